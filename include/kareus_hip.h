@@ -433,6 +433,48 @@ int kr_cross_entropy_bwd(const void* logits, const int64_t* labels, const float*
                          const float* dloss, void* dlogits, int64_t rows, int vocab, int64_t ld,
                          int64_t ld_out, void* stream);
 
+/* Token embedding with a factor: kr_embedding_fwd with out = bf16(scale * weight row).  (The reference multiplies the embedding's
+ * output by a factor in a pass of its own where a model asks for one.)                              */
+int kr_embedding_fwd_scaled(const int64_t* ids, const void* weight, void* out, int s, int b, int hidden,
+                            int64_t vocab_start, int64_t vocab_rows, float scale, void* stream);
+/* The embedding's gradient by sorted tokens: dweight[r, :] = scale * sum of dout over the tokens whose id is vocab_start + r.
+ * ids [b, s], dout [s, b, hidden] as above; dweight: [vocab_rows, hidden], bf16, or fp32 if out_fp32 != 0.
+ * accumulate == 0: every row is written (zeros without a token); != 0: the sum is added to dweight in fp32, rounded once, and rows
+ * without a token are neither read nor written (a gradient kept over several microbatches, the reference's main_grad).
+ * Sums are fp32 in a fixed order that depends on the ids alone: no atomics on values, the result is reproducible.
+ * hidden: a multiple of 8, any size; vocab_rows below 2^27, s * b below 2^26 (KR_EUNSUPPORTED; the workspace query then returns 0).
+ * workspace: 16-byte aligned device memory of the queried size, used by this call only while it runs on the stream.      */
+size_t kr_embedding_bwd_sorted_workspace_bytes(int s, int b, int hidden, int64_t vocab_rows);
+int kr_embedding_bwd_sorted(const int64_t* ids, const void* dout, void* dweight, int out_fp32, int s, int b, int hidden,
+                            int64_t vocab_start, int64_t vocab_rows, float scale, int accumulate,
+                            void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- 8-bit blocks ----------------------------------------------------------------------------
+ * A matrix operand in 8-bit blocks: e4m3 bytes [rows, ld], contiguous along the contraction (ld a multiple of 16, at least the
+ * contraction rounded up to a multiple of 128; the bytes behind the contraction up to that multiple are read and must be 0), and
+ * scale bytes, one per row and block of 128 contraction elements, block b's at s + b * lds (lds a multiple of 4, at least rows):
+ * an element stands for value * 2^(scale - 127).  The quantised operands of the reference's linear layers (quantizer arguments of
+ * kareus/transformer_engine/pytorch/ops/basic/basic_linear.py:391-604).
+ *
+ * kr_block_quantize: bf16 x [rows, cols] (row stride ld, or rows in runs as above: run_rows 1 for a plain matrix, any power of two
+ * that divides rows) -> the operand of its rows (q, s: contraction over cols) and / or of its columns (qt [cols, ldqt], st:
+ * contraction over rows), whichever of q and qt is not NULL, from one read of x.  A block's scale is the smallest power of two that
+ * brings its largest finite magnitude to 448 or below (2^-127 at least; that for a block of zeros), values are rounded to the
+ * nearest, ties to even; infinities and NaN become NaN.  tiles != 0: one scale per 128 x 128 tile, so that both orientations hold
+ * the same values (weights).  cols, ld, run_ld: multiples of 8.  Padding bytes are written (0).
+ *
+ * kr_block_gemm: C [M, N] bf16 (row stride ldc) = A . B^T over K, A with M rows and B with N; accumulate != 0 adds the product to C,
+ * rounded once.  fp32 accumulation.  N, ldc: multiples of 8; M and K: any.  max_cus > 0 limits the launch to that many compute
+ * units.  workspace: NULL or kr_block_gemm_workspace_bytes() bytes (16-byte aligned): with it a product of few tiles and a long
+ * contraction is cut along K; a smaller one is not used.                                              */
+int kr_block_quantize(const void* x, int rows, int cols, int64_t ld, int run_rows, int64_t run_ld, int tiles,
+                      void* q, int64_t ldq, void* s, int64_t lds, void* qt, int64_t ldqt, void* st, int64_t ldst,
+                      void* stream);
+size_t kr_block_gemm_workspace_bytes(int M, int N, int K, int max_cus);
+int kr_block_gemm(int M, int N, int K, const void* A, int64_t lda, const void* sa, int64_t lsa,
+                  const void* B, int64_t ldb, const void* sb, int64_t lsb, void* C, int64_t ldc, int accumulate,
+                  int max_cus, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -12,6 +12,8 @@ from typing import Tuple
 import torch
 from torch import Tensor
 
+from ..block_scaled import BLOCK, BlockOperand, BlockScaled, blocks_of
+
 
 class EagerBackend:
     name = "eager"
@@ -249,12 +251,69 @@ class EagerBackend:
     # Vocabulary-shard embedding: rows of other shards give zeros
     # (3rdparty/Megatron-LM/megatron/core/tensor_parallel/layers.py:245-263); output [s, b, h]
     # (models/common/embeddings/language_model_embedding.py:114-116).
-    def embedding_fwd(self, ids: Tensor, weight: Tensor, vocab_start: int = 0) -> Tensor:
+    def embedding_fwd(self, ids: Tensor, weight: Tensor, vocab_start: int = 0, scale: float = 1.0) -> Tensor:
         rel = ids - vocab_start
         other = (rel < 0) | (rel >= weight.shape[0])
         out = weight[rel.masked_fill(other, 0)]
         out = out.masked_fill(other[..., None], 0.0)
+        if scale != 1.0:
+            out = (out.float() * scale).to(weight.dtype)
         return out.transpose(0, 1).contiguous()
+
+    def embedding_bwd_sorted(self, ids: Tensor, dout: Tensor, vocab_rows: int, vocab_start: int = 0, scale: float = 1.0,
+                             out: Tensor = None, accumulate: bool = False) -> Tensor:
+        rel = (ids - vocab_start).transpose(0, 1).reshape(-1)
+        keep = (rel >= 0) & (rel < vocab_rows)
+        dw = torch.zeros(vocab_rows, dout.shape[-1], dtype=torch.float32, device=dout.device)
+        dw.index_add_(0, rel[keep], dout.reshape(-1, dout.shape[-1])[keep].float())
+        dw *= scale
+        if out is None:
+            if accumulate:
+                raise RuntimeError("embedding_bwd_sorted: accumulate needs the gradient to add to")
+            return dw.to(dout.dtype)
+        return out.copy_(out.float() + dw if accumulate else dw)
+
+    # 8-bit blocks: e = smallest with amax 2^-e <= 448 (frexp: amax = f 2^p, f in [0.5, 1); 448 = 0.875 2^9)
+    @staticmethod
+    def _block_operand(x: Tensor, tiles: bool) -> BlockOperand:
+        r, c = x.shape
+        rb, cb = blocks_of(r), blocks_of(c)
+        p = x.new_zeros((rb * BLOCK, cb * BLOCK), dtype=torch.float32)
+        p[:r, :c] = x
+        size = torch.where(torch.isfinite(p), p.abs(), torch.zeros_like(p)).view(rb, BLOCK, cb, BLOCK)
+        amax = size.amax((1, 3), keepdim=True).expand(rb, BLOCK, cb, 1) if tiles else size.amax(3, keepdim=True)
+        f, e = torch.frexp(amax.reshape(rb * BLOCK, cb))
+        e = torch.where(f > 0.875, e - 8, e - 9).to(torch.int32)
+        e = torch.where(f > 0, e, torch.full_like(e, -127)).clamp(-127, 127)
+        power = ((127 - e) << 23).view(torch.float32)
+        v = p.view(rb * BLOCK, cb, BLOCK) * power[..., None]
+        q = torch.where(torch.isfinite(v), v, torch.full_like(v, float("nan"))).to(torch.float8_e4m3fn)
+        scales = (e + 127).to(torch.uint8).t()[:, :(r + 3) // 4 * 4].contiguous()
+        return BlockOperand(q.view(rb * BLOCK, cb * BLOCK)[:r], scales, c)
+
+    def quantize_blocks(self, x: Tensor, by_row: bool = True, by_col: bool = False, tiles: bool = False) -> BlockScaled:
+        x = x.reshape(-1, x.shape[-1])
+        return BlockScaled(self._block_operand(x, tiles) if by_row else None,
+                           self._block_operand(x.t(), tiles) if by_col else None)
+
+    @staticmethod
+    def _block_values(t: BlockOperand) -> Tensor:
+        e = t.scales[:blocks_of(t.length), :t.rows].t().to(torch.int32)
+        power = torch.where(e > 0, (e << 23).view(torch.float32), torch.full(e.shape, 2.0 ** -127, device=e.device))
+        nb = blocks_of(t.length)
+        v = t.data[:, :nb * BLOCK].float().reshape(t.rows, nb, BLOCK) * power[..., None]
+        return v.view(t.rows, nb * BLOCK)[:, :t.length]
+
+    def block_matmul(self, a: BlockOperand, b: BlockOperand, out: Tensor = None, accumulate: bool = False,
+                     dtype: torch.dtype = torch.bfloat16) -> Tensor:
+        if a.length != b.length:
+            raise RuntimeError(f"block_matmul: contractions of {a.length} and {b.length}")
+        c = self._block_values(a) @ self._block_values(b).t()
+        if out is None:
+            if accumulate:
+                raise RuntimeError("block_matmul: accumulate needs the matrix to add to")
+            return c.to(dtype)
+        return out.copy_(out.float() + c if accumulate else c)
 
     def embedding_bwd(self, ids: Tensor, dout: Tensor, vocab_rows: int, vocab_start: int = 0) -> Tensor:
         rel = (ids - vocab_start).transpose(0, 1).reshape(-1)          # [s, b] order like dout

@@ -7,6 +7,7 @@ dtype other than bf16 raises.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 from typing import Tuple
@@ -14,6 +15,7 @@ from typing import Tuple
 import torch
 from torch import Tensor
 
+from ..block_scaled import BlockOperand, BlockScaled, blocks_of
 from . import reserved_compute_units
 
 _LIB_NAME = "libkareus_hip.so"
@@ -77,8 +79,15 @@ _SIGNATURES = {
     "kr_attn_bwd_workspace_bytes": (_c_size_t, [_c_int] * 5),
     "kr_attn_bwd": (_c_int, [_c_void_p] * 10 + [_c_int] * 5 + [_c_float] + [_c_i64] * 28 + [_c_void_p]),
     "kr_attn_bwd_flags": (_c_int, [_c_void_p] * 10 + [_c_int] * 5 + [_c_float] + [_c_i64] * 28 + [_c_int, _c_void_p]),
+    "kr_embedding_fwd_scaled": (_c_int, [_c_void_p] * 3 + [_c_int] * 3 + [_c_i64, _c_i64, _c_float, _c_void_p]),
+    "kr_embedding_bwd_sorted_workspace_bytes": (_c_size_t, [_c_int] * 3 + [_c_i64]),
+    "kr_embedding_bwd_sorted": (_c_int, [_c_void_p] * 3 + [_c_int] * 4 + [_c_i64, _c_i64, _c_float, _c_int, _c_void_p, _c_size_t, _c_void_p]),
+    "kr_block_quantize": (_c_int, [_c_void_p, _c_int, _c_int, _c_i64, _c_int, _c_i64, _c_int] + [_c_void_p, _c_i64] * 4 + [_c_void_p]),
+    "kr_block_gemm_workspace_bytes": (_c_size_t, [_c_int] * 4),
+    "kr_block_gemm": (_c_int, [_c_int] * 3 + [_c_void_p, _c_i64] * 5 + [_c_int, _c_int, _c_void_p, _c_size_t, _c_void_p]),
 }
 
+_HERE = contextlib.nullcontext()
 KR_GEMM_TN, KR_GEMM_NN, KR_GEMM_NT = 0, 1, 2
 KR_ATTN_BESIDE_OTHER_STREAMS = 0x100
 KR_ATTN_GENERAL_KERNELS = 0x200
@@ -434,6 +443,113 @@ class HipBackend:
         self._check(rc, f"kr_gemm_bf16_nt_segments(M={m}, N={n}, k_seg={k_seg}, nseg={nseg})")
         return out
 
+    # -- 8-bit blocks -------------------------------------------------------------------
+    @staticmethod
+    def _same_device(name: str, *tensors: Tensor) -> None:
+        for t in tensors[1:]:
+            if t.device != tensors[0].device:
+                raise RuntimeError(f"{name}: tensors on {tensors[0].device} and {t.device}")
+
+    @classmethod
+    def _current(cls, t: Tensor):
+        """A ``with`` block in which the tensor's device is the current one."""
+        if t.device.index == (cls._raw_device() if cls._raw_device is not None else torch.cuda.current_device()):
+            return _HERE
+        return torch.cuda.device(t.device)
+
+    def quantize_blocks(self, x: Tensor, by_row: bool = True, by_col: bool = False, tiles: bool = False) -> BlockScaled:
+        """A bf16 matrix [rows, cols] (or a [s, r, cols] nanobatch slice whose rows come in runs, read in place) in 8-bit blocks:
+        e4m3 with a power-of-two scale per 128 elements along the columns (``by_row``) and / or the rows (``by_col``), from one
+        read.  ``tiles``: one scale per 128 x 128 tile, so that both orientations hold the same values."""
+        self._dev(x)
+        self._bf16(x)
+        if not (by_row or by_col):
+            raise RuntimeError("quantize_blocks: neither orientation asked for")
+        if x.dim() < 2:
+            raise RuntimeError("quantize_blocks: needs a matrix")
+        op = self._operand(x) if x.dim() <= 3 and x.data_ptr() % 16 == 0 else None
+        if op is None:
+            x = x.reshape(-1, x.shape[-1]).contiguous()
+            if x.data_ptr() % 16:
+                x = x.clone()
+            op = (x.shape[0], x.shape[1], 1, 0)
+        rows, ld, run_rows, run_ld = op
+        cols = x.shape[-1]
+        if cols % 8:
+            raise RuntimeError(f"quantize_blocks: {cols} columns are no multiple of 8")
+        made = []
+        for want, n, length in ((by_row, rows, cols), (by_col, cols, rows)):
+            made.append(BlockOperand(torch.empty((n, blocks_of(length) * 128), dtype=torch.float8_e4m3fn, device=x.device),
+                                     torch.empty((blocks_of(length), (n + 3) // 4 * 4), dtype=torch.uint8, device=x.device),
+                                     length) if want else None)
+        if rows and cols:
+            args = []
+            for t in made:
+                args += [None, 0, None, 0] if t is None else [t.data.data_ptr(), t.data.shape[1], t.scales.data_ptr(), t.scales.shape[1]]
+            with self._current(x):
+                rc = self.lib.kr_block_quantize(x.data_ptr(), rows, cols, max(ld, cols), run_rows, run_ld, int(tiles), *args,
+                                                self._stream())
+            self._check(rc, f"kr_block_quantize(rows={rows}, cols={cols})")
+        return BlockScaled(*made)
+
+    def _block_operand(self, t: BlockOperand) -> None:
+        d, s = t.data, t.scales
+        if d.dtype != torch.float8_e4m3fn or s.dtype != torch.uint8:
+            raise RuntimeError(f"block_matmul: an operand is float8_e4m3fn with uint8 scales, got {d.dtype} and {s.dtype}")
+        if not d.is_cuda or not s.is_cuda:
+            raise RuntimeError("the hip backend needs tensors on the HIP device")
+        if d.dim() != 2 or d.shape[1] < blocks_of(t.length) * 128 or (d.numel() and d.stride(1) != 1):
+            raise RuntimeError(f"block_matmul: {tuple(d.shape)} values with strides {d.stride()} do not hold rows of {t.length} "
+                               "contraction elements up to a multiple of 128")
+        if s.dim() != 2 or s.shape[0] < blocks_of(t.length) or s.shape[1] < d.shape[0] or (s.numel() and s.stride(1) != 1):
+            raise RuntimeError(f"block_matmul: {tuple(s.shape)} scales with strides {s.stride()} for {d.shape[0]} rows in "
+                               f"{blocks_of(t.length)} blocks")
+
+    def block_matmul(self, a: BlockOperand, b: BlockOperand, out: Tensor = None, accumulate: bool = False,
+                     dtype: torch.dtype = torch.bfloat16) -> Tensor:
+        """``a . b^T`` of two operands in 8-bit blocks over the same contraction, [a.rows, b.rows] in bf16 with fp32 sums:
+        ``y = x . W^T`` from ``(x.by_row, W.by_row)``, ``dx = dy . W`` from ``(dy.by_row, W.by_col)``, ``dW = dy^T . x`` from
+        ``(dy.by_col, x.by_col)``.  ``accumulate``: added to ``out``, rounded once."""
+        self._block_operand(a)
+        self._block_operand(b)
+        if dtype != torch.bfloat16:
+            raise RuntimeError(f"the hip backend computes in bf16, got {dtype}")
+        m, n, k = a.rows, b.rows, a.length
+        if b.length != k:
+            raise RuntimeError(f"block_matmul: contractions of {k} and {b.length}")
+        if out is None:
+            if accumulate:
+                raise RuntimeError("block_matmul: accumulate needs the matrix to add to")
+            out = torch.empty((m, n), dtype=dtype, device=a.data.device)
+        else:
+            self._dev(out)
+            self._bf16(out)
+            if tuple(out.shape) != (m, n) or (out.numel() and out.stride(1) != 1):
+                raise RuntimeError(f"block_matmul: out must be [{m}, {n}] with a contiguous last dimension")
+        self._same_device("block_matmul", a.data, a.scales, b.data, b.scales, out)
+        if not m or not n:
+            return out
+        if not k:
+            return out if accumulate else out.zero_()
+        max_cus = 0
+        reserved = reserved_compute_units()
+        if reserved:
+            max_cus = max(self._num_cus(a.data.device) - reserved, 8)
+        with self._current(out):
+            nbytes = self.lib.kr_block_gemm_workspace_bytes(m, n, k, max_cus)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=out.device) if nbytes else None
+            rc = self.lib.kr_block_gemm(m, n, k, a.data.data_ptr(), self._pitch(a.data), a.scales.data_ptr(), self._pitch(a.scales),
+                                        b.data.data_ptr(), self._pitch(b.data), b.scales.data_ptr(), self._pitch(b.scales),
+                                        out.data_ptr(), self._pitch(out), int(accumulate), max_cus,
+                                        None if ws is None else ws.data_ptr(), nbytes, self._stream())
+        self._check(rc, f"kr_block_gemm(M={m}, N={n}, K={k})")
+        return out
+
+    @staticmethod
+    def _pitch(t: Tensor) -> int:
+        """Elements from one row to the next (a single row may have any stride)."""
+        return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
     # -- RMSNorm ----------------------------------------------------------------------
     @staticmethod
     def _rows(t: Tensor) -> Tensor:
@@ -767,8 +883,8 @@ class HipBackend:
             return t.reshape(t.shape[0], -1)
 
     # -- embedding and loss ---------------------------------------------------------------
-    def embedding_fwd(self, ids: Tensor, weight: Tensor, vocab_start: int = 0) -> Tensor:
-        """ids [b, s] int64 -> [s, b, hidden]; ids outside this shard's rows give zeros."""
+    def embedding_fwd(self, ids: Tensor, weight: Tensor, vocab_start: int = 0, scale: float = 1.0) -> Tensor:
+        """ids [b, s] int64 -> ``scale *`` rows of the weight, [s, b, hidden]; ids outside this shard's rows give zeros."""
         self._dev(weight)
         self._on_device(ids)
         self._bf16(weight)
@@ -777,6 +893,17 @@ class HipBackend:
         ids = ids.contiguous()
         b, s = ids.shape
         out = torch.empty((s, b, weight.shape[1]), dtype=weight.dtype, device=weight.device)
+        if scale != 1.0:
+            if not ids.numel():
+                return out
+            self._same_device("embedding_fwd", weight, ids)
+            if weight.dim() != 2 or not weight.is_contiguous():
+                raise RuntimeError("embedding_fwd: the table must be a dense [rows, hidden] matrix")
+            with self._current(weight):
+                rc = self.lib.kr_embedding_fwd_scaled(ids.data_ptr(), weight.data_ptr(), out.data_ptr(), s, b, weight.shape[1],
+                                                      vocab_start, weight.shape[0], float(scale), self._stream())
+            self._check(rc, f"kr_embedding_fwd_scaled(s={s}, b={b}, hidden={weight.shape[1]})")
+            return out
         rc = self.lib.kr_embedding_fwd(ids.data_ptr(), weight.data_ptr(), out.data_ptr(), s, b,
                                        weight.shape[1], vocab_start, weight.shape[0], self._stream())
         self._check(rc, "kr_embedding_fwd")
@@ -793,6 +920,38 @@ class HipBackend:
                                        vocab_start, vocab_rows, self._stream())
         self._check(rc, "kr_embedding_bwd")
         return dw
+
+    def embedding_bwd_sorted(self, ids: Tensor, dout: Tensor, vocab_rows: int, vocab_start: int = 0, scale: float = 1.0,
+                             out: Tensor = None, accumulate: bool = False) -> Tensor:
+        """The gradient of :meth:`embedding_fwd` with respect to the weight, ``[vocab_rows, hidden]``, by sorted tokens: sums in
+        fp32 in an order that the ids fix.  ``out`` (dense bf16 or fp32; by default a new bf16 tensor) is written whole, or with
+        ``accumulate`` has the gradient added to it (rounded once), where rows without a token are left alone."""
+        self._dev(dout)
+        self._on_device(ids)
+        self._bf16(dout)
+        if ids.dim() != 2 or dout.dim() != 3 or dout.shape[:2] != (ids.shape[1], ids.shape[0]):
+            raise RuntimeError(f"embedding_bwd_sorted: ids must be [b, s] and dout [s, b, hidden], got {tuple(ids.shape)} and "
+                               f"{tuple(dout.shape)}")
+        hidden = dout.shape[2]
+        if out is None:
+            if accumulate:
+                raise RuntimeError("embedding_bwd_sorted: accumulate needs the gradient to add to")
+            out = torch.empty((vocab_rows, hidden), dtype=dout.dtype, device=dout.device)
+        elif tuple(out.shape) != (vocab_rows, hidden) or not out.is_contiguous() or out.dtype not in (torch.bfloat16, torch.float32):
+            raise RuntimeError(f"embedding_bwd_sorted: out must be a dense bf16 or fp32 [{vocab_rows}, {hidden}] matrix")
+        self._same_device("embedding_bwd_sorted", dout, ids, out)
+        if not ids.numel() or not out.numel():
+            return out if accumulate else out.zero_()
+        ids, dout = ids.contiguous(), dout.contiguous()
+        b, s = ids.shape
+        with self._current(dout):
+            nbytes = self.lib.kr_embedding_bwd_sorted_workspace_bytes(s, b, hidden, vocab_rows)
+            ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dout.device)
+            rc = self.lib.kr_embedding_bwd_sorted(ids.data_ptr(), dout.data_ptr(), out.data_ptr(), int(out.dtype == torch.float32),
+                                                  s, b, hidden, vocab_start, vocab_rows, float(scale), int(accumulate),
+                                                  ws.data_ptr(), nbytes, self._stream())
+        self._check(rc, f"kr_embedding_bwd_sorted(s={s}, b={b}, hidden={hidden}, vocab_rows={vocab_rows})")
+        return out
 
     def cross_entropy_fwd(self, logits: Tensor, labels: Tensor) -> Tuple[Tensor, Tensor]:
         """logits [rows, vocab] bf16, labels [rows] int64 -> (loss [rows] fp32, lse [rows] fp32)."""

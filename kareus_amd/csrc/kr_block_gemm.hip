@@ -1,0 +1,503 @@
+// Product of two matrices held in 8-bit blocks: C[M,N] = A . B^T, A [M,K] and B [N,K] e4m3, contiguous along the contraction,
+// one power-of-two scale per row and block of 128 contraction elements, fp32 accumulation, bf16 store.
+//
+//   C[m, n] (+)= sum_kb 2^(sa[kb, m] - 127 + sb[kb, n] - 127) sum_{k in block kb} a[m, k] b[n, k]
+//
+// The matrix instruction (v_mfma_scale_f32_32x32x64_f8f6f4, 131072 FLOP in 64 cycles, twice the rate of the unscaled 8-bit ones)
+// multiplies by 2^(scale - 127) of both operands' rows on its way into the sum, so the scales cost nothing but their loads.
+#include "kr_common.h"
+
+#include <algorithm>
+
+namespace {
+
+typedef __attribute__((__vector_size__(8 * sizeof(int)))) int i32x8;
+typedef __attribute__((__vector_size__(4 * sizeof(int)))) int i32x4;
+
+constexpr int BK = 128;        // contraction elements (and bytes) of a K-step: one scale block
+constexpr int NTHREADS = 256;
+constexpr int kXcds = 8;
+constexpr int kGroupM = 4;
+enum Out { kStore, kAccumulate, kPartial };
+
+struct Args {
+  const uint8_t* a;
+  const uint8_t* sa;
+  const uint8_t* b;
+  const uint8_t* sb;
+  bf16* c;
+  float* partial;
+  int64_t lda, ldb, ldc;
+  int lsa, lsb;            // bytes from one scale block's row to the next (multiples of 4)
+  int m, n, ksteps, steps_per, splits;
+};
+
+__device__ __forceinline__ uint32_t lds_addr(const uint8_t* p) { return (uint32_t)(uintptr_t)(KR_LDS const uint8_t*)p; }
+
+// One direct global -> LDS load: lane p's 16 bytes land at lds + 16 p (lds wave-uniform).  Inline assembly, so that the compiler does
+// not drain it in front of every barrier; the K loop waits for all of them by hand.
+template <int IMM>
+__device__ __forceinline__ void dma_b128(const void* base, uint32_t byte_off, uint32_t lds_base) {
+  asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+               :
+               : "s"(lds_base), "v"(byte_off), "s"(base), "n"(IMM)
+               : "memory", "m0", "scc");
+}
+
+// ids congruent mod 8 run on one XCD: each XCD takes a compact band of C
+__device__ __forceinline__ void tile_of(int pid, int nblocks, int tiles_m, int tiles_n, int& tm, int& tn) {
+  const int q = nblocks / kXcds, r = nblocks % kXcds;
+  const int xcd = pid % kXcds, local = pid / kXcds;
+  const int lid = xcd * q + (xcd < r ? xcd : r) + local;
+  const int per_band = kGroupM * tiles_n;
+  const int band = lid / per_band;
+  const int first_m = band * kGroupM;
+  const int band_rows = (tiles_m - first_m) < kGroupM ? (tiles_m - first_m) : kGroupM;
+  const int in_band = lid - band * per_band;
+  tn = in_band / band_rows;
+  tm = first_m + in_band - tn * band_rows;
+}
+
+// The scales of a wave's 32 W rows, one lane's part: the W bytes of rows W j .. W j + W - 1.
+template <int W>
+__device__ __forceinline__ int load_scales(const uint8_t* p) {
+  if constexpr (W == 4) return *reinterpret_cast<const int*>(p);
+  if constexpr (W == 2) return *reinterpret_cast<const uint16_t*>(p);
+  return *p;
+}
+
+// WT x WN tiles of 32 x 32 per wave, four waves as 2 x 2: 64 WT x 64 WN of C per workgroup.
+//   * Row j of a wave's MFMA tile g is row W j + g of its 32 W rows (W = WT for A, WN for B), so that one load per lane brings the
+//     scales of all its tiles for a K-step, packed as the instruction's byte selector takes them, and a lane ends up with 4 WN
+//     consecutive columns of C.  Rows lie in LDS in tile order: the load of a tile places them.
+//   * Two K-steps lie in LDS.  Each is computed in two halves of 64; behind the barrier in the middle of step t all of t is in
+//     registers or used up and the loads of t + 2 go where it lay, with one to one and a half K-steps to land.
+//   * An LDS row is 128 bytes, its 16-byte chunks XORed with (row >> 1) & 7: the 16 rows that a fragment read takes at a time cover
+//     all banks once.
+template <int WT, int WN, int OUT>
+__global__ __launch_bounds__(NTHREADS, WT * WN <= 4 ? 2 : 1) void block_gemm_kernel(Args g) {
+#ifdef __HIP_DEVICE_COMPILE__   // (the host's pass over this file cannot place the registers that the assembly names)
+  constexpr int BM = 64 * WT, BN = 64 * WN;
+  constexpr int NA = 2 * WT, NB = 2 * WN;                       // loads per wave of an operand's K-step
+  constexpr uint32_t SLOT = (BM + BN) * BK;                     // bytes of a K-step in LDS
+  constexpr int ROWB = 64 * WN;                                 // bytes of a staged row of a wave's output
+  extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave >> 1, wn = wave & 1;
+  const uint32_t smem_b = lds_addr(smem);
+  const uint32_t stage = smem_b + 2 * SLOT + (uint32_t)wave * (32 * ROWB);
+  const int tiles_m = (g.m + BM - 1) / BM, tiles_n = (g.n + BN - 1) / BN;
+  const int ntiles = tiles_m * tiles_n;
+  const int total = ntiles * (OUT == kPartial ? g.splits : 1);
+
+  struct Item {
+    int m0, n0, k0, nk, split;
+  };
+  auto select = [&](int v) {
+    Item it;
+    it.split = v / ntiles;
+    int tm, tn;
+    tile_of(v - it.split * ntiles, ntiles, tiles_m, tiles_n, tm, tn);
+    it.m0 = tm * BM;
+    it.n0 = tn * BN;
+    it.k0 = OUT == kPartial ? it.split * g.steps_per : 0;
+    it.nk = OUT == kPartial ? (g.ksteps - it.k0 < g.steps_per ? g.ksteps - it.k0 : g.steps_per) : g.ksteps;
+    return it;
+  };
+
+  // ---- requests: a cursor over the K-steps of all items of this workgroup, two steps ahead of the computation ----
+  int r_item = blockIdx.x;
+  int r_left;
+  const uint8_t *ra, *rb, *rsa, *rsb;   // of the K-step to request next (wave-uniform)
+  uint32_t la[NA], lb[NB];
+  uint32_t lsa, lsb;
+  auto aim = [&](int v) {
+    const Item it = select(v);
+    r_left = it.nk;
+    ra = g.a + (int64_t)it.m0 * g.lda + (int64_t)it.k0 * BK;
+    rb = g.b + (int64_t)it.n0 * g.ldb + (int64_t)it.k0 * BK;
+    rsa = g.sa + (int64_t)it.k0 * g.lsa;
+    rsb = g.sb + (int64_t)it.k0 * g.lsb;
+    int l2 = lane;
+    asm volatile("" : "+v"(l2));
+    // load i of a wave fills LDS rows 8 (wave + 4 i) .. + 7; beyond the matrix: its last row (never stored)
+    const int sub = l2 >> 3;
+#pragma unroll
+    for (int i = 0; i < NA; ++i) {
+      const int row = 8 * (wave + 4 * i) + sub;
+      const int w = row / (32 * WT), t = row % (32 * WT) / 32, j = row % 32;
+      int r = 32 * WT * w + WT * j + t;
+      r = it.m0 + r < g.m ? r : g.m - 1 - it.m0;
+      la[i] = (uint32_t)r * (uint32_t)g.lda + (uint32_t)(((l2 & 7) ^ ((row >> 1) & 7)) << 4);
+    }
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      const int row = 8 * (wave + 4 * i) + sub;
+      const int w = row / (32 * WN), t = row % (32 * WN) / 32, j = row % 32;
+      int r = 32 * WN * w + WN * j + t;
+      r = it.n0 + r < g.n ? r : g.n - 1 - it.n0;
+      lb[i] = (uint32_t)r * (uint32_t)g.ldb + (uint32_t)(((l2 & 7) ^ ((row >> 1) & 7)) << 4);
+    }
+    const int sra = it.m0 + 32 * WT * wm + WT * (l2 & 31), srb = it.n0 + 32 * WN * wn + WN * (l2 & 31);
+    lsa = (uint32_t)(sra < g.lsa - WT ? sra : g.lsa - WT);
+    lsb = (uint32_t)(srb < g.lsb - WN ? srb : g.lsb - WN);
+  };
+  // (behind the last item's last K-step it stays there: the K loop requests that one again rather than branch, two steps in all)
+  auto advance = [&]() {
+    if (--r_left > 0) {
+      ra += BK;
+      rb += BK;
+      rsa += g.lsa;
+      rsb += g.lsb;
+    } else if (r_item + (int)gridDim.x < total) {
+      r_item += gridDim.x;
+      aim(r_item);
+    } else {
+      r_left = 1;
+    }
+  };
+  auto request_a = [&](auto i_tag, uint32_t slot) {
+    constexpr int i = decltype(i_tag)::value;
+    dma_b128<i * 4096>(ra, la[i], slot + (uint32_t)wave * 1024u);
+  };
+  auto request_b = [&](auto i_tag, uint32_t slot) {
+    constexpr int i = decltype(i_tag)::value;
+    dma_b128<BM * BK + i * 4096>(rb, lb[i], slot + (uint32_t)wave * 1024u);
+  };
+
+  // The accumulators of the large tile are the wave's 256 accumulation registers (its MFMAs are inline assembly, to pin them there:
+  // with the builtin the compiler moves and spills them); smaller tiles leave them to the compiler.
+  constexpr bool PINNED = WT * WN > 4;
+  f32x16 acc[WT][WN];
+  struct Frags {
+    i32x8 a[WT], b[WN];
+  } X, Y;
+  auto clear = [&]() {
+#pragma unroll
+    for (int i = 0; i < WT; ++i)
+#pragma unroll
+      for (int j = 0; j < WN; ++j)
+{
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+        if constexpr (PINNED) asm volatile("" : "+a"(acc[i][j]));
+      }
+  };
+
+  // fragment addresses: lane l takes row l % 32 of a tile, chunks 4 h + 2 (l / 32) and + 1 of half h
+  const uint32_t frag0 = (uint32_t)((lane & 31) * BK + (((2 * (lane >> 5)) ^ ((lane >> 1) & 7)) << 4));
+  const uint32_t fa0 = smem_b + (uint32_t)(wm * 32 * WT * BK) + frag0;
+  const uint32_t fb0 = smem_b + (uint32_t)((BM + wn * 32 * WN) * BK) + frag0;
+  auto lds16 = [&](uint32_t a) { return *(KR_LDS const i32x4*)a; };
+  auto frag = [&](uint32_t a, uint32_t b) {
+    const i32x4 lo = lds16(a), hi = lds16(b);
+    return i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+  };
+
+  // One half of a K-step: the MFMAs on `cur`, and between them the fragment reads of half h of the K-step in `slot` and the loads
+  // of one K-step into `dslot` (if DMA).
+  auto half = [&](Frags& cur, Frags& nxt, int sa, int sb, uint32_t slot, int h, auto dma_tag, uint32_t dslot) {
+    constexpr bool DMA = decltype(dma_tag)::value;
+    const uint32_t a0 = (fa0 ^ (uint32_t)(h << 6)) + slot, b0 = (fb0 ^ (uint32_t)(h << 6)) + slot;
+    const uint32_t a1 = a0 ^ 16u, b1 = b0 ^ 16u;
+    auto step = [&](auto gt, auto nt) {
+      constexpr int gi = decltype(gt)::value, ni = decltype(nt)::value;
+      if constexpr (PINNED) {
+        if constexpr (gi == 0 && ni == 0) asm volatile("s_nop 3" ::: "memory");   // (the scales may just have been moved)
+        asm volatile("v_mfma_scale_f32_32x32x64_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[%5,%6,0] op_sel_hi:[%7,%8,0]"
+                     : "+a"(acc[gi][ni])
+                     : "v"(cur.b[ni]), "v"(cur.a[gi]), "v"(sb), "v"(sa), "n"(ni & 1), "n"(gi & 1), "n"(ni >> 1), "n"(gi >> 1));
+      } else {
+        acc[gi][ni] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(cur.b[ni], cur.a[gi], acc[gi][ni], 0, 0, ni, sb, gi, sa);
+      }
+      if constexpr (ni == 0) nxt.a[gi] = frag(a0 + gi * 32 * BK, a1 + gi * 32 * BK);
+      if constexpr (gi == 0) nxt.b[ni] = frag(b0 + ni * 32 * BK, b1 + ni * 32 * BK);
+      if constexpr (DMA) {
+        // the loads ride one behind each MFMA, operand A's first
+        constexpr int per = (NA + NB + WT * WN - 1) / (WT * WN), at = (gi * WN + ni) * per;
+#define KR_REQ(d)                                                                                          \
+  if constexpr (d < per) {                                                                                 \
+    if constexpr (at + d < NA) request_a(std::integral_constant<int, at + d>{}, dslot);                    \
+    else if constexpr (at + d < NA + NB) request_b(std::integral_constant<int, at + d - NA>{}, dslot);     \
+  }
+        KR_REQ(0) KR_REQ(1) KR_REQ(2) KR_REQ(3)
+#undef KR_REQ
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    auto row = [&](auto gt) {
+      step(gt, std::integral_constant<int, 0>{});
+      if constexpr (WN > 1) step(gt, std::integral_constant<int, 1>{});
+      if constexpr (WN > 2) step(gt, std::integral_constant<int, 2>{});
+      if constexpr (WN > 3) step(gt, std::integral_constant<int, 3>{});
+    };
+    row(std::integral_constant<int, 0>{});
+    if constexpr (WT > 1) row(std::integral_constant<int, 1>{});
+    if constexpr (WT > 2) row(std::integral_constant<int, 2>{});
+    if constexpr (WT > 3) row(std::integral_constant<int, 3>{});
+  };
+  auto request_all = [&](uint32_t dslot) {
+    auto one = [&](auto i) {
+      if constexpr (decltype(i)::value < NA) request_a(i, dslot);
+    };
+    auto two = [&](auto i) {
+      if constexpr (decltype(i)::value < NB) request_b(i, dslot);
+    };
+#define KR_ALL(f)                                                                                          \
+  f(std::integral_constant<int, 0>{}); f(std::integral_constant<int, 1>{}); f(std::integral_constant<int, 2>{}); \
+  f(std::integral_constant<int, 3>{}); f(std::integral_constant<int, 4>{}); f(std::integral_constant<int, 5>{}); \
+  f(std::integral_constant<int, 6>{}); f(std::integral_constant<int, 7>{});
+    KR_ALL(one)
+    KR_ALL(two)
+#undef KR_ALL
+  };
+
+  // ---- start: K-steps 0 and 1 requested, half 0 of step 0 read ----
+  Item it = select(blockIdx.x);
+  int item = blockIdx.x;
+  aim(r_item);
+  int sa = load_scales<WT>(rsa + lsa), sb = load_scales<WN>(rsb + lsb);
+  request_all(0 + smem_b);
+  advance();
+  int sa1 = load_scales<WT>(rsa + lsa), sb1 = load_scales<WN>(rsb + lsb);
+  request_all(SLOT + smem_b);
+  advance();
+  clear();
+  __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0)
+  kr_barrier();
+  {
+    const uint32_t a0 = fa0, b0 = fb0;
+#pragma unroll
+    for (int i = 0; i < WT; ++i) X.a[i] = frag(a0 + i * 32 * BK, (a0 ^ 16u) + i * 32 * BK);
+#pragma unroll
+    for (int i = 0; i < WN; ++i) X.b[i] = frag(b0 + i * 32 * BK, (b0 ^ 16u) + i * 32 * BK);
+  }
+  uint32_t slot = 0;   // of the current K-step, 0 or SLOT
+  for (;;) {
+    for (int t = 0; t < it.nk; ++t) {
+      half(X, Y, sa, sb, slot, 1, std::false_type{}, 0u);
+      __builtin_amdgcn_s_waitcnt(0x0f70);
+      kr_barrier();
+      const uint32_t other = SLOT - slot;
+      const int sa2 = load_scales<WT>(rsa + lsa), sb2 = load_scales<WN>(rsb + lsb);
+      // (behind the last K-step it reads what is not there: unused)
+      half(Y, X, sa, sb, other, 0, std::true_type{}, slot + smem_b);
+      advance();
+      sa = sa1;
+      sb = sb1;
+      sa1 = sa2;
+      sb1 = sb2;
+      slot = other;
+    }
+
+    // the compiler does not know the latency of MFMAs in assembly: let the last ones finish before their results are read
+    if constexpr (PINNED) asm volatile("s_nop 15\n\ts_nop 15\n\ts_nop 15\n\ts_nop 15\n\ts_nop 15" ::: "memory");
+
+    // ---- epilogue: lane l holds row WT (l % 32) + g of its wave, columns WN (8 q + 4 (l / 32)) .. + 4 WN - 1 for q = 0..3 ----
+    {
+      int le = lane;
+      asm volatile("" : "+v"(le));
+      const int j = le & 31, hi = le >> 5;
+      const int m_wave = it.m0 + 32 * WT * wm, n_wave = it.n0 + 32 * WN * wn;
+#pragma unroll
+      for (int gi = 0; gi < WT; ++gi) {
+        const int row = m_wave + WT * j + gi;
+        f32x16 val[WN];
+#pragma unroll
+        for (int ni = 0; ni < WN; ++ni) {
+          if constexpr (PINNED) asm volatile("" : "+a"(acc[gi][ni]));
+          val[ni] = acc[gi][ni];
+          if constexpr (PINNED) asm volatile("" : "+v"(val[ni]));
+        }
+        if constexpr (OUT == kPartial) {
+          float* const p = g.partial + ((int64_t)it.split * g.m + row) * g.n;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int col = n_wave + WN * (8 * q + 4 * hi);
+#pragma unroll
+            for (int v = 0; v < WN; ++v) {
+              f32x4 o;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int c = 4 * v + e;
+                o[e] = val[c % WN][4 * q + c / WN];
+              }
+              if (row < g.m && col + 4 * v < g.n) *reinterpret_cast<f32x4*>(p + col + 4 * v) = o;
+            }
+          }
+        } else {
+          bf16 vals[4][4 * WN];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int col = n_wave + WN * (8 * q + 4 * hi);
+#pragma unroll
+            for (int c = 0; c < 4 * WN; ++c) {
+              float v = val[c % WN][4 * q + c / WN];
+              if constexpr (OUT == kAccumulate) {
+                const bool in = row < g.m && col + (c & ~3) < g.n;
+                const bf16x4 old = in ? *reinterpret_cast<const bf16x4*>(g.c + (int64_t)row * g.ldc + col + (c & ~3)) : bf16x4{};
+                v += (float)old[c & 3];
+              }
+              vals[q][c] = (bf16)v;
+            }
+          }
+          // rows of the block through LDS, then whole rows to memory
+          constexpr int PIECES = ROWB / 16 > 0 ? ROWB / 16 : 1;
+          __builtin_amdgcn_wave_barrier();
+          if constexpr (WN == 1) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const bf16x4 o = {vals[q][0], vals[q][1], vals[q][2], vals[q][3]};
+              *(KR_LDS bf16x4*)(stage + j * ROWB + ((q ^ ((j >> 2) & 3)) << 4) + 8 * hi) = o;
+            }
+          } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+              for (int v = 0; v < WN / 2; ++v) {
+                bf16x8 o;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) o[e] = vals[q][8 * v + e];
+                const int piece = WN / 2 * (2 * q + hi) + v;
+                const int x = WN == 4 ? j & 15 : (j >> 1) & 7;
+                *(KR_LDS bf16x8*)(stage + j * ROWB + ((piece ^ x) << 4)) = o;
+              }
+          }
+          __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+          __builtin_amdgcn_wave_barrier();
+          __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+          const int piece = le % PIECES, r0 = le / PIECES;
+          constexpr int RPP = 64 / PIECES;
+#pragma unroll
+          for (int p = 0; p < 32 / RPP; ++p) {
+            const int jj = p * RPP + r0;
+            const int x = WN == 4 ? jj & 15 : WN == 2 ? (jj >> 1) & 7 : (jj >> 2) & 3;
+            const bf16x8 v = *(KR_LDS const bf16x8*)(stage + jj * ROWB + ((piece ^ x) << 4));
+            const int rr = m_wave + WT * jj + gi;
+            if (rr < g.m && n_wave + 8 * piece < g.n) stg8_stream(g.c + (int64_t)rr * g.ldc + n_wave + 8 * piece, v);
+          }
+          __builtin_amdgcn_wave_barrier();
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      clear();
+    }
+    item += gridDim.x;
+    if (item >= total) break;
+    it = select(item);
+  }
+  __builtin_amdgcn_s_waitcnt(0x0f70);   // the loads requested again: LDS is given up only when they have landed
+#endif
+}
+
+// C = bf16(sum of the cuts' fp32 partial products, in order [+ C])
+__global__ __launch_bounds__(256) void block_gemm_reduce_kernel(const float* __restrict__ partial, bf16* __restrict__ C,
+                                                                int64_t ldc, int M, int N, int splits, int accumulate) {
+  const int nv = N / 8;
+  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (idx >= (int64_t)M * nv) return;
+  const int m = (int)(idx / nv), n = (int)(idx % nv) * 8;
+  float acc[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) acc[e] = 0.f;
+  for (int sp = 0; sp < splits; ++sp) {
+    const float* src = partial + ((int64_t)sp * M + m) * N + n;
+    const f32x4 a = *reinterpret_cast<const f32x4*>(src), b = *reinterpret_cast<const f32x4*>(src + 4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      acc[e] += a[e];
+      acc[4 + e] += b[e];
+    }
+  }
+  bf16* dst = C + (int64_t)m * ldc + n;
+  if (accumulate) {
+    const bf16x8 old = ldg8(dst);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] += (float)old[e];
+  }
+  bf16x8 o;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) o[e] = (bf16)acc[e];
+  stg8(dst, o);
+}
+
+struct Plan {
+  int w, splits, steps_per;   // w: tiles per wave along both sides (4: 256 x 256, 2: 128 x 128, 1: 64 x 64)
+};
+
+Plan choose_plan(int M, int N, int K, int cus) {
+  const int ksteps = (K + BK - 1) / BK;
+  Plan p{4, 1, ksteps};
+  auto tiles = [&](int w) { return (int64_t)((M + 64 * w - 1) / (64 * w)) * ((N + 64 * w - 1) / (64 * w)); };
+  if (tiles(4) < cus) p.w = 2;
+  if (tiles(2) < cus) p.w = 1;
+  return p;
+}
+
+int device_cus() {
+  int dev = 0, n = 0;
+  if (hipGetDevice(&dev) != hipSuccess) return 256;
+  if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) return 256;
+  return n;
+}
+
+template <int W, int OUT>
+int launch(const Args& g, int cus, hipStream_t stream) {
+  constexpr size_t lds = 2 * (128 * W) * BK + 4 * 32 * 64 * W;
+  static const hipError_t raised = hipFuncSetAttribute((const void*)block_gemm_kernel<W, W, OUT>,
+                                                       hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+  if (raised != hipSuccess) return KR_ELAUNCH;
+  const int64_t tiles = (int64_t)((g.m + 64 * W - 1) / (64 * W)) * ((g.n + 64 * W - 1) / (64 * W)) * g.splits;
+  if (tiles > 0x3fffffff) return KR_EUNSUPPORTED;
+  const int64_t grid = std::min<int64_t>(tiles, (int64_t)cus * (W <= 2 ? 2 : 1));
+  hipLaunchKernelGGL((block_gemm_kernel<W, W, OUT>), dim3((unsigned)grid), dim3(NTHREADS), lds, stream, g);
+  return kr_launch_status();
+}
+
+template <int OUT>
+int launch_w(const Plan& p, const Args& g, int cus, hipStream_t stream) {
+  if (p.w == 4) return launch<4, OUT>(g, cus, stream);
+  if (p.w == 2) return launch<2, OUT>(g, cus, stream);
+  return launch<1, OUT>(g, cus, stream);
+}
+
+}  // namespace
+
+extern "C" size_t kr_block_gemm_workspace_bytes(int M, int N, int K, int max_cus) {
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  const int all = device_cus();
+  const Plan p = choose_plan(M, N, K, max_cus > 0 && max_cus < all ? max_cus : all);
+  return p.splits > 1 ? (size_t)p.splits * M * N * sizeof(float) : 0;
+}
+
+extern "C" int kr_block_gemm(int M, int N, int K, const void* A, int64_t lda, const void* sa, int64_t lsa, const void* B,
+                             int64_t ldb, const void* sb, int64_t lsb, void* C, int64_t ldc, int accumulate, int max_cus,
+                             void* workspace, size_t workspace_bytes, void* stream) {
+  if (!A || !sa || !B || !sb || !C || M <= 0 || N <= 0 || K <= 0) return KR_EINVAL;
+  if (N % 8 || ldc % 8 || lda % 16 || ldb % 16 || lsa % 4 || lsb % 4) return KR_EUNSUPPORTED;
+  const int64_t kp = ((int64_t)K + BK - 1) / BK * BK;
+  if (lda < kp || ldb < kp || lsa < M || lsb < N || ldc < N) return KR_EINVAL;
+  if (!kr_aligned16(A) || !kr_aligned16(B) || !kr_aligned16(C) || !kr_aligned16(workspace) ||
+      (reinterpret_cast<uintptr_t>(sa) & 3) || (reinterpret_cast<uintptr_t>(sb) & 3))
+    return KR_EINVAL;
+  // a tile's rows are addressed with 32-bit offsets from its first
+  if (lda > (1 << 23) || ldb > (1 << 23) || lsa > 0x7fffffff || lsb > 0x7fffffff || M > 0x7fffff00 || N > 0x7fffff00)
+    return KR_EUNSUPPORTED;
+  const int all = device_cus();
+  const int cus = max_cus > 0 && max_cus < all ? max_cus : all;
+  Plan p = choose_plan(M, N, K, cus);
+  if (p.splits > 1 && (!workspace || workspace_bytes < (size_t)p.splits * M * N * sizeof(float))) p = Plan{p.w, 1, (K + BK - 1) / BK};
+  Args g{(const uint8_t*)A, (const uint8_t*)sa, (const uint8_t*)B, (const uint8_t*)sb, (bf16*)C, (float*)workspace,
+         lda, ldb, ldc, (int)lsa, (int)lsb, M, N, (K + BK - 1) / BK, p.steps_per, p.splits};
+  if (p.splits > 1) {
+    const int rc = launch_w<kPartial>(p, g, cus, (hipStream_t)stream);
+    if (rc != KR_OK) return rc;
+    const int64_t threads = (int64_t)M * (N / 8);
+    if ((threads + 255) / 256 > 0x7fffffff) return KR_EUNSUPPORTED;
+    hipLaunchKernelGGL(block_gemm_reduce_kernel, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, (hipStream_t)stream,
+                       (const float*)workspace, (bf16*)C, ldc, M, N, p.splits, accumulate);
+    return kr_launch_status();
+  }
+  return accumulate ? launch_w<kAccumulate>(p, g, cus, (hipStream_t)stream) : launch_w<kStore>(p, g, cus, (hipStream_t)stream);
+}
