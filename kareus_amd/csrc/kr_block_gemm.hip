@@ -8,6 +8,8 @@
 #include "kr_common.h"
 
 #include <algorithm>
+#include <type_traits>
+#include <utility>
 
 namespace {
 
@@ -44,6 +46,15 @@ __device__ __forceinline__ void dma_b128(const void* base, uint32_t byte_off, ui
                : "memory", "m0", "scc");
 }
 
+__device__ __forceinline__ void dma_b32(const void* base, uint32_t byte_off, uint32_t lds_base) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2"
+               :
+               : "s"(lds_base), "v"(byte_off), "s"(base)
+               : "memory", "m0");
+}
+// s_waitcnt immediate for vmcnt(n); lgkmcnt and expcnt untouched
+constexpr int vm_wait(int n) { return 0x0f70 | (n & 15) | ((n >> 4) << 14); }
+
 // ids congruent mod 8 run on one XCD: each XCD takes a compact band of C
 __device__ __forceinline__ void tile_of(int pid, int nblocks, int tiles_m, int tiles_n, int& tm, int& tn) {
   const int q = nblocks / kXcds, r = nblocks % kXcds;
@@ -58,35 +69,51 @@ __device__ __forceinline__ void tile_of(int pid, int nblocks, int tiles_m, int t
   tm = first_m + in_band - tn * band_rows;
 }
 
-// The scales of a wave's 32 W rows, one lane's part: the W bytes of rows W j .. W j + W - 1.
 template <int W>
-__device__ __forceinline__ int load_scales(const uint8_t* p) {
-  if constexpr (W == 4) return *reinterpret_cast<const int*>(p);
-  if constexpr (W == 2) return *reinterpret_cast<const uint16_t*>(p);
-  return *p;
+__device__ __forceinline__ int lds_scales(uint32_t a) {
+  if constexpr (W == 4) return *(KR_LDS const int*)a;
+  if constexpr (W == 2) return *(KR_LDS const uint16_t*)a;
+  return *(KR_LDS const uint8_t*)a;
+}
+template <int N>
+using Int = std::integral_constant<int, N>;
+template <class F, int... I>
+__device__ __forceinline__ void each(F&& f, std::integer_sequence<int, I...>) {
+  (f(Int<I>{}), ...);
+}
+
+// LDS of one instance: eight blocks of 64 contraction bytes (both operands' halves of two K-steps), two K-steps' scales, staging
+constexpr int stage_row(int wn) { return wn == 4 ? 128 : 64; }
+constexpr uint32_t block_bytes(int w) { return 64 * w * 64; }
+constexpr size_t lds_bytes(int wt, int wn) {
+  return 4 * (size_t)(block_bytes(wt > wn ? wt : wn) * 2) + 2 * 512 + 4 * 32 * stage_row(wn);
 }
 
 // WT x WN tiles of 32 x 32 per wave, four waves as 2 x 2: 64 WT x 64 WN of C per workgroup.
-//   * Row j of a wave's MFMA tile g is row W j + g of its 32 W rows (W = WT for A, WN for B), so that one load per lane brings the
-//     scales of all its tiles for a K-step, packed as the instruction's byte selector takes them, and a lane ends up with 4 WN
-//     consecutive columns of C.  Rows lie in LDS in tile order: the load of a tile places them.
-//   * Two K-steps lie in LDS.  Each is computed in two halves of 64; behind the barrier in the middle of step t all of t is in
-//     registers or used up and the loads of t + 2 go where it lay, with one to one and a half K-steps to land.
-//   * An LDS row is 128 bytes, its 16-byte chunks XORed with (row >> 1) & 7: the 16 rows that a fragment read takes at a time cover
-//     all banks once.
+//   * Row j of a wave's MFMA tile g is row W j + g of its 32 W rows (W = WT for A, WN for B), so that the scales of all its tiles for a
+//     K-step are W consecutive bytes, as the instruction's byte selector takes them, and a lane ends up with 4 WN consecutive columns
+//     of C.  Rows lie in LDS in tile order: the load of a tile places them.
+//   * A K-step is two phases, one per half of 64 contraction elements: a phase is the MFMAs on the fragments in registers, and between
+//     them the fragment reads of the next phase and the loads of one operand two K-steps ahead.  In LDS the halves are blocks of
+//     their own: the block that a phase has read is free behind the barrier at its end, so eight blocks hold the two K-steps that the
+//     loads run ahead, every phase loads as much as the others, and every load has one phase to land at least.
+//   * The barrier stands in front of a phase's last MFMA, which runs while the waves meet.
+//   * A block's row is 64 bytes, its 16-byte chunks XORed with (row >> 2) & 3: the 16 rows that a fragment read takes at a time cover
+//     all banks once.  Both halves of a row's 128 bytes are requested one behind the other: one line fetched from the L2.
 template <int WT, int WN, int OUT>
 __global__ __launch_bounds__(NTHREADS, WT * WN <= 4 ? 2 : 1) void block_gemm_kernel(Args g) {
 #ifdef __HIP_DEVICE_COMPILE__   // (the host's pass over this file cannot place the registers that the assembly names)
   constexpr int BM = 64 * WT, BN = 64 * WN;
-  constexpr int NA = 2 * WT, NB = 2 * WN;                       // loads per wave of an operand's K-step
-  constexpr uint32_t SLOT = (BM + BN) * BK;                     // bytes of a K-step in LDS
-  constexpr int ROWB = 64 * WN;                                 // bytes of a staged row of a wave's output
+  constexpr int NA = 2 * WT, NB = 2 * WN;                       // loads per wave of an operand's K-step, both halves
+  constexpr uint32_t BLK = block_bytes(WT > WN ? WT : WN);
+  constexpr int SLOTS = WT * WN;                                // MFMAs of a phase
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave >> 1, wn = wave & 1;
   const uint32_t smem_b = lds_addr(smem);
-  const uint32_t stage = smem_b + 2 * SLOT + (uint32_t)wave * (32 * ROWB);
+  const uint32_t scales_b = smem_b + 8 * BLK;
+  const uint32_t stage = scales_b + 1024 + (uint32_t)wave * (32 * stage_row(WN));
   const int tiles_m = (g.m + BM - 1) / BM, tiles_n = (g.n + BN - 1) / BN;
   const int ntiles = tiles_m * tiles_n;
   const int total = ntiles * (OUT == kPartial ? g.splits : 1);
@@ -109,47 +136,45 @@ __global__ __launch_bounds__(NTHREADS, WT * WN <= 4 ? 2 : 1) void block_gemm_ker
   // ---- requests: a cursor over the K-steps of all items of this workgroup, two steps ahead of the computation ----
   int r_item = blockIdx.x;
   int r_left;
-  const uint8_t *ra, *rb, *rsa, *rsb;   // of the K-step to request next (wave-uniform)
-  uint32_t la[NA], lb[NB];
-  uint32_t lsa, lsb;
+  const uint8_t *ra, *rb, *rs;          // of the K-step to request next (wave-uniform); rs: the scales this wave loads
+  uint32_t la[WT], lb[WN], ls;
+  const int64_t rs_step = wn ? g.lsb : g.lsa;
   auto aim = [&](int v) {
     const Item it = select(v);
     r_left = it.nk;
     ra = g.a + (int64_t)it.m0 * g.lda + (int64_t)it.k0 * BK;
     rb = g.b + (int64_t)it.n0 * g.ldb + (int64_t)it.k0 * BK;
-    rsa = g.sa + (int64_t)it.k0 * g.lsa;
-    rsb = g.sb + (int64_t)it.k0 * g.lsb;
+    rs = (wn ? g.sb : g.sa) + (int64_t)it.k0 * rs_step;
     int l2 = lane;
     asm volatile("" : "+v"(l2));
-    // load i of a wave fills LDS rows 8 (wave + 4 i) .. + 7; beyond the matrix: its last row (never stored)
-    const int sub = l2 >> 3;
+    // load i of a wave fills block rows 16 (wave + 4 i) .. + 15; beyond the matrix: its last row (never stored)
+    const int sub = l2 >> 2;
+    const int chunk = ((l2 & 3) ^ ((sub >> 2) & 3)) << 4;
 #pragma unroll
-    for (int i = 0; i < NA; ++i) {
-      const int row = 8 * (wave + 4 * i) + sub;
+    for (int i = 0; i < WT; ++i) {
+      const int row = 16 * (wave + 4 * i) + sub;
       const int w = row / (32 * WT), t = row % (32 * WT) / 32, j = row % 32;
       int r = 32 * WT * w + WT * j + t;
       r = it.m0 + r < g.m ? r : g.m - 1 - it.m0;
-      la[i] = (uint32_t)r * (uint32_t)g.lda + (uint32_t)(((l2 & 7) ^ ((row >> 1) & 7)) << 4);
+      la[i] = (uint32_t)r * (uint32_t)g.lda + (uint32_t)chunk;
     }
 #pragma unroll
-    for (int i = 0; i < NB; ++i) {
-      const int row = 8 * (wave + 4 * i) + sub;
+    for (int i = 0; i < WN; ++i) {
+      const int row = 16 * (wave + 4 * i) + sub;
       const int w = row / (32 * WN), t = row % (32 * WN) / 32, j = row % 32;
       int r = 32 * WN * w + WN * j + t;
       r = it.n0 + r < g.n ? r : g.n - 1 - it.n0;
-      lb[i] = (uint32_t)r * (uint32_t)g.ldb + (uint32_t)(((l2 & 7) ^ ((row >> 1) & 7)) << 4);
+      lb[i] = (uint32_t)r * (uint32_t)g.ldb + (uint32_t)chunk;
     }
-    const int sra = it.m0 + 32 * WT * wm + WT * (l2 & 31), srb = it.n0 + 32 * WN * wn + WN * (l2 & 31);
-    lsa = (uint32_t)(sra < g.lsa - WT ? sra : g.lsa - WT);
-    lsb = (uint32_t)(srb < g.lsb - WN ? srb : g.lsb - WN);
+    const int sr = (wn ? it.n0 : it.m0) + 4 * l2, most = (int)rs_step - 4;
+    ls = (uint32_t)(sr < most ? sr : most);
   };
   // (behind the last item's last K-step it stays there: the K loop requests that one again rather than branch, two steps in all)
   auto advance = [&]() {
     if (--r_left > 0) {
       ra += BK;
       rb += BK;
-      rsa += g.lsa;
-      rsb += g.lsb;
+      rs += rs_step;
     } else if (r_item + (int)gridDim.x < total) {
       r_item += gridDim.x;
       aim(r_item);
@@ -157,14 +182,17 @@ __global__ __launch_bounds__(NTHREADS, WT * WN <= 4 ? 2 : 1) void block_gemm_ker
       r_left = 1;
     }
   };
-  auto request_a = [&](auto i_tag, uint32_t slot) {
-    constexpr int i = decltype(i_tag)::value;
-    dma_b128<i * 4096>(ra, la[i], slot + (uint32_t)wave * 1024u);
+  // load d of an operand's K-step: half d & 1 of the rows of load d / 2; to block k0 (half 0) or k1
+  auto request_a = [&](auto d, uint32_t k0, uint32_t k1) {
+    constexpr int i = decltype(d)::value;
+    dma_b128<(i >> 1) * 4096>(ra + 64 * (i & 1), la[i >> 1], (i & 1 ? k1 : k0) + (uint32_t)wave * 1024u);
   };
-  auto request_b = [&](auto i_tag, uint32_t slot) {
-    constexpr int i = decltype(i_tag)::value;
-    dma_b128<BM * BK + i * 4096>(rb, lb[i], slot + (uint32_t)wave * 1024u);
+  auto request_b = [&](auto d, uint32_t k0, uint32_t k1) {
+    constexpr int i = decltype(d)::value;
+    dma_b128<(i >> 1) * 4096>(rb + 64 * (i & 1), lb[i >> 1], (i & 1 ? k1 : k0) + (uint32_t)wave * 1024u);
   };
+  // a K-step's scales: waves 0 and 2 load A's 256 bytes, 1 and 3 B's (the same bytes to the same place)
+  auto request_scales = [&](uint32_t slot) { dma_b32(rs, ls, slot + (uint32_t)wn * 256u); };
 
   // The accumulators of the large tile are the wave's 256 accumulation registers (its MFMAs are inline assembly, to pin them there:
   // with the builtin the compiler moves and spills them); smaller tiles leave them to the compiler.
@@ -177,118 +205,107 @@ __global__ __launch_bounds__(NTHREADS, WT * WN <= 4 ? 2 : 1) void block_gemm_ker
 #pragma unroll
     for (int i = 0; i < WT; ++i)
 #pragma unroll
-      for (int j = 0; j < WN; ++j)
-{
+      for (int j = 0; j < WN; ++j) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
         if constexpr (PINNED) asm volatile("" : "+a"(acc[i][j]));
       }
   };
 
-  // fragment addresses: lane l takes row l % 32 of a tile, chunks 4 h + 2 (l / 32) and + 1 of half h
-  const uint32_t frag0 = (uint32_t)((lane & 31) * BK + (((2 * (lane >> 5)) ^ ((lane >> 1) & 7)) << 4));
-  const uint32_t fa0 = smem_b + (uint32_t)(wm * 32 * WT * BK) + frag0;
-  const uint32_t fb0 = smem_b + (uint32_t)((BM + wn * 32 * WN) * BK) + frag0;
-  auto lds16 = [&](uint32_t a) { return *(KR_LDS const i32x4*)a; };
-  auto frag = [&](uint32_t a, uint32_t b) {
-    const i32x4 lo = lds16(a), hi = lds16(b);
+  // fragment addresses: lane l takes row l % 32 of a tile, chunks 2 (l / 32) and + 1 of a half
+  const uint32_t frag0 = (uint32_t)((lane & 31) * 64 + (((2 * (lane >> 5)) ^ ((lane >> 2) & 3)) << 4));
+  const uint32_t fa = (uint32_t)(wm * 32 * WT * 64) + frag0, fb = (uint32_t)(wn * 32 * WN * 64) + frag0;
+  auto frag = [&](uint32_t a) {
+    const i32x4 lo = *(KR_LDS const i32x4*)a, hi = *(KR_LDS const i32x4*)(a ^ 16u);
     return i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
   };
+  const uint32_t sca = (uint32_t)(32 * WT * wm + WT * (lane & 31)), scb = 256u + (uint32_t)(32 * WN * wn + WN * (lane & 31));
 
-  // One half of a K-step: the MFMAs on `cur`, and between them the fragment reads of half h of the K-step in `slot` and the loads
-  // of one K-step into `dslot` (if DMA).
-  auto half = [&](Frags& cur, Frags& nxt, int sa, int sb, uint32_t slot, int h, auto dma_tag, uint32_t dslot) {
-    constexpr bool DMA = decltype(dma_tag)::value;
-    const uint32_t a0 = (fa0 ^ (uint32_t)(h << 6)) + slot, b0 = (fb0 ^ (uint32_t)(h << 6)) + slot;
-    const uint32_t a1 = a0 ^ 16u, b1 = b0 ^ 16u;
-    auto step = [&](auto gt, auto nt) {
-      constexpr int gi = decltype(gt)::value, ni = decltype(nt)::value;
+  // One phase: the MFMAs on `cur`, and between them the fragments of the next from blocks na / nb, `loads` (called with 0 ..
+  // NLOADS - 1) and, in front of the last MFMA, `meet`.
+  auto phase = [&](Frags& cur, Frags& nxt, int sa, int sb, uint32_t na, uint32_t nb, auto nloads_tag, auto loads, auto meet) {
+    constexpr int NLOADS = decltype(nloads_tag)::value;
+    const uint32_t a0 = fa + na, b0 = fb + nb;
+    auto fetch = [&](auto f) {   // fragments in the order that the next phase takes them
+      constexpr int i = decltype(f)::value;
+      if constexpr (i == 0) nxt.a[0] = frag(a0);
+      else if constexpr (i <= WN) nxt.b[i - 1] = frag(b0 + (i - 1) * 32 * 64);
+      else nxt.a[i - WN] = frag(a0 + (i - WN) * 32 * 64);
+    };
+    constexpr int NF = WT + WN;
+    constexpr int LAST = SLOTS >= 4 ? SLOTS - 1 : SLOTS;   // the MFMA that `meet` stands in front of
+    // fragment f is read behind MFMA f * (LAST - 2) / NF, load d behind MFMA d * (LAST - 1) / NLOADS
+    each([&](auto s) {
+      constexpr int slot = decltype(s)::value, gi = slot / WN, ni = slot % WN;
+      if constexpr (slot == LAST) meet();
       if constexpr (PINNED) {
-        if constexpr (gi == 0 && ni == 0) asm volatile("s_nop 3" ::: "memory");   // (the scales may just have been moved)
+        if constexpr (slot == 0) asm volatile("s_nop 3" ::: "memory");   // (the scales may just have been moved)
         asm volatile("v_mfma_scale_f32_32x32x64_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[%5,%6,0] op_sel_hi:[%7,%8,0]"
                      : "+a"(acc[gi][ni])
                      : "v"(cur.b[ni]), "v"(cur.a[gi]), "v"(sb), "v"(sa), "n"(ni & 1), "n"(gi & 1), "n"(ni >> 1), "n"(gi >> 1));
       } else {
         acc[gi][ni] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(cur.b[ni], cur.a[gi], acc[gi][ni], 0, 0, ni, sb, gi, sa);
       }
-      if constexpr (ni == 0) nxt.a[gi] = frag(a0 + gi * 32 * BK, a1 + gi * 32 * BK);
-      if constexpr (gi == 0) nxt.b[ni] = frag(b0 + ni * 32 * BK, b1 + ni * 32 * BK);
-      if constexpr (DMA) {
-        // the loads ride one behind each MFMA, operand A's first
-        constexpr int per = (NA + NB + WT * WN - 1) / (WT * WN), at = (gi * WN + ni) * per;
-#define KR_REQ(d)                                                                                          \
-  if constexpr (d < per) {                                                                                 \
-    if constexpr (at + d < NA) request_a(std::integral_constant<int, at + d>{}, dslot);                    \
-    else if constexpr (at + d < NA + NB) request_b(std::integral_constant<int, at + d - NA>{}, dslot);     \
-  }
-        KR_REQ(0) KR_REQ(1) KR_REQ(2) KR_REQ(3)
-#undef KR_REQ
-      }
+      each([&](auto f) {
+        constexpr int span = LAST - 2 > 1 ? LAST - 2 : 1;
+        if constexpr (decltype(f)::value * span / NF == slot) fetch(f);
+      }, std::make_integer_sequence<int, NF>{});
+      each([&](auto d) {
+        constexpr int span = LAST - 1 > 1 ? LAST - 1 : 1;
+        if constexpr (decltype(d)::value * span / NLOADS == slot) loads(d);
+      }, std::make_integer_sequence<int, NLOADS>{});
       __builtin_amdgcn_sched_barrier(0);
-    };
-    auto row = [&](auto gt) {
-      step(gt, std::integral_constant<int, 0>{});
-      if constexpr (WN > 1) step(gt, std::integral_constant<int, 1>{});
-      if constexpr (WN > 2) step(gt, std::integral_constant<int, 2>{});
-      if constexpr (WN > 3) step(gt, std::integral_constant<int, 3>{});
-    };
-    row(std::integral_constant<int, 0>{});
-    if constexpr (WT > 1) row(std::integral_constant<int, 1>{});
-    if constexpr (WT > 2) row(std::integral_constant<int, 2>{});
-    if constexpr (WT > 3) row(std::integral_constant<int, 3>{});
-  };
-  auto request_all = [&](uint32_t dslot) {
-    auto one = [&](auto i) {
-      if constexpr (decltype(i)::value < NA) request_a(i, dslot);
-    };
-    auto two = [&](auto i) {
-      if constexpr (decltype(i)::value < NB) request_b(i, dslot);
-    };
-#define KR_ALL(f)                                                                                          \
-  f(std::integral_constant<int, 0>{}); f(std::integral_constant<int, 1>{}); f(std::integral_constant<int, 2>{}); \
-  f(std::integral_constant<int, 3>{}); f(std::integral_constant<int, 4>{}); f(std::integral_constant<int, 5>{}); \
-  f(std::integral_constant<int, 6>{}); f(std::integral_constant<int, 7>{});
-    KR_ALL(one)
-    KR_ALL(two)
-#undef KR_ALL
+    }, std::make_integer_sequence<int, SLOTS>{});
+    if constexpr (LAST == SLOTS) meet();
   };
 
   // ---- start: K-steps 0 and 1 requested, half 0 of step 0 read ----
+  struct Blocks {
+    uint32_t a0, a1, b0, b1, sc;
+  };
+  Blocks now = {smem_b, smem_b + BLK, smem_b + 2 * BLK, smem_b + 3 * BLK, scales_b};
+  Blocks next = {smem_b + 4 * BLK, smem_b + 5 * BLK, smem_b + 6 * BLK, smem_b + 7 * BLK, scales_b + 512};
+  auto request_step = [&](const Blocks& to) {
+    each([&](auto d) { request_a(d, to.a0, to.a1); }, std::make_integer_sequence<int, NA>{});
+    request_scales(to.sc);
+    each([&](auto d) { request_b(d, to.b0, to.b1); }, std::make_integer_sequence<int, NB>{});
+    advance();
+  };
   Item it = select(blockIdx.x);
   int item = blockIdx.x;
   aim(r_item);
-  int sa = load_scales<WT>(rsa + lsa), sb = load_scales<WN>(rsb + lsb);
-  request_all(0 + smem_b);
-  advance();
-  int sa1 = load_scales<WT>(rsa + lsa), sb1 = load_scales<WN>(rsb + lsb);
-  request_all(SLOT + smem_b);
-  advance();
+  request_step(now);
+  request_step(next);
   clear();
   __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0)
   kr_barrier();
-  {
-    const uint32_t a0 = fa0, b0 = fb0;
 #pragma unroll
-    for (int i = 0; i < WT; ++i) X.a[i] = frag(a0 + i * 32 * BK, (a0 ^ 16u) + i * 32 * BK);
+  for (int i = 0; i < WT; ++i) X.a[i] = frag(fa + now.a0 + i * 32 * 64);
 #pragma unroll
-    for (int i = 0; i < WN; ++i) X.b[i] = frag(b0 + i * 32 * BK, (b0 ^ 16u) + i * 32 * BK);
-  }
-  uint32_t slot = 0;   // of the current K-step, 0 or SLOT
+  for (int i = 0; i < WN; ++i) X.b[i] = frag(fb + now.b0 + i * 32 * 64);
+  int sa = lds_scales<WT>(now.sc + sca), sb = lds_scales<WN>(now.sc + scb);
+  kr_barrier();                         // (every wave has read what the first phase's loads overwrite)
   for (;;) {
     for (int t = 0; t < it.nk; ++t) {
-      half(X, Y, sa, sb, slot, 1, std::false_type{}, 0u);
-      __builtin_amdgcn_s_waitcnt(0x0f70);
-      kr_barrier();
-      const uint32_t other = SLOT - slot;
-      const int sa2 = load_scales<WT>(rsa + lsa), sb2 = load_scales<WN>(rsb + lsb);
-      // (behind the last K-step it reads what is not there: unused)
-      half(Y, X, sa, sb, other, 0, std::true_type{}, slot + smem_b);
+      // half 0: half 1 of this step is read; A two steps ahead goes where both operands' half 0 lay
+      phase(X, Y, sa, sb, now.a1, now.b1, Int<NA + 1>{},
+            [&](auto d) {
+              if constexpr (decltype(d)::value < NA) request_a(d, now.a0, now.b0);
+              else request_scales(now.sc);
+            },
+            [&]() {
+              __builtin_amdgcn_s_waitcnt(vm_wait(NA + 1));   // the next step has landed
+              kr_barrier();
+            });
+      // half 1: half 0 of the next step and its scales are read; B two steps ahead goes where this step's half 1 lay
+      const int sa1 = lds_scales<WT>(next.sc + sca), sb1 = lds_scales<WN>(next.sc + scb);
+      phase(Y, X, sa, sb, next.a0, next.b0, Int<NB>{}, [&](auto d) { request_b(d, now.a1, now.b1); }, [&]() { kr_barrier(); });
       advance();
       sa = sa1;
       sb = sb1;
-      sa1 = sa2;
-      sb1 = sb2;
-      slot = other;
+      const Blocks ahead = {now.a0, now.b0, now.a1, now.b1, now.sc};
+      now = next;
+      next = ahead;
     }
 
     // the compiler does not know the latency of MFMAs in assembly: let the last ones finish before their results are read
@@ -327,57 +344,56 @@ __global__ __launch_bounds__(NTHREADS, WT * WN <= 4 ? 2 : 1) void block_gemm_ker
             }
           }
         } else {
-          bf16 vals[4][4 * WN];
+          // rows of the block through LDS (64 or 128 bytes of each at a time), then whole pieces of rows to memory
+          constexpr int SW = stage_row(WN), PASSES = 64 * WN / SW, QP = 4 / PASSES, PIECES = SW / 16, RPP = 64 / PIECES;
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int col = n_wave + WN * (8 * q + 4 * hi);
+          for (int h = 0; h < PASSES; ++h) {
+            __builtin_amdgcn_wave_barrier();
 #pragma unroll
-            for (int c = 0; c < 4 * WN; ++c) {
-              float v = val[c % WN][4 * q + c / WN];
+            for (int ql = 0; ql < QP; ++ql) {
+              const int q = h * QP + ql;
+              const int col = n_wave + WN * (8 * q + 4 * hi);
+              float v[4 * WN];
+#pragma unroll
+              for (int c = 0; c < 4 * WN; ++c) v[c] = val[c % WN][4 * q + c / WN];
               if constexpr (OUT == kAccumulate) {
-                const bool in = row < g.m && col + (c & ~3) < g.n;
-                const bf16x4 old = in ? *reinterpret_cast<const bf16x4*>(g.c + (int64_t)row * g.ldc + col + (c & ~3)) : bf16x4{};
-                v += (float)old[c & 3];
+#pragma unroll
+                for (int c4 = 0; c4 < WN; ++c4) {
+                  const bool in = row < g.m && col + 4 * c4 < g.n;
+                  const bf16x4 old = in ? *reinterpret_cast<const bf16x4*>(g.c + (int64_t)row * g.ldc + col + 4 * c4) : bf16x4{};
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) v[4 * c4 + e] += (float)old[e];
+                }
               }
-              vals[q][c] = (bf16)v;
-            }
-          }
-          // rows of the block through LDS, then whole rows to memory
-          constexpr int PIECES = ROWB / 16 > 0 ? ROWB / 16 : 1;
-          __builtin_amdgcn_wave_barrier();
-          if constexpr (WN == 1) {
+              if constexpr (WN == 1) {
+                const bf16x4 o = {(bf16)v[0], (bf16)v[1], (bf16)v[2], (bf16)v[3]};
+                *(KR_LDS bf16x4*)(stage + j * SW + ((q ^ ((j >> 2) & 3)) << 4) + 8 * hi) = o;
+              } else {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const bf16x4 o = {vals[q][0], vals[q][1], vals[q][2], vals[q][3]};
-              *(KR_LDS bf16x4*)(stage + j * ROWB + ((q ^ ((j >> 2) & 3)) << 4) + 8 * hi) = o;
-            }
-          } else {
+                for (int w = 0; w < WN / 2; ++w) {
+                  bf16x8 o;
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-#pragma unroll
-              for (int v = 0; v < WN / 2; ++v) {
-                bf16x8 o;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) o[e] = vals[q][8 * v + e];
-                const int piece = WN / 2 * (2 * q + hi) + v;
-                const int x = WN == 4 ? j & 15 : (j >> 1) & 7;
-                *(KR_LDS bf16x8*)(stage + j * ROWB + ((piece ^ x) << 4)) = o;
+                  for (int e = 0; e < 8; ++e) o[e] = (bf16)v[8 * w + e];
+                  const int piece = WN / 2 * (2 * ql + hi) + w;
+                  *(KR_LDS bf16x8*)(stage + j * SW + ((piece ^ (SW == 128 ? (j >> 1) & 7 : (j >> 2) & 3)) << 4)) = o;
+                }
               }
-          }
-          __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
-          __builtin_amdgcn_wave_barrier();
-          __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
-          const int piece = le % PIECES, r0 = le / PIECES;
-          constexpr int RPP = 64 / PIECES;
+            }
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+            const int piece = le % PIECES, r0 = le / PIECES;
+            const int col = n_wave + h * (SW / 2) + 8 * piece;
 #pragma unroll
-          for (int p = 0; p < 32 / RPP; ++p) {
-            const int jj = p * RPP + r0;
-            const int x = WN == 4 ? jj & 15 : WN == 2 ? (jj >> 1) & 7 : (jj >> 2) & 3;
-            const bf16x8 v = *(KR_LDS const bf16x8*)(stage + jj * ROWB + ((piece ^ x) << 4));
-            const int rr = m_wave + WT * jj + gi;
-            if (rr < g.m && n_wave + 8 * piece < g.n) stg8_stream(g.c + (int64_t)rr * g.ldc + n_wave + 8 * piece, v);
+            for (int p = 0; p < 32 / RPP; ++p) {
+              const int jj = p * RPP + r0;
+              const bf16x8 v = *(KR_LDS const bf16x8*)(stage + jj * SW + ((piece ^ (SW == 128 ? (jj >> 1) & 7 : (jj >> 2) & 3)) << 4));
+              const int rr = m_wave + WT * jj + gi;
+              if (rr < g.m && col < g.n) stg8_stream(g.c + (int64_t)rr * g.ldc + col, v);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+            __builtin_amdgcn_wave_barrier();
           }
-          __builtin_amdgcn_wave_barrier();
         }
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -444,7 +460,7 @@ int device_cus() {
 
 template <int W, int OUT>
 int launch(const Args& g, int cus, hipStream_t stream) {
-  constexpr size_t lds = 2 * (128 * W) * BK + 4 * 32 * 64 * W;
+  constexpr size_t lds = lds_bytes(W, W);
   static const hipError_t raised = hipFuncSetAttribute((const void*)block_gemm_kernel<W, W, OUT>,
                                                        hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
   if (raised != hipSuccess) return KR_ELAUNCH;
