@@ -461,6 +461,11 @@ class HipBackend:
         """A bf16 matrix [rows, cols] (or a [s, r, cols] nanobatch slice whose rows come in runs, read in place) in 8-bit blocks:
         e4m3 with a power-of-two scale per 128 elements along the columns (``by_row``) and / or the rows (``by_col``), from one
         read.  ``tiles``: one scale per 128 x 128 tile, so that both orientations hold the same values."""
+        done = self._n.quantize_blocks(x, by_row, by_col, tiles)
+        if done is not None:
+            q, s, qt, st = done
+            return BlockScaled(None if q is None else BlockOperand(q, s, x.shape[-1]),
+                               None if qt is None else BlockOperand(qt, st, x.numel() // x.shape[-1]))
         self._dev(x)
         self._bf16(x)
         if not (by_row or by_col):
@@ -510,6 +515,14 @@ class HipBackend:
         """``a . b^T`` of two operands in 8-bit blocks over the same contraction, [a.rows, b.rows] in bf16 with fp32 sums:
         ``y = x . W^T`` from ``(x.by_row, W.by_row)``, ``dx = dy . W`` from ``(dy.by_row, W.by_col)``, ``dW = dy^T . x`` from
         ``(dy.by_col, x.by_col)``.  ``accumulate``: added to ``out``, rounded once."""
+        max_cus = 0
+        reserved = reserved_compute_units()
+        if reserved and a.data.is_cuda:
+            max_cus = max(self._num_cus(a.data.device) - reserved, 8)
+        if a.length == b.length and dtype == torch.bfloat16:
+            done = self._n.block_matmul(a.data, a.scales, b.data, b.scales, a.length, out, accumulate, max_cus)
+            if done is not None:
+                return done
         self._block_operand(a)
         self._block_operand(b)
         if dtype != torch.bfloat16:
@@ -531,10 +544,6 @@ class HipBackend:
             return out
         if not k:
             return out if accumulate else out.zero_()
-        max_cus = 0
-        reserved = reserved_compute_units()
-        if reserved:
-            max_cus = max(self._num_cus(a.data.device) - reserved, 8)
         with self._current(out):
             nbytes = self.lib.kr_block_gemm_workspace_bytes(m, n, k, max_cus)
             ws = torch.empty(nbytes, dtype=torch.uint8, device=out.device) if nbytes else None
@@ -885,6 +894,10 @@ class HipBackend:
     # -- embedding and loss ---------------------------------------------------------------
     def embedding_fwd(self, ids: Tensor, weight: Tensor, vocab_start: int = 0, scale: float = 1.0) -> Tensor:
         """ids [b, s] int64 -> ``scale *`` rows of the weight, [s, b, hidden]; ids outside this shard's rows give zeros."""
+        if scale != 1.0:
+            done = self._n.embedding_fwd_scaled(ids, weight, vocab_start, scale)
+            if done is not None:
+                return done
         self._dev(weight)
         self._on_device(ids)
         self._bf16(weight)
@@ -926,6 +939,9 @@ class HipBackend:
         """The gradient of :meth:`embedding_fwd` with respect to the weight, ``[vocab_rows, hidden]``, by sorted tokens: sums in
         fp32 in an order that the ids fix.  ``out`` (dense bf16 or fp32; by default a new bf16 tensor) is written whole, or with
         ``accumulate`` has the gradient added to it (rounded once), where rows without a token are left alone."""
+        done = self._n.embedding_bwd_sorted(ids, dout, vocab_rows, vocab_start, scale, out, accumulate)
+        if done is not None:
+            return done
         self._dev(dout)
         self._on_device(ids)
         self._bf16(dout)

@@ -8,6 +8,7 @@
 #include "kr_common.h"
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 #include <utility>
 
@@ -72,6 +73,7 @@ __device__ __forceinline__ void tile_of(int pid, int nblocks, int tiles_m, int t
 template <int W>
 __device__ __forceinline__ int lds_scales(uint32_t a) {
   if constexpr (W == 4) return *(KR_LDS const int*)a;
+  if constexpr (W == 3) return *(KR_LDS const uint8_t*)a | *(KR_LDS const uint8_t*)(a + 1) << 8 | *(KR_LDS const uint8_t*)(a + 2) << 16;
   if constexpr (W == 2) return *(KR_LDS const uint16_t*)a;
   return *(KR_LDS const uint8_t*)a;
 }
@@ -101,7 +103,7 @@ constexpr size_t lds_bytes(int wt, int wn) {
 //   * A block's row is 64 bytes, its 16-byte chunks XORed with (row >> 2) & 3: the 16 rows that a fragment read takes at a time cover
 //     all banks once.  Both halves of a row's 128 bytes are requested one behind the other: one line fetched from the L2.
 template <int WT, int WN, int OUT>
-__global__ __launch_bounds__(NTHREADS, WT * WN <= 4 ? 2 : 1) void block_gemm_kernel(Args g) {
+__global__ __launch_bounds__(NTHREADS, WT * WN == 1 ? 3 : WT * WN == 4 ? 2 : 1) void block_gemm_kernel(Args g) {
 #ifdef __HIP_DEVICE_COMPILE__   // (the host's pass over this file cannot place the registers that the assembly names)
   constexpr int BM = 64 * WT, BN = 64 * WN;
   constexpr int NA = 2 * WT, NB = 2 * WN;                       // loads per wave of an operand's K-step, both halves
@@ -407,6 +409,78 @@ __global__ __launch_bounds__(NTHREADS, WT * WN <= 4 ? 2 : 1) void block_gemm_ker
 #endif
 }
 
+// Few rows (up to 16 MT of A): bound by the bytes of B, which stream from memory into registers.  A workgroup owns 16 rows of B; its
+// eight waves take every eighth K-step each, FEW_AHEAD of them requested at a time, and their sums meet in LDS in wave order.
+constexpr int FEW_WAVES = 8, FEW_AHEAD = 4;
+template <int MT, bool ACCUMULATE>
+__global__ __launch_bounds__(64 * FEW_WAVES) void block_gemm_few_rows_kernel(Args g) {
+  __shared__ float sums[FEW_WAVES][MT * 256];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int n0 = blockIdx.x * 16, r16 = lane & 15, k32 = (lane >> 4) * 32;
+  const int nrow = n0 + r16 < g.n ? n0 + r16 : g.n - 1;
+  const uint8_t* const b = g.b + (int64_t)nrow * g.ldb + k32;
+  const uint8_t* a[MT];
+  int mrow[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    mrow[i] = 16 * i + r16 < g.m ? 16 * i + r16 : g.m - 1;
+    a[i] = g.a + (int64_t)mrow[i] * g.lda + k32;
+  }
+  f32x4 acc[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  auto load = [](const uint8_t* p) {
+    const i32x4 lo = *reinterpret_cast<const i32x4*>(p), hi = *reinterpret_cast<const i32x4*>(p + 16);
+    return i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+  };
+  auto steps = [&](int t0, auto count) {
+    constexpr int U = decltype(count)::value;
+    i32x8 fb[U], fa[U][MT];
+    int sb[U], sa[U][MT];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t t = t0 + u * FEW_WAVES;
+      fb[u] = load(b + t * BK);
+      sb[u] = g.sb[t * g.lsb + nrow];
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        fa[u][i] = load(a[i] + t * BK);
+        sa[u][i] = g.sa[t * g.lsa + mrow[i]];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+        acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[u], fa[u][i], acc[i], 0, 0, 0, sb[u], 0, sa[u][i]);
+  };
+  int t = wave;
+  for (; t + (FEW_AHEAD - 1) * FEW_WAVES < g.ksteps; t += FEW_AHEAD * FEW_WAVES) steps(t, Int<FEW_AHEAD>{});
+  for (; t < g.ksteps; t += FEW_WAVES) steps(t, Int<1>{});
+  // lane l: row l % 16 of A's tile, columns 4 (l / 16) .. + 3
+#pragma unroll
+  for (int i = 0; i < MT; ++i) *reinterpret_cast<f32x4*>(&sums[wave][i * 256 + r16 * 16 + (lane >> 4) * 4]) = acc[i];
+  kr_barrier();
+  for (int i = threadIdx.x; i < MT * 64; i += 64 * FEW_WAVES) {   // four columns each
+    const int row = i / 4, col = n0 + (i & 3) * 4;
+    if (row >= g.m || col >= g.n) continue;
+    f32x4 v = *reinterpret_cast<const f32x4*>(&sums[0][i * 4]);
+#pragma unroll
+    for (int w = 1; w < FEW_WAVES; ++w) {
+      const f32x4 o = *reinterpret_cast<const f32x4*>(&sums[w][i * 4]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] += o[e];
+    }
+    bf16* const c = g.c + (int64_t)row * g.ldc + col;
+    if constexpr (ACCUMULATE) {
+      const bf16x4 old = *reinterpret_cast<const bf16x4*>(c);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] += (float)old[e];
+    }
+    *reinterpret_cast<bf16x4*>(c) = bf16x4{(bf16)v[0], (bf16)v[1], (bf16)v[2], (bf16)v[3]};
+  }
+}
+
 // C = bf16(sum of the cuts' fp32 partial products, in order [+ C])
 __global__ __launch_bounds__(256) void block_gemm_reduce_kernel(const float* __restrict__ partial, bf16* __restrict__ C,
                                                                 int64_t ldc, int M, int N, int splits, int accumulate) {
@@ -438,18 +512,75 @@ __global__ __launch_bounds__(256) void block_gemm_reduce_kernel(const float* __r
   stg8(dst, o);
 }
 
+// The tiles, and what a launch of them takes in us as measured (256 compute units): per round of workgroups, and per K-step, for each
+// round and for each tile of a unit's share, but no less than `step_min` (a unit with one tile waits for its loads).
+// us, model and measured: 16384 x 7168 x 4096, 256 x 256 346, 349; 192 x 256 409, 408; 256 x 128 409, 412; 128 x 128 499, 489; 64 x
+// 64 824, 790.  6023 x 4096 x 3584: 90, 83; 74, 75; 81, 81; 97, 92; 167, 151.  1536 x 4096 x 6023: 74, 57; 60, 46; 43, 41; 57, 46; 55,
+// 68.  512 x 4096 x 4096: 52, 40; 43, 32; 31, 25; 25, 24; 18, 18.  1024 x 1024 x 1024: 18, 15; 17, 13; 13, 10; 9, 8; 6, 5.
+struct Tile {
+  int wt, wn;       // MFMA tiles per wave: 64 wt x 64 wn of C per workgroup
+  int per_cu;       // workgroups that a compute unit holds
+  float round, step_round, step_tile, step_min;
+};
+constexpr Tile kTiles[] = {{4, 4, 1, 5.4f, 0.f, 1.38f, 1.38f}, {3, 4, 1, 5.3f, 0.f, 1.1f, 1.1f},   {4, 2, 1, 3.5f, 0.f, 0.8f, 0.8f},
+                           {2, 4, 1, 3.5f, 0.f, 0.79f, 0.79f}, {2, 2, 2, 1.5f, 0.1f, 0.5f, 0.66f}, {1, 1, 3, 0.5f, 0.1f, 0.19f, 0.38f}};
+constexpr int kNumTiles = 6, kFewRows = kNumTiles;   // behind the tiles: block_gemm_few_rows_kernel
+constexpr int kFewRowsMost = 64, kMostSplits = 16;
+constexpr float kLaunch = 2.f, kCutLaunch = 3.6f;
+
 struct Plan {
-  int w, splits, steps_per;   // w: tiles per wave along both sides (4: 256 x 256, 2: 128 x 128, 1: 64 x 64)
+  int tile, splits, steps_per;
 };
 
-Plan choose_plan(int M, int N, int K, int cus) {
+#ifdef FORCE
+static int force_tile = -1, force_splits = 0;
+extern "C" void force(int t, int s) { force_tile = t; force_splits = s; }
+#endif
+
+size_t partial_bytes(int splits, int M, int N) { return splits > 1 ? (size_t)splits * M * N * sizeof(float) : 0; }
+
+// The plan of the least time by the figures above, with at most `most_bytes` of workspace.
+//   * A contraction is cut (partial tiles written and read again at 5 TB/s, and a second launch) only while all pieces fit into one
+//     round: 1536 x 2048 x 32768 whole 159 us, in four pieces 100; 64 x 4096 x 4096 12 and 10; 1024 x 1024 x 1024 5 and 11.
+//   * Few rows: a workgroup reads 16 rows of B and all of A, 33.6 GB/s per unit (us, 16 x 4096 x 4096 5.9 where tiles take 8.3, 64 x 4096
+//     x 4096 11.8 and 10.0, 1 x 28672 x 4096 24.9 and 18.7).
+Plan choose_plan(int M, int N, int K, int cus, size_t most_bytes) {
   const int ksteps = (K + BK - 1) / BK;
-  Plan p{4, 1, ksteps};
-  auto tiles = [&](int w) { return (int64_t)((M + 64 * w - 1) / (64 * w)) * ((N + 64 * w - 1) / (64 * w)); };
-  if (tiles(4) < cus) p.w = 2;
-  if (tiles(2) < cus) p.w = 1;
-  return p;
+#ifdef FORCE
+  if (force_tile >= 0) {
+    Plan p{force_tile, force_splits, (ksteps + force_splits - 1) / force_splits};
+    p.splits = (ksteps + p.steps_per - 1) / p.steps_per;
+    return p;
+  }
+#endif
+  Plan best{0, 1, ksteps};
+  float least = INFINITY;
+  for (int t = 0; t < kNumTiles; ++t) {
+    const Tile& tile = kTiles[t];
+    const int64_t tiles = (int64_t)((M + 64 * tile.wt - 1) / (64 * tile.wt)) * ((N + 64 * tile.wn - 1) / (64 * tile.wn));
+    int last = 0;
+    for (int want = 1; want <= kMostSplits && want <= ksteps; ++want) {
+      const int per = (ksteps + want - 1) / want, splits = (ksteps + per - 1) / per;
+      if (splits == last) continue;
+      last = splits;
+      if (splits > 1 && (tiles * splits > (int64_t)cus * tile.per_cu || partial_bytes(splits, M, N) > most_bytes)) break;
+      const float share = (float)((tiles * splits + cus - 1) / cus), rounds = std::ceil(share / tile.per_cu);
+      float us = kLaunch + rounds * tile.round + per * std::max(tile.step_min, rounds * tile.step_round + share * tile.step_tile);
+      if (splits > 1) us += kCutLaunch + (2.f * splits + 0.5f) * M * N * 4.f / 5e6f;
+      if (us < least) {
+        least = us;
+        best = Plan{t, splits, per};
+      }
+    }
+  }
+  if (M <= kFewRowsMost) {
+    const float groups = std::max(1.f, (float)((N + 15) / 16) / cus), rows = 16.f + (M == 1 ? 1.f : 16.f * ((M + 15) / 16));
+    const float us = 1.5f + std::max(groups * K * rows / 33.6e3f, (float)N * K / 5.5e6f);
+    if (us < least) best = Plan{kFewRows, 1, ksteps};
+  }
+  return best;
 }
+constexpr size_t kMostWorkspace = (size_t)1 << 30;
 
 int device_cus() {
   int dev = 0, n = 0;
@@ -458,24 +589,45 @@ int device_cus() {
   return n;
 }
 
-template <int W, int OUT>
+template <int T, int OUT>
 int launch(const Args& g, int cus, hipStream_t stream) {
-  constexpr size_t lds = lds_bytes(W, W);
-  static const hipError_t raised = hipFuncSetAttribute((const void*)block_gemm_kernel<W, W, OUT>,
+  constexpr Tile t = kTiles[T];
+  constexpr size_t lds = lds_bytes(t.wt, t.wn);
+  static_assert(lds * t.per_cu <= 160 * 1024, "LDS of a compute unit");
+  static const hipError_t raised = hipFuncSetAttribute((const void*)block_gemm_kernel<t.wt, t.wn, OUT>,
                                                        hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
   if (raised != hipSuccess) return KR_ELAUNCH;
-  const int64_t tiles = (int64_t)((g.m + 64 * W - 1) / (64 * W)) * ((g.n + 64 * W - 1) / (64 * W)) * g.splits;
+  const int64_t tiles = (int64_t)((g.m + 64 * t.wt - 1) / (64 * t.wt)) * ((g.n + 64 * t.wn - 1) / (64 * t.wn)) * g.splits;
   if (tiles > 0x3fffffff) return KR_EUNSUPPORTED;
-  const int64_t grid = std::min<int64_t>(tiles, (int64_t)cus * (W <= 2 ? 2 : 1));
-  hipLaunchKernelGGL((block_gemm_kernel<W, W, OUT>), dim3((unsigned)grid), dim3(NTHREADS), lds, stream, g);
+  const int64_t grid = std::min<int64_t>(tiles, (int64_t)cus * t.per_cu);
+  hipLaunchKernelGGL((block_gemm_kernel<t.wt, t.wn, OUT>), dim3((unsigned)grid), dim3(NTHREADS), lds, stream, g);
   return kr_launch_status();
 }
 
+template <int MT>
+int launch_few(const Args& g, int accumulate, hipStream_t stream) {
+  const dim3 grid((unsigned)((g.n + 15) / 16)), block(64 * FEW_WAVES);
+  if (accumulate) hipLaunchKernelGGL((block_gemm_few_rows_kernel<MT, true>), grid, block, 0, stream, g);
+  else hipLaunchKernelGGL((block_gemm_few_rows_kernel<MT, false>), grid, block, 0, stream, g);
+  return kr_launch_status();
+}
+int launch_few_rows(const Args& g, int accumulate, hipStream_t stream) {
+  if (g.m <= 16) return launch_few<1>(g, accumulate, stream);
+  if (g.m <= 32) return launch_few<2>(g, accumulate, stream);
+  return launch_few<4>(g, accumulate, stream);
+}
+
 template <int OUT>
-int launch_w(const Plan& p, const Args& g, int cus, hipStream_t stream) {
-  if (p.w == 4) return launch<4, OUT>(g, cus, stream);
-  if (p.w == 2) return launch<2, OUT>(g, cus, stream);
-  return launch<1, OUT>(g, cus, stream);
+int launch_tile(const Plan& p, const Args& g, int cus, hipStream_t stream) {
+  switch (p.tile) {
+    case 0: return launch<0, OUT>(g, cus, stream);
+    case 1: return launch<1, OUT>(g, cus, stream);
+    case 2: return launch<2, OUT>(g, cus, stream);
+    case 3: return launch<3, OUT>(g, cus, stream);
+    case 4: return launch<4, OUT>(g, cus, stream);
+    case 5: return launch<5, OUT>(g, cus, stream);
+  }
+  return KR_EUNSUPPORTED;
 }
 
 }  // namespace
@@ -483,8 +635,7 @@ int launch_w(const Plan& p, const Args& g, int cus, hipStream_t stream) {
 extern "C" size_t kr_block_gemm_workspace_bytes(int M, int N, int K, int max_cus) {
   if (M <= 0 || N <= 0 || K <= 0) return 0;
   const int all = device_cus();
-  const Plan p = choose_plan(M, N, K, max_cus > 0 && max_cus < all ? max_cus : all);
-  return p.splits > 1 ? (size_t)p.splits * M * N * sizeof(float) : 0;
+  return partial_bytes(choose_plan(M, N, K, max_cus > 0 && max_cus < all ? max_cus : all, kMostWorkspace).splits, M, N);
 }
 
 extern "C" int kr_block_gemm(int M, int N, int K, const void* A, int64_t lda, const void* sa, int64_t lsa, const void* B,
@@ -502,12 +653,12 @@ extern "C" int kr_block_gemm(int M, int N, int K, const void* A, int64_t lda, co
     return KR_EUNSUPPORTED;
   const int all = device_cus();
   const int cus = max_cus > 0 && max_cus < all ? max_cus : all;
-  Plan p = choose_plan(M, N, K, cus);
-  if (p.splits > 1 && (!workspace || workspace_bytes < (size_t)p.splits * M * N * sizeof(float))) p = Plan{p.w, 1, (K + BK - 1) / BK};
+  const Plan p = choose_plan(M, N, K, cus, workspace ? std::min(workspace_bytes, kMostWorkspace) : 0);
   Args g{(const uint8_t*)A, (const uint8_t*)sa, (const uint8_t*)B, (const uint8_t*)sb, (bf16*)C, (float*)workspace,
          lda, ldb, ldc, (int)lsa, (int)lsb, M, N, (K + BK - 1) / BK, p.steps_per, p.splits};
+  if (p.tile == kFewRows) return launch_few_rows(g, accumulate, (hipStream_t)stream);
   if (p.splits > 1) {
-    const int rc = launch_w<kPartial>(p, g, cus, (hipStream_t)stream);
+    const int rc = launch_tile<kPartial>(p, g, cus, (hipStream_t)stream);
     if (rc != KR_OK) return rc;
     const int64_t threads = (int64_t)M * (N / 8);
     if ((threads + 255) / 256 > 0x7fffffff) return KR_EUNSUPPORTED;
@@ -515,5 +666,5 @@ extern "C" int kr_block_gemm(int M, int N, int K, const void* A, int64_t lda, co
                        (const float*)workspace, (bf16*)C, ldc, M, N, p.splits, accumulate);
     return kr_launch_status();
   }
-  return accumulate ? launch_w<kAccumulate>(p, g, cus, (hipStream_t)stream) : launch_w<kStore>(p, g, cus, (hipStream_t)stream);
+  return accumulate ? launch_tile<kAccumulate>(p, g, cus, (hipStream_t)stream) : launch_tile<kStore>(p, g, cus, (hipStream_t)stream);
 }

@@ -15,6 +15,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/ATen.h>
+#include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 
 #include <algorithm>
@@ -1108,6 +1109,166 @@ PyObject* py_attn_chain_bwd(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   });
 }
 
+// ---- 8-bit blocks, sorted embedding gradient ----------------------------------------------------------------
+bool on_current_device(const Tensor& t) { return t.is_cuda() && t.device().index() == c10::hip::current_device(); }
+bool aligned16(const Tensor& t) { return ((uintptr_t)t.data_ptr() & 15) == 0; }
+int64_t blocks_of(int64_t n) { return (n + 127) / 128; }
+
+// quantize_blocks(x, by_row, by_col, tiles) -> (data, scales, data, scales), None for an orientation that was not asked for
+PyObject* py_quantize_blocks(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  return guarded([&]() -> PyObject* {
+    if (n_args != 4 || !bf16_arg(a[0])) return none();
+    const Tensor& x = tensor(a[0]);
+    if (symbolic(x) || !on_current_device(x) || !aligned16(x)) return none();
+    const Operand o = operand(x, 1 << 20);
+    const bool want[2] = {truth(a[1]), truth(a[2])};
+    const int tiles = truth(a[3]);
+    if (!o.ok || o.cols % 8 || !fits_int(o.rows) || !fits_int(o.cols) || (!want[0] && !want[1])) return none();
+    Tensor t[4];
+    int rc;
+    {
+      WithoutInterpreter free;
+      for (int i = 0; i < 2; ++i) {
+        if (!want[i]) continue;
+        const int64_t n = i ? o.cols : o.rows, k = i ? o.rows : o.cols;
+        t[2 * i] = at::empty({n, blocks_of(k) * 128}, x.options().dtype(at::kFloat8_e4m3fn));
+        t[2 * i + 1] = at::empty({blocks_of(k), (n + 3) / 4 * 4}, x.options().dtype(at::kByte));
+      }
+      auto at_ = [&](int i) { return t[i].defined() ? ptr(t[i]) : nullptr; };
+      auto ld = [&](int i) { return t[i].defined() ? t[i].size(1) : (int64_t)0; };
+      rc = kr_block_quantize(ptr(x), (int)o.rows, (int)o.cols, o.ld, o.run_rows, o.run_ld, tiles, at_(0), ld(0), at_(1), ld(1),
+                             at_(2), ld(2), at_(3), ld(3), stream());
+    }
+    if (rc != KR_OK)
+      return failed("kr_block_quantize(rows=" + std::to_string(o.rows) + ", cols=" + std::to_string(o.cols) + ")", rc);
+    PyObject* out = PyTuple_New(4);
+    if (out == nullptr) return nullptr;
+    for (int i = 0; i < 4; ++i) PyTuple_SET_ITEM(out, i, t[i].defined() ? wrap(std::move(t[i])) : Py_NewRef(Py_None));
+    return out;
+  });
+}
+
+// an operand of a block product: rows of `k` contraction elements, contiguous, in whole blocks
+struct BlockRows {
+  int64_t rows = 0, ld = 0, lds = 0;
+  bool ok = false;
+};
+BlockRows block_rows(PyObject* data, PyObject* scales, int64_t k) {
+  BlockRows r;
+  if (!is_tensor(data) || !is_tensor(scales)) return r;
+  const Tensor &d = tensor(data), &s = tensor(scales);
+  if (symbolic(d) || symbolic(s) || !on_current_device(d) || !on_current_device(s)) return r;
+  if (d.scalar_type() != at::kFloat8_e4m3fn || s.scalar_type() != at::kByte || d.dim() != 2 || s.dim() != 2) return r;
+  if (k <= 0 || d.numel() == 0 || d.stride(1) != 1 || d.size(1) < blocks_of(k) * 128 || s.numel() == 0 || s.stride(1) != 1 ||
+      s.size(0) < blocks_of(k) || s.size(1) < d.size(0))
+    return r;
+  r.rows = d.size(0);
+  r.ld = d.size(0) > 1 ? d.stride(0) : d.size(1);   // (a single row may have any stride)
+  r.lds = s.size(0) > 1 ? s.stride(0) : s.size(1);
+  r.ok = true;
+  return r;
+}
+
+// block_matmul(a data, a scales, b data, b scales, k, out, accumulate, max_cus)
+PyObject* py_block_matmul(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  return guarded([&]() -> PyObject* {
+    if (n_args != 8) return none();
+    const int64_t k = integer(a[4]);
+    const BlockRows ra = block_rows(a[0], a[1], k), rb = block_rows(a[2], a[3], k);
+    const bool accumulate = truth(a[6]);
+    const int max_cus = (int)integer(a[7]);
+    if (!ra.ok || !rb.ok || !fits_int(ra.rows) || !fits_int(rb.rows) || !fits_int(k) || rb.rows % 8) return none();
+    Tensor out;
+    int64_t ldc = rb.rows;
+    if (absent(a[5])) {
+      if (accumulate) return none();
+    } else {
+      if (!bf16_arg(a[5])) return none();
+      out = tensor(a[5]);
+      if (!on_current_device(out) || out.dim() != 2 || out.size(0) != ra.rows || out.size(1) != rb.rows || out.stride(1) != 1) return none();
+      if (ra.rows > 1) ldc = out.stride(0);
+    }
+    const Tensor &da = tensor(a[0]), &sa = tensor(a[1]), &db = tensor(a[2]), &sb = tensor(a[3]);
+    int rc;
+    {
+      WithoutInterpreter free;
+      if (!out.defined()) out = at::empty({ra.rows, rb.rows}, da.options().dtype(at::kBFloat16));
+      const size_t ws_bytes = kr_block_gemm_workspace_bytes((int)ra.rows, (int)rb.rows, (int)k, max_cus);
+      Tensor ws;
+      if (ws_bytes) ws = bytes(ws_bytes, da);
+      rc = kr_block_gemm((int)ra.rows, (int)rb.rows, (int)k, ptr(da), ra.ld, ptr(sa), ra.lds, ptr(db), rb.ld, ptr(sb), rb.lds, ptr(out),
+                         ldc, accumulate, max_cus, ws_bytes ? ptr(ws) : nullptr, ws_bytes, stream());
+    }
+    if (rc != KR_OK)
+      return failed("kr_block_gemm(M=" + std::to_string(ra.rows) + ", N=" + std::to_string(rb.rows) + ", K=" + std::to_string(k) + ")", rc);
+    return absent(a[5]) ? wrap(std::move(out)) : Py_NewRef(a[5]);
+  });
+}
+
+bool ids_arg(PyObject* o) {
+  return is_tensor(o) && on_device(tensor(o), at::kLong) && !symbolic(tensor(o)) && tensor(o).dim() == 2 && tensor(o).is_contiguous() &&
+         on_current_device(tensor(o));
+}
+
+// embedding_fwd_scaled(ids [b, s], weight, vocab_start, scale) -> [s, b, hidden]
+PyObject* py_embedding_fwd_scaled(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  return guarded([&]() -> PyObject* {
+    if (n_args != 4 || !ids_arg(a[0]) || !bf16_arg(a[1])) return none();
+    const Tensor &ids = tensor(a[0]), &w = tensor(a[1]);
+    if (symbolic(w) || !on_current_device(w) || w.dim() != 2 || !w.is_contiguous() || w.numel() == 0 || ids.numel() == 0) return none();
+    const int64_t start = integer(a[2]), b = ids.size(0), s = ids.size(1), h = w.size(1);
+    const float scale = (float)real(a[3]);
+    if (!fits_int(b) || !fits_int(s) || !fits_int(h)) return none();
+    Tensor out;
+    int rc;
+    {
+      WithoutInterpreter free;
+      out = at::empty({s, b, h}, w.options());
+      rc = kr_embedding_fwd_scaled((const int64_t*)ptr(ids), ptr(w), ptr(out), (int)s, (int)b, (int)h, start, w.size(0), scale, stream());
+    }
+    if (rc != KR_OK)
+      return failed("kr_embedding_fwd_scaled(s=" + std::to_string(s) + ", b=" + std::to_string(b) + ", hidden=" + std::to_string(h) + ")", rc);
+    return wrap(std::move(out));
+  });
+}
+
+// embedding_bwd_sorted(ids [b, s], dout [s, b, hidden], vocab_rows, vocab_start, scale, out, accumulate)
+PyObject* py_embedding_bwd_sorted(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  return guarded([&]() -> PyObject* {
+    if (n_args != 7 || !ids_arg(a[0]) || !bf16_arg(a[1])) return none();
+    const Tensor &ids = tensor(a[0]), &dout = tensor(a[1]);
+    if (symbolic(dout) || !on_current_device(dout) || dout.dim() != 3 || !dout.is_contiguous() || dout.size(0) != ids.size(1) ||
+        dout.size(1) != ids.size(0) || dout.numel() == 0)
+      return none();
+    const int64_t rows = integer(a[2]), start = integer(a[3]), b = ids.size(0), s = ids.size(1), h = dout.size(2);
+    const float scale = (float)real(a[4]);
+    const bool accumulate = truth(a[6]);
+    if (rows <= 0 || !fits_int(b) || !fits_int(s) || !fits_int(h)) return none();
+    Tensor out;
+    if (absent(a[5])) {
+      if (accumulate) return none();
+    } else {
+      if (!bf16_arg(a[5]) && !f32_arg(a[5])) return none();
+      out = tensor(a[5]);
+      if (!on_current_device(out) || out.dim() != 2 || out.size(0) != rows || out.size(1) != h || !out.is_contiguous()) return none();
+    }
+    int rc;
+    {
+      WithoutInterpreter free;
+      if (!out.defined()) out = matrix(rows, h, dout);
+      const size_t n = kr_embedding_bwd_sorted_workspace_bytes((int)s, (int)b, (int)h, rows);
+      const Tensor ws = bytes(std::max<size_t>(n, 16), dout);
+      rc = kr_embedding_bwd_sorted((const int64_t*)ptr(ids), ptr(dout), ptr(out), out.scalar_type() == at::kFloat, (int)s, (int)b, (int)h,
+                                   start, rows, scale, accumulate, ptr(ws), n, stream());
+    }
+    if (rc != KR_OK)
+      return failed("kr_embedding_bwd_sorted(s=" + std::to_string(s) + ", b=" + std::to_string(b) + ", hidden=" + std::to_string(h) +
+                        ", vocab_rows=" + std::to_string(rows) + ")",
+                    rc);
+    return absent(a[5]) ? wrap(std::move(out)) : Py_NewRef(a[5]);
+  });
+}
+
 // rmsnorm_dgamma(partials [n, cols] fp32, gamma) -> the weight gradient
 PyObject* py_rmsnorm_dgamma(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   return guarded([&]() -> PyObject* {
@@ -1146,6 +1307,10 @@ PyMethodDef kMethods[] = {
     {"mlp_chain_bwd", (PyCFunction)(void*)py_mlp_chain_bwd, METH_FASTCALL, nullptr},
     {"attn_chain_bwd", (PyCFunction)(void*)py_attn_chain_bwd, METH_FASTCALL, nullptr},
     {"rmsnorm_dgamma", (PyCFunction)(void*)py_rmsnorm_dgamma, METH_FASTCALL, nullptr},
+    {"quantize_blocks", (PyCFunction)(void*)py_quantize_blocks, METH_FASTCALL, nullptr},
+    {"block_matmul", (PyCFunction)(void*)py_block_matmul, METH_FASTCALL, nullptr},
+    {"embedding_fwd_scaled", (PyCFunction)(void*)py_embedding_fwd_scaled, METH_FASTCALL, nullptr},
+    {"embedding_bwd_sorted", (PyCFunction)(void*)py_embedding_bwd_sorted, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 
