@@ -22,6 +22,8 @@ import torch
 from .operators import (
     BiasDropoutAddOp,
     BiasSwigluOp,
+    BlockColumnParallelLinearOp,
+    BlockRowParallelLinearOp,
     NoOpAllReduce,
     PartitionableRMSNorm,
     QKVPostProcessOp,
@@ -116,6 +118,10 @@ class LayerConfig:
     # where four nanobatches stop gaining; it does not look at their number, so two of 1.13x to 1.20x stay on streams.
     # 0: every pass uses the streams.
     in_line_below_ms: float = 0.65
+    # "bf16", or "fp8_blocks": the linear layers' products run on e4m3 operands with a power-of-two scale per 128 elements along the
+    # contraction (weights: per 128 x 128 tile); parameters, activations between the layers and gradients stay in params_dtype, and
+    # the epilogues of fuse_forward_epilogues are operators of their own
+    linear_format: str = "bf16"
 
     def nanobatches_in_line(self, seq: int, seqs: int) -> bool:
         """Whether the nanobatches of a pass ([seq, seqs, hidden] each) run one after the other on the caller's stream
@@ -233,10 +239,15 @@ class DecoderLayer(torch.nn.Module):
             vals = torch.empty(w.shape, dtype=torch.float32).normal_(0.0, c.init_method_std, generator=generator)
             w.copy_(vals.to(w.dtype))
 
+        if c.linear_format not in ("bf16", "fp8_blocks"):
+            raise ValueError(f"unknown linear_format {c.linear_format!r}; choose 'bf16' or 'fp8_blocks'")
+        blocks = c.linear_format == "fp8_blocks"
+        column = BlockColumnParallelLinearOp if blocks else TEColumnParallelLinearOp
+        row = BlockRowParallelLinearOp if blocks else TERowParallelLinearOp
         lin = dict(config=c, init_method=init, bias=False, device=device, dtype=dt, backend=be)
         self.attn_residual_fork = ResidualForkOp(backend=be)
         self.input_layernorm = PartitionableRMSNorm(c.hidden_size, c.layernorm_epsilon, device=device, dtype=dt, backend=be)
-        self.linear_qkv = TEColumnParallelLinearOp(c.hidden_size, c.qkv_width, skip_bias_add=False, **lin)
+        self.linear_qkv = column(c.hidden_size, c.qkv_width, skip_bias_add=False, **lin)
         head_norm = (lambda: RMSNorm(c.kv_channels, c.layernorm_epsilon, device=device, dtype=dt, backend=be)
                      ) if c.qk_layernorm else (lambda: None)
         self.qkv_postprocess = QKVPostProcessOp(c.num_query_groups, c.num_attention_heads, c.kv_channels,
@@ -244,16 +255,15 @@ class DecoderLayer(torch.nn.Module):
         self.rotary = RotaryEmbeddingOp(config=c, backend=be)
         self.core_attention = TEDotProductAttentionOp(config=c, layer_number=layer_number, backend=be,
                                                       attention_dropout=c.attention_dropout)
-        self.linear_proj = TERowParallelLinearOp(c.num_attention_heads * c.kv_channels, c.hidden_size,
-                                                 skip_bias_add=True, **lin)
+        self.linear_proj = row(c.num_attention_heads * c.kv_channels, c.hidden_size, skip_bias_add=True, **lin)
         self.self_attn_bda = BiasDropoutAddOp(has_bias=c.add_bias_linear, dropout_prob=c.hidden_dropout, backend=be)
         self.mlp_residual_fork = ResidualForkOp(backend=be)
         self.pre_mlp_layernorm = PartitionableRMSNorm(c.hidden_size, c.layernorm_epsilon, device=device, dtype=dt, backend=be)
-        self.linear_fc1 = TEColumnParallelLinearOp(c.hidden_size, 2 * c.ffn_hidden_size, skip_bias_add=True, **lin)
+        self.linear_fc1 = column(c.hidden_size, 2 * c.ffn_hidden_size, skip_bias_add=True, **lin)
         self.activation = BiasSwigluOp(has_bias=c.add_bias_linear, backend=be)
-        self.linear_fc2 = TERowParallelLinearOp(c.ffn_hidden_size, c.hidden_size, skip_bias_add=True, **lin)
+        self.linear_fc2 = row(c.ffn_hidden_size, c.hidden_size, skip_bias_add=True, **lin)
         self.mlp_bda = BiasDropoutAddOp(has_bias=c.add_bias_linear, dropout_prob=c.hidden_dropout, backend=be)
-        fuse = bool(getattr(c, "fuse_forward_epilogues", False))
+        fuse = bool(getattr(c, "fuse_forward_epilogues", False)) and not blocks
         self.linear_fc1.fuse_activation = fuse    # SwiGLU forward in fc1's epilogue
         self.linear_fc2.fuse_activation = fuse    # SwiGLU backward in the epilogue of fc2's input gradient
         # (with hidden dropout the residual is added behind the dropout, by the op that follows)

@@ -40,6 +40,33 @@ class _Embedding(torch.autograd.Function):
         return None, get_backend(ctx.backend).embedding_bwd(ids, dout, ctx.rows, ctx.vocab_start), None, None
 
 
+class _SortedEmbedding(torch.autograd.Function):
+    """The embedding times ``scale``, its gradient by sorted tokens.  With ``main_grad`` the gradient goes to the weight's fp32
+    ``main_grad``, which the first backward pass writes whole and later ones add to, and autograd sees none."""
+
+    @staticmethod
+    def forward(ctx, ids, weight, vocab_start, scale, main_grad, backend):
+        ctx.save_for_backward(ids)
+        ctx.vocab_start, ctx.scale, ctx.backend, ctx.rows = vocab_start, scale, backend, weight.shape[0]
+        ctx.main = weight if main_grad else None
+        return get_backend(backend).embedding_fwd(ids, weight.detach(), vocab_start, scale=scale)
+
+    @staticmethod
+    def backward(ctx, dout):
+        (ids,) = ctx.saved_tensors
+        be, w = get_backend(ctx.backend), ctx.main
+        out, add = None, False
+        if w is not None:
+            out = getattr(w, "main_grad", None)
+            add = out is not None
+            if not add:
+                out = torch.empty(w.shape, dtype=torch.float32, device=w.device)
+        dw = be.embedding_bwd_sorted(ids, dout, ctx.rows, ctx.vocab_start, scale=ctx.scale, out=out, accumulate=add)
+        if w is not None:
+            w.main_grad, dw = out, None
+        return None, dw, None, None, None, None
+
+
 class _RMSNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gamma, eps, backend):
@@ -99,30 +126,44 @@ class _CrossEntropy(torch.autograd.Function):
 
 
 class LanguageModelEmbedding(torch.nn.Module):
-    """Word embeddings of one vocabulary shard; ``forward(input_ids [b, s]) -> [s, b, hidden]``."""
+    """Word embeddings of one vocabulary shard; ``forward(input_ids [b, s]) -> scale * rows, [s, b, hidden]``.
+
+    ``sorted_gradient``: the weight's gradient is summed by sorted tokens instead of by vocabulary rows (always so with a scale or
+    ``main_grad``): for many tokens, or ids that fill a batch.  ``main_grad``: it is kept over backward passes in an fp32
+    ``weight.main_grad``, ``None`` until the first (set it back to ``None``, or zero it, for the next step); a pass touches the rows of
+    its tokens only."""
 
     def __init__(self, config: LayerConfig, vocab_rows: int, vocab_start: int = 0, device=None,
-                 generator=None) -> None:
+                 generator=None, scale: float = 1.0, sorted_gradient: bool = False, main_grad: bool = False) -> None:
         super().__init__()
         w = torch.empty(vocab_rows, config.hidden_size, dtype=torch.float32)
         w.normal_(0.0, config.init_method_std, generator=generator)
         self.weight = torch.nn.Parameter(w.to(device=device, dtype=config.params_dtype))
         self.vocab_start, self._backend = int(vocab_start), config.backend
+        self.scale, self.main_grad = float(scale), bool(main_grad)
+        self.sorted_gradient = bool(sorted_gradient) or self.main_grad or self.scale != 1.0
+        if self.main_grad:
+            self.weight.main_grad = None
 
     def forward(self, input_ids: Tensor) -> Tensor:
+        if self.sorted_gradient:
+            return _SortedEmbedding.apply(input_ids, self.weight, self.vocab_start, self.scale, self.main_grad, self._backend)
         return _Embedding.apply(input_ids, self.weight, self.vocab_start, self._backend)
 
 
 class GPTModelShard(torch.nn.Module):
     """``forward(input_ids [b, s], labels [b, s] or None)`` -> loss ``[b, s]`` (fp32) or logits
-    ``[s, b, vocab_rows]``."""
+    ``[s, b, vocab_rows]``.  ``embedding_scale``, ``embedding_sorted_gradient``, ``embedding_main_grad``: see
+    :class:`LanguageModelEmbedding`."""
 
     def __init__(self, config: LayerConfig, vocab_rows: int, vocab_start: int = 0, device=None,
-                 seed: Optional[int] = None) -> None:
+                 seed: Optional[int] = None, embedding_scale: float = 1.0, embedding_sorted_gradient: bool = False,
+                 embedding_main_grad: bool = False) -> None:
         super().__init__()
         gen = torch.Generator().manual_seed(seed + 1) if seed is not None else None
         self.config = config
-        self.embedding = LanguageModelEmbedding(config, vocab_rows, vocab_start, device=device, generator=gen)
+        self.embedding = LanguageModelEmbedding(config, vocab_rows, vocab_start, device=device, generator=gen, scale=embedding_scale,
+                                                sorted_gradient=embedding_sorted_gradient, main_grad=embedding_main_grad)
         self.decoder = LayerStack(config, device=device, seed=seed)
         self.final_layernorm = torch.nn.Parameter(
             torch.ones(config.hidden_size, device=device, dtype=config.params_dtype))

@@ -4,6 +4,7 @@ reference's: the slot table keys on them)."""
 from .attention import TEDotProductAttentionOp
 from .bias_dropout_add import BiasDropoutAddOp
 from .bias_swiglu import BiasSwigluOp
+from .block_linear import BlockColumnParallelLinearOp, BlockRowParallelLinearOp
 from .linear import PartitionableLinear, TEColumnParallelLinearOp, TERowParallelLinearOp
 from .noop_collective import NoOpAllReduce
 from .qkv_postprocess import QKVPostProcessOp
@@ -15,6 +16,8 @@ from . import chains  # noqa: F401  (loaded with the package: the engine asks fo
 __all__ = [
     "BiasDropoutAddOp",
     "BiasSwigluOp",
+    "BlockColumnParallelLinearOp",
+    "BlockRowParallelLinearOp",
     "NoOpAllReduce",
     "PartitionableLinear",
     "PartitionableRMSNorm",

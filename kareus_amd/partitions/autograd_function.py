@@ -204,7 +204,9 @@ class TransformerBlockAutogradFunction(torch.autograd.Function):
         streams = [None] * n if in_line else _nanobatch_streams(config, n)
         chains = _chains(config)
         out_tid = fwd_graph.get_output_channel(seed.fwd_output_channel)
-        ctxs = [NanoBatchContext(batch_idx=i, stream=streams[i], in_line=in_line, chains=chains, output_id=out_tid) for i in range(n)]
+        shared = {} if getattr(config, "linear_format", "bf16") != "bf16" else None   # (8-bit weights, quantised once a pass)
+        ctxs = [NanoBatchContext(batch_idx=i, stream=streams[i], in_line=in_line, chains=chains, output_id=out_tid, shared=shared)
+                for i in range(n)]
         _seed_forward(ctxs, hs, rotary, mask, seed)
 
         # The nanobatch outputs are written side by side into one [s, b, h] tensor, so the
@@ -229,6 +231,8 @@ class TransformerBlockAutogradFunction(torch.autograd.Function):
         _fork(streams)
         _run_forward(fwd_parts, ctxs, schedule, is_grad_enabled)
         _join(streams)
+        if shared is not None:
+            shared.clear()
 
         outs = [c.tensor_store.get(out_tid) for c in ctxs]
 
@@ -285,7 +289,9 @@ class TransformerBlockAutogradFunction(torch.autograd.Function):
         _fork(streams)
         if func_ctx.checkpoint_activations:
             hs = func_ctx.saved_tensors
-            ctxs = [NanoBatchContext(batch_idx=i, stream=streams[i], in_line=func_ctx.in_line, chains=chains) for i in range(n)]
+            shared = {} if getattr(func_ctx.config, "linear_format", "bf16") != "bf16" else None
+            ctxs = [NanoBatchContext(batch_idx=i, stream=streams[i], in_line=func_ctx.in_line, chains=chains, shared=shared)
+                    for i in range(n)]
             _seed_forward(ctxs, hs, rotary, mask, seed)
             # with the generators as they were before the forward pass, and put back afterwards
             # (kareus/megatron/core/partitions/autograd_function.py:263-266)
@@ -295,6 +301,8 @@ class TransformerBlockAutogradFunction(torch.autograd.Function):
                 if func_ctx.fwd_cuda_rng_state is not None:
                     torch.cuda.set_rng_state(func_ctx.fwd_cuda_rng_state)
                 _run_forward(func_ctx.forward_partitions, ctxs, schedule, func_ctx.is_grad_enabled)
+            if shared is not None:
+                shared.clear()
             for c in ctxs:
                 c.finalize_recomputed_contexts()
         else:

@@ -84,12 +84,16 @@ class NanoBatchContext:
     output_id: Optional[str] = None
     # op_id -> tensor that op's forward output is to be written into (consumed when the op runs)
     output_sinks: Dict[int, torch.Tensor] = field(default_factory=dict)
+    # one dict for all nanobatches of a forward (or recomputation) pass, in which operators leave what they all read
+    shared: Optional[Dict[int, Any]] = None
     _saved_tensors: List[Optional[torch.Tensor]] = field(default_factory=list)
     _saved_ranges: Dict[int, Tuple[int, int]] = field(default_factory=dict)
 
     def create_op_context(self, op_id: int) -> OperationContext:
         ctx = OperationContext.__new__(OperationContext)  # every field at its class default
         self.op_contexts[op_id] = ctx
+        if self.shared is not None:
+            ctx.pass_shared = self.shared
         return ctx
 
     def get_op_context(self, op_id: int) -> OperationContext:

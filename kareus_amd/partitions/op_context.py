@@ -31,6 +31,8 @@ class OperationContext:
     requires_grad: bool = True
     # no kernel of another nanobatch's stream runs beside this op's (NanoBatchContext.in_line)
     alone: bool = False
+    # what the nanobatches of one pass share, by operator (NanoBatchContext.shared)
+    pass_shared: Optional[Dict[int, Any]] = None
 
     def save_for_backward(self, *tensors: Optional[torch.Tensor]) -> None:
         self.to_save = tensors

@@ -42,6 +42,8 @@ _GROUP_BY_CLASS: Dict[str, str] = {
     "PartitionableLinear": "linear",
     "TEColumnParallelLinearOp": "linear",
     "TERowParallelLinearOp": "linear",
+    "BlockColumnParallelLinearOp": "linear",
+    "BlockRowParallelLinearOp": "linear",
     "TEDotProductAttentionOp": "attn",
 }
 _MEMORY_BOUND_GROUPS = frozenset({"norm", "rope", "activation"})
