@@ -88,6 +88,7 @@ _SIGNATURES = {
 }
 
 _HERE = contextlib.nullcontext()
+_new = tuple.__new__
 KR_GEMM_TN, KR_GEMM_NN, KR_GEMM_NT = 0, 1, 2
 KR_ATTN_BESIDE_OTHER_STREAMS = 0x100
 KR_ATTN_GENERAL_KERNELS = 0x200
@@ -463,9 +464,9 @@ class HipBackend:
         read.  ``tiles``: one scale per 128 x 128 tile, so that both orientations hold the same values."""
         done = self._n.quantize_blocks(x, by_row, by_col, tiles)
         if done is not None:
-            q, s, qt, st = done
-            return BlockScaled(None if q is None else BlockOperand(q, s, x.shape[-1]),
-                               None if qt is None else BlockOperand(qt, st, x.numel() // x.shape[-1]))
+            q, s, qt, st = done     # (tuple.__new__: half the time of the named tuple's own)
+            return _new(BlockScaled, (None if q is None else _new(BlockOperand, (q, s, x.shape[-1])),
+                                      None if qt is None else _new(BlockOperand, (qt, st, x.numel() // x.shape[-1]))))
         self._dev(x)
         self._bf16(x)
         if not (by_row or by_col):

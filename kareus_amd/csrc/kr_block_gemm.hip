@@ -564,7 +564,8 @@ Plan choose_plan(int M, int N, int K, int cus, size_t most_bytes) {
       if (splits == last) continue;
       last = splits;
       if (splits > 1 && (tiles * splits > (int64_t)cus * tile.per_cu || partial_bytes(splits, M, N) > most_bytes)) break;
-      const float share = (float)((tiles * splits + cus - 1) / cus), rounds = std::ceil(share / tile.per_cu);
+      const int64_t of_unit = splits > 1 ? ((int)tiles * splits + cus - 1) / cus : (tiles + cus - 1) / cus;
+      const float share = (float)of_unit, rounds = (float)((of_unit + tile.per_cu - 1) / tile.per_cu);
       float us = kLaunch + rounds * tile.round + per * std::max(tile.step_min, rounds * tile.step_round + share * tile.step_tile);
       if (splits > 1) us += kCutLaunch + (2.f * splits + 0.5f) * M * N * 4.f / 5e6f;
       if (us < least) {

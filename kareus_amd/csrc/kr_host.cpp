@@ -1114,6 +1114,15 @@ bool on_current_device(const Tensor& t) { return t.is_cuda() && t.device().index
 bool aligned16(const Tensor& t) { return ((uintptr_t)t.data_ptr() & 15) == 0; }
 int64_t blocks_of(int64_t n) { return (n + 127) / 128; }
 
+// a dense matrix inside a byte buffer (a second allocation costs as much as the kernel's launch)
+Tensor part_of(const Tensor& buffer, at::ScalarType type, int64_t byte_offset, int64_t rows, int64_t cols) {
+  Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(buffer.storage()), buffer.key_set(), c10::scalarTypeToTypeMeta(type));
+  c10::TensorImpl* const impl = t.unsafeGetTensorImpl();
+  impl->set_sizes_contiguous({rows, cols});
+  impl->set_storage_offset(byte_offset);   // (elements of one byte)
+  return t;
+}
+
 // quantize_blocks(x, by_row, by_col, tiles) -> (data, scales, data, scales), None for an orientation that was not asked for
 PyObject* py_quantize_blocks(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   return guarded([&]() -> PyObject* {
@@ -1131,8 +1140,10 @@ PyObject* py_quantize_blocks(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
       for (int i = 0; i < 2; ++i) {
         if (!want[i]) continue;
         const int64_t n = i ? o.cols : o.rows, k = i ? o.rows : o.cols;
-        t[2 * i] = at::empty({n, blocks_of(k) * 128}, x.options().dtype(at::kFloat8_e4m3fn));
-        t[2 * i + 1] = at::empty({blocks_of(k), (n + 3) / 4 * 4}, x.options().dtype(at::kByte));
+        const int64_t pitch = blocks_of(k) * 128, scales = (n + 3) / 4 * 4;
+        const Tensor both = bytes((size_t)(n * pitch + blocks_of(k) * scales), x);
+        t[2 * i] = part_of(both, at::kFloat8_e4m3fn, 0, n, pitch);
+        t[2 * i + 1] = part_of(both, at::kByte, n * pitch, blocks_of(k), scales);
       }
       auto at_ = [&](int i) { return t[i].defined() ? ptr(t[i]) : nullptr; };
       auto ld = [&](int i) { return t[i].defined() ? t[i].size(1) : (int64_t)0; };
