@@ -481,6 +481,8 @@ class HipBackend:
             op = (x.shape[0], x.shape[1], 1, 0)
         rows, ld, run_rows, run_ld = op
         cols = x.shape[-1]
+        if rows <= 1:
+            ld = cols               # (the stride of one row says nothing)
         if cols % 8:
             raise RuntimeError(f"quantize_blocks: {cols} columns are no multiple of 8")
         made = []
@@ -493,7 +495,7 @@ class HipBackend:
             for t in made:
                 args += [None, 0, None, 0] if t is None else [t.data.data_ptr(), t.data.shape[1], t.scales.data_ptr(), t.scales.shape[1]]
             with self._current(x):
-                rc = self.lib.kr_block_quantize(x.data_ptr(), rows, cols, max(ld, cols), run_rows, run_ld, int(tiles), *args,
+                rc = self.lib.kr_block_quantize(x.data_ptr(), rows, cols, ld, run_rows, run_ld, int(tiles), *args,
                                                 self._stream())
             self._check(rc, f"kr_block_quantize(rows={rows}, cols={cols})")
         return BlockScaled(*made)

@@ -5,6 +5,16 @@
 //
 // The matrix instruction (v_mfma_scale_f32_32x32x64_f8f6f4, 131072 FLOP in 64 cycles, twice the rate of the unscaled 8-bit ones)
 // multiplies by 2^(scale - 127) of both operands' rows on its way into the sum, so the scales cost nothing but their loads.
+//
+// Precision: a product of two e4m3 values has 8 bits, so it is exact in the unit, which aligns the products of 8 consecutive
+// contraction elements to the largest of them, cuts each 13 binary places below its exponent, and adds such groups to the fp32
+// accumulator at 2^-23 of the largest term (measured with single products beside large ones).  Sums over the cuts of a contraction,
+// over waves and with C are fp32; the one rounding to bf16 is the store's.
+//
+// What bounds it: large products the card's power.  16384 x 28672 x 4096 takes 1403 us (2.74 PFLOP/s) on normally distributed values
+// and 1033 (3.73) on operands of one value, with the same instructions; 16384 x 7168 x 4096 353 and 262 us, 16384 x 4096 x 7168 337
+// and 254.  Products of few rows are bound by B's bytes (1 x 28672 x 4096 18.4 us: 6.4 TB/s, from the 256 MiB cache), those of one
+// tile per unit by their loads' latency and the launch.
 #include "kr_common.h"
 
 #include <algorithm>
@@ -99,7 +109,7 @@ constexpr size_t lds_bytes(int wt, int wn) {
 //     them the fragment reads of the next phase and the loads of one operand two K-steps ahead.  In LDS the halves are blocks of
 //     their own: the block that a phase has read is free behind the barrier at its end, so eight blocks hold the two K-steps that the
 //     loads run ahead, every phase loads as much as the others, and every load has one phase to land at least.
-//   * The barrier stands in front of a phase's last MFMA, which runs while the waves meet.
+//   * The barrier stands in front of a phase's last MFMAs, which run while the waves meet.
 //   * A block's row is 64 bytes, its 16-byte chunks XORed with (row >> 2) & 3: the 16 rows that a fragment read takes at a time cover
 //     all banks once.  Both halves of a row's 128 bytes are requested one behind the other: one line fetched from the L2.
 template <int WT, int WN, int OUT>
@@ -204,14 +214,14 @@ __global__ __launch_bounds__(NTHREADS, WT * WN == 1 ? 3 : WT * WN == 4 ? 2 : 1) 
     i32x8 a[WT], b[WN];
   } X, Y;
   auto clear = [&]() {
+    if constexpr (!PINNED) {
 #pragma unroll
-    for (int i = 0; i < WT; ++i)
+      for (int i = 0; i < WT; ++i)
 #pragma unroll
-      for (int j = 0; j < WN; ++j) {
+        for (int j = 0; j < WN; ++j)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-        if constexpr (PINNED) asm volatile("" : "+a"(acc[i][j]));
-      }
+          for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+    }
   };
 
   // fragment addresses: lane l takes row l % 32 of a tile, chunks 2 (l / 32) and + 1 of a half
@@ -224,8 +234,10 @@ __global__ __launch_bounds__(NTHREADS, WT * WN == 1 ? 3 : WT * WN == 4 ? 2 : 1) 
   const uint32_t sca = (uint32_t)(32 * WT * wm + WT * (lane & 31)), scb = 256u + (uint32_t)(32 * WN * wn + WN * (lane & 31));
 
   // One phase: the MFMAs on `cur`, and between them the fragments of the next from blocks na / nb, `loads` (called with 0 ..
-  // NLOADS - 1) and, in front of the last MFMA, `meet`.
-  auto phase = [&](Frags& cur, Frags& nxt, int sa, int sb, uint32_t na, uint32_t nb, auto nloads_tag, auto loads, auto meet) {
+  // NLOADS - 1) and, in front of the last ones, `meet`.
+  // FIRST: of an item; the pinned accumulators start from the instruction's constant 0 instead of being cleared.
+  auto phase = [&](auto first_tag, Frags& cur, Frags& nxt, int sa, int sb, uint32_t na, uint32_t nb, auto nloads_tag, auto loads, auto meet) {
+    constexpr bool FIRST = decltype(first_tag)::value;
     constexpr int NLOADS = decltype(nloads_tag)::value;
     const uint32_t a0 = fa + na, b0 = fb + nb;
     auto fetch = [&](auto f) {   // fragments in the order that the next phase takes them
@@ -235,16 +247,23 @@ __global__ __launch_bounds__(NTHREADS, WT * WN == 1 ? 3 : WT * WN == 4 ? 2 : 1) 
       else nxt.a[i - WN] = frag(a0 + (i - WN) * 32 * 64);
     };
     constexpr int NF = WT + WN;
-    constexpr int LAST = SLOTS >= 4 ? SLOTS - 1 : SLOTS;   // the MFMA that `meet` stands in front of
+    // the MFMA that `meet` stands in front of.  (Large tile, behind all, in front of the last, the last two, the last three, us: 16384 x
+    // 7168 x 4096 359, 359, 357, 359; 16384 x 28672 x 4096 1440, 1473, 1430, 1454; 16384 x 4096 x 7168 345, 344, 342, 344.)
+    constexpr int LAST = SLOTS >= 12 ? SLOTS - 2 : SLOTS >= 4 ? SLOTS - 1 : SLOTS;
     // fragment f is read behind MFMA f * (LAST - 2) / NF, load d behind MFMA d * (LAST - 1) / NLOADS
     each([&](auto s) {
       constexpr int slot = decltype(s)::value, gi = slot / WN, ni = slot % WN;
       if constexpr (slot == LAST) meet();
       if constexpr (PINNED) {
         if constexpr (slot == 0) asm volatile("s_nop 3" ::: "memory");   // (the scales may just have been moved)
-        asm volatile("v_mfma_scale_f32_32x32x64_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[%5,%6,0] op_sel_hi:[%7,%8,0]"
-                     : "+a"(acc[gi][ni])
-                     : "v"(cur.b[ni]), "v"(cur.a[gi]), "v"(sb), "v"(sa), "n"(ni & 1), "n"(gi & 1), "n"(ni >> 1), "n"(gi >> 1));
+        if constexpr (FIRST)
+          asm volatile("v_mfma_scale_f32_32x32x64_f8f6f4 %0, %1, %2, 0, %3, %4 op_sel:[%5,%6,0] op_sel_hi:[%7,%8,0]"
+                       : "=a"(acc[gi][ni])
+                       : "v"(cur.b[ni]), "v"(cur.a[gi]), "v"(sb), "v"(sa), "n"(ni & 1), "n"(gi & 1), "n"(ni >> 1), "n"(gi >> 1));
+        else
+          asm volatile("v_mfma_scale_f32_32x32x64_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[%5,%6,0] op_sel_hi:[%7,%8,0]"
+                       : "+a"(acc[gi][ni])
+                       : "v"(cur.b[ni]), "v"(cur.a[gi]), "v"(sb), "v"(sa), "n"(ni & 1), "n"(gi & 1), "n"(ni >> 1), "n"(gi >> 1));
       } else {
         acc[gi][ni] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(cur.b[ni], cur.a[gi], acc[gi][ni], 0, 0, ni, sb, gi, sa);
       }
@@ -287,28 +306,30 @@ __global__ __launch_bounds__(NTHREADS, WT * WN == 1 ? 3 : WT * WN == 4 ? 2 : 1) 
   for (int i = 0; i < WN; ++i) X.b[i] = frag(fb + now.b0 + i * 32 * 64);
   int sa = lds_scales<WT>(now.sc + sca), sb = lds_scales<WN>(now.sc + scb);
   kr_barrier();                         // (every wave has read what the first phase's loads overwrite)
+  auto k_step = [&](auto first) {
+    // half 0: half 1 of this step is read; A two steps ahead goes where both operands' half 0 lay
+    phase(first, X, Y, sa, sb, now.a1, now.b1, Int<NA + 1>{},
+          [&](auto d) {
+            if constexpr (decltype(d)::value < NA) request_a(d, now.a0, now.b0);
+            else request_scales(now.sc);
+          },
+          [&]() {
+            __builtin_amdgcn_s_waitcnt(vm_wait(NA + 1));   // the next step has landed
+            kr_barrier();
+          });
+    // half 1: half 0 of the next step and its scales are read; B two steps ahead goes where this step's half 1 lay
+    const int sa1 = lds_scales<WT>(next.sc + sca), sb1 = lds_scales<WN>(next.sc + scb);
+    phase(std::false_type{}, Y, X, sa, sb, next.a0, next.b0, Int<NB>{}, [&](auto d) { request_b(d, now.a1, now.b1); }, [&]() { kr_barrier(); });
+    advance();
+    sa = sa1;
+    sb = sb1;
+    const Blocks ahead = {now.a0, now.b0, now.a1, now.b1, now.sc};
+    now = next;
+    next = ahead;
+  };
   for (;;) {
-    for (int t = 0; t < it.nk; ++t) {
-      // half 0: half 1 of this step is read; A two steps ahead goes where both operands' half 0 lay
-      phase(X, Y, sa, sb, now.a1, now.b1, Int<NA + 1>{},
-            [&](auto d) {
-              if constexpr (decltype(d)::value < NA) request_a(d, now.a0, now.b0);
-              else request_scales(now.sc);
-            },
-            [&]() {
-              __builtin_amdgcn_s_waitcnt(vm_wait(NA + 1));   // the next step has landed
-              kr_barrier();
-            });
-      // half 1: half 0 of the next step and its scales are read; B two steps ahead goes where this step's half 1 lay
-      const int sa1 = lds_scales<WT>(next.sc + sca), sb1 = lds_scales<WN>(next.sc + scb);
-      phase(Y, X, sa, sb, next.a0, next.b0, Int<NB>{}, [&](auto d) { request_b(d, now.a1, now.b1); }, [&]() { kr_barrier(); });
-      advance();
-      sa = sa1;
-      sb = sb1;
-      const Blocks ahead = {now.a0, now.b0, now.a1, now.b1, now.sc};
-      now = next;
-      next = ahead;
-    }
+    k_step(std::integral_constant<bool, PINNED>{});
+    for (int t = 1; t < it.nk; ++t) k_step(std::false_type{});
 
     // the compiler does not know the latency of MFMAs in assembly: let the last ones finish before their results are read
     if constexpr (PINNED) asm volatile("s_nop 15\n\ts_nop 15\n\ts_nop 15\n\ts_nop 15\n\ts_nop 15" ::: "memory");
@@ -319,6 +340,17 @@ __global__ __launch_bounds__(NTHREADS, WT * WN == 1 ? 3 : WT * WN == 4 ? 2 : 1) 
       asm volatile("" : "+v"(le));
       const int j = le & 31, hi = le >> 5;
       const int m_wave = it.m0 + 32 * WT * wm, n_wave = it.n0 + 32 * WN * wn;
+      constexpr int SW = stage_row(WN), PASSES = 64 * WN / SW, QP = 4 / PASSES, PIECES = SW / 16, RPP = 64 / PIECES, PER = 32 / RPP;
+      const int piece = le % PIECES, r0 = le / PIECES;
+      bf16x8 held[PER];   // the pass before
+      auto store_pass = [&](int pass) {
+        const int gi = pass / PASSES, col = n_wave + pass % PASSES * (SW / 2) + 8 * piece;
+#pragma unroll
+        for (int p = 0; p < PER; ++p) {
+          const int rr = m_wave + WT * (p * RPP + r0) + gi;
+          if (rr < g.m && col < g.n) stg8_stream(g.c + (int64_t)rr * g.ldc + col, held[p]);
+        }
+      };
 #pragma unroll
       for (int gi = 0; gi < WT; ++gi) {
         const int row = m_wave + WT * j + gi;
@@ -346,11 +378,11 @@ __global__ __launch_bounds__(NTHREADS, WT * WN == 1 ? 3 : WT * WN == 4 ? 2 : 1) 
             }
           }
         } else {
-          // rows of the block through LDS (64 or 128 bytes of each at a time), then whole pieces of rows to memory
-          constexpr int SW = stage_row(WN), PASSES = 64 * WN / SW, QP = 4 / PASSES, PIECES = SW / 16, RPP = 64 / PIECES;
+          // rows of the block through LDS (64 or 128 bytes of each at a time), then whole pieces of rows to memory.  A wave's LDS
+          // instructions run in order, so nothing waits between a pass's writes and reads, nor before the next pass's writes; a
+          // pass is stored when the next has been written and asked for.
 #pragma unroll
           for (int h = 0; h < PASSES; ++h) {
-            __builtin_amdgcn_wave_barrier();
 #pragma unroll
             for (int ql = 0; ql < QP; ++ql) {
               const int q = h * QP + ql;
@@ -384,18 +416,20 @@ __global__ __launch_bounds__(NTHREADS, WT * WN == 1 ? 3 : WT * WN == 4 ? 2 : 1) 
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
             __builtin_amdgcn_wave_barrier();
             __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
-            const int piece = le % PIECES, r0 = le / PIECES;
-            const int col = n_wave + h * (SW / 2) + 8 * piece;
+            bf16x8 read[PER];
 #pragma unroll
-            for (int p = 0; p < 32 / RPP; ++p) {
+            for (int p = 0; p < PER; ++p) {
               const int jj = p * RPP + r0;
-              const bf16x8 v = *(KR_LDS const bf16x8*)(stage + jj * SW + ((piece ^ (SW == 128 ? (jj >> 1) & 7 : (jj >> 2) & 3)) << 4));
-              const int rr = m_wave + WT * jj + gi;
-              if (rr < g.m && col < g.n) stg8_stream(g.c + (int64_t)rr * g.ldc + col, v);
+              read[p] = *(KR_LDS const bf16x8*)(stage + jj * SW + ((piece ^ (SW == 128 ? (jj >> 1) & 7 : (jj >> 2) & 3)) << 4));
             }
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
             __builtin_amdgcn_wave_barrier();
+            if (gi * PASSES + h > 0) store_pass(gi * PASSES + h - 1);
+#pragma unroll
+            for (int p = 0; p < PER; ++p) held[p] = read[p];
+            __builtin_amdgcn_sched_barrier(0);
           }
+          if (gi == WT - 1) store_pass(WT * PASSES - 1);
         }
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -532,11 +566,6 @@ struct Plan {
   int tile, splits, steps_per;
 };
 
-#ifdef FORCE
-static int force_tile = -1, force_splits = 0;
-extern "C" void force(int t, int s) { force_tile = t; force_splits = s; }
-#endif
-
 size_t partial_bytes(int splits, int M, int N) { return splits > 1 ? (size_t)splits * M * N * sizeof(float) : 0; }
 
 // The plan of the least time by the figures above, with at most `most_bytes` of workspace.
@@ -544,28 +573,23 @@ size_t partial_bytes(int splits, int M, int N) { return splits > 1 ? (size_t)spl
 //     round: 1536 x 2048 x 32768 whole 159 us, in four pieces 100; 64 x 4096 x 4096 12 and 10; 1024 x 1024 x 1024 5 and 11.
 //   * Few rows: a workgroup reads 16 rows of B and all of A, 33.6 GB/s per unit (us, 16 x 4096 x 4096 5.9 where tiles take 8.3, 64 x 4096
 //     x 4096 11.8 and 10.0, 1 x 28672 x 4096 24.9 and 18.7).
-Plan choose_plan(int M, int N, int K, int cus, size_t most_bytes) {
+// limited: the caller has named the units; a workgroup each, and no kernel that is not persistent.
+Plan choose_plan(int M, int N, int K, int cus, bool limited, size_t most_bytes) {
   const int ksteps = (K + BK - 1) / BK;
-#ifdef FORCE
-  if (force_tile >= 0) {
-    Plan p{force_tile, force_splits, (ksteps + force_splits - 1) / force_splits};
-    p.splits = (ksteps + p.steps_per - 1) / p.steps_per;
-    return p;
-  }
-#endif
   Plan best{0, 1, ksteps};
   float least = INFINITY;
   for (int t = 0; t < kNumTiles; ++t) {
     const Tile& tile = kTiles[t];
+    const int per_cu = limited ? 1 : tile.per_cu;
     const int64_t tiles = (int64_t)((M + 64 * tile.wt - 1) / (64 * tile.wt)) * ((N + 64 * tile.wn - 1) / (64 * tile.wn));
     int last = 0;
     for (int want = 1; want <= kMostSplits && want <= ksteps; ++want) {
       const int per = (ksteps + want - 1) / want, splits = (ksteps + per - 1) / per;
       if (splits == last) continue;
       last = splits;
-      if (splits > 1 && (tiles * splits > (int64_t)cus * tile.per_cu || partial_bytes(splits, M, N) > most_bytes)) break;
+      if (splits > 1 && (tiles * splits > (int64_t)cus * per_cu || partial_bytes(splits, M, N) > most_bytes)) break;
       const int64_t of_unit = splits > 1 ? ((int)tiles * splits + cus - 1) / cus : (tiles + cus - 1) / cus;
-      const float share = (float)of_unit, rounds = (float)((of_unit + tile.per_cu - 1) / tile.per_cu);
+      const float share = (float)of_unit, rounds = (float)((of_unit + per_cu - 1) / per_cu);
       float us = kLaunch + rounds * tile.round + per * std::max(tile.step_min, rounds * tile.step_round + share * tile.step_tile);
       if (splits > 1) us += kCutLaunch + (2.f * splits + 0.5f) * M * N * 4.f / 5e6f;
       if (us < least) {
@@ -574,7 +598,7 @@ Plan choose_plan(int M, int N, int K, int cus, size_t most_bytes) {
       }
     }
   }
-  if (M <= kFewRowsMost) {
+  if (M <= kFewRowsMost && !limited) {
     const float groups = std::max(1.f, (float)((N + 15) / 16) / cus), rows = 16.f + (M == 1 ? 1.f : 16.f * ((M + 15) / 16));
     const float us = 1.5f + std::max(groups * K * rows / 33.6e3f, (float)N * K / 5.5e6f);
     if (us < least) best = Plan{kFewRows, 1, ksteps};
@@ -591,7 +615,7 @@ int device_cus() {
 }
 
 template <int T, int OUT>
-int launch(const Args& g, int cus, hipStream_t stream) {
+int launch(const Args& g, int cus, bool limited, hipStream_t stream) {
   constexpr Tile t = kTiles[T];
   constexpr size_t lds = lds_bytes(t.wt, t.wn);
   static_assert(lds * t.per_cu <= 160 * 1024, "LDS of a compute unit");
@@ -600,7 +624,7 @@ int launch(const Args& g, int cus, hipStream_t stream) {
   if (raised != hipSuccess) return KR_ELAUNCH;
   const int64_t tiles = (int64_t)((g.m + 64 * t.wt - 1) / (64 * t.wt)) * ((g.n + 64 * t.wn - 1) / (64 * t.wn)) * g.splits;
   if (tiles > 0x3fffffff) return KR_EUNSUPPORTED;
-  const int64_t grid = std::min<int64_t>(tiles, (int64_t)cus * t.per_cu);
+  const int64_t grid = std::min<int64_t>(tiles, (int64_t)cus * (limited ? 1 : t.per_cu));
   hipLaunchKernelGGL((block_gemm_kernel<t.wt, t.wn, OUT>), dim3((unsigned)grid), dim3(NTHREADS), lds, stream, g);
   return kr_launch_status();
 }
@@ -619,14 +643,14 @@ int launch_few_rows(const Args& g, int accumulate, hipStream_t stream) {
 }
 
 template <int OUT>
-int launch_tile(const Plan& p, const Args& g, int cus, hipStream_t stream) {
+int launch_tile(const Plan& p, const Args& g, int cus, bool limited, hipStream_t stream) {
   switch (p.tile) {
-    case 0: return launch<0, OUT>(g, cus, stream);
-    case 1: return launch<1, OUT>(g, cus, stream);
-    case 2: return launch<2, OUT>(g, cus, stream);
-    case 3: return launch<3, OUT>(g, cus, stream);
-    case 4: return launch<4, OUT>(g, cus, stream);
-    case 5: return launch<5, OUT>(g, cus, stream);
+    case 0: return launch<0, OUT>(g, cus, limited, stream);
+    case 1: return launch<1, OUT>(g, cus, limited, stream);
+    case 2: return launch<2, OUT>(g, cus, limited, stream);
+    case 3: return launch<3, OUT>(g, cus, limited, stream);
+    case 4: return launch<4, OUT>(g, cus, limited, stream);
+    case 5: return launch<5, OUT>(g, cus, limited, stream);
   }
   return KR_EUNSUPPORTED;
 }
@@ -636,7 +660,8 @@ int launch_tile(const Plan& p, const Args& g, int cus, hipStream_t stream) {
 extern "C" size_t kr_block_gemm_workspace_bytes(int M, int N, int K, int max_cus) {
   if (M <= 0 || N <= 0 || K <= 0) return 0;
   const int all = device_cus();
-  return partial_bytes(choose_plan(M, N, K, max_cus > 0 && max_cus < all ? max_cus : all, kMostWorkspace).splits, M, N);
+  const bool limited = max_cus > 0 && max_cus < all;
+  return partial_bytes(choose_plan(M, N, K, limited ? max_cus : all, limited, kMostWorkspace).splits, M, N);
 }
 
 extern "C" int kr_block_gemm(int M, int N, int K, const void* A, int64_t lda, const void* sa, int64_t lsa, const void* B,
@@ -653,13 +678,14 @@ extern "C" int kr_block_gemm(int M, int N, int K, const void* A, int64_t lda, co
   if (lda > (1 << 23) || ldb > (1 << 23) || lsa > 0x7fffffff || lsb > 0x7fffffff || M > 0x7fffff00 || N > 0x7fffff00)
     return KR_EUNSUPPORTED;
   const int all = device_cus();
-  const int cus = max_cus > 0 && max_cus < all ? max_cus : all;
-  const Plan p = choose_plan(M, N, K, cus, workspace ? std::min(workspace_bytes, kMostWorkspace) : 0);
+  const bool limited = max_cus > 0 && max_cus < all;
+  const int cus = limited ? max_cus : all;
+  const Plan p = choose_plan(M, N, K, cus, limited, workspace ? std::min(workspace_bytes, kMostWorkspace) : 0);
   Args g{(const uint8_t*)A, (const uint8_t*)sa, (const uint8_t*)B, (const uint8_t*)sb, (bf16*)C, (float*)workspace,
          lda, ldb, ldc, (int)lsa, (int)lsb, M, N, (K + BK - 1) / BK, p.steps_per, p.splits};
   if (p.tile == kFewRows) return launch_few_rows(g, accumulate, (hipStream_t)stream);
   if (p.splits > 1) {
-    const int rc = launch_tile<kPartial>(p, g, cus, (hipStream_t)stream);
+    const int rc = launch_tile<kPartial>(p, g, cus, limited, (hipStream_t)stream);
     if (rc != KR_OK) return rc;
     const int64_t threads = (int64_t)M * (N / 8);
     if ((threads + 255) / 256 > 0x7fffffff) return KR_EUNSUPPORTED;
@@ -667,5 +693,5 @@ extern "C" int kr_block_gemm(int M, int N, int K, const void* A, int64_t lda, co
                        (const float*)workspace, (bf16*)C, ldc, M, N, p.splits, accumulate);
     return kr_launch_status();
   }
-  return accumulate ? launch_tile<kAccumulate>(p, g, cus, (hipStream_t)stream) : launch_tile<kStore>(p, g, cus, (hipStream_t)stream);
+  return accumulate ? launch_tile<kAccumulate>(p, g, cus, limited, (hipStream_t)stream) : launch_tile<kStore>(p, g, cus, limited, (hipStream_t)stream);
 }
