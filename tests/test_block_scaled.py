@@ -207,6 +207,24 @@ def test_product_added_to_what_is_there(m, n, k):
     check_product(m, n, k, out=inputs(m, n, 9) * 10, accumulate=True)
 
 
+# by the planner on 256 units: 256 x 256 whole and cut, 192 x 256, 256 x 128, 128 x 256, 128 x 128 whole and cut
+TILES = [(5745, 2184, 261), (401, 5552, 15129), (1848, 5184, 386), (523, 4672, 10903), (5737, 1352, 871), (133, 3096, 14755),
+         (2960, 1368, 796), (147, 5448, 5716), (1753, 1776, 259), (66, 4368, 5880)]
+
+
+@pytest.mark.parametrize("accumulate", [False, True])
+@pytest.mark.parametrize("m,n,k", TILES)
+@on_gpu
+def test_product_of_every_tile(m, n, k, accumulate):
+    check_product(m, n, k, out=inputs(m, n, 9) * 10 if accumulate else None, accumulate=accumulate)
+
+
+@pytest.mark.parametrize("m,n,k", [(2, 72, 384), (17, 4104, 1100), (33, 264, 5000), (64, 72, 349)])
+@on_gpu
+def test_product_of_few_rows_added_to_what_is_there(m, n, k):
+    check_product(m, n, k, out=inputs(m, n, 9) * 10, accumulate=True)
+
+
 @on_gpu
 def test_product_leaves_what_is_around_its_output():
     whole = torch.full((300, 400), 7.0, dtype=torch.bfloat16, device="cuda")
