@@ -461,7 +461,8 @@ int kr_embedding_bwd_sorted(const int64_t* ids, const void* dout, void* dweight,
  * contraction over rows), whichever of q and qt is not NULL, from one read of x.  A block's scale is the smallest power of two that
  * brings its largest finite magnitude to 448 or below (2^-127 at least; that for a block of zeros), values are rounded to the
  * nearest, ties to even; infinities and NaN become NaN.  tiles != 0: one scale per 128 x 128 tile, so that both orientations hold
- * the same values (weights).  cols, ld, run_ld: multiples of 8.  Padding bytes are written (0).
+ * the same values (weights).  cols, ld, run_ld: multiples of 8; at most 128 * 65535 rows.  Padding bytes
+ * are written (0).
  *
  * kr_block_gemm: C [M, N] bf16 (row stride ldc) = A . B^T over K, A with M rows and B with N; accumulate != 0 adds the product to C,
  * rounded once.  fp32 accumulation.  N, ldc: multiples of 8; M and K: any.  max_cus > 0 limits the launch to that many compute

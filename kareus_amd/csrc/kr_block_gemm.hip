@@ -178,7 +178,8 @@ __global__ __launch_bounds__(NTHREADS, WT * WN == 1 ? 3 : WT * WN == 4 ? 2 : 1) 
       r = it.n0 + r < g.n ? r : g.n - 1 - it.n0;
       lb[i] = (uint32_t)r * (uint32_t)g.ldb + (uint32_t)chunk;
     }
-    const int sr = (wn ? it.n0 : it.m0) + 4 * l2, most = (int)rs_step - 4;
+    // four rows' scales a lane; beyond the matrix: those of its last row
+    const int sr = (wn ? it.n0 : it.m0) + 4 * l2, most = ((wn ? g.n : g.m) - 1) & ~3;
     ls = (uint32_t)(sr < most ? sr : most);
   };
   // (behind the last item's last K-step it stays there: the K loop requests that one again rather than branch, two steps in all)

@@ -253,6 +253,19 @@ def test_product_of_longer_pitches_and_unset_padding():
 
 
 @on_gpu
+def test_product_of_parts_of_larger_operands():
+    """Rows and scales that end where their buffers end, behind others': only what belongs to the product is read."""
+    be = get_backend("hip")
+    m, n, k = 130, 72, 200
+    whole_a, whole_b = be.quantize_blocks(inputs(132 + m, k)).by_row, be.quantize_blocks(inputs(200 + n, k, 3)).by_row
+    whole = be.block_matmul(whole_a, whole_b)
+    a = BlockOperand(whole_a.data[132:], whole_a.scales[:, 132:132 + m], k)
+    b = BlockOperand(whole_b.data[200:], whole_b.scales[:, 200:], k)
+    assert not a.scales.is_contiguous() and not b.scales.is_contiguous()
+    assert torch.equal(be.block_matmul(a, b), whole[132:, 200:])
+
+
+@on_gpu
 def test_not_a_number_stays_in_its_row():
     be = get_backend("hip")
     x, w = inputs(70, 256), inputs(72, 256, 2)
