@@ -516,7 +516,8 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void block_gemm_few_rows_kernel(Arg
   }
 }
 
-// C = bf16(sum of the cuts' fp32 partial products, in order [+ C])
+// C = bf16(sum of the cuts' fp32 partial products, in order [+ C]).  (The whole product, us, a cut's loads at a time and four cuts':
+// 75 x 608 x 17951 in twelve 13.2, 11.0; 91 x 272 x 3875 in sixteen 10.2, 7.0; 1536 x 2048 x 32768 in four 100, 100.)
 __global__ __launch_bounds__(256) void block_gemm_reduce_kernel(const float* __restrict__ partial, bf16* __restrict__ C,
                                                                 int64_t ldc, int M, int N, int splits, int accumulate) {
   const int nv = N / 8;
@@ -526,15 +527,28 @@ __global__ __launch_bounds__(256) void block_gemm_reduce_kernel(const float* __r
   float acc[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) acc[e] = 0.f;
-  for (int sp = 0; sp < splits; ++sp) {
-    const float* src = partial + ((int64_t)sp * M + m) * N + n;
-    const f32x4 a = *reinterpret_cast<const f32x4*>(src), b = *reinterpret_cast<const f32x4*>(src + 4);
+  const float* src = partial + (int64_t)m * N + n;
+  const int64_t step = (int64_t)M * N;
+  auto add = [&](auto count) {   // cuts whose loads are all asked for before the first is used
+    constexpr int U = decltype(count)::value;
+    f32x4 a[U], b[U];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      acc[e] += a[e];
-      acc[4 + e] += b[e];
+    for (int u = 0; u < U; ++u) {
+      a[u] = *reinterpret_cast<const f32x4*>(src);
+      b[u] = *reinterpret_cast<const f32x4*>(src + 4);
+      src += step;
     }
-  }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        acc[e] += a[u][e];
+        acc[4 + e] += b[u][e];
+      }
+  };
+  int left = splits;
+  for (; left >= 4; left -= 4) add(Int<4>{});
+  for (; left > 0; --left) add(Int<1>{});
   bf16* dst = C + (int64_t)m * ldc + n;
   if (accumulate) {
     const bf16x8 old = ldg8(dst);
