@@ -593,6 +593,11 @@ Plan choose_plan(int M, int N, int K, int cus, bool limited, size_t most_bytes) 
   const int ksteps = (K + BK - 1) / BK;
   Plan best{0, 1, ksteps};
   float least = INFINITY;
+  if (M <= kFewRowsMost && !limited) {
+    const float groups = std::max(1.f, (float)((N + 15) / 16) / cus), rows = 16.f + (M == 1 ? 1.f : 16.f * ((M + 15) / 16));
+    least = 1.5f + std::max(groups * K * rows / 33.6e3f, (float)N * K / 5.5e6f);
+    best.tile = kFewRows;
+  }
   for (int t = 0; t < kNumTiles; ++t) {
     const Tile& tile = kTiles[t];
     const int per_cu = limited ? 1 : tile.per_cu;
@@ -602,6 +607,7 @@ Plan choose_plan(int M, int N, int K, int cus, bool limited, size_t most_bytes) 
       const int per = (ksteps + want - 1) / want, splits = (ksteps + per - 1) / per;
       if (splits == last) continue;
       last = splits;
+      if (splits > 1 && kLaunch + kCutLaunch + tile.round >= least) break;   // (whatever it is cut into)
       if (splits > 1 && (tiles * splits > (int64_t)cus * per_cu || partial_bytes(splits, M, N) > most_bytes)) break;
       const int64_t of_unit = splits > 1 ? ((int)tiles * splits + cus - 1) / cus : (tiles + cus - 1) / cus;
       const float share = (float)of_unit, rounds = (float)((of_unit + per_cu - 1) / per_cu);
@@ -612,11 +618,6 @@ Plan choose_plan(int M, int N, int K, int cus, bool limited, size_t most_bytes) 
         best = Plan{t, splits, per};
       }
     }
-  }
-  if (M <= kFewRowsMost && !limited) {
-    const float groups = std::max(1.f, (float)((N + 15) / 16) / cus), rows = 16.f + (M == 1 ? 1.f : 16.f * ((M + 15) / 16));
-    const float us = 1.5f + std::max(groups * K * rows / 33.6e3f, (float)N * K / 5.5e6f);
-    if (us < least) best = Plan{kFewRows, 1, ksteps};
   }
   return best;
 }
