@@ -180,6 +180,53 @@ def test_one_stream_step_in_a_graph():
             assert torch.equal(model(sets[0][0]), want[0])
 
 
+@on_gpu
+def test_forward_and_backward_in_a_graph():
+    s, b, h = 96, 2, 512
+    sizes = dict(hidden_size=h, num_attention_heads=4, num_query_groups=2, kv_channels=128, ffn_hidden_size=768)
+    model = LayerStack(config("hip", torch.bfloat16, num_nanobatches=1, **sizes), device="cuda", seed=7)
+    weights = list(model.parameters())
+    sets = [batch(s, b, h, "cuda", torch.bfloat16, i) for i in range(3)]
+
+    def step(x, go):
+        return torch.autograd.grad(model(x), [x] + weights, go)
+
+    want = [[t.clone() for t in step(x.detach().clone().requires_grad_(True), go)] for x, go in sets]
+    held, held_go = sets[0][0].detach().clone().requires_grad_(True), sets[0][1].clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(held, held_go)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(held, held_go)
+    for r in range(4):
+        with torch.no_grad():
+            held.copy_(sets[r % 3][0])
+            held_go.copy_(sets[r % 3][1])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, c) for a, c in zip(out, want[r % 3]))
+        eager = step(sets[1][0].detach().clone().requires_grad_(True), sets[1][1])
+        assert all(torch.equal(a, c) for a, c in zip(eager, want[1]))
+
+
+@pytest.mark.parametrize("key,slot", [("fwd_attn", "attn_0"), ("fwd_mlp", "linear_0"), ("bwd_mlp", "linear_0"), ("bwd_attn", "attn_0")])
+@on_gpu
+def test_profiled_partitions(key, slot):
+    """A partition alone, run twice on the same saved tensors."""
+    from kareus_amd.profiling import PartitionTest
+
+    cfg = config("hip", torch.bfloat16, hidden_size=512, num_attention_heads=4, num_query_groups=2, kv_channels=128, ffn_hidden_size=768)
+    t = PartitionTest(key, cfg, 2, 128, device="cuda")
+    for _ in range(2):
+        grads = t.test_config((slot, "none"), (16, 1024))
+        torch.cuda.synchronize()
+        if key.startswith("bwd"):
+            assert all(g is None or g.isfinite().all() for op in grads.values() for g in op)
+
+
 # ---- model shards ------------------------------------------------------------------------------------
 def shard(backend, dtype, device=None, **kw):
     return GPTModelShard(config(backend, dtype, num_nanobatches=2), vocab_rows=104, device=device, seed=11, **kw)
