@@ -1137,13 +1137,27 @@ PyObject* py_quantize_blocks(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     int rc;
     {
       WithoutInterpreter free;
+      int64_t n[2], pitch[2], blocks[2], scales[2], size[2];
+      for (int i = 0; i < 2; ++i) {
+        n[i] = i ? o.cols : o.rows;
+        blocks[i] = blocks_of(i ? o.rows : o.cols);
+        pitch[i] = blocks[i] * 128;
+        scales[i] = (n[i] + 3) / 4 * 4;
+        size[i] = want[i] ? (n[i] * pitch[i] + blocks[i] * scales[i] + 255) / 256 * 256 : 0;
+      }
+      // an allocation per orientation, so that one is freed without the other; one for both up to 2 MB (5.0 us a call instead of 5.7)
+      const bool together = size[0] + size[1] <= (2 << 20);
+      Tensor buffer;
+      int64_t from = 0;
       for (int i = 0; i < 2; ++i) {
         if (!want[i]) continue;
-        const int64_t n = i ? o.cols : o.rows, k = i ? o.rows : o.cols;
-        const int64_t pitch = blocks_of(k) * 128, scales = (n + 3) / 4 * 4;
-        const Tensor both = bytes((size_t)(n * pitch + blocks_of(k) * scales), x);
-        t[2 * i] = part_of(both, at::kFloat8_e4m3fn, 0, n, pitch);
-        t[2 * i + 1] = part_of(both, at::kByte, n * pitch, blocks_of(k), scales);
+        if (!buffer.defined() || !together) {
+          buffer = bytes((size_t)(together ? size[0] + size[1] : size[i]), x);
+          from = 0;
+        }
+        t[2 * i] = part_of(buffer, at::kFloat8_e4m3fn, from, n[i], pitch[i]);
+        t[2 * i + 1] = part_of(buffer, at::kByte, from + n[i] * pitch[i], blocks[i], scales[i]);
+        from += size[i];
       }
       auto at_ = [&](int i) { return t[i].defined() ? ptr(t[i]) : nullptr; };
       auto ld = [&](int i) { return t[i].defined() ? t[i].size(1) : (int64_t)0; };
