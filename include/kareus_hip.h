@@ -468,7 +468,12 @@ int kr_embedding_bwd_sorted(const int64_t* ids, const void* dout, void* dweight,
  * rounded once.  Accumulators, cuts and the sum with C are fp32; of the products of eight consecutive contraction elements the matrix
  * unit drops, towards zero, what lies below 2^-13 of the largest sum of two exponents among them.  N, ldc: multiples of 8; M and K:
  * any.  max_cus > 0 limits the launch to that many compute units.  workspace: NULL or kr_block_gemm_workspace_bytes() bytes (16-byte aligned): with it a product of few tiles and a long
- * contraction is cut along K; a smaller one is not used.                                              */
+ * contraction is cut along K; a smaller one is not used.
+ *
+ * kr_block_gemm_segments: C = sum over i of A_i . B_i^T in one launch, one fp32 sum over all of them and one rounding (the gradient of a
+ * weight over several microbatches or parts of one): nseg (1 to 16) pairs of operands with M and N rows, the i-th K[i] long, each as
+ * above with its own strides.  The workspace's query takes the blocks of 128 of all of them, sum of ceil(K[i] / 128).  The arrays are
+ * read before the call returns.                                                                        */
 int kr_block_quantize(const void* x, int rows, int cols, int64_t ld, int run_rows, int64_t run_ld, int tiles,
                       void* q, int64_t ldq, void* s, int64_t lds, void* qt, int64_t ldqt, void* st, int64_t ldst,
                       void* stream);
@@ -476,6 +481,11 @@ size_t kr_block_gemm_workspace_bytes(int M, int N, int K, int max_cus);
 int kr_block_gemm(int M, int N, int K, const void* A, int64_t lda, const void* sa, int64_t lsa,
                   const void* B, int64_t ldb, const void* sb, int64_t lsb, void* C, int64_t ldc, int accumulate,
                   int max_cus, void* workspace, size_t workspace_bytes, void* stream);
+#define KR_BLOCK_GEMM_MAX_SEGMENTS 16
+size_t kr_block_gemm_segments_workspace_bytes(int M, int N, int blocks, int max_cus);
+int kr_block_gemm_segments(int M, int N, int nseg, const int* K, const void* const* A, const int64_t* lda, const void* const* sa,
+                           const int64_t* lsa, const void* const* B, const int64_t* ldb, const void* const* sb, const int64_t* lsb,
+                           void* C, int64_t ldc, int max_cus, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

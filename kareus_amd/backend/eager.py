@@ -315,6 +315,14 @@ class EagerBackend:
             return c.to(dtype)
         return out.copy_(out.float() + c if accumulate else c)
 
+    def block_matmul_segments(self, a, b, out: Tensor = None, dtype: torch.dtype = torch.bfloat16) -> Tensor:
+        """``sum_i a[i] . b[i]^T``, rounded once."""
+        total = None
+        for x, y in zip(a, b):
+            c = self.block_matmul(x, y, dtype=torch.float32)
+            total = c if total is None else total + c
+        return total.to(dtype) if out is None else out.copy_(total)
+
     def embedding_bwd(self, ids: Tensor, dout: Tensor, vocab_rows: int, vocab_start: int = 0) -> Tensor:
         rel = (ids - vocab_start).transpose(0, 1).reshape(-1)          # [s, b] order like dout
         keep = (rel >= 0) & (rel < vocab_rows)

@@ -84,6 +84,8 @@ _SIGNATURES = {
     "kr_embedding_bwd_sorted": (_c_int, [_c_void_p] * 3 + [_c_int] * 4 + [_c_i64, _c_i64, _c_float, _c_int, _c_void_p, _c_size_t, _c_void_p]),
     "kr_block_quantize": (_c_int, [_c_void_p, _c_int, _c_int, _c_i64, _c_int, _c_i64, _c_int] + [_c_void_p, _c_i64] * 4 + [_c_void_p]),
     "kr_block_gemm_workspace_bytes": (_c_size_t, [_c_int] * 4),
+    "kr_block_gemm_segments_workspace_bytes": (_c_size_t, [_c_int] * 4),
+    "kr_block_gemm_segments": (_c_int, [_c_int] * 3 + [_c_void_p] * 10 + [_c_i64, _c_int, _c_void_p, _c_size_t, _c_void_p]),
     "kr_block_gemm": (_c_int, [_c_int] * 3 + [_c_void_p, _c_i64] * 5 + [_c_int, _c_int, _c_void_p, _c_size_t, _c_void_p]),
 }
 
@@ -513,6 +515,12 @@ class HipBackend:
             raise RuntimeError(f"block_matmul: {tuple(s.shape)} scales with strides {s.stride()} for {d.shape[0]} rows in "
                                f"{blocks_of(t.length)} blocks")
 
+    def _block_out(self, out: Tensor, m: int, n: int, name: str) -> None:
+        self._dev(out)
+        self._bf16(out)
+        if tuple(out.shape) != (m, n) or (out.numel() and out.stride(1) != 1):
+            raise RuntimeError(f"{name}: out must be [{m}, {n}] with a contiguous last dimension")
+
     def block_matmul(self, a: BlockOperand, b: BlockOperand, out: Tensor = None, accumulate: bool = False,
                      dtype: torch.dtype = torch.bfloat16) -> Tensor:
         """``a . b^T`` of two operands in 8-bit blocks over the same contraction, [a.rows, b.rows] in bf16 with fp32 sums:
@@ -539,10 +547,7 @@ class HipBackend:
                 raise RuntimeError("block_matmul: accumulate needs the matrix to add to")
             out = torch.empty((m, n), dtype=dtype, device=a.data.device)
         else:
-            self._dev(out)
-            self._bf16(out)
-            if tuple(out.shape) != (m, n) or (out.numel() and out.stride(1) != 1):
-                raise RuntimeError(f"block_matmul: out must be [{m}, {n}] with a contiguous last dimension")
+            self._block_out(out, m, n, "block_matmul")
         self._same_device("block_matmul", a.data, a.scales, b.data, b.scales, out)
         if not m or not n:
             return out
@@ -557,6 +562,64 @@ class HipBackend:
                                         None if ws is None else ws.data_ptr(), nbytes, self._stream())
         self._check(rc, f"kr_block_gemm(M={m}, N={n}, K={k})")
         return out
+
+    MAX_BLOCK_SEGMENTS = 16   # KR_BLOCK_GEMM_MAX_SEGMENTS
+
+    def block_matmul_segments(self, a, b, out: Tensor = None, dtype: torch.dtype = torch.bfloat16) -> Tensor:
+        """``sum_i a[i] . b[i]^T`` of pairs of operands in 8-bit blocks, the rows of all ``a`` alike and those of all ``b``, in bf16: one
+        launch, one sum over all pairs and one rounding.  The weight gradient over the nanobatches of a pass."""
+        if len(a) != len(b) or not len(a):
+            raise RuntimeError(f"block_matmul_segments: {len(a)} and {len(b)} operands")
+        max_cus = 0
+        reserved = reserved_compute_units()
+        if reserved and a[0].data.is_cuda:
+            max_cus = max(self._num_cus(a[0].data.device) - reserved, 8)
+        if dtype == torch.bfloat16 and type(a) is list and type(b) is list:
+            done = self._n.block_matmul_segments(a, b, out, max_cus)
+            if done is not None:
+                return done
+        if dtype != torch.bfloat16:
+            raise RuntimeError(f"the hip backend computes in bf16, got {dtype}")
+        m, n = a[0].rows, b[0].rows
+        for x, y in zip(a, b):
+            self._block_operand(x)
+            self._block_operand(y)
+            if x.length != y.length:
+                raise RuntimeError(f"block_matmul_segments: contractions of {x.length} and {y.length}")
+            if x.rows != m or y.rows != n:
+                raise RuntimeError(f"block_matmul_segments: operands of {x.rows} and {y.rows} rows behind {m} and {n}")
+        if out is None:
+            out = torch.empty((m, n), dtype=dtype, device=a[0].data.device)
+        else:
+            self._block_out(out, m, n, "block_matmul_segments")
+        self._same_device("block_matmul_segments", out, *[t for o in (*a, *b) for t in (o.data, o.scales)])
+        pairs = [(x, y) for x, y in zip(a, b) if x.length]
+        if not m or not n or not pairs:
+            return out.zero_()
+        with self._current(out):
+            while len(pairs) > self.MAX_BLOCK_SEGMENTS:     # (the last ones side by side, as one pair)
+                cut = self.MAX_BLOCK_SEGMENTS - 1
+                pairs[cut:] = [tuple(self._side_by_side(ops) for ops in zip(*pairs[cut:]))]
+            nseg = len(pairs)
+            table = []
+            for ops in zip(*pairs):
+                for tensors in ([o.data for o in ops], [o.scales for o in ops]):
+                    table.append((_c_void_p * nseg)(*[t.data_ptr() for t in tensors]))
+                    table.append((_c_i64 * nseg)(*[self._pitch(t) for t in tensors]))
+            blocks = sum(blocks_of(x.length) for x, _ in pairs)
+            nbytes = self.lib.kr_block_gemm_segments_workspace_bytes(m, n, blocks, max_cus)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=out.device) if nbytes else None
+            rc = self.lib.kr_block_gemm_segments(m, n, nseg, (_c_int * nseg)(*[x.length for x, _ in pairs]), *table, out.data_ptr(), self._pitch(out),
+                                                 max_cus,                                                 None if ws is None else ws.data_ptr(), nbytes, self._stream())
+        self._check(rc, f"kr_block_gemm_segments(M={m}, N={n}, blocks={blocks}, nseg={nseg})")
+        return out
+
+    @staticmethod
+    def _side_by_side(ops) -> BlockOperand:
+        """The operands' contractions one behind the other, each in whole blocks."""
+        return BlockOperand(torch.cat([o.data[:, :blocks_of(o.length) * 128].view(torch.uint8) for o in ops], 1).view(torch.float8_e4m3fn),
+                            torch.cat([torch.nn.functional.pad(o.scales[:blocks_of(o.length), :o.rows], (0, -o.rows % 4)) for o in ops]),
+                            sum(blocks_of(o.length) * 128 for o in ops))
 
     @staticmethod
     def _pitch(t: Tensor) -> int:

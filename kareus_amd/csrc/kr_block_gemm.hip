@@ -47,6 +47,13 @@ struct Args {
   int lsa, lsb;            // bytes from one scale block's row to the next (multiples of 4)
   int m, n, ksteps, steps_per, splits;
 };
+// The pieces that a contraction lies in, one behind the other, each of whole blocks (Args: m, n, ksteps of all of them, the output)
+constexpr int kMostSegments = KR_BLOCK_GEMM_MAX_SEGMENTS;
+struct Segments {
+  const uint8_t *a[kMostSegments], *sa[kMostSegments], *b[kMostSegments], *sb[kMostSegments];
+  int lda[kMostSegments], ldb[kMostSegments], lsa[kMostSegments], lsb[kMostSegments], ksteps[kMostSegments];
+};
+struct OnePiece {};
 
 __device__ __forceinline__ uint32_t lds_addr(const uint8_t* p) { return (uint32_t)(uintptr_t)(KR_LDS const uint8_t*)p; }
 
@@ -115,13 +122,16 @@ constexpr size_t lds_bytes(int wt, int wn) {
 //   * The barrier stands in front of a phase's last MFMAs, which run while the waves meet.
 //   * A block's row is 64 bytes, its 16-byte chunks XORed with (row >> 2) & 3: the 16 rows that a fragment read takes at a time cover
 //     all banks once.  Both halves of a row's 128 bytes are requested one behind the other: one line fetched from the L2.
-template <int WT, int WN, int OUT>
-__global__ __launch_bounds__(NTHREADS, WT * WN == 1 ? 3 : WT * WN == 4 ? 2 : 1) void block_gemm_kernel(Args g) {
+//   * A contraction in pieces (Segments) moves the requests from one piece's operands to the next's between two K-steps; the computation
+//     does not know of it.
+template <int WT, int WN, int OUT, class Contraction>
+__global__ __launch_bounds__(NTHREADS, WT * WN == 1 ? 3 : WT * WN == 4 ? 2 : 1) void block_gemm_kernel(Args g, Contraction pieces) {
 #ifdef __HIP_DEVICE_COMPILE__   // (the host's pass over this file cannot place the registers that the assembly names)
   constexpr int BM = 64 * WT, BN = 64 * WN;
   constexpr int NA = 2 * WT, NB = 2 * WN;                       // loads per wave of an operand's K-step, both halves
   constexpr uint32_t BLK = block_bytes(WT > WN ? WT : WN);
   constexpr int SLOTS = WT * WN;                                // MFMAs of a phase
+  constexpr bool SEGMENTS = std::is_same_v<Contraction, Segments>;
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -153,13 +163,10 @@ __global__ __launch_bounds__(NTHREADS, WT * WN == 1 ? 3 : WT * WN == 4 ? 2 : 1) 
   int r_left;
   const uint8_t *ra, *rb, *rs;          // of the K-step to request next (wave-uniform); rs: the scales this wave loads
   uint32_t la[WT], lb[WN], ls;
-  const int64_t rs_step = wn ? g.lsb : g.lsa;
-  auto aim = [&](int v) {
-    const Item it = select(v);
-    r_left = it.nk;
-    ra = g.a + (int64_t)it.m0 * g.lda + (int64_t)it.k0 * BK;
-    rb = g.b + (int64_t)it.n0 * g.ldb + (int64_t)it.k0 * BK;
-    rs = (wn ? g.sb : g.sa) + (int64_t)it.k0 * rs_step;
+  int64_t rs_step = wn ? g.lsb : g.lsa;
+  int r_m0, r_n0, r_piece, r_left_piece;   // SEGMENTS
+  // rows of the tile at (m0, n0), `lda` and `ldb` bytes apart
+  auto address = [&](int m0, int n0, uint32_t lda, uint32_t ldb) {
     int l2 = lane;
     asm volatile("" : "+v"(l2));
     // load i of a wave fills block rows 16 (wave + 4 i) .. + 15; beyond the matrix: its last row (never stored)
@@ -170,24 +177,58 @@ __global__ __launch_bounds__(NTHREADS, WT * WN == 1 ? 3 : WT * WN == 4 ? 2 : 1) 
       const int row = 16 * (wave + 4 * i) + sub;
       const int w = row / (32 * WT), t = row % (32 * WT) / 32, j = row % 32;
       int r = 32 * WT * w + WT * j + t;
-      r = it.m0 + r < g.m ? r : g.m - 1 - it.m0;
-      la[i] = (uint32_t)r * (uint32_t)g.lda + (uint32_t)chunk;
+      r = m0 + r < g.m ? r : g.m - 1 - m0;
+      la[i] = (uint32_t)r * lda + (uint32_t)chunk;
     }
 #pragma unroll
     for (int i = 0; i < WN; ++i) {
       const int row = 16 * (wave + 4 * i) + sub;
       const int w = row / (32 * WN), t = row % (32 * WN) / 32, j = row % 32;
       int r = 32 * WN * w + WN * j + t;
-      r = it.n0 + r < g.n ? r : g.n - 1 - it.n0;
-      lb[i] = (uint32_t)r * (uint32_t)g.ldb + (uint32_t)chunk;
+      r = n0 + r < g.n ? r : g.n - 1 - n0;
+      lb[i] = (uint32_t)r * ldb + (uint32_t)chunk;
     }
     // four rows' scales a lane; beyond the matrix: those of its last row
-    const int sr = (wn ? it.n0 : it.m0) + 4 * l2, most = ((wn ? g.n : g.m) - 1) & ~3;
+    const int sr = (wn ? n0 : m0) + 4 * l2, most = ((wn ? g.n : g.m) - 1) & ~3;
     ls = (uint32_t)(sr < most ? sr : most);
+  };
+  auto enter = [&](int piece, int step) {   // (SEGMENTS: K-step `step` of a piece, for the tile at r_m0, r_n0)
+    if constexpr (SEGMENTS) {
+      r_piece = piece;
+      r_left_piece = pieces.ksteps[piece] - step;
+      const int lda = pieces.lda[piece], ldb = pieces.ldb[piece];
+      ra = pieces.a[piece] + (int64_t)r_m0 * lda + (int64_t)step * BK;
+      rb = pieces.b[piece] + (int64_t)r_n0 * ldb + (int64_t)step * BK;
+      rs_step = wn ? pieces.lsb[piece] : pieces.lsa[piece];
+      rs = (wn ? pieces.sb[piece] : pieces.sa[piece]) + (int64_t)step * rs_step;
+      address(r_m0, r_n0, (uint32_t)lda, (uint32_t)ldb);
+    }
+  };
+  auto aim = [&](int v) {
+    const Item it = select(v);
+    r_left = it.nk;
+    if constexpr (SEGMENTS) {
+      r_m0 = it.m0;
+      r_n0 = it.n0;
+      int piece = 0, step = it.k0;
+      while (step >= pieces.ksteps[piece]) step -= pieces.ksteps[piece++];
+      enter(piece, step);
+    } else {
+      ra = g.a + (int64_t)it.m0 * g.lda + (int64_t)it.k0 * BK;
+      rb = g.b + (int64_t)it.n0 * g.ldb + (int64_t)it.k0 * BK;
+      rs = (wn ? g.sb : g.sa) + (int64_t)it.k0 * rs_step;
+      address(it.m0, it.n0, (uint32_t)g.lda, (uint32_t)g.ldb);
+    }
   };
   // (behind the last item's last K-step it stays there: the K loop requests that one again rather than branch, two steps in all)
   auto advance = [&]() {
     if (--r_left > 0) {
+      if constexpr (SEGMENTS) {
+        if (--r_left_piece == 0) {
+          enter(r_piece + 1, 0);
+          return;
+        }
+      }
       ra += BK;
       rb += BK;
       rs += rs_step;
@@ -592,11 +633,12 @@ size_t partial_bytes(int splits, int M, int N) { return splits > 1 ? (size_t)spl
 //   * Few rows: a workgroup reads 16 rows of B and all of A, 33.6 GB/s per unit (us, 16 x 4096 x 4096 5.9 where tiles take 8.3, 64 x 4096
 //     x 4096 11.8 and 10.0, 1 x 28672 x 4096 24.9 and 18.7).
 // limited: the caller has named the units; a workgroup each, and no kernel that is not persistent.
-Plan choose_plan(int M, int N, int K, int cus, bool limited, size_t most_bytes) {
+// segments: the contraction lies in pieces, which the kernel for few rows does not know.
+Plan choose_plan(int M, int N, int K, int cus, bool limited, size_t most_bytes, bool segments = false) {
   const int ksteps = (K + BK - 1) / BK;
   Plan best{0, 1, ksteps};
   float least = INFINITY;
-  if (M <= kFewRowsMost && !limited) {
+  if (M <= kFewRowsMost && !limited && !segments) {
     const float groups = std::max(1.f, (float)((N + 15) / 16) / cus), rows = 16.f + (M == 1 ? 1.f : 16.f * ((M + 15) / 16));
     least = 1.5f + std::max(groups * K * rows / 33.6e3f, (float)N * K / 5.5e6f);
     best.tile = kFewRows;
@@ -633,18 +675,18 @@ int device_cus() {
   return n;
 }
 
-template <int T, int OUT>
-int launch(const Args& g, int cus, bool limited, hipStream_t stream) {
+template <int T, int OUT, class Contraction>
+int launch(const Args& g, const Contraction& pieces, int cus, bool limited, hipStream_t stream) {
   constexpr Tile t = kTiles[T];
   constexpr size_t lds = lds_bytes(t.wt, t.wn);
   static_assert(lds * t.per_cu <= 160 * 1024, "LDS of a compute unit");
-  static const hipError_t raised = hipFuncSetAttribute((const void*)block_gemm_kernel<t.wt, t.wn, OUT>,
+  static const hipError_t raised = hipFuncSetAttribute((const void*)block_gemm_kernel<t.wt, t.wn, OUT, Contraction>,
                                                        hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
   if (raised != hipSuccess) return KR_ELAUNCH;
   const int64_t tiles = (int64_t)((g.m + 64 * t.wt - 1) / (64 * t.wt)) * ((g.n + 64 * t.wn - 1) / (64 * t.wn)) * g.splits;
   if (tiles > 0x3fffffff) return KR_EUNSUPPORTED;
   const int64_t grid = std::min<int64_t>(tiles, (int64_t)cus * (limited ? 1 : t.per_cu));
-  hipLaunchKernelGGL((block_gemm_kernel<t.wt, t.wn, OUT>), dim3((unsigned)grid), dim3(NTHREADS), lds, stream, g);
+  hipLaunchKernelGGL((block_gemm_kernel<t.wt, t.wn, OUT, Contraction>), dim3((unsigned)grid), dim3(NTHREADS), lds, stream, g, pieces);
   return kr_launch_status();
 }
 
@@ -661,17 +703,25 @@ int launch_few_rows(const Args& g, int accumulate, hipStream_t stream) {
   return launch_few<4>(g, accumulate, stream);
 }
 
-template <int OUT>
-int launch_tile(const Plan& p, const Args& g, int cus, bool limited, hipStream_t stream) {
+template <int OUT, class Contraction>
+int launch_tile(const Plan& p, const Args& g, const Contraction& pieces, int cus, bool limited, hipStream_t stream) {
   switch (p.tile) {
-    case 0: return launch<0, OUT>(g, cus, limited, stream);
-    case 1: return launch<1, OUT>(g, cus, limited, stream);
-    case 2: return launch<2, OUT>(g, cus, limited, stream);
-    case 3: return launch<3, OUT>(g, cus, limited, stream);
-    case 4: return launch<4, OUT>(g, cus, limited, stream);
-    case 5: return launch<5, OUT>(g, cus, limited, stream);
+    case 0: return launch<0, OUT>(g, pieces, cus, limited, stream);
+    case 1: return launch<1, OUT>(g, pieces, cus, limited, stream);
+    case 2: return launch<2, OUT>(g, pieces, cus, limited, stream);
+    case 3: return launch<3, OUT>(g, pieces, cus, limited, stream);
+    case 4: return launch<4, OUT>(g, pieces, cus, limited, stream);
+    case 5: return launch<5, OUT>(g, pieces, cus, limited, stream);
   }
   return KR_EUNSUPPORTED;
+}
+
+int launch_reduce(const Plan& p, const Args& g, int accumulate, hipStream_t stream) {
+  const int64_t threads = (int64_t)g.m * (g.n / 8);
+  if ((threads + 255) / 256 > 0x7fffffff) return KR_EUNSUPPORTED;
+  hipLaunchKernelGGL(block_gemm_reduce_kernel, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, stream, g.partial, g.c, g.ldc, g.m, g.n,
+                     p.splits, accumulate);
+  return kr_launch_status();
 }
 
 }  // namespace
@@ -703,14 +753,59 @@ extern "C" int kr_block_gemm(int M, int N, int K, const void* A, int64_t lda, co
   Args g{(const uint8_t*)A, (const uint8_t*)sa, (const uint8_t*)B, (const uint8_t*)sb, (bf16*)C, (float*)workspace,
          lda, ldb, ldc, (int)lsa, (int)lsb, M, N, (K + BK - 1) / BK, p.steps_per, p.splits};
   if (p.tile == kFewRows) return launch_few_rows(g, accumulate, (hipStream_t)stream);
+  const hipStream_t st = (hipStream_t)stream;
   if (p.splits > 1) {
-    const int rc = launch_tile<kPartial>(p, g, cus, limited, (hipStream_t)stream);
-    if (rc != KR_OK) return rc;
-    const int64_t threads = (int64_t)M * (N / 8);
-    if ((threads + 255) / 256 > 0x7fffffff) return KR_EUNSUPPORTED;
-    hipLaunchKernelGGL(block_gemm_reduce_kernel, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, (hipStream_t)stream,
-                       (const float*)workspace, (bf16*)C, ldc, M, N, p.splits, accumulate);
-    return kr_launch_status();
+    const int rc = launch_tile<kPartial>(p, g, OnePiece{}, cus, limited, st);
+    return rc != KR_OK ? rc : launch_reduce(p, g, accumulate, st);
   }
-  return accumulate ? launch_tile<kAccumulate>(p, g, cus, limited, (hipStream_t)stream) : launch_tile<kStore>(p, g, cus, limited, (hipStream_t)stream);
+  return accumulate ? launch_tile<kAccumulate>(p, g, OnePiece{}, cus, limited, st) : launch_tile<kStore>(p, g, OnePiece{}, cus, limited, st);
+}
+
+extern "C" size_t kr_block_gemm_segments_workspace_bytes(int M, int N, int blocks, int max_cus) {
+  if (M <= 0 || N <= 0 || blocks <= 0 || blocks > 0x7fffffff / BK) return 0;
+  const int all = device_cus();
+  const bool limited = max_cus > 0 && max_cus < all;
+  return partial_bytes(choose_plan(M, N, blocks * BK, limited ? max_cus : all, limited, kMostWorkspace, true).splits, M, N);
+}
+
+extern "C" int kr_block_gemm_segments(int M, int N, int nseg, const int* K, const void* const* A, const int64_t* lda, const void* const* sa,
+                                      const int64_t* lsa, const void* const* B, const int64_t* ldb, const void* const* sb,
+                                      const int64_t* lsb, void* C, int64_t ldc, int max_cus, void* workspace, size_t workspace_bytes,
+                                      void* stream) {
+  if (!K || !A || !lda || !sa || !lsa || !B || !ldb || !sb || !lsb || !C || M <= 0 || N <= 0 || nseg <= 0) return KR_EINVAL;
+  if (nseg > kMostSegments || N % 8 || ldc % 8 || M > 0x7fffff00 || N > 0x7fffff00) return KR_EUNSUPPORTED;
+  if (ldc < N || !kr_aligned16(C) || !kr_aligned16(workspace)) return KR_EINVAL;
+  Segments pieces{};
+  int64_t blocks = 0;
+  for (int i = 0; i < nseg; ++i) {
+    if (!A[i] || !sa[i] || !B[i] || !sb[i] || K[i] <= 0) return KR_EINVAL;
+    if (lda[i] % 16 || ldb[i] % 16 || lsa[i] % 4 || lsb[i] % 4) return KR_EUNSUPPORTED;
+    const int64_t steps = ((int64_t)K[i] + BK - 1) / BK;
+    if (lda[i] < steps * BK || ldb[i] < steps * BK || lsa[i] < M || lsb[i] < N) return KR_EINVAL;
+    if (!kr_aligned16(A[i]) || !kr_aligned16(B[i]) || (reinterpret_cast<uintptr_t>(sa[i]) & 3) || (reinterpret_cast<uintptr_t>(sb[i]) & 3))
+      return KR_EINVAL;
+    if (lda[i] > (1 << 23) || ldb[i] > (1 << 23) || lsa[i] > 0x7fffffff || lsb[i] > 0x7fffffff) return KR_EUNSUPPORTED;
+    pieces.a[i] = (const uint8_t*)A[i];
+    pieces.sa[i] = (const uint8_t*)sa[i];
+    pieces.b[i] = (const uint8_t*)B[i];
+    pieces.sb[i] = (const uint8_t*)sb[i];
+    pieces.lda[i] = (int)lda[i];
+    pieces.ldb[i] = (int)ldb[i];
+    pieces.lsa[i] = (int)lsa[i];
+    pieces.lsb[i] = (int)lsb[i];
+    pieces.ksteps[i] = (int)steps;
+    blocks += steps;
+  }
+  if (blocks > 0x7fffffff / BK) return KR_EUNSUPPORTED;
+  const int all = device_cus();
+  const bool limited = max_cus > 0 && max_cus < all;
+  const int cus = limited ? max_cus : all;
+  const Plan p = choose_plan(M, N, (int)blocks * BK, cus, limited, workspace ? std::min(workspace_bytes, kMostWorkspace) : 0, true);
+  const Args g{nullptr, nullptr, nullptr, nullptr, (bf16*)C, (float*)workspace, 0, 0, ldc, 0, 0, M, N, (int)blocks, p.steps_per, p.splits};
+  const hipStream_t st = (hipStream_t)stream;
+  if (p.splits > 1) {
+    const int rc = launch_tile<kPartial>(p, g, pieces, cus, limited, st);
+    return rc != KR_OK ? rc : launch_reduce(p, g, 0, st);
+  }
+  return launch_tile<kStore>(p, g, pieces, cus, limited, st);
 }

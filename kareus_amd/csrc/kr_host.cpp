@@ -1194,6 +1194,15 @@ BlockRows block_rows(PyObject* data, PyObject* scales, int64_t k) {
   return r;
 }
 
+// an output of block products and its row stride
+bool block_out(PyObject* o, int64_t rows, int64_t cols, Tensor& out, int64_t& ld) {
+  if (!bf16_arg(o)) return false;
+  out = tensor(o);
+  if (!on_current_device(out) || out.dim() != 2 || out.size(0) != rows || out.size(1) != cols || out.stride(1) != 1) return false;
+  ld = rows > 1 ? out.stride(0) : cols;
+  return true;
+}
+
 // block_matmul(a data, a scales, b data, b scales, k, out, accumulate, max_cus)
 PyObject* py_block_matmul(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   return guarded([&]() -> PyObject* {
@@ -1208,10 +1217,7 @@ PyObject* py_block_matmul(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     if (absent(a[5])) {
       if (accumulate) return none();
     } else {
-      if (!bf16_arg(a[5])) return none();
-      out = tensor(a[5]);
-      if (!on_current_device(out) || out.dim() != 2 || out.size(0) != ra.rows || out.size(1) != rb.rows || out.stride(1) != 1) return none();
-      if (ra.rows > 1) ldc = out.stride(0);
+      if (!block_out(a[5], ra.rows, rb.rows, out, ldc)) return none();
     }
     const Tensor &da = tensor(a[0]), &sa = tensor(a[1]), &db = tensor(a[2]), &sb = tensor(a[3]);
     int rc;
@@ -1227,6 +1233,61 @@ PyObject* py_block_matmul(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     if (rc != KR_OK)
       return failed("kr_block_gemm(M=" + std::to_string(ra.rows) + ", N=" + std::to_string(rb.rows) + ", K=" + std::to_string(k) + ")", rc);
     return absent(a[5]) ? wrap(std::move(out)) : Py_NewRef(a[5]);
+  });
+}
+
+// block_matmul_segments([(data, scales, k), ..], [(data, scales, k), ..], out, max_cus): sum of the pairs' products
+PyObject* py_block_matmul_segments(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  return guarded([&]() -> PyObject* {
+    constexpr int most = KR_BLOCK_GEMM_MAX_SEGMENTS;
+    if (n_args != 4 || !PyList_Check(a[0]) || !PyList_Check(a[1])) return none();
+    const Py_ssize_t nseg = PyList_GET_SIZE(a[0]);
+    if (nseg < 1 || nseg > most || PyList_GET_SIZE(a[1]) != nseg) return none();
+    const int max_cus = (int)integer(a[3]);
+    Tensor held[4 * most];   // the lists may change while the interpreter is free
+    const void* p[4][most];
+    int64_t ld[4][most], m = 0, n = 0, blocks = 0;
+    int k[most];
+    for (Py_ssize_t i = 0; i < nseg; ++i) {
+      PyObject* const pair[2] = {PyList_GET_ITEM(a[0], i), PyList_GET_ITEM(a[1], i)};
+      if (!PyTuple_Check(pair[0]) || !PyTuple_Check(pair[1]) || PyTuple_GET_SIZE(pair[0]) != 3 || PyTuple_GET_SIZE(pair[1]) != 3) return none();
+      const int64_t length = integer(PyTuple_GET_ITEM(pair[0], 2));
+      if (integer(PyTuple_GET_ITEM(pair[1], 2)) != length || !fits_int(length)) return none();
+      for (int o = 0; o < 2; ++o) {
+        PyObject *data = PyTuple_GET_ITEM(pair[o], 0), *scales = PyTuple_GET_ITEM(pair[o], 1);
+        const BlockRows r = block_rows(data, scales, length);
+        int64_t& rows = o ? n : m;
+        if (!r.ok || !fits_int(r.rows) || (i != 0 && r.rows != rows)) return none();
+        rows = r.rows;
+        held[4 * i + 2 * o] = tensor(data);
+        held[4 * i + 2 * o + 1] = tensor(scales);
+        p[2 * o][i] = ptr(held[4 * i + 2 * o]);
+        p[2 * o + 1][i] = ptr(held[4 * i + 2 * o + 1]);
+        ld[2 * o][i] = r.ld;
+        ld[2 * o + 1][i] = r.lds;
+      }
+      k[i] = (int)length;
+      blocks += blocks_of(length);
+    }
+    if (n % 8 || !fits_int(blocks)) return none();
+    Tensor out;
+    int64_t ldc = n;
+    if (!absent(a[2]) && !block_out(a[2], m, n, out, ldc)) return none();
+    int rc;
+    {
+      WithoutInterpreter free;
+      if (!out.defined()) out = at::empty({m, n}, held[0].options().dtype(at::kBFloat16));
+      const size_t ws_bytes = kr_block_gemm_segments_workspace_bytes((int)m, (int)n, (int)blocks, max_cus);
+      Tensor ws;
+      if (ws_bytes) ws = bytes(ws_bytes, held[0]);
+      rc = kr_block_gemm_segments((int)m, (int)n, (int)nseg, k, p[0], ld[0], p[1], ld[1], p[2], ld[2], p[3], ld[3], ptr(out), ldc, max_cus,
+                                  ws_bytes ? ptr(ws) : nullptr, ws_bytes, stream());
+    }
+    if (rc != KR_OK)
+      return failed("kr_block_gemm_segments(M=" + std::to_string(m) + ", N=" + std::to_string(n) + ", blocks=" + std::to_string(blocks) +
+                        ", nseg=" + std::to_string(nseg) + ")",
+                    rc);
+    return absent(a[2]) ? wrap(std::move(out)) : Py_NewRef(a[2]);
   });
 }
 
@@ -1334,6 +1395,7 @@ PyMethodDef kMethods[] = {
     {"rmsnorm_dgamma", (PyCFunction)(void*)py_rmsnorm_dgamma, METH_FASTCALL, nullptr},
     {"quantize_blocks", (PyCFunction)(void*)py_quantize_blocks, METH_FASTCALL, nullptr},
     {"block_matmul", (PyCFunction)(void*)py_block_matmul, METH_FASTCALL, nullptr},
+    {"block_matmul_segments", (PyCFunction)(void*)py_block_matmul_segments, METH_FASTCALL, nullptr},
     {"embedding_fwd_scaled", (PyCFunction)(void*)py_embedding_fwd_scaled, METH_FASTCALL, nullptr},
     {"embedding_bwd_sorted", (PyCFunction)(void*)py_embedding_bwd_sorted, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},

@@ -6,6 +6,7 @@ saved is what the backward reads: the input's columns and the weight's columns i
 reference's layers take the same place with TransformerEngine quantizers
 (kareus/transformer_engine/pytorch/ops/basic/basic_linear.py:391-604, 606-915).
 
+The weight gradient over the nanobatches of a pass is one product over all their tokens, launched where ``linear.py`` launches its own.
 A pass quantises a weight once: the first nanobatch to get to the layer does, the others of the pass read its result.  The residual add
 and the SwiGLU activation behind and in front of the layers run as operators of their own.
 """
@@ -92,14 +93,22 @@ class BlockLinear(PartitionableLinear):
         return dx.view(*grad_output.shape[:-1], k), (dw,)
 
     def _block_weight_grad(self, be, ctx, dy: BlockOperand, x: BlockOperand):
-        """``dW = dy^T . x``.  With the engine's ``wgrad_sink`` (see ``PartitionableLinear._weight_grad``) the nanobatches' products are
-        added up in one tensor, each rounded to the weight's type: the first nanobatch allocates it, later ones add to it behind the
-        one before them."""
+        """``dW = dy^T . x``.  With the engine's ``wgrad_sink`` (see ``PartitionableLinear._weight_grad``) the nanobatches' operands are
+        contracted in one launch, with one fp32 sum and one rounding.  Where the layer's configuration asks for a product per nanobatch
+        (``wgrad_over_all_nanobatches`` off), the first allocates the gradient and later ones add to it, rounding it to its type
+        each time, as the bf16 layers do there."""
         sink = getattr(ctx, "wgrad_sink", None)
         if sink is None:
             return be.block_matmul(dy, x, dtype=self.weight.dtype)
         api = stream_api()
         here = None if sink.get("in_line") else api.current_stream()
+        if sink.get("n", 0) > 1 and sink.get("defer", True):
+            # (aliases: the engine drops the storage behind the saved tensor objects after each backward op)
+            return self._over_all_nanobatches(
+                sink, ctx, here, dy, x._replace(data=x.data.detach(), scales=x.scales.detach()),
+                lambda dys, xs: self.weight.new_empty(self.weight.shape),
+                lambda dys, xs, dw: be.block_matmul_segments(dys, xs, out=dw, dtype=dw.dtype),
+                lambda pair: (t for o in pair for t in (o.data, o.scales)))
         buf = sink.get("buf")
         if buf is None:
             ret = sink["buf"] = be.block_matmul(dy, x, dtype=self.weight.dtype)

@@ -196,57 +196,22 @@ class PartitionableLinear(BasicOperation, PartitionableOperator):
             return be.linear_wgrad(dy, x2d, split_k=split_k)
         api = stream_api()
         here = None if sink.get("in_line") else api.current_stream()
-        n = sink.get("n", 0)
-        if n > 1 and sink.get("defer", True) and hasattr(be, "linear_wgrad_segments"):
-            ev = None
-            if here is not None:
-                ev = api.new_event()
-                ev.record(here)
-            pairs = sink.setdefault("pairs", [])
+        if sink.get("n", 0) > 1 and sink.get("defer", True) and hasattr(be, "linear_wgrad_segments"):
+            def product(dys, xs, dw):
+                if be.wgrad_segments_ok(dys, xs):
+                    # planned as a GEMM that has the device to itself (cuts of the contraction where the
+                    # output has few tiles): the products of the other nanobatches, which used to fill the
+                    # device beside each other, are inside it
+                    be.linear_wgrad_segments(dys, xs, out=dw, split_k=PartitionableLinear.wgrad_over_all_split_k)
+                else:
+                    be.linear_wgrad(dys[0], xs[0], out=dw, split_k=split_k)
+                    for d, x in zip(dys[1:], xs[1:]):
+                        be.linear_wgrad(d, x, out=dw, accumulate=True, split_k=split_k)
+
             # (aliases: the engine drops the storage behind the saved tensor objects after each backward op)
-            pairs.append((getattr(ctx, "nanobatch_index", len(pairs)), dy.detach(), x2d.detach(), ev, here))
-            if len(pairs) < n:
-                return None
-            pairs.sort(key=lambda p: p[0])
-            sink["pairs"] = None
-            pending = sink.get("pending")
-            turn = sink.get("turn")
-            if turn is None:
-                turn = [0]
-            # launched at once, the launches of a backward pass take the nanobatch streams in rotation; put off
-            # to the end of the pass they all go to the first nanobatch's stream, one after the other
-            target = pairs[0 if pending is not None else turn[0] % n][4]
-            turn[0] += 1
-            dys, xs = [p[1] for p in pairs], [p[2] for p in pairs]
-            with api.stream(target):
-                dw = dys[0].new_empty((dys[0].shape[-1], xs[0].shape[-1]))
-
-            def launch():
-                with api.stream(target):
-                    if target is not None:
-                        for _, _, _, ready, st in pairs:
-                            if ready is not None and st != target:
-                                target.wait_event(ready)
-                    if be.wgrad_segments_ok(dys, xs):
-                        # planned as a GEMM that has the device to itself (cuts of the contraction where the
-                        # output has few tiles): the products of the other nanobatches, which used to fill the
-                        # device beside each other, are inside it
-                        be.linear_wgrad_segments(dys, xs, out=dw, split_k=PartitionableLinear.wgrad_over_all_split_k)
-                    else:
-                        be.linear_wgrad(dys[0], xs[0], out=dw, split_k=split_k)
-                        for d, x in zip(dys[1:], xs[1:]):
-                            be.linear_wgrad(d, x, out=dw, accumulate=True, split_k=split_k)
-                    if target is not None:
-                        # the operands were allocated on their own nanobatch's stream
-                        for t in dys + xs:
-                            if t.is_cuda:
-                                t.record_stream(target)
-
-            if pending is not None:
-                pending.append(launch)
-            else:
-                launch()
-            return dw
+            return PartitionableLinear._over_all_nanobatches(
+                sink, ctx, here, dy.detach(), x2d.detach(),
+                lambda dys, xs: dys[0].new_empty((dys[0].shape[-1], xs[0].shape[-1])), product, lambda pair: pair)
         buf = sink.get("buf")
         if buf is None:
             buf = sink["buf"] = be.linear_wgrad(dy, x2d, split_k=split_k)
@@ -261,6 +226,55 @@ class PartitionableLinear(BasicOperation, PartitionableOperator):
             ev.record(here)
             sink["event"] = ev
         return ret
+
+    @staticmethod
+    def _over_all_nanobatches(sink, ctx, here, dy, x, allocate, product, tensors):
+        """Leaves a nanobatch's operands of the weight gradient in the sink; the last nanobatch to get here has
+        ``product(dys, xs, dw)`` launched on those of all, in nanobatch order, and returns ``dw = allocate(dys, xs)``, the others
+        None.  ``tensors((dy, x))``: what the two hold on the device."""
+        api = stream_api()
+        n = sink["n"]
+        ev = None
+        if here is not None:
+            ev = api.new_event()
+            ev.record(here)
+        pairs = sink.setdefault("pairs", [])
+        pairs.append((getattr(ctx, "nanobatch_index", len(pairs)), dy, x, ev, here))
+        if len(pairs) < n:
+            return None
+        pairs.sort(key=lambda p: p[0])
+        sink["pairs"] = None
+        pending = sink.get("pending")
+        turn = sink.get("turn")
+        if turn is None:
+            turn = [0]
+        # launched at once, the launches of a backward pass take the nanobatch streams in rotation; put off
+        # to the end of the pass they all go to the first nanobatch's stream, one after the other
+        target = pairs[0 if pending is not None else turn[0] % n][4]
+        turn[0] += 1
+        dys, xs = [p[1] for p in pairs], [p[2] for p in pairs]
+        with api.stream(target):
+            dw = allocate(dys, xs)
+
+        def launch():
+            with api.stream(target):
+                if target is not None:
+                    for _, _, _, ready, st in pairs:
+                        if ready is not None and st != target:
+                            target.wait_event(ready)
+                product(dys, xs, dw)
+                if target is not None:
+                    # the operands were allocated on their own nanobatch's stream
+                    for pair in zip(dys, xs):
+                        for t in tensors(pair):
+                            if t.is_cuda:
+                                t.record_stream(target)
+
+        if pending is not None:
+            pending.append(launch)
+        else:
+            launch()
+        return dw
 
     def __repr__(self) -> str:
         return (f"{type(self).__name__}(in_features={self.weight.shape[1]}, "
