@@ -2,13 +2,15 @@
 
 ``y = x . W^T``, ``dx = dy . W`` and ``dW = dy^T . x`` as in ``linear.py``, each of ``x``, ``dy`` (a scale per 128 elements along the
 contraction) and ``W`` (a scale per 128 x 128 tile) rounded to e4m3 on its way in; sums in fp32, results in the parameters' type.  What is
-saved is what the backward reads: the input's columns and the weight's columns in 8-bit blocks, half the bytes of the bf16 input.  The
-reference's layers take the same place with TransformerEngine quantizers
+saved is what the backward reads: the input's columns and the weight's columns in 8-bit blocks, a byte for each element of either (the
+bf16 layers save two for each of the input), and for matrices that take at most 2 MB in both orientations the rows' as well, which lie in
+the same allocation.  The reference's layers take the same place with TransformerEngine quantizers
 (kareus/transformer_engine/pytorch/ops/basic/basic_linear.py:391-604, 606-915).
 
 The weight gradient over the nanobatches of a pass is one product over all their tokens, launched where ``linear.py`` launches its own.
-A pass quantises a weight once: the first nanobatch to get to the layer does, the others of the pass read its result.  The residual add
-and the SwiGLU activation behind and in front of the layers run as operators of their own.
+A pass quantises a weight once: the first nanobatch to get to the layer does, the others of the pass read its result, and the last one
+drops the rows' orientation; the columns are saved for the backward.  The residual add and the SwiGLU activation behind and in front of
+the layers run as operators of their own.
 """
 
 from __future__ import annotations
@@ -44,9 +46,13 @@ class BlockLinear(PartitionableLinear):
                 if here is not None:
                     ready = api.new_event()
                     ready.record(here)
-                shared[id(self)] = (blocks, ready, here)
+                shared[id(self)] = [blocks, ready, here, shared.readers - 1]
             return blocks, here
-        blocks, ready, where = entry
+        blocks, ready, where, left = entry
+        if left == 1:
+            del shared[id(self)]    # (the memory is the streams' that were asked to read it until they have)
+        else:
+            entry[3] = left - 1
         if here is not None and ready is not None and where != here:
             here.wait_event(ready)
             for t in blocks:

@@ -25,7 +25,7 @@ from typing import Dict, List, Optional, Sequence
 import torch
 from torch import Tensor
 
-from .context_manager import NanoBatchContext, TensorStore
+from .context_manager import NanoBatchContext, PassShared, TensorStore
 from .streams import stream_api
 from .tensor_graph import TensorGraph
 
@@ -78,6 +78,11 @@ def _chains(config) -> bool:
     from ..operators.chains import chains_allowed
 
     return chains_allowed()
+
+
+def _shared(config, n: int) -> Optional[PassShared]:
+    """For what a pass makes once for all its nanobatches: weights in 8-bit blocks."""
+    return PassShared(n) if n > 1 and getattr(config, "linear_format", "bf16") != "bf16" else None
 
 
 def _scheduled(partitions) -> bool:
@@ -204,7 +209,7 @@ class TransformerBlockAutogradFunction(torch.autograd.Function):
         streams = [None] * n if in_line else _nanobatch_streams(config, n)
         chains = _chains(config)
         out_tid = fwd_graph.get_output_channel(seed.fwd_output_channel)
-        shared = {} if getattr(config, "linear_format", "bf16") != "bf16" else None   # (8-bit weights, quantised once a pass)
+        shared = _shared(config, n)
         ctxs = [NanoBatchContext(batch_idx=i, stream=streams[i], in_line=in_line, chains=chains, output_id=out_tid, shared=shared)
                 for i in range(n)]
         _seed_forward(ctxs, hs, rotary, mask, seed)
@@ -231,8 +236,6 @@ class TransformerBlockAutogradFunction(torch.autograd.Function):
         _fork(streams)
         _run_forward(fwd_parts, ctxs, schedule, is_grad_enabled)
         _join(streams)
-        if shared is not None:
-            shared.clear()
 
         outs = [c.tensor_store.get(out_tid) for c in ctxs]
 
@@ -289,7 +292,7 @@ class TransformerBlockAutogradFunction(torch.autograd.Function):
         _fork(streams)
         if func_ctx.checkpoint_activations:
             hs = func_ctx.saved_tensors
-            shared = {} if getattr(func_ctx.config, "linear_format", "bf16") != "bf16" else None
+            shared = _shared(func_ctx.config, n)
             ctxs = [NanoBatchContext(batch_idx=i, stream=streams[i], in_line=func_ctx.in_line, chains=chains, shared=shared)
                     for i in range(n)]
             _seed_forward(ctxs, hs, rotary, mask, seed)
@@ -301,8 +304,6 @@ class TransformerBlockAutogradFunction(torch.autograd.Function):
                 if func_ctx.fwd_cuda_rng_state is not None:
                     torch.cuda.set_rng_state(func_ctx.fwd_cuda_rng_state)
                 _run_forward(func_ctx.forward_partitions, ctxs, schedule, func_ctx.is_grad_enabled)
-            if shared is not None:
-                shared.clear()
             for c in ctxs:
                 c.finalize_recomputed_contexts()
         else:

@@ -61,6 +61,15 @@ class TensorStore:
                 self.set(port.tensor_id, tensor)
 
 
+class PassShared(dict):
+    """What the nanobatches of one forward (or recomputation) pass share, by operator.  ``readers``: how many they are; the last one to
+    take an entry drops it."""
+
+    def __init__(self, readers: int) -> None:
+        super().__init__()
+        self.readers = readers
+
+
 @dataclass
 class NanoBatchContext:
     """Everything one nanobatch carries across partitions.
@@ -84,8 +93,8 @@ class NanoBatchContext:
     output_id: Optional[str] = None
     # op_id -> tensor that op's forward output is to be written into (consumed when the op runs)
     output_sinks: Dict[int, torch.Tensor] = field(default_factory=dict)
-    # one dict for all nanobatches of a forward (or recomputation) pass, in which operators leave what they all read
-    shared: Optional[Dict[int, Any]] = None
+    # one for all nanobatches of a pass, in which operators leave what they all read (None: nothing does, or there is one nanobatch)
+    shared: Optional[PassShared] = None
     _saved_tensors: List[Optional[torch.Tensor]] = field(default_factory=list)
     _saved_ranges: Dict[int, Tuple[int, int]] = field(default_factory=dict)
 

@@ -32,7 +32,7 @@ class OperationContext:
     # no kernel of another nanobatch's stream runs beside this op's (NanoBatchContext.in_line)
     alone: bool = False
     # what the nanobatches of one pass share, by operator (NanoBatchContext.shared)
-    pass_shared: Optional[Dict[int, Any]] = None
+    pass_shared: Optional[Any] = None
 
     def save_for_backward(self, *tensors: Optional[torch.Tensor]) -> None:
         self.to_save = tensors

@@ -309,3 +309,36 @@ def test_backend_refuses_segments_on_the_device():
         be.block_matmul_segments([a], [b._replace(scales=b.scales[:1])])
     with pytest.raises(RuntimeError, match="kr_block_gemm_segments"):      # four columns: not a multiple of 8
         be.block_matmul_segments([b], [whole_operand(4, 200, 3, "cuda")[0]])
+
+
+# ---- a weight's blocks while a pass runs ----------------------------------------------------------------
+@pytest.mark.parametrize("grad", [False, True])
+@pytest.mark.parametrize("n,kw", [(1, dict()), (2, dict()), (4, dict()), (2, dict(checkpoint_activations=True)), (1, dict(checkpoint_activations=True))])
+def test_a_weights_rows_are_dropped_behind_its_last_nanobatch(monkeypatch, n, kw, grad):
+    """Six layers: at no time are the rows' orientations of more than two layers' four weights alive (nanobatches run less than a layer
+    apart), forward, recomputed and without gradients, and each weight is quantised once a pass."""
+    import weakref
+
+    be = get_backend("eager")
+    made, alive, passes = [], [], []
+    whole = be.quantize_blocks
+
+    def quantise(x, by_row=True, by_col=False, tiles=False):
+        got = whole(x, by_row, by_col, tiles)
+        if tiles:
+            made.append(weakref.ref(got.by_row.data))
+            alive.append(sum(r() is not None for r in made))
+        return got
+
+    monkeypatch.setattr(be, "quantize_blocks", quantise, raising=False)
+    model = LayerStack(config("eager", torch.float32, num_layers=6, num_nanobatches=n, **kw), seed=7)
+    x = torch.randn(8, 4, 256, generator=torch.Generator().manual_seed(1)).requires_grad_(grad)
+    with torch.set_grad_enabled(grad):
+        y = model(x)
+        passes.append(len(made))
+        assert all(r() is None for r in made)
+        if grad:
+            y.sum().backward()
+            passes.append(len(made))
+    assert passes == [24] + ([48 if kw else 24] if grad else [])
+    assert max(alive) <= (1 if n == 1 else 8)
