@@ -452,7 +452,8 @@ int kr_embedding_bwd_sorted(const int64_t* ids, const void* dout, void* dweight,
 /* ---- 8-bit blocks ----------------------------------------------------------------------------
  * A matrix operand in 8-bit blocks: e4m3 bytes [rows, ld], contiguous along the contraction (ld a multiple of 16, at least the
  * contraction rounded up to a multiple of 128; the bytes behind the contraction up to that multiple are read and must be 0), and
- * scale bytes, one per row and block of 128 contraction elements, block b's at s + b * lds (lds a multiple of 4, at least rows):
+ * scale bytes, one per row and block of 128 contraction elements, block b's at s + b * lds (s 4-byte aligned, lds a multiple of 4, at
+ * least rows; they are read four rows at a time, so that up to three bytes behind the last block's rows belong to the buffer):
  * an element stands for value * 2^(scale - 127).  The quantised operands of the reference's linear layers (quantizer arguments of
  * kareus/transformer_engine/pytorch/ops/basic/basic_linear.py:391-604).
  *

@@ -515,6 +515,17 @@ class HipBackend:
             raise RuntimeError(f"block_matmul: {tuple(s.shape)} scales with strides {s.stride()} for {d.shape[0]} rows in "
                                f"{blocks_of(t.length)} blocks")
 
+    @staticmethod
+    def _block_scales(t: BlockOperand) -> Tuple[Tensor, int]:
+        """An operand's scales where the kernels can read them, four rows at a time, and the bytes from one block's to the next's."""
+        s, rows, blocks = t.scales, t.rows, blocks_of(t.length)
+        read = (rows + 3) // 4 * 4
+        pitch = s.stride(0) if blocks > 1 else read     # (a single row may have any stride)
+        if (s.data_ptr() % 4 == 0 and pitch % 4 == 0 and pitch >= rows
+                and s.storage_offset() + (blocks - 1) * pitch + read <= s.untyped_storage().nbytes()):
+            return s, pitch
+        return torch.nn.functional.pad(s[:blocks, :rows], (0, read - rows)).contiguous(), read
+
     def _block_out(self, out: Tensor, m: int, n: int, name: str) -> None:
         self._dev(out)
         self._bf16(out)
@@ -556,10 +567,10 @@ class HipBackend:
         with self._current(out):
             nbytes = self.lib.kr_block_gemm_workspace_bytes(m, n, k, max_cus)
             ws = torch.empty(nbytes, dtype=torch.uint8, device=out.device) if nbytes else None
-            rc = self.lib.kr_block_gemm(m, n, k, a.data.data_ptr(), self._pitch(a.data), a.scales.data_ptr(), self._pitch(a.scales),
-                                        b.data.data_ptr(), self._pitch(b.data), b.scales.data_ptr(), self._pitch(b.scales),
-                                        out.data_ptr(), self._pitch(out), int(accumulate), max_cus,
-                                        None if ws is None else ws.data_ptr(), nbytes, self._stream())
+            (sa, lsa), (sb, lsb) = self._block_scales(a), self._block_scales(b)
+            rc = self.lib.kr_block_gemm(m, n, k, a.data.data_ptr(), self._block_pitch(a), sa.data_ptr(), lsa,
+                                        b.data.data_ptr(), self._block_pitch(b), sb.data_ptr(), lsb, out.data_ptr(), self._pitch(out),
+                                        int(accumulate), max_cus, None if ws is None else ws.data_ptr(), nbytes, self._stream())
         self._check(rc, f"kr_block_gemm(M={m}, N={n}, K={k})")
         return out
 
@@ -601,11 +612,13 @@ class HipBackend:
                 cut = self.MAX_BLOCK_SEGMENTS - 1
                 pairs[cut:] = [tuple(self._side_by_side(ops) for ops in zip(*pairs[cut:]))]
             nseg = len(pairs)
-            table = []
+            table, held = [], []
             for ops in zip(*pairs):
-                for tensors in ([o.data for o in ops], [o.scales for o in ops]):
+                scales = [self._block_scales(o) for o in ops]
+                held.append(scales)                         # (copies, until they have been asked for)
+                for tensors, pitches in (([o.data for o in ops], map(self._block_pitch, ops)), zip(*scales)):
                     table.append((_c_void_p * nseg)(*[t.data_ptr() for t in tensors]))
-                    table.append((_c_i64 * nseg)(*[self._pitch(t) for t in tensors]))
+                    table.append((_c_i64 * nseg)(*pitches))
             blocks = sum(blocks_of(x.length) for x, _ in pairs)
             nbytes = self.lib.kr_block_gemm_segments_workspace_bytes(m, n, blocks, max_cus)
             ws = torch.empty(nbytes, dtype=torch.uint8, device=out.device) if nbytes else None
@@ -620,6 +633,10 @@ class HipBackend:
         return BlockOperand(torch.cat([o.data[:, :blocks_of(o.length) * 128].view(torch.uint8) for o in ops], 1).view(torch.float8_e4m3fn),
                             torch.cat([torch.nn.functional.pad(o.scales[:blocks_of(o.length), :o.rows], (0, -o.rows % 4)) for o in ops]),
                             sum(blocks_of(o.length) * 128 for o in ops))
+
+    @staticmethod
+    def _block_pitch(t: BlockOperand) -> int:
+        return t.data.stride(0) if t.rows > 1 else blocks_of(t.length) * 128
 
     @staticmethod
     def _pitch(t: Tensor) -> int:

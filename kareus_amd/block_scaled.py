@@ -24,8 +24,9 @@ class BlockOperand(NamedTuple):
 
     ``data`` ``[rows, pitch]`` float8_e4m3fn, contiguous along the contraction, ``pitch`` a multiple of 16 and at least ``length``
     rounded up to a multiple of 128; the values from ``length`` to that multiple are read and have to be zero.
-    ``scales`` ``[blocks, >= rows]`` uint8, a row per block of 128 contraction elements, rows a multiple of 4 bytes apart; the value of
-    an element is ``data * 2^(scale - 127)``."""
+    ``scales`` ``[blocks, >= rows]`` uint8, a row per block of 128 contraction elements; the value of an element is
+    ``data * 2^(scale - 127)``.  Any rows of an operand are one, ``data[i:j]`` and ``scales[:, i:j]``; scales that do not begin at a
+    multiple of 4 bytes, are not a multiple of 4 apart or end with their storage within one are copied for a product."""
 
     data: Tensor
     scales: Tensor

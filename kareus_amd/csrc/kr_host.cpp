@@ -1187,10 +1187,12 @@ BlockRows block_rows(PyObject* data, PyObject* scales, int64_t k) {
   if (k <= 0 || d.numel() == 0 || d.stride(1) != 1 || d.size(1) < blocks_of(k) * 128 || s.numel() == 0 || s.stride(1) != 1 ||
       s.size(0) < blocks_of(k) || s.size(1) < d.size(0))
     return r;
+  const int64_t blocks = blocks_of(k), read = (d.size(0) + 3) / 4 * 4;   // (scales are read four rows at a time)
   r.rows = d.size(0);
-  r.ld = d.size(0) > 1 ? d.stride(0) : d.size(1);   // (a single row may have any stride)
-  r.lds = s.size(0) > 1 ? s.stride(0) : s.size(1);
-  r.ok = true;
+  r.ld = d.size(0) > 1 ? d.stride(0) : blocks * 128;                     // (a single row may have any stride)
+  r.lds = blocks > 1 ? s.stride(0) : read;
+  r.ok = r.lds % 4 == 0 && r.lds >= r.rows && ((uintptr_t)s.data_ptr() & 3) == 0 &&
+         s.storage_offset() + (blocks - 1) * r.lds + read <= (int64_t)s.storage().nbytes();   // (others are copied)
   return r;
 }
 
