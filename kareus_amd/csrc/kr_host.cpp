@@ -1191,8 +1191,9 @@ BlockRows block_rows(PyObject* data, PyObject* scales, int64_t k) {
   r.rows = d.size(0);
   r.ld = d.size(0) > 1 ? d.stride(0) : blocks * 128;                     // (a single row may have any stride)
   r.lds = blocks > 1 ? s.stride(0) : read;
-  r.ok = r.lds % 4 == 0 && r.lds >= r.rows && ((uintptr_t)s.data_ptr() & 3) == 0 &&
-         s.storage_offset() + (blocks - 1) * r.lds + read <= (int64_t)s.storage().nbytes();   // (others are copied)
+  // (others are copied)
+  r.ok = r.lds % 4 == 0 && r.lds >= r.rows && ((uintptr_t)s.const_data_ptr() & 3) == 0 &&
+         (read <= s.size(1) || s.storage_offset() + (blocks - 1) * r.lds + read <= (int64_t)s.storage().nbytes());
   return r;
 }
 
