@@ -562,47 +562,51 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void block_gemm_few_rows_kernel(Arg
 
 // C = bf16(sum of the cuts' fp32 partial products, in order [+ C]).  (The whole product, us, a cut's loads at a time and four cuts':
 // 75 x 608 x 17951 in twelve 13.2, 11.0; 91 x 272 x 3875 in sixteen 10.2, 7.0; 1536 x 2048 x 32768 in four 100, 100.)
+// STRIDED: for a caller that has named the units, a workgroup each; otherwise one piece a thread (75 x 608 x 17951 11.4 us, 11.8 with
+// the loop).
+template <bool STRIDED>
 __global__ __launch_bounds__(256) void block_gemm_reduce_kernel(const float* __restrict__ partial, bf16* __restrict__ C,
                                                                 int64_t ldc, int M, int N, int splits, int accumulate) {
   const int nv = N / 8;
-  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (idx >= (int64_t)M * nv) return;
-  const int m = (int)(idx / nv), n = (int)(idx % nv) * 8;
-  float acc[8];
+  for (int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x; idx < (int64_t)M * nv; idx += (int64_t)gridDim.x * 256) {
+    const int m = (int)(idx / nv), n = (int)(idx % nv) * 8;
+    float acc[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) acc[e] = 0.f;
-  const float* src = partial + (int64_t)m * N + n;
-  const int64_t step = (int64_t)M * N;
-  auto add = [&](auto count) {   // cuts whose loads are all asked for before the first is used
-    constexpr int U = decltype(count)::value;
-    f32x4 a[U], b[U];
+    for (int e = 0; e < 8; ++e) acc[e] = 0.f;
+    const float* src = partial + (int64_t)m * N + n;
+    const int64_t step = (int64_t)M * N;
+    auto add = [&](auto count) {   // cuts whose loads are all asked for before the first is used
+      constexpr int U = decltype(count)::value;
+      f32x4 a[U], b[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      a[u] = *reinterpret_cast<const f32x4*>(src);
-      b[u] = *reinterpret_cast<const f32x4*>(src + 4);
-      src += step;
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        acc[e] += a[u][e];
-        acc[4 + e] += b[u][e];
+      for (int u = 0; u < U; ++u) {
+        a[u] = *reinterpret_cast<const f32x4*>(src);
+        b[u] = *reinterpret_cast<const f32x4*>(src + 4);
+        src += step;
       }
-  };
-  int left = splits;
-  for (; left >= 4; left -= 4) add(Int<4>{});
-  for (; left > 0; --left) add(Int<1>{});
-  bf16* dst = C + (int64_t)m * ldc + n;
-  if (accumulate) {
-    const bf16x8 old = ldg8(dst);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) acc[e] += (float)old[e];
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          acc[e] += a[u][e];
+          acc[4 + e] += b[u][e];
+        }
+    };
+    int left = splits;
+    for (; left >= 4; left -= 4) add(Int<4>{});
+    for (; left > 0; --left) add(Int<1>{});
+    bf16* dst = C + (int64_t)m * ldc + n;
+    if (accumulate) {
+      const bf16x8 old = ldg8(dst);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] += (float)old[e];
+    }
+    bf16x8 o;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = (bf16)acc[e];
+    stg8(dst, o);
+    if constexpr (!STRIDED) return;
   }
-  bf16x8 o;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) o[e] = (bf16)acc[e];
-  stg8(dst, o);
 }
 
 // The tiles, and what a launch of them takes in us as measured (256 compute units): per round of workgroups, and per K-step, for each
@@ -632,7 +636,7 @@ size_t partial_bytes(int splits, int M, int N) { return splits > 1 ? (size_t)spl
 //     round: 1536 x 2048 x 32768 whole 159 us, in four pieces 100; 64 x 4096 x 4096 12 and 10; 1024 x 1024 x 1024 5 and 11.
 //   * Few rows: a workgroup reads 16 rows of B and all of A, 33.6 GB/s per unit (us, 16 x 4096 x 4096 5.9 where tiles take 8.3, 64 x 4096
 //     x 4096 11.8 and 10.0, 1 x 28672 x 4096 24.9 and 18.7).
-// limited: the caller has named the units; a workgroup each, and no kernel that is not persistent.
+// limited: the caller has named the units; a workgroup of each launch for each, and no kernel that takes more.
 // segments: the contraction lies in pieces, which the kernel for few rows does not know.
 Plan choose_plan(int M, int N, int K, int cus, bool limited, size_t most_bytes, bool segments = false) {
   const int ksteps = (K + BK - 1) / BK;
@@ -716,11 +720,11 @@ int launch_tile(const Plan& p, const Args& g, const Contraction& pieces, int cus
   return KR_EUNSUPPORTED;
 }
 
-int launch_reduce(const Plan& p, const Args& g, int accumulate, hipStream_t stream) {
-  const int64_t threads = (int64_t)g.m * (g.n / 8);
-  if ((threads + 255) / 256 > 0x7fffffff) return KR_EUNSUPPORTED;
-  hipLaunchKernelGGL(block_gemm_reduce_kernel, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, stream, g.partial, g.c, g.ldc, g.m, g.n,
-                     p.splits, accumulate);
+int launch_reduce(const Plan& p, const Args& g, int accumulate, int cus, bool limited, hipStream_t stream) {
+  const int64_t groups = ((int64_t)g.m * (g.n / 8) + 255) / 256;
+  const int64_t grid = std::min<int64_t>(groups, limited ? cus : 0x7fffffff);
+  hipLaunchKernelGGL((grid < groups ? block_gemm_reduce_kernel<true> : block_gemm_reduce_kernel<false>), dim3((unsigned)grid), dim3(256), 0,
+                     stream, g.partial, g.c, g.ldc, g.m, g.n, p.splits, accumulate);
   return kr_launch_status();
 }
 
@@ -756,7 +760,7 @@ extern "C" int kr_block_gemm(int M, int N, int K, const void* A, int64_t lda, co
   const hipStream_t st = (hipStream_t)stream;
   if (p.splits > 1) {
     const int rc = launch_tile<kPartial>(p, g, OnePiece{}, cus, limited, st);
-    return rc != KR_OK ? rc : launch_reduce(p, g, accumulate, st);
+    return rc != KR_OK ? rc : launch_reduce(p, g, accumulate, cus, limited, st);
   }
   return accumulate ? launch_tile<kAccumulate>(p, g, OnePiece{}, cus, limited, st) : launch_tile<kStore>(p, g, OnePiece{}, cus, limited, st);
 }
@@ -805,7 +809,7 @@ extern "C" int kr_block_gemm_segments(int M, int N, int nseg, const int* K, cons
   const hipStream_t st = (hipStream_t)stream;
   if (p.splits > 1) {
     const int rc = launch_tile<kPartial>(p, g, pieces, cus, limited, st);
-    return rc != KR_OK ? rc : launch_reduce(p, g, 0, st);
+    return rc != KR_OK ? rc : launch_reduce(p, g, 0, cus, limited, st);
   }
   return launch_tile<kStore>(p, g, pieces, cus, limited, st);
 }
