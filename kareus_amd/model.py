@@ -25,6 +25,7 @@ from torch import Tensor
 
 from .backend import get_backend
 from .block import LayerConfig, LayerStack
+from .partitions.streams import stream_api
 
 
 class _Embedding(torch.autograd.Function):
@@ -40,15 +41,60 @@ class _Embedding(torch.autograd.Function):
         return None, get_backend(ctx.backend).embedding_bwd(ids, dout, ctx.rows, ctx.vocab_start), None, None
 
 
+class _MainGradOrder:
+    """Sums into one ``main_grad`` run one behind the other, whatever streams their forward passes ran on, and the stream that called
+    ``backward()`` goes on behind them: what autograd sees to for the gradients that it accumulates itself."""
+
+    def __init__(self) -> None:
+        self.last = None    # (event behind the last sum, its stream, the captured pass that it is part of)
+
+    def __reduce__(self):   # (a copy of a module, or one that was saved, has no sums under way)
+        return _MainGradOrder, ()
+
+    @staticmethod
+    def _captured(weight: Tensor):
+        """An event of a capture means nothing outside it, and one from before it nothing inside, where the device was waited for."""
+        return torch._C._current_graph_task_id() if weight.is_cuda and torch.cuda.is_current_stream_capturing() else None
+
+    def begin(self, weight: Tensor, out: Tensor) -> None:
+        here = stream_api().current_stream()
+        if here is not None and self.last is not None:
+            event, stream, captured = self.last
+            if stream != here and captured == self._captured(weight):
+                self._behind(here, event, out)
+
+    def end(self, weight: Tensor, out: Tensor) -> None:
+        api = stream_api()
+        here = api.current_stream()
+        if here is None:
+            return
+        event = api.new_event()
+        event.record(here)
+        self.last = (event, here, self._captured(weight))
+
+        def done() -> None:
+            caller = api.current_stream()
+            if caller != here:
+                self._behind(caller, event, out)
+
+        torch.autograd.Variable._execution_engine.queue_callback(done)
+
+    @staticmethod
+    def _behind(stream, event, out: Tensor) -> None:
+        stream.wait_event(event)
+        if out.is_cuda:
+            out.record_stream(stream)
+
+
 class _SortedEmbedding(torch.autograd.Function):
-    """The embedding times ``scale``, its gradient by sorted tokens.  With ``main_grad`` the gradient goes to the weight's fp32
+    """The embedding times ``scale``, its gradient by sorted tokens.  With ``order`` the gradient goes to the weight's fp32
     ``main_grad``, which the first backward pass writes whole and later ones add to, and autograd sees none."""
 
     @staticmethod
-    def forward(ctx, ids, weight, vocab_start, scale, main_grad, backend):
+    def forward(ctx, ids, weight, vocab_start, scale, order, backend):
         ctx.save_for_backward(ids)
         ctx.vocab_start, ctx.scale, ctx.backend, ctx.rows = vocab_start, scale, backend, weight.shape[0]
-        ctx.main = weight if main_grad else None
+        ctx.main, ctx.order = weight if order is not None else None, order
         return get_backend(backend).embedding_fwd(ids, weight.detach(), vocab_start, scale=scale)
 
     @staticmethod
@@ -61,8 +107,10 @@ class _SortedEmbedding(torch.autograd.Function):
             add = out is not None
             if not add:
                 out = torch.empty(w.shape, dtype=torch.float32, device=w.device)
+            ctx.order.begin(w, out)
         dw = be.embedding_bwd_sorted(ids, dout, ctx.rows, ctx.vocab_start, scale=ctx.scale, out=out, accumulate=add)
         if w is not None:
+            ctx.order.end(w, out)
             w.main_grad, dw = out, None
         return None, dw, None, None, None, None
 
@@ -142,12 +190,13 @@ class LanguageModelEmbedding(torch.nn.Module):
         self.vocab_start, self._backend = int(vocab_start), config.backend
         self.scale, self.main_grad = float(scale), bool(main_grad)
         self.sorted_gradient = bool(sorted_gradient) or self.main_grad or self.scale != 1.0
+        self._order = _MainGradOrder() if self.main_grad else None
         if self.main_grad:
             self.weight.main_grad = None
 
     def forward(self, input_ids: Tensor) -> Tensor:
         if self.sorted_gradient:
-            return _SortedEmbedding.apply(input_ids, self.weight, self.vocab_start, self.scale, self.main_grad, self._backend)
+            return _SortedEmbedding.apply(input_ids, self.weight, self.vocab_start, self.scale, self._order, self._backend)
         return _Embedding.apply(input_ids, self.weight, self.vocab_start, self._backend)
 
 
