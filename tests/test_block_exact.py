@@ -161,3 +161,23 @@ def test_few_rows_sums_are_the_matrix_units(m, n, k):
     for w in range(1, 8):
         total = (total + unit_product(a, b, range(w, blocks_of(k), 8))).float().double()
     assert torch.equal(be.block_matmul(a, b), total.float().to(torch.bfloat16))
+
+
+@pytest.mark.parametrize("m,n,k", [(256, 512, 30000), (75, 608, 17951)])
+@on_gpu
+def test_a_smaller_workspace_is_kept_to(m, n, k):
+    """Whatever a caller hands over, from all that was asked for to none: the same exact result, and nothing behind it is written."""
+    from kareus_amd.backend import hip
+
+    lib = hip.load_library()
+    (a, av), (b, bv) = whole_operand(m, k, "dense", 1, "cuda"), whole_operand(n, k, "dense", 2, "cuda")
+    want = (av @ bv.t()).float().to(torch.bfloat16)
+    asked = lib.kr_block_gemm_workspace_bytes(m, n, k, 0)
+    assert asked >= 8 * m * n
+    for size in (asked, asked - 16, asked // 2 // 16 * 16, 8 * m * n, 4 * m * n, 0):
+        space = torch.full((asked + 4096,), 77, dtype=torch.uint8, device="cuda")
+        out = torch.empty(m, n, dtype=torch.bfloat16, device="cuda")
+        rc = lib.kr_block_gemm(m, n, k, a.data.data_ptr(), a.data.shape[1], a.scales.data_ptr(), a.scales.shape[1], b.data.data_ptr(), b.data.shape[1],
+                               b.scales.data_ptr(), b.scales.shape[1], out.data_ptr(), n, 0, 0, space.data_ptr(), size,
+                               torch.cuda.current_stream().cuda_stream)
+        assert rc == 0 and torch.equal(out, want) and (space[size:] == 77).all()
