@@ -128,7 +128,12 @@ class LayerConfig:
         instead of on their own: where an estimate of one nanobatch's device time per layer, forward and backward,
         is below what its launches cost the host.  Products at 0.75 PFLOP/s, attention at 0.4, forty passes over
         the hidden states at 5 TB/s, the weights read twice at 4.5 TB/s.  Not under a plan: its overlap windows and
-        resource shapes are about the streams, and a pass without them would run none of it."""
+        resource shapes are about the streams, and a pass without them would run none of it.
+
+        Layers over 8-bit blocks: products at 1.5 PFLOP/s, and 2.3 times the line, since their operators run one by one and
+        quantise in launches of their own.  Measured, ms, streams and in line (estimate of one nanobatch): 1B layer, 4 x 2048
+        tokens, two nanobatches 3.85, 2.62 (1.49), four 6.19, 3.36 (0.77); Qwen3 TP=8 shard, 8 x 4096, two 2.78, 2.48 (1.26), four 4.64,
+        3.32 (0.63); 8B TP=4 shard, 4 x 4096, four 4.96, 5.12 (1.51), two 3.90, 4.25 (2.97); 8B layer, 2 x 8192, two 14.4, 14.8 (12.7)."""
         if not self.streams_are_own or self.backend != "hip" or self.kareus_scheduler is not None:
             return False
         made, named = self.made_streams, self.nanobatch_streams
@@ -136,9 +141,10 @@ class LayerConfig:
             return False
         t, h, hd, nq = seq * seqs, self.hidden_size, self.kv_channels, self.num_attention_heads
         weights = h * (self.qkv_width + nq * hd + 3 * self.ffn_hidden_size)
-        ms = (6.0 * t * weights / 0.75e12 + 7.0 * seqs * nq * hd * float(seq) ** 2 / 0.4e12
+        blocks = self.linear_format != "bf16"
+        ms = (6.0 * t * weights / (1.5e12 if blocks else 0.75e12) + 7.0 * seqs * nq * hd * float(seq) ** 2 / 0.4e12
               + 80.0 * t * h / 5e9 + 4.0 * weights / 4.5e9)
-        return ms < self.in_line_below_ms
+        return ms < self.in_line_below_ms * (2.3 if blocks else 1.0)
 
     @property
     def qkv_width(self) -> int:

@@ -342,3 +342,17 @@ def test_a_weights_rows_are_dropped_behind_its_last_nanobatch(monkeypatch, n, kw
             passes.append(len(made))
     assert passes == [24] + ([48 if kw else 24] if grad else [])
     assert max(alive) <= (1 if n == 1 else 8)
+
+
+# ---- streams or one behind the other ----------------------------------------------------------------------
+@pytest.mark.parametrize("h,nq,nkv,hd,ffn,seq,seqs,bf16,blocks", [
+    (2048, 32, 8, 64, 8192, 2048, 2, False, True), (2048, 32, 8, 64, 8192, 2048, 1, False, True), (2048, 2, 1, 128, 768, 4096, 4, False, True),
+    (2048, 2, 1, 128, 768, 4096, 2, False, True), (4096, 8, 2, 128, 3584, 4096, 1, False, False), (4096, 8, 2, 128, 3584, 4096, 2, False, False),
+    (4096, 32, 8, 128, 14336, 8192, 1, False, False), (512, 8, 8, 64, 1376, 128, 1, True, True)])
+def test_small_nanobatches_of_8_bit_layers_run_in_line(h, nq, nkv, hd, ffn, seq, seqs, bf16, blocks):
+    """By what was faster, measured: an 8-bit layer's nanobatch needs less of the device and more of the host than a bf16 layer's."""
+    for form, want in (("bf16", bf16), ("fp8_blocks", blocks)):
+        cfg = LayerConfig(h, nq, nkv, hd, ffn, linear_format=form, streams_are_own=True)
+        assert cfg.nanobatches_in_line(seq, seqs) is want
+        cfg.in_line_below_ms = 0.0
+        assert cfg.nanobatches_in_line(seq, seqs) is False
