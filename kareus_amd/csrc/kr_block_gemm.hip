@@ -16,8 +16,9 @@
 // What bounds it: large products the card's power.  16384 x 28672 x 4096 takes 1403 us (2.74 PFLOP/s) on normally distributed values
 // and 1033 (3.73) on operands of one value, with the same instructions; 16384 x 7168 x 4096 353 and 262 us, 16384 x 4096 x 7168 337
 // and 254.  Products of few rows are bound by B's bytes (1 x 28672 x 4096 18.4 us: 6.4 TB/s, from the 256 MiB cache), those of one
-// tile per unit by their loads' latency and the launch.  The tiles below 192 x 256 are bound by LDS: a K-step of 128 x 256 writes 48 KB
-// and reads 96, 0.5 us at 128 bytes a cycle where its MFMAs are 0.43 (three K-steps under way instead of two: no faster).
+// tile per unit by their loads' latency and the launch.  The tiles below 192 x 256 need LDS for longer than the matrix pipe: a K-step of
+// 128 x 256 writes 48 KB and reads 96, 0.5 us at 128 bytes a cycle where its MFMAs are 0.43; it takes 0.73, and what the rest is has not
+// been shown (three K-steps under way instead of two: no faster).
 #include "kr_common.h"
 
 #include <algorithm>

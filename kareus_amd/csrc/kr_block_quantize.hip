@@ -62,7 +62,7 @@ __device__ __forceinline__ unsigned mags(unsigned w) {
 }
 
 // Four values (two words) times 2^-e as e4m3.  The instruction divides by its scale's power of two before it rounds (nearest, ties to
-// even; what is not finite becomes NaN; every bf16 value checked against the definition at scales from 2^-126 to 2^120).  TINY: the
+// even; what is not finite becomes NaN; tests check every bf16 value at every scale).  TINY: the
 // block's scale may be 2^-127, which is no normal fp32 number: multiplied in two steps.
 template <bool TINY>
 __device__ __forceinline__ unsigned pack4(unsigned lo, unsigned hi, int e, float scale) {

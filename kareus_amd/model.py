@@ -177,7 +177,9 @@ class LanguageModelEmbedding(torch.nn.Module):
     """Word embeddings of one vocabulary shard; ``forward(input_ids [b, s]) -> scale * rows, [s, b, hidden]``.
 
     ``sorted_gradient``: the weight's gradient is summed by sorted tokens instead of by vocabulary rows (always so with a scale or
-    ``main_grad``): for many tokens, or ids that fill a batch.  ``main_grad``: it is kept over backward passes in an fp32
+    ``main_grad``), which takes as long whatever the ids are.  By rows a workgroup adds up all tokens of its rows, so that ids which come
+    often cost most (us by rows and sorted, into 32064 x 4096: 16056 tokens of evenly spread ids 102, 109, as frequent as in text 1388, 112,
+    with 30 % of one id 5393, 106; 512 tokens 38, 47; 64, 48; 167, 47).  ``main_grad``: it is kept over backward passes in an fp32
     ``weight.main_grad``, ``None`` until the first (set it back to ``None``, or zero it, for the next step); a pass touches the rows of
     its tokens only."""
 

@@ -9,6 +9,9 @@ compute-only forward partition over the same operators so one forward pass can f
 operator contexts that every timed backward run re-uses (the backward partition is created in
 ``profiling_mode``, which keeps saved activations alive).
 
+A layer over 8-bit blocks quantises its weight in every partition timed here; in a pass only the first nanobatch to reach the layer does, and
+the times of the others' partitions are shorter by that launch.
+
 Tensor ids of the seeded channels are ``ext_<channel>``; the hand-over operator reads
 ``comm_in_<channel>`` from the *other* nanobatch's store and writes ``comm_out_<channel>``.
 """
