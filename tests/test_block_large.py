@@ -9,6 +9,14 @@ from kareus_amd.backend import get_backend
 pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not torch.cuda.is_available(), reason="needs a HIP device")]
 
 
+@pytest.fixture(autouse=True)
+def give_memory_back():
+    """(Nothing that outlives a test is put into the large pieces that these leave in the allocator.)"""
+    yield
+    if torch.cuda.is_available():
+        torch.cuda.empty_cache()
+
+
 def needs(gb):
     if torch.cuda.mem_get_info()[0] < gb << 30:
         pytest.skip(f"needs {gb} GB")

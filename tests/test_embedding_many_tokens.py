@@ -10,6 +10,14 @@ from kareus_amd.backend import get_backend
 pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not torch.cuda.is_available(), reason="needs a HIP device")]
 
 
+@pytest.fixture(autouse=True)
+def give_memory_back():
+    """(Nothing that outlives a test is put into the large pieces that these leave in the allocator.)"""
+    yield
+    if torch.cuda.is_available():
+        torch.cuda.empty_cache()
+
+
 def ids_of(kind, b, s, rows, seed=0):
     g = torch.Generator().manual_seed(seed)
     if kind == "text":
