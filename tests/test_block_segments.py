@@ -356,3 +356,35 @@ def test_small_nanobatches_of_8_bit_layers_run_in_line(h, nq, nkv, hd, ffn, seq,
         assert cfg.nanobatches_in_line(seq, seqs) is want
         cfg.in_line_below_ms = 0.0
         assert cfg.nanobatches_in_line(seq, seqs) is False
+
+
+@on_gpu
+def test_two_nanobatches_forward_and_backward_in_a_graph():
+    sizes = dict(hidden_size=512, num_attention_heads=4, num_query_groups=2, kv_channels=128, ffn_hidden_size=768)
+    model = LayerStack(config("hip", torch.bfloat16, num_nanobatches=2, num_layers=2, **sizes), device="cuda", seed=7)
+    weights = list(model.parameters())
+    g = torch.Generator().manual_seed(1)
+    sets = [[torch.randn(96, 2, 512, generator=g).to("cuda", torch.bfloat16) for _ in range(2)] for _ in range(3)]
+
+    def step(x, go):
+        return torch.autograd.grad(model(x), [x] + weights, go)
+
+    want = [[t.clone() for t in step(x.clone().requires_grad_(True), go)] for x, go in sets]
+    held, held_go = sets[0][0].clone().requires_grad_(True), sets[0][1].clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(held, held_go)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(held, held_go)
+    for r in range(4):
+        with torch.no_grad():
+            held.copy_(sets[r % 3][0])
+            held_go.copy_(sets[r % 3][1])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, c) for a, c in zip(out, want[r % 3]))
+        eager = step(sets[1][0].clone().requires_grad_(True), sets[1][1])
+        assert all(torch.equal(a, c) for a, c in zip(eager, want[1]))
