@@ -317,6 +317,8 @@ class EagerBackend:
 
     def block_matmul_segments(self, a, b, out: Tensor = None, dtype: torch.dtype = torch.bfloat16) -> Tensor:
         """``sum_i a[i] . b[i]^T``, rounded once."""
+        if len(a) != len(b) or not len(a):
+            raise RuntimeError(f"block_matmul_segments: {len(a)} and {len(b)} operands")
         total = None
         for x, y in zip(a, b):
             c = self.block_matmul(x, y, dtype=torch.float32)

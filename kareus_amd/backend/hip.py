@@ -622,8 +622,8 @@ class HipBackend:
             blocks = sum(blocks_of(x.length) for x, _ in pairs)
             nbytes = self.lib.kr_block_gemm_segments_workspace_bytes(m, n, blocks, max_cus)
             ws = torch.empty(nbytes, dtype=torch.uint8, device=out.device) if nbytes else None
-            rc = self.lib.kr_block_gemm_segments(m, n, nseg, (_c_int * nseg)(*[x.length for x, _ in pairs]), *table, out.data_ptr(), self._pitch(out),
-                                                 max_cus,                                                 None if ws is None else ws.data_ptr(), nbytes, self._stream())
+            rc = self.lib.kr_block_gemm_segments(m, n, nseg, (_c_int * nseg)(*[x.length for x, _ in pairs]), *table, out.data_ptr(),
+                                                 self._pitch(out), max_cus, None if ws is None else ws.data_ptr(), nbytes, self._stream())
         self._check(rc, f"kr_block_gemm_segments(M={m}, N={n}, blocks={blocks}, nseg={nseg})")
         return out
 

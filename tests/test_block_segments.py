@@ -293,6 +293,9 @@ def test_backend_refuses_segments():
         be.block_matmul_segments([], [])
     with pytest.raises(RuntimeError, match="bf16"):
         be.block_matmul_segments([good], [good], dtype=torch.float32)
+    for pair in (([good], []), ([], [])):
+        with pytest.raises(RuntimeError, match="operands"):
+            get_backend("eager").block_matmul_segments(*pair)
 
 
 @on_gpu
