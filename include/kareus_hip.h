@@ -220,6 +220,27 @@ int kr_rmsnorm_bwd_add_noalloc(const void* dy, const void* x, const float* rstd,
                                int64_t dy_ld, int64_t x_ld, int64_t dres_ld, int64_t dx_ld,
                                void* stream);
 
+/* ---- Layer norm ---------------------------------------------------------------------------
+ * mean, rstd: [rows] fp32, written by the forward, read by the backward.  x: [rows, cols] bf16 (row stride x_ld, or rows in runs,
+ * see "Row runs" above; run_rows 1 for a plain matrix); y: [rows, cols] dense; gamma, beta, dgamma, dbeta: [cols] bf16.
+ *   y = bf16((x - mean) rstd gamma + beta), the variance from the differences to the mean
+ *   dx = bf16(rstd (g - mean(g) - xh mean(g xh)) + dres), g = dy gamma, xh = (x - mean) rstd; dres [rows, cols] may be NULL: the
+ *   gradient of a residual branch forked off in front of the norm, added before the one rounding.
+ *   dgamma = sum of dy xh, dbeta = sum of dy over the rows, in fp32 and in a fixed order, rounded once.
+ * cols: a multiple of 8, at most 16384; strides multiples of 8.  dx overlaps no input; it may be a slice of a larger tensor.
+ * workspace: kr_layernorm_bwd_workspace_bytes() bytes, 16-byte aligned.  With dgamma and dbeta NULL the call leaves there its
+ * kr_layernorm_bwd_partial_rows() fp32 rows of [2][cols] sums, and kr_layernorm_dparams adds those of several calls (the nanobatches
+ * of a microbatch, workspaces back to back).  The queries return 0 for widths that are not supported.      */
+int kr_layernorm_fwd(const void* x, const void* gamma, const void* beta, void* y, float* mean, float* rstd, int rows, int cols,
+                     int64_t x_ld, int x_run_rows, int64_t x_run_ld, float eps, void* stream);
+size_t kr_layernorm_bwd_workspace_bytes(int rows, int cols);
+int kr_layernorm_bwd_partial_rows(int rows, int cols);
+int kr_layernorm_bwd(const void* dy, const void* x, const float* mean, const float* rstd, const void* gamma, const void* dres,
+                     void* dx, void* dgamma, void* dbeta, void* workspace, int rows, int cols, int64_t dy_ld,
+                     int64_t x_ld, int x_run_rows, int64_t x_run_ld, int64_t dres_ld, int dres_run_rows, int64_t dres_run_ld,
+                     int64_t dx_ld, int dx_run_rows, int64_t dx_run_ld, void* stream);
+int kr_layernorm_dparams(const float* partial, int nparts, int cols, void* dgamma, void* dbeta, void* stream);
+
 /* ---- Query / key layernorm of the QKV split -----------------------------------------------
  * RMSNorm over the head dimension of every query head (weights gamma_q [hd]) and every key head
  * (gamma_k [hd]) of a fused QKV projection output: replaces the q_layernorm / k_layernorm calls of
@@ -261,6 +282,21 @@ int kr_rope(const void* t, void* out, const float* freqs,
             int64_t t_stride_s, int64_t t_stride_b, int64_t t_stride_h,
             int64_t o_stride_s, int64_t o_stride_b, int64_t o_stride_h,
             int backward, int group_size, int group_rotate, void* stream);
+
+/* ---- Rotary positions on several axes ---------------------------------------------------
+ * kr_rope with an angle for every sequence and token: frequency f (channels f and f + hd / 2) turns by
+ * positions[axis(f)][bi][si] * inv_freq[f], formed in 64 bits.  positions: [axes, b, s] int64 through strides; inv_freq: [hd / 2]
+ * fp64; axes: 1 to KR_ROPE_MAX_AXES.  sections [axes] (host memory, read before the call returns): how many frequencies an axis
+ * has, hd / 2 in all: one axis behind the other, or, interleaved != 0, in turn (f % axes) while that axis has any left, the first
+ * axis behind that.  t, out, their strides and groups as kr_rope's; heads that are not rotated are copied unless out is t.
+ * out is t or overlaps it nowhere.  hd: a multiple of 16, at most 256.                          */
+#define KR_ROPE_MAX_AXES 4
+int kr_rope_axes(const void* t, void* out, const int64_t* positions, int64_t p_stride_axis, int64_t p_stride_b,
+                 int64_t p_stride_s, int axes, const double* inv_freq, const int* sections, int interleaved,
+                 int s, int b, int heads, int hd,
+                 int64_t t_stride_s, int64_t t_stride_b, int64_t t_stride_h,
+                 int64_t o_stride_s, int64_t o_stride_b, int64_t o_stride_h,
+                 int backward, int group_size, int group_rotate, void* stream);
 
 /* ---- SwiGLU ----------------------------------------------------------------------------
  * Replaces the Inductor kernels of fused_swiglu_forward / fused_swiglu_backward
@@ -488,6 +524,20 @@ size_t kr_block_gemm_segments_workspace_bytes(int M, int N, int blocks, int max_
 int kr_block_gemm_segments(int M, int N, int nseg, const int* K, const void* const* A, const int64_t* lda, const void* const* sa,
                            const int64_t* lsa, const void* const* B, const int64_t* ldb, const void* const* sb, const int64_t* lsb,
                            void* C, int64_t ldc, int max_cus, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- Gradient norm and clipping -----------------------------------------------------------------
+ * n tensors, the i-th of counts[i] elements one behind the other at grads[i] (any alignment of its type; 0 elements: the pointer is
+ * not looked at), bf16 or, fp32[i] != 0, fp32.  The arrays are in host memory and read before the call returns.
+ * kr_grad_norm: norm = sqrt(sum of all squares), 64-bit sums in a fixed order, one fp32 on the device.
+ * kr_grad_clip: the norm, and every gradient times min(1, max_norm / (norm + eps)): in place (out NULL; rounded once; with a factor of
+ * 1 nothing is written), or in fp32 at out[i].  A norm that is infinite or not a number gives the factor that the formula gives.
+ * A tensor that appears twice, or overlaps another or an output, is the caller's to leave out.
+ * workspace: kr_grad_norm_workspace_bytes() bytes, 16-byte aligned.                                  */
+size_t kr_grad_norm_workspace_bytes(int n);
+int kr_grad_norm(int n, const void* const* grads, const int64_t* counts, const int* fp32, float* norm, void* workspace,
+                 size_t workspace_bytes, void* stream);
+int kr_grad_clip(int n, const void* const* grads, const int64_t* counts, const int* fp32, void* const* out, double max_norm,
+                 double eps, float* norm, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -31,6 +31,17 @@ def get_backend(name: str = "hip"):
     return _CACHE[name]
 
 
+def check_window(causal: bool, window: int, sinks: int) -> None:
+    """Raises unless a call of attention asks for a mask that there is: ``window`` 0 (none) or the keys that a query sees up to its own,
+    ``sinks`` the first keys that stay visible."""
+    if window < 0 or sinks < 0:
+        raise RuntimeError(f"attention: window {window} and sinks {sinks} must not be negative")
+    if sinks and not window:
+        raise RuntimeError("attention: sinks say what stays visible beside a window, and there is none")
+    if window and not causal:
+        raise RuntimeError("attention: a window is causal")
+
+
 # ---- compute-unit budget of the launches of the current thread ---------------------------------
 # A schedule gives every partition a resource shape (kareus/megatron/core/partitions/
 # partition_base.py:117-128: ``sm_num``, the compute units the work overlapping the partition is to

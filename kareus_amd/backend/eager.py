@@ -13,6 +13,9 @@ import torch
 from torch import Tensor
 
 from ..block_scaled import BLOCK, BlockOperand, BlockScaled, blocks_of
+from ..gradients import check_gradients
+from ..rotary_axes import RotaryAxes, axis_of_frequency
+from . import check_window
 
 
 class EagerBackend:
@@ -113,6 +116,42 @@ class EagerBackend:
             return dx, None
         return dx, dgamma.to(gamma.dtype)
 
+    # mean and 1 / sqrt(variance + eps) per row in fp32, the variance from the differences to the mean; y = (x - mean) rs gamma + beta
+    def layernorm_fwd(self, x: Tensor, gamma: Tensor, beta: Tensor, eps: float) -> Tuple[Tensor, Tensor, Tensor]:
+        xf = x.reshape(-1, x.shape[-1]).float()
+        mean = xf.mean(dim=-1)
+        d = xf - mean[:, None]
+        rstd = torch.rsqrt(d.pow(2).mean(dim=-1) + eps)
+        return (d * rstd[:, None] * gamma.float() + beta.float()).to(x.dtype), mean, rstd
+
+    # dx = rs (g - mean(g) - xhat mean(g xhat)) + residual gradient, g = gamma dy; dgamma = sum dy xhat, dbeta = sum dy
+    def layernorm_partial_rows(self, rows: int, cols: int) -> int:
+        return 1
+
+    def layernorm_dparams(self, partials: Tensor, gamma: Tensor) -> Tuple[Tensor, Tensor]:
+        dgamma, dbeta = partials.sum(dim=0).to(gamma.dtype).chunk(2)
+        return dgamma, dbeta
+
+    def layernorm_bwd(self, dy: Tensor, x: Tensor, mean: Tensor, rstd: Tensor, gamma: Tensor, residual_grad: Tensor = None,
+                      out: Tensor = None, partials_out: Tensor = None) -> Tuple[Tensor, Tensor, Tensor]:
+        cols = x.shape[-1]
+        xhat = (x.reshape(-1, cols).float() - mean[:, None]) * rstd[:, None]
+        dyf = dy.reshape(-1, cols).float()
+        g = dyf * gamma.float()
+        dx = rstd[:, None] * (g - g.mean(dim=-1, keepdim=True) - xhat * (g * xhat).mean(dim=-1, keepdim=True))
+        if residual_grad is not None:
+            dx = dx + residual_grad.reshape(-1, cols).float()
+        dx = dx.to(x.dtype)
+        if out is not None:
+            out.copy_(dx.view(out.shape))
+            dx = out
+        sums = torch.cat(((dyf * xhat).sum(dim=0), dyf.sum(dim=0)))
+        if partials_out is not None:
+            partials_out.copy_(sums.view(1, -1))
+            return dx, None, None
+        dgamma, dbeta = sums.to(gamma.dtype).chunk(2)
+        return dx, dgamma, dbeta
+
     # y = t cos f + rotate_half(t) sin f, rotate_half([a, b]) = [-b, a]; trig in fp32
     # (kareus/megatron/core/models/common/embedding/rope_utils.py:147-182)
     @staticmethod
@@ -199,11 +238,67 @@ class EagerBackend:
         out = torch.cat([dx.to(dmixed5.dtype), dmixed5[..., per + 1:, :]], dim=3)
         return out, dgam[:per].sum(0).to(gamma_q.dtype), dgam[per].to(gamma_k.dtype)
 
+    # Rotation by positions on several axes, the angles in 64 bits
+    @staticmethod
+    def _rope_axes(t: Tensor, at: RotaryAxes, sign: float) -> Tensor:
+        s, b, hd = t.shape[0], t.shape[1], t.shape[-1]
+        at.check(s, b, hd)
+        place = at.positions[axis_of_frequency(at.sections, at.interleaved, at.positions.device)]     # [hd / 2, b, s]
+        angle = (place.double() * at.inv_freq[:, None, None]).permute(2, 1, 0).view((s, b) + (1,) * (t.dim() - 3) + (hd // 2,))
+        cos, sin = torch.cos(angle).float(), torch.sin(angle).float() * sign
+        x, y = t.float().chunk(2, dim=-1)
+        return torch.cat((x * cos - y * sin, y * cos + x * sin), dim=-1).to(t.dtype)
+
+    def rope_axes_fwd(self, t: Tensor, at: RotaryAxes) -> Tensor:
+        return self._rope_axes(t.flatten(2, 3) if t.dim() == 5 else t, at, 1.0)
+
+    def rope_axes_bwd(self, g: Tensor, at: RotaryAxes) -> Tensor:
+        return self._rope_axes(g.flatten(2, 3) if g.dim() == 5 else g, at, -1.0)
+
+    def rope_axes_fused(self, fused: Tensor, per: int, at: RotaryAxes, backward: bool = False, out: Tensor = None) -> Tensor:
+        if fused.dim() != 5 or fused.shape[3] != per + 2:
+            raise RuntimeError("rope_axes_fused: needs a fused buffer [s, b, groups, per + 2, hd]")
+        turned = self._rope_axes(fused[:, :, :, :per + 1], at, -1.0 if backward else 1.0)
+        if out is None:
+            out = torch.empty_like(fused)
+        out[:, :, :, per + 1] = fused[:, :, :, per + 1]
+        out[:, :, :, :per + 1] = turned
+        return out
+
+    # The 2-norm over all tensors in 64 bits, and all tensors times min(1, max_norm / (norm + eps))
+    def grad_norm(self, tensors) -> Tensor:
+        tensors = list(tensors)
+        check_gradients(tensors)
+        if not tensors:
+            return torch.zeros(())
+        return torch.stack([t.double().square().sum() for t in tensors]).sum().sqrt().float()
+
+    def clip_grad_norm(self, tensors, max_norm: float, eps: float = 1e-6, out=None) -> Tensor:
+        tensors = list(tensors)
+        check_gradients(tensors, max_norm, eps, out)
+        if not tensors:
+            return torch.zeros(())
+        norm = torch.stack([t.double().square().sum() for t in tensors]).sum().sqrt()
+        factor = (max_norm / (norm + eps)).clamp(max=1.0).float()
+        for t, to in zip(tensors, tensors if out is None else out):
+            to.copy_(t.float() * factor)
+        return norm.float()
+
     # Causal GQA attention on [s, b, heads, hd] tensors; query head i reads KV head
     # i // (nq / nkv); lse = logsumexp of the scaled, masked scores, [b, nq, s] fp32
     # (kareus/flash_attn/flash_attn_interface.py:473-493).
+    # (window > 0: a query sees the last `window` keys up to its own, and the first `sinks`)
+    @staticmethod
+    def _visible(s: int, causal: bool, window: int, sinks: int, device) -> Tensor:
+        check_window(causal, window, sinks)
+        if not causal:
+            return torch.ones(s, s, dtype=torch.bool, device=device)
+        i = torch.arange(s, device=device)
+        back = i[:, None] - i
+        return (back >= 0) & ((back < window) | (i < sinks)) if window else back >= 0
+
     def attn_fwd(self, q: Tensor, k: Tensor, v: Tensor, scale: float, causal: bool = True,
-                 beside_other_streams: bool = False):
+                 beside_other_streams: bool = False, window: int = 0, sinks: int = 0):
         if q.dim() == 5:
             q = q.flatten(2, 3)
         s, b, nq, hd = q.shape
@@ -213,15 +308,14 @@ class EagerBackend:
         kf = k.float().permute(1, 2, 0, 3).repeat_interleave(rep, dim=1)
         vf = v.float().permute(1, 2, 0, 3).repeat_interleave(rep, dim=1)
         scores = (qf @ kf.transpose(-1, -2)) * scale
-        if causal:
-            mask = torch.ones(s, s, dtype=torch.bool, device=q.device).tril()
-            scores = scores.masked_fill(~mask, float("-inf"))
+        scores = scores.masked_fill(~self._visible(s, causal, window, sinks, q.device), float("-inf"))
         lse = torch.logsumexp(scores, dim=-1)
         p = torch.exp(scores - lse[..., None])
         o = (p @ vf).permute(2, 0, 1, 3).contiguous()
         return o.to(q.dtype), lse.contiguous()
 
-    def attn_bwd(self, do, q, k, v, o, lse, scale: float, causal: bool = True, beside_other_streams: bool = False):
+    def attn_bwd(self, do, q, k, v, o, lse, scale: float, causal: bool = True, beside_other_streams: bool = False,
+                 window: int = 0, sinks: int = 0):
         if q.dim() == 5:
             q = q.flatten(2, 3)
         s, b, nq, hd = q.shape
@@ -233,9 +327,7 @@ class EagerBackend:
         dof = do.float().reshape(s, b, nq, hd).permute(1, 2, 0, 3)
         of = o.float().reshape(s, b, nq, hd).permute(1, 2, 0, 3)
         scores = (qf @ kf.transpose(-1, -2)) * scale
-        if causal:
-            mask = torch.ones(s, s, dtype=torch.bool, device=q.device).tril()
-            scores = scores.masked_fill(~mask, float("-inf"))
+        scores = scores.masked_fill(~self._visible(s, causal, window, sinks, q.device), float("-inf"))
         p = torch.exp(scores - lse[..., None])
         dv = p.transpose(-1, -2) @ dof
         dp = dof @ vf.transpose(-1, -2)

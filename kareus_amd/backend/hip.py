@@ -16,7 +16,9 @@ import torch
 from torch import Tensor
 
 from ..block_scaled import BlockOperand, BlockScaled, blocks_of
-from . import reserved_compute_units
+from ..gradients import check_gradients
+from ..rotary_axes import RotaryAxes
+from . import check_window, reserved_compute_units
 
 _LIB_NAME = "libkareus_hip.so"
 _c_void_p, _c_int, _c_i64, _c_float, _c_size_t = (
@@ -69,6 +71,16 @@ _SIGNATURES = {
     "kr_embedding_bwd": (_c_int, [_c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_i64, _c_i64, _c_void_p]),
     "kr_cross_entropy_fwd": (_c_int, [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_i64, _c_int, _c_i64, _c_void_p]),
     "kr_cross_entropy_bwd": (_c_int, [_c_void_p] * 5 + [_c_i64, _c_int, _c_i64, _c_i64, _c_void_p]),
+    "kr_layernorm_fwd": (_c_int, [_c_void_p] * 6 + [_c_int, _c_int, _c_i64, _c_int, _c_i64, _c_float, _c_void_p]),
+    "kr_layernorm_bwd_workspace_bytes": (_c_size_t, [_c_int, _c_int]),
+    "kr_layernorm_bwd_partial_rows": (_c_int, [_c_int, _c_int]),
+    "kr_layernorm_bwd": (_c_int, [_c_void_p] * 10 + [_c_int, _c_int, _c_i64] + [_c_i64, _c_int, _c_i64] * 3 + [_c_void_p]),
+    "kr_layernorm_dparams": (_c_int, [_c_void_p, _c_int, _c_int, _c_void_p, _c_void_p, _c_void_p]),
+    "kr_rope_axes": (_c_int, [_c_void_p] * 3 + [_c_i64] * 3 + [_c_int, _c_void_p, _c_void_p] + [_c_int] * 5 + [_c_i64] * 6 +
+                     [_c_int] * 3 + [_c_void_p]),
+    "kr_grad_norm_workspace_bytes": (_c_size_t, [_c_int]),
+    "kr_grad_norm": (_c_int, [_c_int] + [_c_void_p] * 5 + [_c_size_t, _c_void_p]),
+    "kr_grad_clip": (_c_int, [_c_int] + [_c_void_p] * 4 + [ctypes.c_double, ctypes.c_double, _c_void_p, _c_void_p, _c_size_t, _c_void_p]),
     "kr_attn_fwd": (_c_int, [_c_void_p] * 5 + [_c_int] * 5 + [_c_float] + [_c_i64] * 14 + [_c_void_p]),
     "kr_attn_fwd_flags": (_c_int, [_c_void_p] * 5 + [_c_int] * 5 + [_c_float] + [_c_i64] * 14 + [_c_int, _c_void_p]),
     "kr_attn_fwd_workspace_bytes": (_c_size_t, [_c_int] * 5),
@@ -754,6 +766,131 @@ class HipBackend:
         self._check(rc, "kr_rmsnorm_bwd_add")
         return dx, dgamma
 
+    # -- layer norm -------------------------------------------------------------------
+    def _norm_weights(self, name: str, cols: int, *weights: Tensor) -> None:
+        self._dev(*weights)
+        self._bf16(*weights)
+        for w in weights:
+            if w.shape != (cols,) or not w.is_contiguous():
+                raise RuntimeError(f"{name}: a weight vector has shape {tuple(w.shape)}, rows have {cols} elements")
+
+    def _norm_rows(self, name: str, t: Tensor) -> Tuple[Tensor, Tuple[int, int, int, int]]:
+        """``t`` as the kernels address it, copied only where they cannot, and its ``_operand``."""
+        self._dev(t)
+        self._bf16(t)
+        if t.dim() < 2:
+            raise RuntimeError(f"{name}: needs rows, got {tuple(t.shape)}")
+        v = self.rows_view(t) if t.numel() and t.data_ptr() % 16 == 0 else None
+        op = None if v is None else self._operand(v)
+        if op is None:
+            v = t.reshape(-1, t.shape[-1]).contiguous()
+            if v.data_ptr() % 16:
+                v = v.clone()
+            op = (v.shape[0], v.shape[1], 1, 0)
+        rows, ld, run_rows, run_ld = op
+        return v, (rows, (v.shape[-1] + 7) // 8 * 8 if rows == 1 else ld, run_rows, run_ld)    # (one row's stride says nothing)
+
+    def layernorm_fwd(self, x: Tensor, gamma: Tensor, beta: Tensor, eps: float) -> Tuple[Tensor, Tensor, Tensor]:
+        """``(x - mean) rstd gamma + beta`` per row of ``x`` ([rows, cols], or a [s, r, cols] nanobatch slice whose rows come in runs, read in
+        place), the statistics in fp32.  Returns the dense [rows, cols] result, mean [rows] and rstd [rows]."""
+        done = self._n.layernorm_fwd(x, gamma, beta, eps)
+        if done is not None:
+            return done
+        x, (rows, ld, run_rows, run_ld) = self._norm_rows("layernorm_fwd", x)
+        cols = x.shape[-1]
+        self._norm_weights("layernorm_fwd", cols, gamma, beta)
+        self._same_device("layernorm_fwd", x, gamma, beta)
+        y = torch.empty((rows, cols), dtype=x.dtype, device=x.device)
+        mean, rstd = torch.empty((2, rows), dtype=torch.float32, device=x.device)
+        if rows:
+            with self._current(x):
+                rc = self.lib.kr_layernorm_fwd(x.data_ptr(), gamma.data_ptr(), beta.data_ptr(), y.data_ptr(), mean.data_ptr(),
+                                               rstd.data_ptr(), rows, cols, ld, run_rows, run_ld, eps, self._stream())
+            self._check(rc, f"kr_layernorm_fwd(rows={rows}, cols={cols})")
+        return y, mean, rstd
+
+    def layernorm_partial_rows(self, rows: int, cols: int) -> int:
+        """fp32 partial rows, [2 cols] each, that one backward call over [rows, cols] leaves."""
+        return self.lib.kr_layernorm_bwd_partial_rows(rows, cols)
+
+    def layernorm_dparams(self, partials: Tensor, gamma: Tensor) -> Tuple[Tensor, Tensor]:
+        """Sums of the partial rows ([n, 2 cols] fp32) of all nanobatches -> the gradients of weight and bias."""
+        cols = gamma.shape[0]
+        if (partials.dtype != torch.float32 or partials.dim() != 2 or partials.shape[1] != 2 * cols or not partials.is_contiguous()
+                or not partials.is_cuda):
+            raise RuntimeError(f"layernorm_dparams: partial rows must be dense fp32 [n, {2 * cols}] on the HIP device")
+        self._norm_weights("layernorm_dparams", cols, gamma)
+        dgamma, dbeta = torch.empty_like(gamma), torch.empty_like(gamma)
+        if not partials.shape[0]:
+            return dgamma.zero_(), dbeta.zero_()
+        with self._current(partials):
+            rc = self.lib.kr_layernorm_dparams(partials.data_ptr(), partials.shape[0], cols, dgamma.data_ptr(), dbeta.data_ptr(),
+                                               self._stream())
+        self._check(rc, "kr_layernorm_dparams")
+        return dgamma, dbeta
+
+    def layernorm_bwd(self, dy: Tensor, x: Tensor, mean: Tensor, rstd: Tensor, gamma: Tensor, residual_grad: Tensor = None,
+                      out: Tensor = None, partials_out: Tensor = None) -> Tuple[Tensor, Tensor, Tensor]:
+        """The input gradient and the gradients of weight and bias.  ``residual_grad`` (rows as ``x``'s): the gradient of the residual branch
+        forked off in front of the norm, added before the one rounding.  ``out``: where the input gradient goes (rows, or rows in runs).
+        ``partials_out`` ([layernorm_partial_rows, 2 cols] fp32, dense): the gradients of weight and bias are left there as partial rows
+        for ``layernorm_dparams`` and None is returned in their place."""
+        done = self._n.layernorm_bwd(dy, x, mean, rstd, gamma, residual_grad, out, partials_out)
+        if done is not None:
+            return done
+        name = "layernorm_bwd"
+        x, (rows, x_ld, x_runs, x_run_ld) = self._norm_rows(name, x)
+        cols = x.shape[-1]
+        dy, (dy_rows, dy_ld, dy_runs, _) = self._norm_rows(name, dy)
+        if dy_runs > 1:
+            dy, dy_ld = dy.reshape(-1, cols).contiguous(), cols
+        if dy_rows != rows or dy.shape[-1] != cols:
+            raise RuntimeError(f"{name}: dy must be [{rows}, {cols}] like x")
+        self._norm_weights(name, cols, gamma)
+        for t in (mean, rstd):
+            if t.dtype != torch.float32 or t.numel() != rows or not t.is_contiguous() or not t.is_cuda:
+                raise RuntimeError(f"{name}: mean and rstd are the forward's dense fp32 [{rows}]")
+        tensors = [x, dy, mean, rstd, gamma]
+        res, res_ptr, res_op = None, None, (rows, 0, 1, 0)
+        if residual_grad is not None:
+            res, res_op = self._norm_rows(name, residual_grad)
+            if res_op[0] != rows or res.shape[-1] != cols:
+                raise RuntimeError(f"{name}: residual_grad must have the shape of x")
+            res_ptr = res.data_ptr()
+            tensors.append(res)
+        if out is None:
+            dx, dx_op = torch.empty((rows, cols), dtype=x.dtype, device=x.device), (rows, cols, 1, 0)
+        else:
+            self._dev(out)
+            self._bf16(out)
+            dx, dx_op = out, self._operand(out)
+            if dx_op is None or dx_op[0] != rows or out.shape[-1] != cols or out.data_ptr() % 16:
+                raise RuntimeError(f"{name}: out must be [{rows}, {cols}] with a single row stride, or in row runs")
+            if rows == 1:
+                dx_op = (1, (cols + 7) // 8 * 8, 1, 0)
+            tensors.append(out)
+        dgamma = dbeta = None
+        if partials_out is not None:
+            if (partials_out.dtype != torch.float32 or not partials_out.is_contiguous() or not partials_out.is_cuda
+                    or tuple(partials_out.shape) != (self.layernorm_partial_rows(rows, cols), 2 * cols)):
+                raise RuntimeError(f"{name}: partials_out must be dense fp32 [partial rows, {2 * cols}]")
+            tensors.append(partials_out)
+        else:
+            dgamma, dbeta = torch.empty_like(gamma), torch.empty_like(gamma)
+        self._same_device(name, *tensors)
+        if not rows:
+            return dx, None if dgamma is None else dgamma.zero_(), None if dbeta is None else dbeta.zero_()
+        with self._current(x):
+            ws = partials_out
+            if ws is None:
+                ws = torch.empty(max(self.lib.kr_layernorm_bwd_workspace_bytes(rows, cols), 16), dtype=torch.uint8, device=x.device)
+            rc = self.lib.kr_layernorm_bwd(dy.data_ptr(), x.data_ptr(), mean.data_ptr(), rstd.data_ptr(), gamma.data_ptr(), res_ptr,
+                                           dx.data_ptr(), None if dgamma is None else dgamma.data_ptr(),
+                                           None if dbeta is None else dbeta.data_ptr(), ws.data_ptr(), rows, cols, dy_ld, x_ld, x_runs,
+                                           x_run_ld, res_op[1], res_op[2], res_op[3], dx_op[1], dx_op[2], dx_op[3], self._stream())
+        self._check(rc, f"kr_layernorm_bwd(rows={rows}, cols={cols})")
+        return dx, dgamma, dbeta
+
     # -- RoPE -------------------------------------------------------------------------
     def _freqs2d(self, freqs: Tensor, hd: int) -> Tensor:
         if freqs.dtype != torch.float32:
@@ -800,6 +937,113 @@ class HipBackend:
             raise RuntimeError("fused QKV buffer must be contiguous [s, b, ng, per+2, hd]")
         flat = fused.view(s, b, ng * slots, hd)
         self._rope(flat, freqs, backward, out=flat, group_size=slots, group_rotate=per + 1)
+
+    # -- rotary positions on several axes -----------------------------------------------
+    def _rope_axes(self, t: Tensor, out: Tensor, at: RotaryAxes, backward: bool, group_size: int, group_rotate: int) -> Tensor:
+        """``t``, ``out``: [s, b, heads, hd]."""
+        self._dev(t)
+        self._bf16(t, out)
+        s, b, heads, hd = t.shape
+        at.check(s, b, hd)
+        self._same_device("rope_axes", t, at.positions, out)
+        if not t.numel():
+            return out
+        # (a dimension of one may have any stride)
+        strides = [8 if n == 1 else st for x in (t, out) for n, st in zip(x.shape[:3], x.stride())]
+        sections = (_c_int * len(at.sections))(*at.sections)
+        p = at.positions
+        with self._current(t):
+            rc = self.lib.kr_rope_axes(t.data_ptr(), out.data_ptr(), p.data_ptr(), *p.stride(), p.shape[0], at.inv_freq.data_ptr(), sections,
+                                       int(at.interleaved), s, b, heads, hd, *strides,
+                                       int(backward), group_size, group_rotate, self._stream())
+        self._check(rc, f"kr_rope_axes(s={s}, b={b}, heads={heads}, hd={hd})")
+        return out
+
+    def _rope_axes_new(self, t: Tensor, at: RotaryAxes, backward: bool) -> Tensor:
+        if t.dim() == 5:
+            t = t.flatten(2, 3)
+        if t.dim() != 4 or t.shape[-1] % 16:
+            raise RuntimeError(f"rope_axes: needs [s, b, heads, hd] with hd a multiple of 16, got {tuple(t.shape)}")
+        if (t.numel() and t.stride(3) != 1) or t.data_ptr() % 16 or any(st % 8 or st <= 0 for n, st in zip(t.shape[:3], t.stride()) if n > 1):
+            t = t.contiguous()
+            if t.data_ptr() % 16:
+                t = t.clone()
+        return self._rope_axes(t, torch.empty(t.shape, dtype=t.dtype, device=t.device), at, backward, 1, 1)
+
+    def rope_axes_fwd(self, t: Tensor, at: RotaryAxes) -> Tensor:
+        """[s, b, heads, hd] (or [s, b, groups, heads, hd]) rotated by positions on several axes."""
+        return self._rope_axes_new(t, at, False)
+
+    def rope_axes_bwd(self, g: Tensor, at: RotaryAxes) -> Tensor:
+        return self._rope_axes_new(g, at, True)
+
+    def rope_axes_fused(self, fused: Tensor, per: int, at: RotaryAxes, backward: bool = False, out: Tensor = None) -> Tensor:
+        """The query and key heads of a dense fused QKV buffer [s, b, groups, per + 2, hd] rotated, its value heads as they are, in one
+        launch: into a new buffer, or into ``out``, which may be ``fused`` (the value heads are then left alone)."""
+        done = self._n.rope_axes_fused(fused, per, at.positions, at.inv_freq, at.sections, at.interleaved, backward, out)
+        if done is not None:
+            return done
+        for t in (fused,) if out is None else (fused, out):
+            if t.dim() != 5 or t.shape[3] != per + 2 or t.shape != fused.shape or not t.is_contiguous() or t.data_ptr() % 16:
+                raise RuntimeError("rope_axes_fused: needs dense fused buffers [s, b, groups, per + 2, hd], 16-byte aligned")
+        if out is None:
+            out = torch.empty_like(fused)
+        elif out.data_ptr() != fused.data_ptr() and out.numel() and (
+                out.data_ptr() < fused.data_ptr() + 2 * fused.numel() and fused.data_ptr() < out.data_ptr() + 2 * out.numel()):
+            raise RuntimeError("rope_axes_fused: out overlaps fused")
+        self._rope_axes(fused.flatten(2, 3), out.flatten(2, 3), at, backward, per + 2, per + 1)
+        return out
+
+    # -- gradient norm and clipping -------------------------------------------------------
+    def _gradient_table(self, tensors, out):
+        n = len(tensors)
+        if not all(t.is_cuda for t in tensors):
+            raise RuntimeError("the hip backend needs tensors on the HIP device")
+        return (n, (_c_void_p * n)(*[t.data_ptr() for t in tensors]), (_c_i64 * n)(*[t.numel() for t in tensors]),
+                (_c_int * n)(*[int(t.dtype == torch.float32) for t in tensors]),
+                None if out is None else (_c_void_p * n)(*[t.data_ptr() for t in out]))
+
+    def _no_gradients(self) -> Tensor:
+        return torch.zeros((), device="cuda" if torch.cuda.is_available() else None)
+
+    def grad_norm(self, tensors) -> Tensor:
+        """The 2-norm of all ``tensors`` (dense bf16 or fp32) as one vector: fp32, on their device.  Sums are 64 bits, in a fixed order."""
+        tensors = list(tensors)
+        if not tensors:
+            return self._no_gradients()
+        done = self._n.grad_norm(tensors)
+        if done is not None:
+            return done
+        check_gradients(tensors)
+        n, grads, counts, fp32, _ = self._gradient_table(tensors, None)
+        with self._current(tensors[0]):
+            norm = torch.empty((), dtype=torch.float32, device=tensors[0].device)
+            nbytes = self.lib.kr_grad_norm_workspace_bytes(n)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=norm.device)
+            rc = self.lib.kr_grad_norm(n, grads, counts, fp32, norm.data_ptr(), ws.data_ptr(), nbytes, self._stream())
+        self._check(rc, f"kr_grad_norm(n={n})")
+        return norm
+
+    def clip_grad_norm(self, tensors, max_norm: float, eps: float = 1e-6, out=None) -> Tensor:
+        """Scales all ``tensors`` by ``min(1, max_norm / (norm + eps))``, in place or, in fp32, into the tensors ``out``; returns their norm
+        before that.  Nothing waits for the device: the factor stays on it."""
+        tensors = list(tensors)
+        out = None if out is None else list(out)
+        if not tensors:
+            check_gradients(tensors, max_norm, eps, out)
+            return self._no_gradients()
+        done = self._n.clip_grad_norm(tensors, max_norm, eps, out)
+        if done is not None:
+            return done
+        check_gradients(tensors, max_norm, eps, out)
+        table = self._gradient_table(tensors, out)
+        with self._current(tensors[0]):
+            norm = torch.empty((), dtype=torch.float32, device=tensors[0].device)
+            nbytes = self.lib.kr_grad_norm_workspace_bytes(table[0])
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=norm.device)
+            rc = self.lib.kr_grad_clip(*table, float(max_norm), float(eps), norm.data_ptr(), ws.data_ptr(), nbytes, self._stream())
+        self._check(rc, f"kr_grad_clip(n={table[0]})")
+        return norm
 
     # -- SwiGLU / add -------------------------------------------------------------------
     def swiglu_fwd(self, x: Tensor) -> Tensor:

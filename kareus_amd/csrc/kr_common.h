@@ -86,6 +86,28 @@ __device__ __forceinline__ void kr_barrier() {
   __syncthreads();
 }
 
+// Row runs: the rows of a tensor may come in runs of 2^sh consecutive rows (stride ld) whose starts are
+// `outer` elements apart — a nanobatch of 2^sh sequences cut out of a [s, b, h] tensor along b, used in
+// place.  A plain matrix has sh = 0 (outer unused).
+struct KrRuns {
+  int sh;
+  int64_t outer;
+};
+__device__ __forceinline__ int64_t kr_row_at(int64_t row, int64_t ld, KrRuns r) {
+  return r.sh ? (row >> r.sh) * r.outer + (row & ((1 << r.sh) - 1)) * ld : row * ld;
+}
+// rows per run (a power of two, 1 = plain) and distance between run starts -> KrRuns
+static inline int kr_make_runs(int run_rows, int64_t run_ld, int rows, KrRuns* out) {
+  *out = KrRuns{0, 0};
+  if (run_rows == 1) return KR_OK;
+  if (run_rows < 1 || (run_rows & (run_rows - 1)) || run_ld <= 0) return KR_EINVAL;
+  if (run_rows > 1024 || run_ld % 8 || rows % run_rows) return KR_EUNSUPPORTED;
+  int sh = 0;
+  while ((1 << sh) < run_rows) ++sh;
+  *out = KrRuns{sh, run_ld};
+  return KR_OK;
+}
+
 static inline bool kr_aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 static inline int kr_launch_status() {

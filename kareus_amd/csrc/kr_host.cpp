@@ -23,6 +23,8 @@
 #include <mutex>
 #include <string>
 #include <unordered_map>
+#include <utility>
+#include <vector>
 
 #include "../../include/kareus_hip.h"
 
@@ -1358,6 +1360,243 @@ PyObject* py_embedding_bwd_sorted(PyObject*, PyObject* const* a, Py_ssize_t n_ar
   });
 }
 
+// ---- layer norm ---------------------------------------------------------------------------------------------
+// layernorm_fwd(x, gamma, beta, eps) -> (y [rows, cols], mean [rows], rstd [rows])
+PyObject* py_layernorm_fwd(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  return guarded([&]() -> PyObject* {
+    if (n_args != 4 || !bf16_arg(a[0])) return none();
+    const Tensor& x = tensor(a[0]);
+    const Operand o = operand(x);
+    if (!o.ok || !is_gamma(a[1], o.cols) || !is_gamma(a[2], o.cols) || !fits_int(o.rows) || o.cols % 8) return none();
+    const Tensor &gamma = tensor(a[1]), &beta = tensor(a[2]);
+    for (const Tensor* t : {&x, &gamma, &beta})
+      if (!on_current_device(*t) || !aligned16(*t)) return none();
+    const float eps = (float)real(a[3]);
+    Tensor y, mean, rstd;
+    int rc;
+    {
+      WithoutInterpreter free;
+      y = matrix(o.rows, o.cols, x);
+      mean = at::empty({o.rows}, x.options().dtype(at::kFloat));
+      rstd = at::empty({o.rows}, x.options().dtype(at::kFloat));
+      rc = kr_layernorm_fwd(ptr(x), ptr(gamma), ptr(beta), ptr(y), (float*)ptr(mean), (float*)ptr(rstd), (int)o.rows, (int)o.cols,
+                            o.ld, o.run_rows, o.run_ld, eps, stream());
+    }
+    if (rc != KR_OK)
+      return failed("kr_layernorm_fwd(rows=" + std::to_string(o.rows) + ", cols=" + std::to_string(o.cols) + ")", rc);
+    PyObject *py = wrap(std::move(y)), *pm = wrap(std::move(mean)), *pr = wrap(std::move(rstd));
+    return Py_BuildValue("(NNN)", py, pm, pr);
+  });
+}
+
+// layernorm_bwd(dy, x, mean, rstd, gamma, residual_grad, out, partials) -> (dx, dgamma or None, dbeta or None)
+PyObject* py_layernorm_bwd(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  return guarded([&]() -> PyObject* {
+    if (n_args != 8 || !bf16_arg(a[0]) || !bf16_arg(a[1]) || !f32_arg(a[2]) || !f32_arg(a[3])) return none();
+    const Tensor &dy = tensor(a[0]), &x = tensor(a[1]), &mean = tensor(a[2]), &rstd = tensor(a[3]);
+    const Operand od = operand2(dy), ox = operand(x);
+    if (!od.ok || !ox.ok || od.rows != ox.rows || od.cols != ox.cols || !fits_int(ox.rows) || !is_gamma(a[4], ox.cols) ||
+        ox.cols % 8)
+      return none();
+    const Tensor& gamma = tensor(a[4]);
+    for (const Tensor* t : {&dy, &x, &gamma})
+      if (!on_current_device(*t) || !aligned16(*t)) return none();
+    for (const Tensor* t : {&mean, &rstd})
+      if (!on_current_device(*t) || !t->is_contiguous() || t->numel() != ox.rows) return none();
+    Operand orr, oc;
+    if (!absent(a[5])) {
+      if (!bf16_arg(a[5])) return none();
+      const Tensor& r = tensor(a[5]);
+      orr = operand(r);
+      if (!orr.ok || orr.rows != ox.rows || orr.cols != ox.cols || !on_current_device(r) || !aligned16(r)) return none();
+    }
+    Tensor dx, dgamma, dbeta, ws;
+    if (absent(a[6])) {
+      oc.ld = ox.cols;
+    } else {
+      if (!bf16_arg(a[6])) return none();
+      dx = tensor(a[6]);
+      oc = operand3(dx);
+      if (!oc.ok || oc.rows != ox.rows || oc.cols != ox.cols || oc.ld < oc.cols || !on_current_device(dx) || !aligned16(dx))
+        return none();
+    }
+    const int rows = (int)ox.rows, cols = (int)ox.cols;
+    if (!absent(a[7])) {
+      if (!f32_arg(a[7])) return none();
+      ws = tensor(a[7]);
+      if (ws.dim() != 2 || !ws.is_contiguous() || ws.size(1) != 2 * ox.cols || !on_current_device(ws) || !aligned16(ws) ||
+          ws.size(0) != kr_layernorm_bwd_partial_rows(rows, cols))
+        return none();
+    }
+    int rc;
+    {
+      WithoutInterpreter free;
+      if (!dx.defined()) dx = matrix(rows, cols, x);
+      if (!ws.defined()) {
+        dgamma = at::empty({ox.cols}, x.options());
+        dbeta = at::empty({ox.cols}, x.options());
+        ws = bytes(kr_layernorm_bwd_workspace_bytes(rows, cols), x);
+      }
+      rc = kr_layernorm_bwd(ptr(dy), ptr(x), (const float*)ptr(mean), (const float*)ptr(rstd), ptr(gamma), ptr_or_null(a[5]), ptr(dx),
+                            dgamma.defined() ? ptr(dgamma) : nullptr, dbeta.defined() ? ptr(dbeta) : nullptr, ptr(ws), rows, cols,
+                            od.ld, ox.ld, ox.run_rows, ox.run_ld, orr.ld, orr.run_rows, orr.run_ld, oc.ld, oc.run_rows, oc.run_ld,
+                            stream());
+    }
+    if (rc != KR_OK) return failed("kr_layernorm_bwd(rows=" + std::to_string(rows) + ", cols=" + std::to_string(cols) + ")", rc);
+    PyObject* pdx = absent(a[6]) ? wrap(std::move(dx)) : Py_NewRef(a[6]);
+    PyObject* pdg = dgamma.defined() ? wrap(std::move(dgamma)) : Py_NewRef(Py_None);
+    PyObject* pdb = dbeta.defined() ? wrap(std::move(dbeta)) : Py_NewRef(Py_None);
+    return Py_BuildValue("(NNN)", pdx, pdg, pdb);
+  });
+}
+
+// ---- rotary positions on several axes ------------------------------------------------------------------------
+// rope_axes_fused(fused [s, b, ng, per + 2, hd], per, positions [axes, b, s], inv_freq [hd / 2] fp64, sections, interleaved, backward,
+// out or None) -> out
+PyObject* py_rope_axes_fused(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  return guarded([&]() -> PyObject* {
+    if (n_args != 8 || !bf16_arg(a[0]) || !is_tensor(a[2]) || !is_tensor(a[3]) || !PyTuple_Check(a[4])) return none();
+    const Tensor &f = tensor(a[0]), &p = tensor(a[2]), &inv = tensor(a[3]);
+    const int64_t per = integer(a[1]);
+    if (f.dim() != 5 || !f.is_contiguous() || f.size(3) != per + 2 || !f.numel() || !on_current_device(f) || !aligned16(f)) return none();
+    const int64_t s = f.size(0), b = f.size(1), slots = f.size(3), heads = f.size(2) * slots, hd = f.size(4);
+    const Py_ssize_t axes = PyTuple_GET_SIZE(a[4]);
+    if (!fits_int(s) || !fits_int(b) || !fits_int(heads) || axes < 1 || axes > KR_ROPE_MAX_AXES) return none();
+    if (!on_device(p, at::kLong) || !on_current_device(p) || p.dim() != 3 || p.size(0) != axes || p.size(1) != b || p.size(2) != s)
+      return none();
+    if (!on_device(inv, at::kDouble) || !on_current_device(inv) || inv.dim() != 1 || !inv.is_contiguous() || inv.size(0) * 2 != hd)
+      return none();
+    int sections[KR_ROPE_MAX_AXES] = {0, 0, 0, 0};
+    int64_t total = 0;
+    for (Py_ssize_t i = 0; i < axes; ++i) {
+      const int64_t v = integer(PyTuple_GET_ITEM(a[4], i));
+      if (v < 0 || v > hd) return none();
+      sections[i] = (int)v;
+      total += v;
+    }
+    if (total * 2 != hd) return none();
+    const bool interleaved = truth(a[5]), backward = truth(a[6]);
+    Tensor out;
+    if (!absent(a[7])) {
+      if (!bf16_arg(a[7])) return none();
+      out = tensor(a[7]);
+      if (out.sizes() != f.sizes() || !out.is_contiguous() || !on_current_device(out) || !aligned16(out)) return none();
+      const char *x = (const char*)f.data_ptr(), *y = (const char*)out.data_ptr();
+      if (x != y && y < x + f.nbytes() && x < y + f.nbytes()) return none();
+    }
+    int rc;
+    {
+      WithoutInterpreter free;
+      if (!out.defined()) out = at::empty(f.sizes(), f.options());
+      rc = kr_rope_axes(ptr(f), ptr(out), (const int64_t*)ptr(p), p.stride(0), p.stride(1), p.stride(2), (int)axes,
+                        (const double*)ptr(inv), sections, interleaved, (int)s, (int)b, (int)heads, (int)hd, b * heads * hd,
+                        heads * hd, hd, b * heads * hd, heads * hd, hd, backward, (int)slots, (int)slots - 1, stream());
+    }
+    if (rc != KR_OK)
+      return failed("kr_rope_axes(s=" + std::to_string(s) + ", b=" + std::to_string(b) + ", heads=" + std::to_string(heads) +
+                        ", hd=" + std::to_string(hd) + ")",
+                    rc);
+    return absent(a[7]) ? wrap(std::move(out)) : Py_NewRef(a[7]);
+  });
+}
+
+// ---- gradient norm and clipping --------------------------------------------------------------------------------
+// The gradients of a list as the library takes them; false for any that the Python side has to word an error about.
+struct Gradients {
+  std::vector<Tensor> held;  // (the lists may change while the interpreter is free)
+  std::vector<const void*> ptrs;
+  std::vector<void*> out;
+  std::vector<int64_t> counts;
+  std::vector<int> fp32;
+};
+bool same_layout(const Tensor& a, const Tensor& b) {
+  if (a.sizes() != b.sizes()) return false;
+  if (a.numel())
+    for (int64_t d = 0; d < a.dim(); ++d)
+      if (a.size(d) != 1 && a.stride(d) != b.stride(d)) return false;
+  return true;
+}
+bool gradients(PyObject* list, PyObject* out, Gradients& g) {
+  if (!PyList_Check(list) || !PyList_GET_SIZE(list)) return false;
+  const Py_ssize_t n = PyList_GET_SIZE(list);
+  if (n > (1 << 20) || (!absent(out) && (!PyList_Check(out) || PyList_GET_SIZE(out) != n))) return false;
+  std::vector<std::pair<uintptr_t, uintptr_t>> places;
+  auto add = [&](PyObject* o, bool f32_only) {
+    if (!is_tensor(o)) return false;
+    const Tensor& t = tensor(o);
+    if (!on_current_device(t) || t.layout() != at::kStrided || symbolic(t)) return false;
+    const bool f32 = t.scalar_type() == at::kFloat;
+    if (!f32 && (f32_only || t.scalar_type() != at::kBFloat16)) return false;
+    if (t.numel()) {
+      if (!t.is_non_overlapping_and_dense()) return false;
+      const uintptr_t at = (uintptr_t)t.data_ptr();
+      places.emplace_back(at, at + t.nbytes());
+    }
+    g.held.push_back(t);
+    return true;
+  };
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    PyObject* o = PyList_GET_ITEM(list, i);
+    if (!add(o, false)) return false;
+    const Tensor& t = tensor(o);
+    g.ptrs.push_back(t.data_ptr());
+    g.counts.push_back(t.numel());
+    g.fp32.push_back(t.scalar_type() == at::kFloat);
+    if (!absent(out)) {
+      PyObject* to = PyList_GET_ITEM(out, i);
+      if (!add(to, true) || !same_layout(t, tensor(to))) return false;
+      g.out.push_back(tensor(to).data_ptr());
+    }
+  }
+  std::sort(places.begin(), places.end());
+  for (size_t i = 1; i < places.size(); ++i)
+    if (places[i - 1].second > places[i].first) return false;
+  return true;
+}
+
+// grad_norm(tensors) -> norm
+PyObject* py_grad_norm(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  return guarded([&]() -> PyObject* {
+    Gradients g;
+    if (n_args != 1 || !gradients(a[0], Py_None, g)) return none();
+    Tensor norm;
+    int rc;
+    const int n = (int)g.ptrs.size();
+    {
+      WithoutInterpreter free;
+      norm = at::empty({}, g.held[0].options().dtype(at::kFloat));
+      const size_t nbytes = kr_grad_norm_workspace_bytes(n);
+      const Tensor ws = bytes(nbytes, g.held[0]);
+      rc = kr_grad_norm(n, g.ptrs.data(), g.counts.data(), g.fp32.data(), (float*)ptr(norm), ptr(ws), nbytes, stream());
+    }
+    if (rc != KR_OK) return failed("kr_grad_norm(n=" + std::to_string(n) + ")", rc);
+    return wrap(std::move(norm));
+  });
+}
+
+// clip_grad_norm(tensors, max_norm, eps, out or None) -> norm
+PyObject* py_clip_grad_norm(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  return guarded([&]() -> PyObject* {
+    Gradients g;
+    if (n_args != 4 || !gradients(a[0], a[3], g)) return none();
+    const double max_norm = real(a[1]), eps = real(a[2]);
+    if (!(max_norm >= 0.0) || !(eps >= 0.0)) return none();
+    Tensor norm;
+    int rc;
+    const int n = (int)g.ptrs.size();
+    {
+      WithoutInterpreter free;
+      norm = at::empty({}, g.held[0].options().dtype(at::kFloat));
+      const size_t nbytes = kr_grad_norm_workspace_bytes(n);
+      const Tensor ws = bytes(nbytes, g.held[0]);
+      rc = kr_grad_clip(n, g.ptrs.data(), g.counts.data(), g.fp32.data(), absent(a[3]) ? nullptr : g.out.data(), max_norm, eps,
+                        (float*)ptr(norm), ptr(ws), nbytes, stream());
+    }
+    if (rc != KR_OK) return failed("kr_grad_clip(n=" + std::to_string(n) + ")", rc);
+    return wrap(std::move(norm));
+  });
+}
+
 // rmsnorm_dgamma(partials [n, cols] fp32, gamma) -> the weight gradient
 PyObject* py_rmsnorm_dgamma(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   return guarded([&]() -> PyObject* {
@@ -1395,6 +1634,11 @@ PyMethodDef kMethods[] = {
     {"mlp_chain_fwd", (PyCFunction)(void*)py_mlp_chain_fwd, METH_FASTCALL, nullptr},
     {"mlp_chain_bwd", (PyCFunction)(void*)py_mlp_chain_bwd, METH_FASTCALL, nullptr},
     {"attn_chain_bwd", (PyCFunction)(void*)py_attn_chain_bwd, METH_FASTCALL, nullptr},
+    {"layernorm_fwd", (PyCFunction)(void*)py_layernorm_fwd, METH_FASTCALL, nullptr},
+    {"layernorm_bwd", (PyCFunction)(void*)py_layernorm_bwd, METH_FASTCALL, nullptr},
+    {"rope_axes_fused", (PyCFunction)(void*)py_rope_axes_fused, METH_FASTCALL, nullptr},
+    {"grad_norm", (PyCFunction)(void*)py_grad_norm, METH_FASTCALL, nullptr},
+    {"clip_grad_norm", (PyCFunction)(void*)py_clip_grad_norm, METH_FASTCALL, nullptr},
     {"rmsnorm_dgamma", (PyCFunction)(void*)py_rmsnorm_dgamma, METH_FASTCALL, nullptr},
     {"quantize_blocks", (PyCFunction)(void*)py_quantize_blocks, METH_FASTCALL, nullptr},
     {"block_matmul", (PyCFunction)(void*)py_block_matmul, METH_FASTCALL, nullptr},

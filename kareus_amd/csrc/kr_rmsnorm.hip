@@ -17,16 +17,7 @@ constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * KR_WAVE;
 constexpr int kMaxBwdBlocks = 512;
 
-// Row runs: the rows of a tensor may come in runs of 2^sh consecutive rows (stride ld) whose starts are
-// `outer` elements apart — a nanobatch of 2^sh sequences cut out of a [s, b, h] tensor along b, used in
-// place.  A plain matrix has sh = 0 (outer unused).
-struct Runs {
-  int sh;
-  int64_t outer;
-};
-__device__ __forceinline__ int64_t row_at(int64_t row, int64_t ld, Runs r) {
-  return r.sh ? (row >> r.sh) * r.outer + (row & ((1 << r.sh) - 1)) * ld : row * ld;
-}
+using Runs = KrRuns;
 
 // KEEP: plain stores for small results, which the next launch finds in the memory-side cache (see rmsnorm_fwd_impl).
 template <int NCHUNK, bool KEEP>
@@ -46,7 +37,7 @@ __global__ __launch_bounds__(kThreads) void rmsnorm_fwd_kernel(const bf16* __res
     g[c] = v < nvec ? ldg8(gamma + v * 8) : zero8();
   }
   for (int row = blockIdx.x * kWaves + wave; row < rows; row += gridDim.x * kWaves) {
-    const bf16* xr = x + row_at(row, x_ld, x_runs);
+    const bf16* xr = x + kr_row_at(row, x_ld, x_runs);
     bf16x8 xv[NCHUNK];
     float ss = 0.f;
 #pragma unroll
@@ -124,9 +115,9 @@ __global__ __launch_bounds__(kThreads) void rmsnorm_bwd_kernel(
     const bool active = SPLIT == 1 || row < rows;  // SPLIT == 1: the loop bound is the wave's own
     if (SPLIT == 1 && row >= rows) break;
     const int64_t r64 = active ? row : 0;
-    const bf16* xr = x + row_at(r64, x_ld, x_runs);
+    const bf16* xr = x + kr_row_at(r64, x_ld, x_runs);
     const bf16* dr = dy + r64 * dy_ld;
-    const bf16* rr = ADD ? dres + row_at(r64, dres_ld, dres_runs) : nullptr;
+    const bf16* rr = ADD ? dres + kr_row_at(r64, dres_ld, dres_runs) : nullptr;
     const float rs = active ? rstd[r64] : 0.f;
     bf16x8 xv[NCHUNK], dv[NCHUNK], rv[ADD && FULL ? NCHUNK : 1];
 #pragma unroll
@@ -157,7 +148,7 @@ __global__ __launch_bounds__(kThreads) void rmsnorm_bwd_kernel(
       parity ^= 1;  // the next row uses the other buffer: one barrier per row is enough
     }
     dot *= inv_cols;
-    bf16* oxr = dx + row_at(r64, dx_ld, dx_runs);
+    bf16* oxr = dx + kr_row_at(r64, dx_ld, dx_runs);
 #pragma unroll
     for (int c = 0; c < NCHUNK; ++c) {
       const int v = v0 + c * 64;
@@ -274,17 +265,6 @@ inline int chunks_for(int cols) { return (cols / 8 + 63) / 64; }
   }
 
 namespace {
-// rows per run (a power of two, 1 = plain) and distance between run starts -> Runs; false if invalid
-bool make_runs(int run_rows, int64_t run_ld, int rows, Runs* out, int* rc) {
-  *out = Runs{0, 0};
-  if (run_rows == 1) return true;
-  if (run_rows < 1 || (run_rows & (run_rows - 1)) || run_ld <= 0) { *rc = KR_EINVAL; return false; }
-  if (run_rows > 1024 || run_ld % 8 || rows % run_rows) { *rc = KR_EUNSUPPORTED; return false; }
-  int sh = 0;
-  while ((1 << sh) < run_rows) ++sh;
-  *out = Runs{sh, run_ld};
-  return true;
-}
 int rmsnorm_fwd_impl(const void* x, const void* gamma, void* y, float* rstd, int rows, int cols,
                      int64_t x_ld, Runs x_runs, float eps, void* stream);
 }  // namespace
@@ -299,8 +279,8 @@ extern "C" int kr_rmsnorm_fwd_runs(const void* x, const void* gamma, void* y, fl
                                    int cols, int64_t x_ld, int x_run_rows, int64_t x_run_ld, float eps,
                                    void* stream) {
   Runs xr;
-  int rc = KR_OK;
-  if (rows <= 0 || !make_runs(x_run_rows, x_run_ld, rows, &xr, &rc)) return rc == KR_OK ? KR_EINVAL : rc;
+  if (rows <= 0) return KR_EINVAL;
+  if (const int rc = kr_make_runs(x_run_rows, x_run_ld, rows, &xr)) return rc;
   return rmsnorm_fwd_impl(x, gamma, y, rstd, rows, cols, x_ld, xr, eps, stream);
 }
 
@@ -356,11 +336,11 @@ extern "C" int kr_rmsnorm_bwd_add_runs(const void* dy, const void* x, const floa
                                        int64_t dx_ld, int dx_run_rows, int64_t dx_run_ld,
                                        void* stream) {
   BwdRuns runs;
-  int rc = KR_OK;
   if (rows <= 0) return KR_EINVAL;
-  if (!make_runs(x_run_rows, x_run_ld, rows, &runs.x, &rc)) return rc;
-  if (dres && !make_runs(dres_run_rows, dres_run_ld, rows, &runs.dres, &rc)) return rc;
-  if (!make_runs(dx_run_rows, dx_run_ld, rows, &runs.dx, &rc)) return rc;
+  if (const int rc = kr_make_runs(x_run_rows, x_run_ld, rows, &runs.x)) return rc;
+  if (dres)
+    if (const int rc = kr_make_runs(dres_run_rows, dres_run_ld, rows, &runs.dres)) return rc;
+  if (const int rc = kr_make_runs(dx_run_rows, dx_run_ld, rows, &runs.dx)) return rc;
   return rmsnorm_bwd_impl(dy, x, rstd, gamma, dres, dx, dgamma, workspace, rows, cols, dy_ld, x_ld,
                           dres_ld, dx_ld, stream, runs);
 }
