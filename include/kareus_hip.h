@@ -437,6 +437,35 @@ int kr_attn_bwd_flags(const void* dout, const void* q, const void* k, const void
                       int64_t dv_stride_s, int64_t dv_stride_b, int64_t dv_stride_h,
                       int flags, void* stream);
 
+/* Causal attention with a window and sinks: query i sees key j <= i where i - j < window (window >= 1: the last `window` keys, its own
+ * among them) or j < sinks (the first keys stay visible to all).  Tensors, strides, lse and flags as kr_attn_fwd_flags' and
+ * kr_attn_bwd_flags' (KR_ATTN_BESIDE_OTHER_STREAMS at most); hd 64 or 128, sequence strides below 2^31 / 127 elements unless hd = 128
+ * and s is a multiple of 128 (KR_EUNSUPPORTED otherwise); scale positive.  Only key tiles with a visible key are read: work and
+ * time go with s * (window + sinks).  Where window + sinks reach s nothing is hidden and the calls are those above.  Keys and values
+ * have to be finite, hidden ones too: a tile's hidden probabilities are zeros that its values are multiplied by.
+ * workspace: kr_attn_window_bwd_workspace_bytes() bytes, 16-byte aligned.                         */
+int kr_attn_window_fwd(const void* q, const void* k, const void* v, void* o, float* lse,
+                       int s, int b, int nq, int nkv, int hd, float scale,
+                       int64_t q_stride_s, int64_t q_stride_b, int64_t q_stride_g, int64_t q_stride_h,
+                       int64_t k_stride_s, int64_t k_stride_b, int64_t k_stride_h,
+                       int64_t v_stride_s, int64_t v_stride_b, int64_t v_stride_h,
+                       int64_t o_stride_s, int64_t o_stride_b, int64_t o_stride_g, int64_t o_stride_h,
+                       int window, int sinks, int flags, void* stream);
+size_t kr_attn_window_bwd_workspace_bytes(int s, int b, int nq, int nkv, int hd, int window, int sinks);
+int kr_attn_window_bwd(const void* dout, const void* q, const void* k, const void* v,
+                       const void* o, const float* lse,
+                       void* dq, void* dk, void* dv, void* workspace,
+                       int s, int b, int nq, int nkv, int hd, float scale,
+                       int64_t q_stride_s, int64_t q_stride_b, int64_t q_stride_g, int64_t q_stride_h,
+                       int64_t k_stride_s, int64_t k_stride_b, int64_t k_stride_h,
+                       int64_t v_stride_s, int64_t v_stride_b, int64_t v_stride_h,
+                       int64_t o_stride_s, int64_t o_stride_b, int64_t o_stride_g, int64_t o_stride_h,
+                       int64_t do_stride_s, int64_t do_stride_b, int64_t do_stride_g, int64_t do_stride_h,
+                       int64_t dq_stride_s, int64_t dq_stride_b, int64_t dq_stride_g, int64_t dq_stride_h,
+                       int64_t dk_stride_s, int64_t dk_stride_b, int64_t dk_stride_h,
+                       int64_t dv_stride_s, int64_t dv_stride_b, int64_t dv_stride_h,
+                       int window, int sinks, int flags, void* stream);
+
 /* ---- Ends of the layer stack: embedding and loss ------------------------------------------
  * Token embedding of one vocabulary shard.  Replaces F.embedding / weight[masked_input] and the
  * [b s h] -> [s b h] transpose of

@@ -81,6 +81,9 @@ _SIGNATURES = {
     "kr_grad_norm_workspace_bytes": (_c_size_t, [_c_int]),
     "kr_grad_norm": (_c_int, [_c_int] + [_c_void_p] * 5 + [_c_size_t, _c_void_p]),
     "kr_grad_clip": (_c_int, [_c_int] + [_c_void_p] * 4 + [ctypes.c_double, ctypes.c_double, _c_void_p, _c_void_p, _c_size_t, _c_void_p]),
+    "kr_attn_window_fwd": (_c_int, [_c_void_p] * 5 + [_c_int] * 5 + [_c_float] + [_c_i64] * 14 + [_c_int] * 3 + [_c_void_p]),
+    "kr_attn_window_bwd_workspace_bytes": (_c_size_t, [_c_int] * 7),
+    "kr_attn_window_bwd": (_c_int, [_c_void_p] * 10 + [_c_int] * 5 + [_c_float] + [_c_i64] * 28 + [_c_int] * 3 + [_c_void_p]),
     "kr_attn_fwd": (_c_int, [_c_void_p] * 5 + [_c_int] * 5 + [_c_float] + [_c_i64] * 14 + [_c_void_p]),
     "kr_attn_fwd_flags": (_c_int, [_c_void_p] * 5 + [_c_int] * 5 + [_c_float] + [_c_i64] * 14 + [_c_int, _c_void_p]),
     "kr_attn_fwd_workspace_bytes": (_c_size_t, [_c_int] * 5),
@@ -1353,11 +1356,15 @@ class HipBackend:
         return s, b, nq, nkv, hd
 
     def attn_fwd(self, q: Tensor, k: Tensor, v: Tensor, scale: float, causal: bool = True,
-                 beside_other_streams: bool = False, general_kernels: bool = False):
+                 beside_other_streams: bool = False, general_kernels: bool = False, window: int = 0, sinks: int = 0):
         """``beside_other_streams``: kernels of other streams use the compute units this launch leaves idle,
         so it is shaped for the least compute-unit time, not for its own latency.
         ``general_kernels``: any shape but head dimension 128 with whole 128-row tiles takes the general fp32
-        kernels instead of the MFMA ones."""
+        kernels instead of the MFMA ones.
+        ``window`` > 0: a query sees the last ``window`` keys up to its own and the first ``sinks``; only key tiles with a visible key are
+        read.  (Head dimensions other than 64 and 128 are padded to these through copies.  Keys and values have to be finite.)"""
+        if window or sinks:
+            return self._attn_window_fwd(q, k, v, scale, causal, beside_other_streams, general_kernels, window, sinks)
         if not causal:
             raise RuntimeError("only causal attention is implemented")
         flags = (KR_ATTN_BESIDE_OTHER_STREAMS if beside_other_streams else 0) | (KR_ATTN_GENERAL_KERNELS if general_kernels else 0)
@@ -1381,10 +1388,12 @@ class HipBackend:
 
     def attn_bwd(self, do: Tensor, q: Tensor, k: Tensor, v: Tensor, o: Tensor, lse: Tensor,
                  scale: float, causal: bool = True, beside_other_streams: bool = False,
-                 general_kernels: bool = False):
+                 general_kernels: bool = False, window: int = 0, sinks: int = 0):
         """Returns (dq, dk, dv).  If ``q`` is a grouped [s, b, ng, per, hd] view, the three
         gradients are views of one buffer laid out like the fused QKV projection output and
         carry it as ``_kr_mixed`` so the QKV-split backward can hand it on without a copy."""
+        if window or sinks:
+            return self._attn_window_bwd(do, q, k, v, o, lse, scale, causal, beside_other_streams, general_kernels, window, sinks)
         if not causal:
             raise RuntimeError("only causal attention is implemented")
         flags = (KR_ATTN_BESIDE_OTHER_STREAMS if beside_other_streams else 0) | (KR_ATTN_GENERAL_KERNELS if general_kernels else 0)
@@ -1425,6 +1434,111 @@ class HipBackend:
             for t in (dq, dk, dv):
                 t._kr_mixed = mixed
                 t._kr_fused5 = fused
+        return dq, dk, dv
+
+    # -- attention with a window and sinks ------------------------------------------------
+    def _window_case(self, q: Tensor, k: Tensor, v: Tensor, scale: float, causal: bool, general_kernels: bool, window: int, sinks: int):
+        check_window(causal, window, sinks)
+        if general_kernels:
+            raise RuntimeError("attention: the general kernels have no window")
+        if not scale > 0:
+            raise RuntimeError(f"attention: a window needs a positive scale, got {scale}")
+        self._dev(q, k, v)
+        self._bf16(q, k, v)
+        if q.dim() not in (4, 5) or k.dim() != 4 or k.shape != v.shape:
+            raise RuntimeError(f"attention: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} do not match")
+        s, b, nq, nkv, hd = self._q_dims(q, k)
+        if (k.shape[0], k.shape[1], q.shape[-1]) != (s, b, hd) or nkv == 0 or nq % nkv or not 0 < hd <= 128 or hd % 8:
+            raise RuntimeError(f"attention: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} do not match, or a head dimension "
+                               "that is no multiple of 8 up to 128")
+        self._same_device("attention", q, k, v)
+        return s, b, nq, nkv, hd
+
+    @staticmethod
+    def _window_tensor(t: Tensor, hd: int) -> Tensor:
+        """``t`` with heads of ``hd`` channels (zeros behind its own) where the kernels can read it."""
+        if t.shape[-1] != hd:
+            return torch.nn.functional.pad(t, (0, hd - t.shape[-1]))
+        if (t.stride(-1) != 1 or t.data_ptr() % 16 or any(n > 1 and (st % 8 or st <= 0) for n, st in zip(t.shape, t.stride()[:-1]))
+                or 127 * t.stride(0) + 128 >= 1 << 31):
+            t = t.contiguous()
+            return t.clone() if t.data_ptr() % 16 else t
+        return t
+
+    @classmethod
+    def _window_strides(cls, t: Tensor, per: int, query: bool):
+        """Strides as the library takes them (a dimension of one may have any)."""
+        st = [8 if n == 1 else x for n, x in zip(t.shape, t.stride())]
+        if not query:
+            return st[0], st[1], st[2]
+        if t.dim() == 5:
+            return st[0], st[1], st[2], st[3]
+        return st[0], st[1], per * st[2], st[2]
+
+    def _attn_window_fwd(self, q, k, v, scale, causal, beside, general_kernels, window, sinks):
+        flags = KR_ATTN_BESIDE_OTHER_STREAMS if beside else 0
+        if causal and not general_kernels:
+            done = self._n.attn_window_fwd(q, k, v, scale, window, sinks, flags)
+            if done is not None:
+                return done
+        s, b, nq, nkv, hd = self._window_case(q, k, v, scale, causal, general_kernels, window, sinks)
+        per, wide = nq // nkv, 64 if hd <= 64 else 128
+        o = torch.empty((s, b, nq, wide), dtype=q.dtype, device=q.device)
+        lse = torch.empty((b, nq, s), dtype=torch.float32, device=q.device)
+        if o.numel():
+            q, k, v = (self._window_tensor(t, wide) for t in (q, k, v))
+            with self._current(q):
+                rc = self.lib.kr_attn_window_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), s, b, nq, nkv,
+                                                 wide, scale, *self._window_strides(q, per, True), *self._window_strides(k, per, False),
+                                                 *self._window_strides(v, per, False), *self._window_strides(o, per, True),
+                                                 min(window, 1 << 30), min(sinks, 1 << 30), flags, self._stream())
+            self._check(rc, f"kr_attn_window_fwd(s={s}, b={b}, nq={nq}, nkv={nkv}, hd={hd}, window={window}, sinks={sinks})")
+        return (o if wide == hd else o[..., :hd].contiguous()), lse
+
+    def _attn_window_bwd(self, do, q, k, v, o, lse, scale, causal, beside, general_kernels, window, sinks):
+        flags = KR_ATTN_BESIDE_OTHER_STREAMS if beside else 0
+        if causal and not general_kernels:
+            done = self._n.attn_window_bwd(do, q, k, v, o, lse, scale, window, sinks, flags)
+            if done is not None:
+                dq, dk, dv, mixed, fused = done
+                for t in (dq, dk, dv):
+                    t._kr_mixed = mixed
+                    t._kr_fused5 = fused
+                return dq, dk, dv
+        s, b, nq, nkv, hd = self._window_case(q, k, v, scale, causal, general_kernels, window, sinks)
+        self._dev(do, o, lse)
+        self._bf16(do, o)
+        self._same_device("attention", q, do, o, lse)
+        if do.numel() != q.numel() or o.numel() != q.numel() or do.shape[:2] != (s, b) or o.shape[:2] != (s, b):
+            raise RuntimeError(f"attention: dO {tuple(do.shape)} and O {tuple(o.shape)} for q {tuple(q.shape)}")
+        if lse.dtype != torch.float32 or tuple(lse.shape) != (b, nq, s) or not lse.is_contiguous():
+            raise RuntimeError(f"attention: lse must be the forward's fp32 [{b}, {nq}, {s}]")
+        per, wide = nq // nkv, 64 if hd <= 64 else 128
+        grouped = q.dim() == 5
+        fused = torch.empty((s, b, nkv, per + 2, wide), dtype=q.dtype, device=q.device)
+        dq, dk, dv = fused[:, :, :, :per], fused[:, :, :, per], fused[:, :, :, per + 1]
+        if fused.numel():
+            do4, o4 = (self._window_tensor(t.reshape(s, b, nq, hd), wide) for t in (do, o))
+            q, k, v = (self._window_tensor(t, wide) for t in (q, k, v))
+            with self._current(q):
+                nbytes = self.lib.kr_attn_window_bwd_workspace_bytes(s, b, nq, nkv, wide, min(window, 1 << 30), min(sinks, 1 << 30))
+                ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=q.device)
+                rc = self.lib.kr_attn_window_bwd(
+                    do4.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), o4.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(),
+                    dv.data_ptr(), ws.data_ptr(), s, b, nq, nkv, wide, scale, *self._window_strides(q, per, True),
+                    *self._window_strides(k, per, False), *self._window_strides(v, per, False), *self._window_strides(o4, per, True),
+                    *self._window_strides(do4, per, True), *self._window_strides(dq, per, True), *self._window_strides(dk, per, False),
+                    *self._window_strides(dv, per, False), min(window, 1 << 30), min(sinks, 1 << 30), flags, self._stream())
+            self._check(rc, f"kr_attn_window_bwd(s={s}, b={b}, nq={nq}, nkv={nkv}, hd={hd}, window={window}, sinks={sinks})")
+        if wide != hd:
+            fused = fused[..., :hd].contiguous()
+            dq, dk, dv = fused[:, :, :, :per], fused[:, :, :, per], fused[:, :, :, per + 1]
+        if not grouped:
+            return dq.reshape(s, b, nq, hd), dk.contiguous(), dv.contiguous()
+        mixed = fused.view(s, b, nkv * (per + 2) * hd)
+        for t in (dq, dk, dv):
+            t._kr_mixed = mixed
+            t._kr_fused5 = fused
         return dq, dk, dv
 
 

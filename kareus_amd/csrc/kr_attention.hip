@@ -17,9 +17,17 @@
 //   P nor V is ever transposed through memory.
 // Tensors are addressed through (seq, batch, head) strides, so sequence-major [s, b, h, d]
 // views of the fused QKV projection are consumed in place.
+// This file is built twice: with KR_ATTN_WINDOW_TU for attention with a window and sinks (WIN instances of the kernels and the
+// kr_attn_window_* entry points), without for everything else.
 #include <initializer_list>
 
 #include "kr_common.h"
+
+#ifdef KR_ATTN_WINDOW_TU
+constexpr bool kWindow = true;
+#else
+constexpr bool kWindow = false;
+#endif
 
 namespace {
 
@@ -90,6 +98,48 @@ __device__ __forceinline__ void longest_first(int pid, int nblocks, int ntiles, 
   } else {  // a last, incomplete group keeps the plain order
     rank = lid % ntiles;
     pair = lid / ntiles;
+  }
+}
+
+// Attention with a window (WIN instances): query i sees key j <= i where i - j < window or j < sinks.  A row's keys are two stretches,
+// the sinks' tiles and, behind what lies between, the window's; where they meet or overlap they are one.
+struct Band {
+  int window, sinks;
+};
+// The key tiles of queries q0 .. q0 + rows - 1: list position n is tile of(n), n < total.
+template <int TK>
+struct BandTiles {
+  int first, sink_tiles, total;  // first tile of the window; the sinks' tiles in front of it
+  __device__ __forceinline__ BandTiles(Band band, int q0, int rows) {
+    const int lo = q0 - band.window + 1;
+    first = lo > 0 ? lo / TK : 0;
+    sink_tiles = (band.sinks + TK - 1) / TK;
+    if (sink_tiles > first) sink_tiles = first;
+    total = sink_tiles + (q0 + rows) / TK - first;
+  }
+  __device__ __forceinline__ int of(int n) const { return n < sink_tiles ? n : n - sink_tiles + first; }
+};
+// Whether some of the keys key0 .. key0 + n - 1 are out of sight, behind the window, for some of the queries up to q_last; whether
+// all are for all queries from q_first on.
+__device__ __forceinline__ bool band_hides(Band band, int key0, int n, int q_last) {
+  return q_last - key0 >= band.window && key0 + n > band.sinks;
+}
+__device__ __forceinline__ bool band_hides_all(Band band, int key0, int n, int q_first) {
+  return q_first - (key0 + n - 1) >= band.window && key0 >= band.sinks;
+}
+// Workgroup -> (tile, (batch, head) pair): rows of a window are of one length, so tiles go in sequence, a contiguous range of them to an
+// XCD; the heads of a KV group side by side (GROUPED), which share their keys, or a head's tiles, which share its queries.
+template <bool GROUPED>
+__device__ __forceinline__ void band_order(int pid, int nblocks, int ntiles, int nheads, int per, int& tile, int& pair) {
+  const int q = nblocks / kXcds, r = nblocks % kXcds, xcd = pid % kXcds;
+  const int id = xcd * q + (xcd < r ? xcd : r) + pid / kXcds;
+  if (GROUPED) {
+    const int in_group = id % per, rest = id / per;
+    tile = rest % ntiles;
+    pair = rest / ntiles * per + in_group;
+  } else {
+    tile = id % ntiles;
+    pair = id / ntiles;
   }
 }
 
@@ -269,6 +319,29 @@ namespace {
 
 
 // query-like tensors: head h of KV group g = h / per sits at g*g_ + (h % per)*h_
+// The query tile behind the last one that sees any of the keys key0 .. key0 + 127 in its window (sp: queries, in whole 128-row tiles).
+template <int TQ>
+__device__ __forceinline__ int band_query_tiles(Band band, int key0, int sp) {
+  const int64_t end = ((int64_t)key0 + 127 + band.window - 1) / TQ + 1;
+  return end < sp / TQ ? (int)end : sp / TQ;
+}
+// What queries behind the window add to the gradients of the sinks' keys (attn_bwd_sinks_kernel): sums of `chunks` stretches of queries for
+// each 32-key block of a (batch, head) pair, in the layout of a wave's accumulators, [which][channel block, value][lane].
+template <int D>
+__device__ __forceinline__ void add_sink_sums(const float* sums, int chunks, int blocks, int pair, int block, int lane,
+                                              f32x16 (&dkacc)[D / 32], f32x16 (&dvacc)[D / 32]) {
+  constexpr int N = D / 32 * 16 * 64;
+  const float* at = sums + ((int64_t)pair * blocks + block) * chunks * 2 * N + lane;
+  for (int c = 0; c < chunks; ++c, at += 2 * N)
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        dkacc[dt][e] += at[(dt * 16 + e) * 64];
+        dvacc[dt][e] += at[N + (dt * 16 + e) * 64];
+      }
+}
+
 struct QLayout {
   int64_t s_, b_, g_, h_;
   __device__ __forceinline__ int64_t at(int bi, int head, int per) const {
@@ -418,13 +491,13 @@ __device__ __forceinline__ bf16x8 bt_cols(uint32_t base, int g, int dt) {
 // straight from global memory into blocked [64][128] LDS tiles.  A SIMD hosts one wave of each
 // half, so its matrix pipe and its vector ALU are busy at the same time instead of taking
 // turns, which is what happens when co-resident waves are in the same phase.
-template <int D, bool RAGGED>
+template <int D, bool RAGGED, bool WIN>
 __global__ __launch_bounds__(512, 1) void attn_fwd_pp_kernel(
     const bf16* __restrict__ q, const bf16* __restrict__ k, const bf16* __restrict__ v,
     bf16* __restrict__ o, float* __restrict__ lse, int s, int nq, int nkv, float scale_log2,
     int64_t q_ss, int64_t q_sb, int64_t q_sg, int64_t q_sh, int64_t k_ss, int64_t k_sb,
     int64_t k_sh, int64_t v_ss, int64_t v_sb, int64_t v_sh, int64_t o_ss, int64_t o_sb,
-    int64_t o_sg, int64_t o_sh) {
+    int64_t o_sg, int64_t o_sh, Band band) {
   extern __shared__ __attribute__((aligned(16))) bf16 smem[];
   constexpr int NB = tile_rows<D> / 32;  // 32-key blocks of a tile
   constexpr int DT = D / 32, KK = D / 16;
@@ -435,12 +508,16 @@ __global__ __launch_bounds__(512, 1) void attn_fwd_pp_kernel(
   const int lane = tid & 63, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int nqt = (s + BQ - 1) / BQ;
-  int rank, pair;
-  longest_first(blockIdx.x, gridDim.x, nqt, rank, pair);
-  const int qt = nqt - 1 - rank;
+  const int per = nq / nkv;
+  int qt, rank, pair;
+  if constexpr (WIN) {
+    band_order<true>(blockIdx.x, gridDim.x, nqt, nq, per, qt, pair);
+  } else {
+    longest_first(blockIdx.x, gridDim.x, nqt, rank, pair);
+    qt = nqt - 1 - rank;
+  }
   const int head = pair % nq;
   const int bi = pair / nq;
-  const int per = nq / nkv;
   const int kvh = head / per, hj = head % per;
 
   const int q0 = qt * BQ;
@@ -462,11 +539,13 @@ __global__ __launch_bounds__(512, 1) void attn_fwd_pp_kernel(
     for (int e = 0; e < 16; ++e) oacc[dt][e] = 0.f;
   float m_run = -INFINITY, l_run = 0.f;
 
-  const int total_tiles = (q0 + BQ) / TK;       // key tiles up to the workgroup's last row
+  const BandTiles<TK> tiles(WIN ? band : Band{1, 0}, q0, BQ);
+  const int total_tiles = WIN ? tiles.total : (q0 + BQ) / TK;  // key tiles up to the workgroup's last row
   const int nsteps = (total_tiles + 1) / 2;     // steps of the workgroup
-  // With 128-key tiles their number can be odd: half 1 then has one tile less (none at all for the first
+  // With 128-key tiles, or a window's, their number can be odd: half 1 then has one tile less (none at all for the first
   // 128 queries) and idles through the last step.
-  const int nmine = D == 128 ? nsteps : (total_tiles + 1 - half) / 2;
+  constexpr bool EVEN = D == 128 && !WIN;
+  const int nmine = EVEN ? nsteps : (total_tiles + 1 - half) / 2;
   // LDS tile = 16 blocks; block b holds rows b, b+16, b+32, b+48 of the tile, 256 bytes each, in
   // the order one wave-wide request delivers them (lane p at +16 p: row b + 16 (p / 16), chunk
   // p % 16 — 16 consecutive lanes fetch one contiguous row), followed by a little padding.  With
@@ -476,7 +555,7 @@ __global__ __launch_bounds__(512, 1) void attn_fwd_pp_kernel(
   constexpr uint32_t KBLK = 1024 + 16, VBLK = 1024 + 64, KTILE = 16 * KBLK, VTILE = 16 * VBLK;
   const uint32_t kbuf = (uint32_t)(uintptr_t)(KR_LDS const bf16*)smem + half * 2 * (KTILE + VTILE);
   const uint32_t vbuf = kbuf + 2 * KTILE;
-  auto key_of = [&](int j) { return (2 * j + half) * TK; };
+  auto key_of = [&](int j) { return (WIN ? tiles.of(2 * j + half) : 2 * j + half) * TK; };
   // row-major fragment (K): row 32 t + lane%32, chunk 2 kk + h  ->  + 512 t + 32 kk
   const uint32_t kfrag_lane = (uint32_t)((lane & 15) * KBLK + ((lane >> 4) & 1) * 256 + h * 16);
   // transposed fragment (V): rows 16 g + 4 h + p/4 (+8), channels 32 dt + 16 (lane/16 % 2) +
@@ -502,16 +581,16 @@ __global__ __launch_bounds__(512, 1) void attn_fwd_pp_kernel(
     if (RAGGED && key_of(j) + TK > s)
       request_clamped<D>(kb, k_ss, key_of(j), wave + 4 * i, s, lane, dst);
     else
-      dma_b128(kreq + i * k_rows4, k_lane_off, dst);
-    if (i == 3) kreq += k_tiles2;
+      dma_b128((WIN ? kb + (int64_t)(key_of(j) + wave) * k_ss : kreq) + i * k_rows4, k_lane_off, dst);
+    if (!WIN && i == 3) kreq += k_tiles2;
   };
   auto request_v_part = [&](uint32_t tile, int j, int i) {
     const uint32_t dst = tile + (wave + 4 * i) * VBLK;
     if (RAGGED && key_of(j) + TK > s)
       request_clamped<D>(vb, v_ss, key_of(j), wave + 4 * i, s, lane, dst);
     else
-      dma_b128(vreq + i * v_rows4, v_lane_off, dst);
-    if (i == 3) vreq += v_tiles2;
+      dma_b128((WIN ? vb + (int64_t)(key_of(j) + wave) * v_ss : vreq) + i * v_rows4, v_lane_off, dst);
+    if (!WIN && i == 3) vreq += v_tiles2;
   };
   auto request_k = [&](uint32_t tile, int j) {
 #pragma unroll
@@ -531,13 +610,13 @@ __global__ __launch_bounds__(512, 1) void attn_fwd_pp_kernel(
     }
   };
 
-  if (D == 128 || nmine > 0) {
+  if (EVEN || nmine > 0) {
     request_k(kbuf, 0);
     if (nmine > 1) request_k(kbuf + KTILE, 1);
     request_v(vbuf, 0);
   }
   __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
-  if (D == 128 || nmine > 0) zero_v_tail(0);
+  if (EVEN || nmine > 0) zero_v_tail(0);
   kr_barrier();
   if (half == 1) kr_barrier();  // half 1 starts one period late
 
@@ -585,8 +664,8 @@ __global__ __launch_bounds__(512, 1) void attn_fwd_pp_kernel(
     // ---- matrix period: O^T += V^T . P^T of tile j-1, then S^T = K . Q^T of tile j
     f32x16 sacc[NB];
     __builtin_amdgcn_s_setprio(1);
-    const bool mine = D == 128 || j < nmine;
-    if (j > 0 && (D == 128 || j - 1 < nmine)) pv_step(j - 1);
+    const bool mine = EVEN || j < nmine;
+    if (j > 0 && (EVEN || j - 1 < nmine)) pv_step(j - 1);
     if (mine) {
       uint32_t ka = kbuf + (j & 1) * KTILE + kfrag_lane;
       asm volatile("" : "+v"(ka));
@@ -633,6 +712,18 @@ __global__ __launch_bounds__(512, 1) void attn_fwd_pp_kernel(
 #pragma unroll
           for (int e = 0; e < 16; ++e)
             if (t * 32 + 8 * (e >> 2) + (e & 3) > lim) sacc[t][e] = -INFINITY;
+      }
+      if (WIN && band_hides(band, key0, TK, qw0 + 31)) {
+        asm volatile("" ::: "memory");
+        const int at = key0 + 4 * h;
+        const int lim = qrow - band.window - at, from = band.sinks - at;  // offsets from `from` to lim are keys behind the window
+#pragma unroll
+        for (int t = 0; t < NB; ++t)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int c = t * 32 + 8 * (e >> 2) + (e & 3);
+            if (c <= lim && c >= from) sacc[t][e] = -INFINITY;
+          }
       }
       float mx = -INFINITY;
 #pragma unroll
@@ -688,7 +779,7 @@ __global__ __launch_bounds__(512, 1) void attn_fwd_pp_kernel(
   }
   // last matrix period: the product of the final tile
   __builtin_amdgcn_s_setprio(1);
-  if (D == 128 || nsteps - 1 < nmine) pv_step(nsteps - 1);
+  if (EVEN || nsteps - 1 < nmine) pv_step(nsteps - 1);
   __builtin_amdgcn_s_setprio(0);
   kr_barrier();
   if (half == 0) kr_barrier();  // the period half 1 is behind by
@@ -1062,13 +1153,14 @@ __global__ __launch_bounds__(256) void attn_delta_kernel(const bf16* __restrict_
 // tile one block ahead).
 // PARTIAL = true: fp32 results for this query head go to part_k / part_v [b, nq, qsplit, sp, D].
 // (Head dimension 128; attn_bwd_dkdv64_kernel below takes 64.)
-template <bool RAGGED, bool PARTIAL>
+template <bool RAGGED, bool PARTIAL, bool WIN>
 __global__ __launch_bounds__(512, 1) void attn_bwd_dkdv_kernel(
     const bf16* __restrict__ q, const bf16* __restrict__ k, const bf16* __restrict__ v,
     const bf16* __restrict__ dout, const float* __restrict__ neg_lse2, const float* __restrict__ neg_delta,
     bf16* __restrict__ dk, bf16* __restrict__ dv, float* __restrict__ part_k,
     float* __restrict__ part_v, int s, int nq, int nkv, int qsplit, int hpw, float scale, float scale_log2,
-    QLayout ql, KLayout kl, KLayout vl, QLayout dol, KLayout dkl, KLayout dvl) {
+    QLayout ql, KLayout kl, KLayout vl, QLayout dol, KLayout dkl, KLayout dvl, Band band, const float* __restrict__ sink_sums,
+    int sink_chunks) {
   extern __shared__ __attribute__((aligned(16))) bf16 smem[];
   constexpr int D = HD, TQ = tile_rows<D>;  // queries of a tile: two blocks of 32
   constexpr int DT = D / 32, KK = D / 16;
@@ -1087,7 +1179,10 @@ __global__ __launch_bounds__(512, 1) void attn_bwd_dkdv_kernel(
   const int nkt = sp / 128;
   // (a key tile's parts count as tiles of half its length; low key tiles see the most queries)
   int rank, hg;
-  longest_first(blockIdx.x, gridDim.x, nkt * qsplit, rank, hg);
+  if constexpr (WIN)
+    band_order<false>(blockIdx.x, gridDim.x, nkt * qsplit, nq / hpw, 1, rank, hg);
+  else
+    longest_first(blockIdx.x, gridDim.x, nkt * qsplit, rank, hg);
   const int part = rank % qsplit, kt = rank / qsplit;
   // A workgroup takes `hpw` consecutive query heads of one KV group, one after the other: its K / V
   // fragments and its dK / dV accumulators serve them all, so a group leaves per / hpw partial
@@ -1104,7 +1199,8 @@ __global__ __launch_bounds__(512, 1) void attn_bwd_dkdv_kernel(
   const int krow = kw0 + (lane & 31);
   const int qt_first = key0 / TQ;
   // this part's query tiles, per head
-  const int niter = (sp / TQ - qt_first - part + qsplit - 1) / qsplit;
+  const int qt_end = WIN ? band_query_tiles<TQ>(band, key0, sp) : sp / TQ;
+  const int niter = (qt_end - qt_first - part + qsplit - 1) / qsplit;
   const int nit_all = niter * hpw;                                       // ... over all heads of the workgroup
   const uint32_t lds0 = (uint32_t)(uintptr_t)(KR_LDS const bf16*)smem;
   const uint32_t xch_lane = lds0 + XCH + wave * 4096 + lane * 16;  // + parity * 16384 + slot * 1024
@@ -1175,6 +1271,15 @@ __global__ __launch_bounds__(512, 1) void attn_bwd_dkdv_kernel(
         for (int e = 0; e < 16; ++e) {
           float x = 8 * (e >> 2) + (e & 3) < lim ? -INFINITY : sacc[e];
           asm volatile("" : "+v"(x));  // keeps this a branch: off the diagonal no mask code runs
+          sacc[e] = x;
+        }
+      }
+      if (WIN && qs0 + 31 - kw0 >= band.window) {
+        const int lim = krow - qs0 - 4 * h + band.window;  // element offsets from it on are queries past the key's window
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          float x = 8 * (e >> 2) + (e & 3) >= lim ? -INFINITY : sacc[e];
+          asm volatile("" : "+v"(x));
           sacc[e] = x;
         }
       }
@@ -1386,6 +1491,9 @@ __global__ __launch_bounds__(512, 1) void attn_bwd_dkdv_kernel(
     }
   }
 
+  if (WIN && part == 0 && kw0 < band.sinks)
+    for (int hh = 0; hh < hpw; ++hh)
+      add_sink_sums<D>(sink_sums, sink_chunks, (band.sinks + 31) / 32, bi * nq + head + hh, kw0 / 32, lane, dkacc, dvacc);
   // The hand-over slice this wave read last is its own: use the other one (block parity 0, read
   // one barrier earlier by this wave only) for the output transposition.
   RowStage rs;
@@ -1423,13 +1531,14 @@ __global__ __launch_bounds__(512, 1) void attn_bwd_dkdv_kernel(
 // Everything read from LDS is requested about four slots before it is used.  dP starts from -delta, read straight into
 // the accumulator, which takes the subtraction out of every score.
 // PARTIAL = true: fp32 results for this group of heads go to part_k / part_v [b, nq / hpw, qsplit, sp, 64].
-template <bool RAGGED, bool PARTIAL>
+template <bool RAGGED, bool PARTIAL, bool WIN>
 __global__ __launch_bounds__(512, 1) void attn_bwd_dkdv64_kernel(
     const bf16* __restrict__ q, const bf16* __restrict__ k, const bf16* __restrict__ v,
     const bf16* __restrict__ dout, const float* __restrict__ neg_lse2, const float* __restrict__ neg_delta,
     bf16* __restrict__ dk, bf16* __restrict__ dv, float* __restrict__ part_k,
     float* __restrict__ part_v, int s, int nq, int nkv, int qsplit, int hpw, float scale, float scale_log2,
-    QLayout ql, KLayout kl, KLayout vl, QLayout dol, KLayout dkl, KLayout dvl) {
+    QLayout ql, KLayout kl, KLayout vl, QLayout dol, KLayout dkl, KLayout dvl, Band band, const float* __restrict__ sink_sums,
+    int sink_chunks) {
   extern __shared__ __attribute__((aligned(16))) bf16 smem[];
   constexpr int D = 64, TQ = tile_rows<D>, DT = D / 32, KK = D / 16;
   constexpr uint32_t STAGE = 2 * BT_BYTES + 8 * TQ;  // Q tile | dO tile | -lse[TQ] fp32 | -delta[TQ] fp32
@@ -1441,7 +1550,10 @@ __global__ __launch_bounds__(512, 1) void attn_bwd_dkdv64_kernel(
   const int sp = RAGGED ? (s + 127) / 128 * 128 : s;  // rows of the statistics and of the partial results
   const int nkt = sp / 128;
   int rank, hg;
-  longest_first(blockIdx.x, gridDim.x, nkt * qsplit, rank, hg);
+  if constexpr (WIN)
+    band_order<false>(blockIdx.x, gridDim.x, nkt * qsplit, nq / hpw, 1, rank, hg);
+  else
+    longest_first(blockIdx.x, gridDim.x, nkt * qsplit, rank, hg);
   const int part = rank % qsplit, kt = rank / qsplit;  // low key tiles see the most queries
   const int nhg = nq / hpw;
   const int hgroup = hg % nhg;
@@ -1452,7 +1564,8 @@ __global__ __launch_bounds__(512, 1) void attn_bwd_dkdv64_kernel(
   const int kw0 = kt * 128 + wave * 32;
   const int krow = kw0 + (lane & 31);
   const int kld = RAGGED && krow >= s ? s - 1 : krow;
-  const int niter = (nkt - kt - part + qsplit - 1) / qsplit;  // this part's query tiles, per head
+  const int qt_end = WIN ? band_query_tiles<TQ>(band, kt * 128, sp) : nkt;
+  const int niter = (qt_end - kt - part + qsplit - 1) / qsplit;  // this part's query tiles, per head
   const int nit_all = niter * hpw;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(KR_LDS const bf16*)smem;
 
@@ -1504,7 +1617,7 @@ __global__ __launch_bounds__(512, 1) void attn_bwd_dkdv64_kernel(
   auto requested = [&]() {  // on to the next tile; the next head starts over at the diagonal
     if (++req_it >= nit_all) return;
     req_qt += qsplit;
-    if (req_qt >= nkt) {
+    if (req_qt >= qt_end) {
       req_qt = kt + part;
       ++req_head;
       seek();
@@ -1568,6 +1681,15 @@ __global__ __launch_bounds__(512, 1) void attn_bwd_dkdv64_kernel(
       for (int e = 0; e < 16; ++e) {
         float v = 8 * (e >> 2) + (e & 3) < lim ? -INFINITY : x.s[e];
         asm volatile("" : "+v"(v));  // keeps this a branch: off the diagonal no mask code runs
+        x.s[e] = v;
+      }
+    }
+    if (WIN && qs0 + 31 - kw0 >= band.window) {
+      const int lim = krow - qs0 - 4 * h + band.window;  // element offsets from it on are queries past the key's window
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        float v = 8 * (e >> 2) + (e & 3) >= lim ? -INFINITY : x.s[e];
+        asm volatile("" : "+v"(v));
         x.s[e] = v;
       }
     }
@@ -1694,7 +1816,7 @@ __global__ __launch_bounds__(512, 1) void attn_bwd_dkdv64_kernel(
       uint32_t rows_n = there + rows_half, stats_n = there + stat_lane;
       asm volatile("" : "+v"(rows), "+v"(cols), "+v"(stats), "+v"(rows_n), "+v"(stats_n));
       const int q0 = qt * TQ + qoff;
-      qt = qt + qsplit >= nkt ? kt + part : qt + qsplit;  // of the next tile
+      qt = qt + qsplit >= qt_end ? kt + part : qt + qsplit;  // of the next tile
       // from the last slots of block 0 on the next tile is read (behind the last one a stale stage, unused)
       block(a, b, cols, stats, 0, rows, stats, 1, rows_n, stats_n, 0, q0 + 32, [](int) {}, [&] {
         __builtin_amdgcn_s_waitcnt(0x0f75);  // vmcnt(5): of this wave's requests only those of tile it + 2 may be on their way
@@ -1708,6 +1830,9 @@ __global__ __launch_bounds__(512, 1) void attn_bwd_dkdv64_kernel(
     }
   }
   __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): the requests behind the last tile
+  if (WIN && part == 0 && half == 0 && kw0 < band.sinks)
+    for (int hh = 0; hh < hpw; ++hh)
+      add_sink_sums<D>(sink_sums, sink_chunks, (band.sinks + 31) / 32, bi * nq + head + hh, kw0 / 32, lane, dkacc, dvacc);
   // The stages are free.  Wave w of the first half gives its dV to wave w of the second and gets its dK ([value][wave]
   // [lane] layout, 32 KB each); the first half stores dK, the second dV, through 4 KB per wave behind them.
   kr_barrier();
@@ -1735,6 +1860,143 @@ __global__ __launch_bounds__(512, 1) void attn_bwd_dkdv64_kernel(
   } else {
     store_rows_bf16<D, RAGGED>(rs, acc, mul, dv + dvl.at(bi, kvh) + (int64_t)kw0 * dvl.s_, dvl.s_, s - kw0);
   }
+}
+
+// dK and dV of the sinks' keys from the queries that have them behind their window, i - j >= window and j < sinks (the dK/dV kernels
+// above take i - j < window and add this kernel's sums to their accumulators).  These few keys are seen by every later query: a key
+// tile's workgroup that took them too would run as many times longer than the others as a row is longer than its window.
+// A workgroup has 32 keys of one (batch, query head), their K and V fragments in every wave's registers, and a stretch of the
+// queries, 128 at a time, 32 to a wave; the waves' sums are added at the end.  `chunks` stretches to a key block, each leaving its sum.
+template <int D, bool RAGGED>
+__global__ __launch_bounds__(256, 1) void attn_bwd_sinks_kernel(
+    const bf16* __restrict__ q, const bf16* __restrict__ k, const bf16* __restrict__ v, const bf16* __restrict__ dout,
+    const float* __restrict__ neg_lse2, const float* __restrict__ neg_delta, float* __restrict__ sums, int s, int nq, int nkv,
+    int chunks, float scale_log2, QLayout ql, KLayout kl, KLayout vl, QLayout dol, Band band) {
+  extern __shared__ __attribute__((aligned(16))) bf16 smem[];
+  constexpr int TQ = tile_rows<D>, NT = 128 / TQ, DT = D / 32, KK = D / 16, N = DT * 16 * 64;
+  constexpr uint32_t STAGE = 2 * NT * BT_BYTES;  // Q tiles | dO tiles of 128 queries
+  static_assert(4 * 2 * N * 4 <= 2 * STAGE, "the waves' sums must fit");
+
+  const int lane = threadIdx.x & 63, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int blocks = (band.sinks + 31) / 32;
+  const int ch = blockIdx.x % chunks, block = blockIdx.x / chunks % blocks, pair = blockIdx.x / chunks / blocks;
+  const int head = pair % nq, bi = pair / nq, per = nq / nkv, kvh = head / per;
+  const int sp = RAGGED ? (s + 127) / 128 * 128 : s;
+  const int kw0 = block * 32, krow = kw0 + (lane & 31), kld = krow < s ? krow : s - 1;
+  const bf16* kp = k + kl.at(bi, kvh) + (int64_t)kld * kl.s_;
+  const bf16* vp = v + vl.at(bi, kvh) + (int64_t)kld * vl.s_;
+  bf16x8 kf[KK], vf[KK];
+#pragma unroll
+  for (int kk = 0; kk < KK; ++kk) {
+    kf[kk] = ldg8(kp + kk * 16 + h * 8);
+    vf[kk] = ldg8(vp + kk * 16 + h * 8);
+  }
+  const bf16* qb = q + ql.at(bi, head, per);
+  const bf16* dob = dout + dol.at(bi, head, per);
+  const int64_t stat0 = ((int64_t)bi * nq + head) * sp;
+  const int qb0 = (kw0 + band.window) / 128, nqb = sp / 128 > qb0 ? sp / 128 - qb0 : 0;
+  const int lo = qb0 + (int)((int64_t)nqb * ch / chunks), hi = qb0 + (int)((int64_t)nqb * (ch + 1) / chunks);
+  const uint32_t area = (uint32_t)(uintptr_t)(KR_LDS const bf16*)smem;
+  auto request = [&](int it, int buf) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const int row0 = it * 128 + t * TQ;
+      const uint32_t to = area + buf * STAGE + t * BT_BYTES;
+      if (RAGGED && row0 + TQ > s) {
+        bt_request_clamped<D>(qb, ql.s_, row0, s, to, wave, lane);
+        bt_request_clamped<D>(dob, dol.s_, row0, s, to + NT * BT_BYTES, wave, lane);
+      } else {
+        bt_request<D>(qb + (int64_t)row0 * ql.s_, ql.s_, to, wave, lane);
+        bt_request<D>(dob + (int64_t)row0 * dol.s_, dol.s_, to + NT * BT_BYTES, wave, lane);
+      }
+    }
+  };
+  auto zero_tail = [&](int it, int buf) {
+    if (RAGGED) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const int row0 = it * 128 + t * TQ;
+        if (row0 + TQ > s) {
+          const uint32_t to = area + buf * STAGE + t * BT_BYTES;
+          bt_zero_tail<D>(row0, s, to, wave, lane);
+          bt_zero_tail<D>(row0, s, to + NT * BT_BYTES, wave, lane);
+        }
+      }
+    }
+  };
+  f32x16 dkacc[DT], dvacc[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) dkacc[dt][e] = dvacc[dt][e] = 0.f;
+  if (lo < hi) {
+    request(lo, 0);
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+    zero_tail(lo, 0);
+  }
+  kr_barrier();
+  settle_scalar_loads();
+  const int tile = D == 64 ? 0 : wave >> 1, sub = D == 64 ? wave : wave & 1;  // where this wave's 32 queries lie
+  for (int it = lo; it < hi; ++it) {
+    const int buf = (it - lo) & 1;
+    if (it + 1 < hi) request(it + 1, buf ^ 1);
+    const int qs0 = it * 128 + wave * 32;
+    if (qs0 + 31 - kw0 >= band.window) {
+      f32x4 l4[4], d4[4];
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        l4[g] = *reinterpret_cast<const f32x4*>(neg_lse2 + stat0 + qs0 + 8 * g + 4 * h);
+        d4[g] = *reinterpret_cast<const f32x4*>(neg_delta + stat0 + qs0 + 8 * g + 4 * h);
+      }
+      uint32_t q_rows = area + buf * STAGE + tile * BT_BYTES + bt_rows_lane(lane), do_rows = q_rows + NT * BT_BYTES;
+      uint32_t q_cols = area + buf * STAGE + tile * BT_BYTES + bt_cols_lane(lane), do_cols = q_cols + NT * BT_BYTES;
+      if (D == 64 || sub) {  // (sub is the wave's, not the compiler's: the tile's 32-row block as an address)
+        q_rows += (sub & 1) * 512 + (sub >> 1) * 128;
+        do_rows += (sub & 1) * 512 + (sub >> 1) * 128;
+        q_cols += (sub & 1) * 512 + (sub >> 1) * 128;
+        do_cols += (sub & 1) * 512 + (sub >> 1) * 128;
+      }
+      f32x16 sacc, dpacc;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) sacc[e] = dpacc[e] = 0.f;
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) {
+        sacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bt_rows<D>(q_rows, 0, kk), kf[kk], sacc, 0, 0, 0);
+        dpacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bt_rows<D>(do_rows, 0, kk), vf[kk], dpacc, 0, 0, 0);
+      }
+      bf16x8 pb[2], dsb[2];
+      const int lim = krow - qs0 - 4 * h + band.window;  // element offsets from it on are queries past the key's window
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const float x = __builtin_fmaf(sacc[e], scale_log2, l4[e >> 2][e & 3]);
+        const float p = 8 * (e >> 2) + (e & 3) >= lim && krow < band.sinks ? __builtin_amdgcn_exp2f(x) : 0.f;
+        pb[e >> 3][e & 7] = (bf16)p;
+        dsb[e >> 3][e & 7] = (bf16)(p * (dpacc[e] + d4[e >> 2][e & 3]));
+      }
+#pragma unroll
+      for (int k2 = 0; k2 < 2; ++k2)
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+          dvacc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bt_cols<D>(do_cols, k2, dt), pb[k2], dvacc[dt], 0, 0, 0);
+          dkacc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bt_cols<D>(q_cols, k2, dt), dsb[k2], dkacc[dt], 0, 0, 0);
+        }
+    }
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's share of the next tiles has landed
+    if (it + 1 < hi) zero_tail(it + 1, buf ^ 1);
+    kr_barrier();
+  }
+  float* const xch = reinterpret_cast<float*>(smem);  // [wave][which][value][lane]; the stages are free
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      xch[(wave * 2 * DT * 16 + dt * 16 + e) * 64 + lane] = dkacc[dt][e];
+      xch[(wave * 2 * DT * 16 + DT * 16 + dt * 16 + e) * 64 + lane] = dvacc[dt][e];
+    }
+  kr_barrier();
+  float* const to = sums + (int64_t)blockIdx.x * 2 * N;
+  for (int i = threadIdx.x; i < 2 * N; i += 256) to[i] = (xch[i] + xch[2 * N + i]) + (xch[4 * N + i] + xch[6 * N + i]);
 }
 
 // dk/dv[b, kvh, i, :] = sum over the group's query heads of the fp32 partials; one thread per
@@ -1783,12 +2045,12 @@ __global__ __launch_bounds__(256) void attn_group_reduce_kernel(
 // LDS at the end.  Chosen by the host when there are few workgroups.
 // When there are more 256-query tiles than compute units (or other streams run beside the launch; see attn_forms)
 // the host takes attn_bwd_dq_w64_kernel below instead.
-template <int D, bool RAGGED, int HALVES>
+template <int D, bool RAGGED, int HALVES, bool WIN>
 __global__ __launch_bounds__(256 * HALVES, HALVES == 1 ? 2 : 1) void attn_bwd_dq_kernel(
     const bf16* __restrict__ q, const bf16* __restrict__ k, const bf16* __restrict__ v,
     const bf16* __restrict__ dout, const float* __restrict__ lse, const float* __restrict__ neg_delta,
     bf16* __restrict__ dq, int s, int nq, int nkv, float scale, float scale_log2, QLayout ql,
-    KLayout kl, KLayout vl, QLayout dol, QLayout dql) {
+    KLayout kl, KLayout vl, QLayout dol, QLayout dql, Band band) {
   extern __shared__ __attribute__((aligned(16))) bf16 smem[];
   constexpr uint32_t STAGE = 2 * BT_BYTES;  // K tile | V tile (blocked tiles), bytes
   constexpr int TK = tile_rows<D>, NB = TK / 32, DT = D / 32, KK = D / 16;
@@ -1799,12 +2061,16 @@ __global__ __launch_bounds__(256 * HALVES, HALVES == 1 ? 2 : 1) void attn_bwd_dq
   constexpr int ROWS = BQ;  // queries per workgroup
   const int sp = RAGGED ? (s + 127) / 128 * 128 : s;
   const int nqt = sp / ROWS;
-  int rank, pair;
-  longest_first(blockIdx.x, gridDim.x, nqt, rank, pair);
-  const int qt = nqt - 1 - rank;
+  const int per = nq / nkv;
+  int qt, rank, pair;
+  if constexpr (WIN) {
+    band_order<true>(blockIdx.x, gridDim.x, nqt, nq, per, qt, pair);
+  } else {
+    longest_first(blockIdx.x, gridDim.x, nqt, rank, pair);
+    qt = nqt - 1 - rank;
+  }
   const int head = pair % nq;
   const int bi = pair / nq;
-  const int per = nq / nkv;
   const int kvh = head / per;
   const int q0 = qt * ROWS;
   const int qw0 = q0 + wave * 32;
@@ -1833,14 +2099,15 @@ __global__ __launch_bounds__(256 * HALVES, HALVES == 1 ? 2 : 1) void attn_bwd_dq
 
   // key tiles per half, up to the workgroup's last row (with 128-key tiles half 1 may have one less: its
   // last step then neither requests nor computes)
-  const int ntiles = ((q0 + BQ) / TK + HALVES - 1) / HALVES;
-  auto key_of = [&](int j) { return (HALVES * j + half) * TK; };
+  const BandTiles<TK> tiles(WIN ? band : Band{1, 0}, q0, BQ);
+  const int ntiles = ((WIN ? tiles.total : (q0 + BQ) / TK) + HALVES - 1) / HALVES;
+  auto key_of = [&](int j) { return (WIN ? tiles.of(HALVES * j + half) : HALVES * j + half) * TK; };  // (behind the last one: q0 + BQ)
   // K and V tiles go straight from global memory into two LDS stages: this half's own, or with
   // shared tiles the workgroup's, half 0 bringing in the K tile and half 1 the V tile
   const uint32_t area = (uint32_t)(uintptr_t)(KR_LDS const bf16*)smem + half * 2 * STAGE;
   auto stage_request = [&](int j, int buf) {
     const int key0 = key_of(j);
-    if (D == 64 && HALVES == 2 && key0 >= q0 + BQ) return;
+    if ((D == 64 || WIN) && HALVES == 2 && key0 >= q0 + BQ) return;
     if (RAGGED && key0 + TK > s) {
       bt_request_clamped<D>(kb, kl.s_, key0, s, area + buf * STAGE, wave, lane);
       bt_request_clamped<D>(vb, vl.s_, key0, s, area + buf * STAGE + BT_BYTES, wave, lane);
@@ -1865,7 +2132,7 @@ __global__ __launch_bounds__(256 * HALVES, HALVES == 1 ? 2 : 1) void attn_bwd_dq
     const int cur = j & 1;
     if (j + 1 < ntiles) stage_request(j + 1, cur ^ 1);
     const int key0 = key_of(j);
-    if (key0 <= qw0 + 31) {
+    if (key0 <= qw0 + 31 && !(WIN && band_hides_all(band, key0, TK, qw0))) {
       // one base register per tile and read direction; everything else is an immediate
       uint32_t k_rows = area + cur * STAGE + bt_rows_lane(lane);
       uint32_t v_rows = k_rows + BT_BYTES;
@@ -1874,7 +2141,8 @@ __global__ __launch_bounds__(256 * HALVES, HALVES == 1 ? 2 : 1) void attn_bwd_dq
       const bool need_mask = key0 + TK - 1 > qw0;  // wave-uniform: the tile on the diagonal
 #pragma unroll
       for (int t = 0; t < NB; ++t) {
-        if (D == 64 && key0 + 32 * t > qw0 + 31) continue;  // wave-uniform: beyond the diagonal
+        if ((D == 64 || WIN) && key0 + 32 * t > qw0 + 31) continue;  // wave-uniform: beyond the diagonal
+        if (WIN && band_hides_all(band, key0 + 32 * t, 32, qw0)) continue;
         f32x16 sacc, dpacc;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
@@ -1896,6 +2164,16 @@ __global__ __launch_bounds__(256 * HALVES, HALVES == 1 ? 2 : 1) void attn_bwd_dq
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             float v = 8 * (e >> 2) + (e & 3) > lim ? -INFINITY : sacc[e];
+            asm volatile("" : "+v"(v));
+            sacc[e] = v;
+          }
+        }
+        if (WIN && band_hides(band, key0 + 32 * t, 32, qw0 + 31)) {
+          const int at = key0 + t * 32 + 4 * h, lim = qrow - band.window - at, from = band.sinks - at;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int c = 8 * (e >> 2) + (e & 3);
+            float v = c <= lim && c >= from ? -INFINITY : sacc[e];
             asm volatile("" : "+v"(v));
             sacc[e] = v;
           }
@@ -2268,6 +2546,7 @@ __global__ __launch_bounds__(256, 1) void attn_bwd_dq_w64_kernel(
                                dql.s_, s - (qw0 + 32 * qb));
 }
 
+#ifndef KR_ATTN_WINDOW_TU
 // =============================================================================================
 // General path: any sequence length, head dimensions that are a multiple of 8 up to 128.
 // The kernels above are built for head dimensions 128 and 64.  With KR_ATTN_GENERAL_KERNELS, or in the forward without
@@ -2576,6 +2855,7 @@ __global__ __launch_bounds__(256) void attn_resize_rows_kernel(const float* __re
   dst[idx] = i < len_src ? src[row * len_src + i] : fill;
 }
 
+#endif  // KR_ATTN_WINDOW_TU
 }  // namespace
 
 // Build-time cap, for measuring one form of a kernel against another: the most query heads a
@@ -2626,6 +2906,7 @@ static size_t attn_bwd_fast_bytes(int s, int b, int nq, int nkv, int hd) {
   return bytes;
 }
 
+#ifndef KR_ATTN_WINDOW_TU
 extern "C" size_t kr_attn_bwd_workspace_bytes(int s, int b, int nq, int nkv, int hd) {
   if (check_attn_common(s, b, nq, nkv, hd) != KR_OK) return 0;
   if (attn_fast_path(s, hd)) return attn_bwd_fast_bytes(s, b, nq, nkv, hd);
@@ -2682,6 +2963,7 @@ int launch_resize_rows(const float* src, float* dst, int64_t n, int len_src, int
 // a KV-like tensor's stride triple as the quadruple the pad kernels take (one head per group)
 QLayout as_qlayout(const KLayout& l) { return QLayout{l.s_, l.b_, l.h_, 0}; }
 }  // namespace
+#endif  // KR_ATTN_WINDOW_TU
 
 // Which form of each kernel a launch takes.  Alone on the GPU a launch wants the shortest latency:
 // with few workgroups the keys of a row (forward, dQ) or the queries of a key tile (dK/dV) are split
@@ -2708,6 +2990,18 @@ static AttnForms attn_forms(int s, int b, int nq, int nkv, int hd, int flags) { 
 }
 
 namespace {
+// Stretches of queries that the sinks' kernel is cut into: workgroups for every unit, but few sums to add.
+int band_sink_chunks(int sp, int b, int nq, Band band) {
+  if (!band.sinks) return 0;
+  const int query_blocks = sp / 128 - band.window / 128, groups = b * nq * ((band.sinks + 31) / 32);
+  int chunks = (kr_compute_units() + groups - 1) / groups;
+  if (chunks > 8) chunks = 8;
+  return chunks < query_blocks ? chunks : query_blocks;
+}
+size_t band_sink_floats(int sp, int b, int nq, int hd, Band band) {
+  return (size_t)b * nq * ((band.sinks + 31) / 32) * band_sink_chunks(sp, b, nq, band) * 2 * (hd / 32) * 16 * 64;
+}
+
 struct BwdCall {
   const bf16 *dout, *q, *k, *v, *o;
   const float* lse;
@@ -2719,11 +3013,12 @@ struct BwdCall {
   KLayout kl, vl, dkl, dvl;
   int flags;
   hipStream_t st;
+  Band band;
 };
 
 // The MFMA backward on tensors as they lie.  The forms are chosen by the length rounded up to whole 128-row
 // tiles: the kernels walk those, whatever part of the last one exists.
-template <int D, bool RAGGED>
+template <int D, bool RAGGED, bool WIN>
 int attn_bwd_mfma(const BwdCall& c) {
   const bf16 *dout = c.dout, *q = c.q, *k = c.k, *v = c.v, *o = c.o;
   const float* lse = c.lse;
@@ -2736,8 +3031,9 @@ int attn_bwd_mfma(const BwdCall& c) {
   float* neg_delta = c.workspace;
   const int64_t rows = (int64_t)b * nq * sp;
   float* neg_lse2 = neg_delta + rows;
-  float* part_k = neg_lse2 + rows;
-  const AttnForms forms = attn_forms(sp, b, nq, c.nkv, D, c.flags);
+  float* const sink_sums = neg_lse2 + rows;
+  float* part_k = sink_sums + (WIN ? band_sink_floats(sp, b, nq, D, c.band) : 0);
+  const AttnForms forms = WIN ? AttnForms{false, false, 1} : attn_forms(sp, b, nq, c.nkv, D, c.flags);
   const int qsplit = forms.qsplit;
   float* part_v = part_k + rows * qsplit * D;
   // query heads of a KV group per dK/dV workgroup: as many as leave two workgroups per compute
@@ -2757,11 +3053,12 @@ int attn_bwd_mfma(const BwdCall& c) {
   constexpr size_t lds_dkdv = D == 64 ? 4 * (2 * BT_BYTES + 8 * tile_rows<D>) : 3 * (2 * BT_BYTES + 8 * tile_rows<D>) + 32768;
   const auto dkdv_kernel = [](bool partial) {
     if constexpr (D == 64)
-      return partial ? attn_bwd_dkdv64_kernel<RAGGED, true> : attn_bwd_dkdv64_kernel<RAGGED, false>;
+      return partial ? attn_bwd_dkdv64_kernel<RAGGED, true, WIN> : attn_bwd_dkdv64_kernel<RAGGED, false, WIN>;
     else
-      return partial ? attn_bwd_dkdv_kernel<RAGGED, true> : attn_bwd_dkdv_kernel<RAGGED, false>;
+      return partial ? attn_bwd_dkdv_kernel<RAGGED, true, WIN> : attn_bwd_dkdv_kernel<RAGGED, false, WIN>;
   };
   constexpr size_t lds_dq = 2 * (2 * BT_BYTES);  // two stages of a K and a V tile
+  constexpr size_t lds_sinks = 2 * (2 * 128 / tile_rows<D> * BT_BYTES);  // two stages of 128 queries and their gradients
   constexpr size_t lds_dq_w64 = 3 * (2 * BT_BYTES) + 4 * 4096;  // three stages + a 4 KB output stage per wave
   static const hipError_t attr_status = [&] {
     hipError_t e = hipFuncSetAttribute((const void*)dkdv_kernel(false), hipFuncAttributeMaxDynamicSharedMemorySize,
@@ -2769,14 +3066,19 @@ int attn_bwd_mfma(const BwdCall& c) {
     if (e == hipSuccess)
       e = hipFuncSetAttribute((const void*)dkdv_kernel(true), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds_dkdv);
     if (e == hipSuccess)
-      e = hipFuncSetAttribute((const void*)attn_bwd_dq_kernel<D, RAGGED, 1>,
+      e = hipFuncSetAttribute((const void*)attn_bwd_dq_kernel<D, RAGGED, 1, WIN>,
                               hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds_dq);
     if (e == hipSuccess)
-      e = hipFuncSetAttribute((const void*)attn_bwd_dq_kernel<D, RAGGED, 2>,
+      e = hipFuncSetAttribute((const void*)attn_bwd_dq_kernel<D, RAGGED, 2, WIN>,
                               hipFuncAttributeMaxDynamicSharedMemorySize, (int)(2 * lds_dq));
-    if (e == hipSuccess)
+    if constexpr (WIN) {
+      if (e == hipSuccess)
+        e = hipFuncSetAttribute((const void*)attn_bwd_sinks_kernel<D, RAGGED>, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                (int)lds_sinks);
+    } else if (e == hipSuccess) {
       e = hipFuncSetAttribute((const void*)attn_bwd_dq_w64_kernel<D, RAGGED>,
                               hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds_dq_w64);
+    }
     return e;
   }();
   if (attr_status != hipSuccess) return KR_ELAUNCH;
@@ -2784,21 +3086,32 @@ int attn_bwd_mfma(const BwdCall& c) {
   const int per = nq / nkv;
   const float scale_log2 = scale * kLog2e;
   const int dq_blocks = (sp / BQ) * nq * b;
+  int sink_chunks = 0;
   if (forms.shared_dq) {
     // 256-query tiles (see attn_forms): one wave per SIMD, 64 rows each.
     // It comes first: it also computes delta and the log2-domain copy of lse that the dK/dV kernel reads.
-    hipLaunchKernelGGL((attn_bwd_dq_w64_kernel<D, RAGGED>), dim3(dq_blocks / 2), dim3(256), lds_dq_w64, st,
-                       q, k, v, dout, o, lse,
-                       neg_delta, neg_lse2, dq, s, nq, nkv, scale, scale_log2, ql, kl, vl, dol, ol, dql);
+    if constexpr (!WIN)
+      hipLaunchKernelGGL((attn_bwd_dq_w64_kernel<D, RAGGED>), dim3(dq_blocks / 2), dim3(256), lds_dq_w64, st,
+                         q, k, v, dout, o, lse,
+                         neg_delta, neg_lse2, dq, s, nq, nkv, scale, scale_log2, ql, kl, vl, dol, ol, dql);
   } else {
     hipLaunchKernelGGL((attn_delta_kernel<D>), dim3((unsigned)((rows * (D / 8) + 255) / 256)), dim3(256), 0, st,
                        dout, o, lse, neg_delta, neg_lse2, s, sp, nq, per, rows, dol, ol);
   }
   if (hipGetLastError() != hipSuccess) return KR_ELAUNCH;
+  if constexpr (WIN) {
+    if (c.band.sinks) {
+      sink_chunks = band_sink_chunks(sp, b, nq, c.band);
+      hipLaunchKernelGGL((attn_bwd_sinks_kernel<D, RAGGED>), dim3((unsigned)(b * nq * ((c.band.sinks + 31) / 32) * sink_chunks)), dim3(256),
+                         lds_sinks, st, q, k, v, dout, neg_lse2, neg_delta, sink_sums, s, nq, nkv, sink_chunks, scale_log2, ql, kl, vl,
+                         dol, c.band);
+      if (hipGetLastError() != hipSuccess) return KR_ELAUNCH;
+    }
+  }
   const dim3 grid_kv((sp / 128) * (nq / hpw) * b * qsplit);
   hipLaunchKernelGGL(dkdv_kernel(partial), grid_kv, dim3(512), lds_dkdv, st, q, k, v, dout, neg_lse2,
                      neg_delta, dk, dv, part_k, part_v, s, nq, nkv, partial ? qsplit : 1, hpw, scale, scale_log2, ql, kl,
-                     vl, dol, dkl, dvl);
+                     vl, dol, dkl, dvl, c.band, (const float*)sink_sums, sink_chunks);
   if (partial) {
     if (hipGetLastError() != hipSuccess) return KR_ELAUNCH;
     const int64_t total = (int64_t)b * nkv * s * (D / 8);
@@ -2809,20 +3122,21 @@ int attn_bwd_mfma(const BwdCall& c) {
   if (hipGetLastError() != hipSuccess) return KR_ELAUNCH;
   if (forms.shared_dq) return kr_launch_status();  // its dQ kernel ran in front of the dK/dV kernel
   if (dq_blocks <= 4 * 256) {  // few workgroups: the longest causal rows set the time
-    hipLaunchKernelGGL((attn_bwd_dq_kernel<D, RAGGED, 2>), dim3(dq_blocks), dim3(512), 2 * lds_dq, st,
+    hipLaunchKernelGGL((attn_bwd_dq_kernel<D, RAGGED, 2, WIN>), dim3(dq_blocks), dim3(512), 2 * lds_dq, st,
                        q, k, v, dout, lse,
                        neg_delta, dq, s, nq, nkv, scale, scale_log2, ql, kl, vl, dol,
-                       dql);
+                       dql, c.band);
   } else {
-    hipLaunchKernelGGL((attn_bwd_dq_kernel<D, RAGGED, 1>), dim3(dq_blocks), dim3(256), lds_dq, st,
+    hipLaunchKernelGGL((attn_bwd_dq_kernel<D, RAGGED, 1, WIN>), dim3(dq_blocks), dim3(256), lds_dq, st,
                        q, k, v, dout, lse,
                        neg_delta, dq, s, nq, nkv, scale, scale_log2, ql, kl, vl, dol,
-                       dql);
+                       dql, c.band);
   }
   return kr_launch_status();
 }
 }  // namespace
 
+#ifndef KR_ATTN_WINDOW_TU
 static int attn_bwd_impl(const void* dout, const void* q, const void* k, const void* v,
                            const void* o, const float* lse, void* dq, void* dk, void* dv,
                            void* workspace, int s, int b, int nq, int nkv, int hd, float scale,
@@ -2903,9 +3217,9 @@ static int attn_bwd_impl(const void* dout, const void* q, const void* k, const v
     return kr_launch_status();
   }
   const BwdCall c{(const bf16*)dout, (const bf16*)q, (const bf16*)k, (const bf16*)v, (const bf16*)o, lse, (bf16*)dq,
-                  (bf16*)dk, (bf16*)dv, delta, s, b, nq, nkv, scale, ql, ol, dol, dql, kl, vl, dkl, dvl, flags, st};
-  if (hd == 64) return s % BQ ? attn_bwd_mfma<64, true>(c) : attn_bwd_mfma<64, false>(c);
-  return s % BQ ? attn_bwd_mfma<128, true>(c) : attn_bwd_mfma<128, false>(c);
+                  (bf16*)dk, (bf16*)dv, delta, s, b, nq, nkv, scale, ql, ol, dol, dql, kl, vl, dkl, dvl, flags, st, Band{0, 0}};
+  if (hd == 64) return s % BQ ? attn_bwd_mfma<64, true, kWindow>(c) : attn_bwd_mfma<64, false, kWindow>(c);
+  return s % BQ ? attn_bwd_mfma<128, true, kWindow>(c) : attn_bwd_mfma<128, false, kWindow>(c);
 }
 
 extern "C" int kr_attn_bwd(const void* dout, const void* q, const void* k, const void* v,
@@ -2937,6 +3251,8 @@ extern "C" int kr_attn_bwd_flags(const void* dout, const void* q, const void* k,
                        do_sh, dq_ss, dq_sb, dq_sg, dq_sh, dk_ss, dk_sb, dk_sh, dv_ss, dv_sb, dv_sh, flags, stream);
 }
 
+#endif  // KR_ATTN_WINDOW_TU
+
 namespace {
 struct FwdCall {
   const bf16 *q, *k, *v;
@@ -2948,12 +3264,13 @@ struct FwdCall {
   KLayout kl, vl;
   int flags;
   hipStream_t st;
+  Band band;
 };
 
-template <int D, bool RAGGED>
+template <int D, bool RAGGED, bool WIN>
 int attn_fwd_mfma(const FwdCall& c) {
   const int s = c.s, b = c.b, nq = c.nq, sp = attn_padded_len(s);
-  if (attn_forms(sp, b, nq, c.nkv, D, c.flags).shared_fwd) {
+  if constexpr (!WIN) if (attn_forms(sp, b, nq, c.nkv, D, c.flags).shared_fwd) {
     // 256-query tiles (see attn_forms): the halves share their K / V tiles
     constexpr size_t lds_sh = 3 * 16 * ((1024 + 16) + (1024 + 64));  // 100 KiB
     static const hipError_t attr_sh = hipFuncSetAttribute(
@@ -2969,15 +3286,16 @@ int attn_fwd_mfma(const FwdCall& c) {
   constexpr size_t lds_pp = 2 * 2 * 16 * ((1024 + 16) + (1024 + 64));  // 133 KiB
   static_assert(lds_pp >= 84 * 1024, "hand-over and output staging must fit");
   static const hipError_t attr_status = hipFuncSetAttribute(
-      (const void*)attn_fwd_pp_kernel<D, RAGGED>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds_pp);
+      (const void*)attn_fwd_pp_kernel<D, RAGGED, WIN>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds_pp);
   if (attr_status != hipSuccess) return KR_ELAUNCH;
-  hipLaunchKernelGGL((attn_fwd_pp_kernel<D, RAGGED>), dim3((sp / BQ) * nq * b), dim3(512), lds_pp, c.st,
+  hipLaunchKernelGGL((attn_fwd_pp_kernel<D, RAGGED, WIN>), dim3((sp / BQ) * nq * b), dim3(512), lds_pp, c.st,
                      c.q, c.k, c.v, c.o, c.lse, s, c.nq, c.nkv, c.scale * kLog2e, c.ql.s_, c.ql.b_, c.ql.g_, c.ql.h_, c.kl.s_,
-                     c.kl.b_, c.kl.h_, c.vl.s_, c.vl.b_, c.vl.h_, c.ol.s_, c.ol.b_, c.ol.g_, c.ol.h_);
+                     c.kl.b_, c.kl.h_, c.vl.s_, c.vl.b_, c.vl.h_, c.ol.s_, c.ol.b_, c.ol.g_, c.ol.h_, c.band);
   return kr_launch_status();
 }
 }  // namespace
 
+#ifndef KR_ATTN_WINDOW_TU
 static int attn_fwd_impl(const void* q, const void* k, const void* v, void* o, float* lse, int s,
                            int b, int nq, int nkv, int hd, float scale, int64_t q_ss, int64_t q_sb,
                            int64_t q_sg, int64_t q_sh, int64_t k_ss, int64_t k_sb, int64_t k_sh,
@@ -3043,9 +3361,9 @@ static int attn_fwd_impl(const void* q, const void* k, const void* v, void* o, f
   }
   const FwdCall c{(const bf16*)q, (const bf16*)k, (const bf16*)v, (bf16*)o, lse, s, b, nq, nkv, scale,
                   QLayout{q_ss, q_sb, q_sg, q_sh}, QLayout{o_ss, o_sb, o_sg, o_sh}, KLayout{k_ss, k_sb, k_sh},
-                  KLayout{v_ss, v_sb, v_sh}, flags, (hipStream_t)stream};
-  if (hd == 64) return s % BQ ? attn_fwd_mfma<64, true>(c) : attn_fwd_mfma<64, false>(c);
-  return s % BQ ? attn_fwd_mfma<128, true>(c) : attn_fwd_mfma<128, false>(c);
+                  KLayout{v_ss, v_sb, v_sh}, flags, (hipStream_t)stream, Band{0, 0}};
+  if (hd == 64) return s % BQ ? attn_fwd_mfma<64, true, kWindow>(c) : attn_fwd_mfma<64, false, kWindow>(c);
+  return s % BQ ? attn_fwd_mfma<128, true, kWindow>(c) : attn_fwd_mfma<128, false, kWindow>(c);
 }
 
 extern "C" int kr_attn_fwd(const void* q, const void* k, const void* v, void* o, float* lse, int s,
@@ -3077,3 +3395,89 @@ extern "C" int kr_attn_fwd_ws(const void* q, const void* k, const void* v, void*
   return attn_fwd_impl(q, k, v, o, lse, s, b, nq, nkv, hd, scale, q_ss, q_sb, q_sg, q_sh, k_ss, k_sb, k_sh, v_ss,
                        v_sb, v_sh, o_ss, o_sb, o_sg, o_sh, flags, stream, workspace, workspace_bytes);
 }
+#else  // KR_ATTN_WINDOW_TU
+namespace {
+// What a call asks for, as the kernels take it: no window where every key up to its own is visible to every query.
+int make_band(int s, int hd, float scale, int window, int sinks, int flags, Band* band) {
+  if (window <= 0 || sinks < 0 || !(scale > 0.f)) return KR_EINVAL;
+  if (flags & ~KR_ATTN_BESIDE_OTHER_STREAMS) return KR_EINVAL;
+  if (hd != 64 && hd != 128) return KR_EUNSUPPORTED;
+  if (sinks > s) sinks = s;
+  *band = (int64_t)window + sinks >= s ? Band{0, 0} : Band{window, sinks};
+  return KR_OK;
+}
+int check_tensors(int s, int hd, std::initializer_list<const void*> ptrs, std::initializer_list<int64_t> seq,
+                  std::initializer_list<int64_t> others) {
+  for (const void* p : ptrs)
+    if (!p || !kr_aligned16(p)) return KR_EINVAL;
+  for (int64_t st : seq)
+    if (st % 8) return KR_EINVAL;
+  for (int64_t st : others)
+    if (st % 8) return KR_EINVAL;
+  for (int64_t st : seq)
+    if (st <= 0 || 48 * st + 128 >= ((int64_t)1 << 31)) return KR_EUNSUPPORTED;
+  for (int64_t st : others)
+    if (st <= 0) return KR_EUNSUPPORTED;
+  return attn_in_place(s, hd, seq) ? KR_OK : KR_EUNSUPPORTED;
+}
+}  // namespace
+
+extern "C" int kr_attn_window_fwd(const void* q, const void* k, const void* v, void* o, float* lse, int s, int b, int nq, int nkv,
+                                  int hd, float scale, int64_t q_ss, int64_t q_sb, int64_t q_sg, int64_t q_sh, int64_t k_ss,
+                                  int64_t k_sb, int64_t k_sh, int64_t v_ss, int64_t v_sb, int64_t v_sh, int64_t o_ss, int64_t o_sb,
+                                  int64_t o_sg, int64_t o_sh, int window, int sinks, int flags, void* stream) {
+  if (!lse) return KR_EINVAL;
+  if (const int rc = check_attn_common(s, b, nq, nkv, hd)) return rc;
+  Band band;
+  if (const int rc = make_band(s, hd, scale, window, sinks, flags, &band)) return rc;
+  if (const int rc = check_tensors(s, hd, {q, k, v, o}, {q_ss, k_ss, v_ss, o_ss}, {q_sb, q_sg, q_sh, k_sb, k_sh, v_sb, v_sh, o_sb, o_sg,
+                                                                                  o_sh}))
+    return rc;
+  if (!band.window)
+    return kr_attn_fwd_ws(q, k, v, o, lse, s, b, nq, nkv, hd, scale, q_ss, q_sb, q_sg, q_sh, k_ss, k_sb, k_sh, v_ss, v_sb, v_sh, o_ss,
+                          o_sb, o_sg, o_sh, flags | KR_ATTN_IN_PLACE, nullptr, 0, stream);
+  const FwdCall c{(const bf16*)q, (const bf16*)k, (const bf16*)v, (bf16*)o, lse, s, b, nq, nkv, scale,
+                  QLayout{q_ss, q_sb, q_sg, q_sh}, QLayout{o_ss, o_sb, o_sg, o_sh}, KLayout{k_ss, k_sb, k_sh},
+                  KLayout{v_ss, v_sb, v_sh}, flags, (hipStream_t)stream, band};
+  if (hd == 64) return s % BQ ? attn_fwd_mfma<64, true, kWindow>(c) : attn_fwd_mfma<64, false, kWindow>(c);
+  return s % BQ ? attn_fwd_mfma<128, true, kWindow>(c) : attn_fwd_mfma<128, false, kWindow>(c);
+}
+
+extern "C" size_t kr_attn_window_bwd_workspace_bytes(int s, int b, int nq, int nkv, int hd, int window, int sinks) {
+  Band band;
+  if (check_attn_common(s, b, nq, nkv, hd) != KR_OK || make_band(s, hd, 1.f, window, sinks, 0, &band) != KR_OK) return 0;
+  const int sp = attn_padded_len(s);
+  if (!band.window) return attn_bwd_fast_bytes(sp, b, nq, nkv, hd);
+  const size_t rows = (size_t)b * nq * sp;
+  return (2 * rows + band_sink_floats(sp, b, nq, hd, band) + (nq != nkv ? 2 * rows * hd : 0)) * sizeof(float);
+}
+
+extern "C" int kr_attn_window_bwd(const void* dout, const void* q, const void* k, const void* v, const void* o, const float* lse,
+                                  void* dq, void* dk, void* dv, void* workspace, int s, int b, int nq, int nkv, int hd, float scale,
+                                  int64_t q_ss, int64_t q_sb, int64_t q_sg, int64_t q_sh, int64_t k_ss, int64_t k_sb, int64_t k_sh,
+                                  int64_t v_ss, int64_t v_sb, int64_t v_sh, int64_t o_ss, int64_t o_sb, int64_t o_sg, int64_t o_sh,
+                                  int64_t do_ss, int64_t do_sb, int64_t do_sg, int64_t do_sh, int64_t dq_ss, int64_t dq_sb,
+                                  int64_t dq_sg, int64_t dq_sh, int64_t dk_ss, int64_t dk_sb, int64_t dk_sh, int64_t dv_ss,
+                                  int64_t dv_sb, int64_t dv_sh, int window, int sinks, int flags, void* stream) {
+  if (!lse) return KR_EINVAL;
+  if (const int rc = check_attn_common(s, b, nq, nkv, hd)) return rc;
+  Band band;
+  if (const int rc = make_band(s, hd, scale, window, sinks, flags, &band)) return rc;
+  if (const int rc = check_tensors(s, hd, {dout, q, k, v, o, dq, dk, dv, workspace},
+                                   {q_ss, k_ss, v_ss, o_ss, do_ss, dq_ss, dk_ss, dv_ss},
+                                   {q_sb, q_sg, q_sh, k_sb, k_sh, v_sb, v_sh, o_sb, o_sg, o_sh, do_sb, do_sg, do_sh, dq_sb, dq_sg,
+                                    dq_sh, dk_sb, dk_sh, dv_sb, dv_sh}))
+    return rc;
+  if (!band.window)
+    return kr_attn_bwd_flags(dout, q, k, v, o, lse, dq, dk, dv, workspace, s, b, nq, nkv, hd, scale, q_ss, q_sb, q_sg, q_sh, k_ss, k_sb,
+                             k_sh, v_ss, v_sb, v_sh, o_ss, o_sb, o_sg, o_sh, do_ss, do_sb, do_sg, do_sh, dq_ss, dq_sb, dq_sg, dq_sh,
+                             dk_ss, dk_sb, dk_sh, dv_ss, dv_sb, dv_sh, flags, stream);
+  const BwdCall c{(const bf16*)dout, (const bf16*)q, (const bf16*)k, (const bf16*)v, (const bf16*)o, lse, (bf16*)dq, (bf16*)dk,
+                  (bf16*)dv, (float*)workspace, s, b, nq, nkv, scale, QLayout{q_ss, q_sb, q_sg, q_sh},
+                  QLayout{o_ss, o_sb, o_sg, o_sh}, QLayout{do_ss, do_sb, do_sg, do_sh}, QLayout{dq_ss, dq_sb, dq_sg, dq_sh},
+                  KLayout{k_ss, k_sb, k_sh}, KLayout{v_ss, v_sb, v_sh}, KLayout{dk_ss, dk_sb, dk_sh}, KLayout{dv_ss, dv_sb, dv_sh},
+                  flags, (hipStream_t)stream, band};
+  if (hd == 64) return s % BQ ? attn_bwd_mfma<64, true, kWindow>(c) : attn_bwd_mfma<64, false, kWindow>(c);
+  return s % BQ ? attn_bwd_mfma<128, true, kWindow>(c) : attn_bwd_mfma<128, false, kWindow>(c);
+}
+#endif  // KR_ATTN_WINDOW_TU

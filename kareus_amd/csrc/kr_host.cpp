@@ -1500,6 +1500,97 @@ PyObject* py_rope_axes_fused(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   });
 }
 
+// ---- attention with a window and sinks --------------------------------------------------------------------------
+bool window_tensor(const Tensor& t) {
+  if (!on_current_device(t) || !aligned16(t) || t.stride(-1) != 1) return false;
+  for (int64_t d = 0; d + 1 < t.dim(); ++d)
+    if (t.stride(d) % 8 || t.stride(d) <= 0) return false;
+  return true;
+}
+std::string window_name(const char* what, const AttnShape& c, int64_t window, int64_t sinks) {
+  std::string name = attn_name(what, c);
+  name.back() = ',';
+  return name + " window=" + std::to_string(window) + ", sinks=" + std::to_string(sinks) + ")";
+}
+bool window_args(const AttnShape& c, double scale, int64_t window, int64_t sinks) {
+  return c.ok && (c.hd == 64 || c.hd == 128) && scale > 0 && window > 0 && window <= (1 << 30) && sinks >= 0 && sinks <= (1 << 30);
+}
+
+// attn_window_fwd(q, k, v, scale, window, sinks, flags) -> (o [s, b, nq, hd], lse [b, nq, s])
+PyObject* py_attn_window_fwd(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  return guarded([&]() -> PyObject* {
+    if (n_args != 7 || !bf16_arg(a[0]) || !bf16_arg(a[1]) || !bf16_arg(a[2])) return none();
+    const Tensor &q = tensor(a[0]), &k = tensor(a[1]), &v = tensor(a[2]);
+    const AttnShape c = attn_shape(q, k, v);
+    const double scale = real(a[3]);
+    const int64_t window = integer(a[4]), sinks = integer(a[5]);
+    const int flags = (int)integer(a[6]);
+    if (!window_args(c, scale, window, sinks) || !window_tensor(q) || !window_tensor(k) || !window_tensor(v)) return none();
+    const QStrides sq = q_strides(q, c.per);
+    if (127 * std::max({sq.s, k.stride(0), v.stride(0)}) + 128 >= ((int64_t)1 << 31)) return none();
+    Tensor o, lse;
+    int rc;
+    {
+      WithoutInterpreter free;
+      o = at::empty({c.s, c.b, c.nq, c.hd}, q.options());
+      lse = at::empty({c.b, c.nq, c.s}, q.options().dtype(at::kFloat));
+      const QStrides so = q_strides(o, c.per);
+      rc = kr_attn_window_fwd(ptr(q), ptr(k), ptr(v), ptr(o), (float*)ptr(lse), c.s, c.b, c.nq, c.nkv, c.hd, (float)scale, sq.s, sq.b,
+                              sq.g, sq.h, k.stride(0), k.stride(1), k.stride(2), v.stride(0), v.stride(1), v.stride(2), so.s, so.b,
+                              so.g, so.h, (int)window, (int)sinks, flags, stream());
+    }
+    if (rc != KR_OK) return failed(window_name("kr_attn_window_fwd", c, window, sinks), rc);
+    PyObject *po = wrap(std::move(o)), *pl = wrap(std::move(lse));
+    return Py_BuildValue("(NN)", po, pl);
+  });
+}
+
+// attn_window_bwd(do, q, k, v, o, lse, scale, window, sinks, flags) -> (dq, dk, dv, mixed, fused) as attn_bwd's
+PyObject* py_attn_window_bwd(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  return guarded([&]() -> PyObject* {
+    if (n_args != 10) return none();
+    for (int i = 0; i < 5; ++i)
+      if (!bf16_arg(a[i])) return none();
+    if (!f32_arg(a[5])) return none();
+    const Tensor &dout = tensor(a[0]), &q = tensor(a[1]), &k = tensor(a[2]), &v = tensor(a[3]), &o = tensor(a[4]), &lse = tensor(a[5]);
+    const AttnShape c = attn_shape(q, k, v);
+    const double scale = real(a[6]);
+    const int64_t window = integer(a[7]), sinks = integer(a[8]);
+    const int flags = (int)integer(a[9]);
+    if (!window_args(c, scale, window, sinks) || !attn_bwd_ok(c, q, o, lse) || !dout.is_contiguous() || dout.numel() != o.numel() ||
+        dout.size(0) != c.s || o.size(0) != c.s || dout.dim() < 3 || o.dim() < 3 || dout.size(1) != c.b || o.size(1) != c.b)
+      return none();
+    if (!window_tensor(q) || !window_tensor(k) || !window_tensor(v) || !on_current_device(o) || !on_current_device(dout) ||
+        !on_current_device(lse) || !aligned16(o) || !aligned16(dout))
+      return none();
+    const int64_t s = c.s, b = c.b, ng = c.nkv, hd = c.hd, group = (c.per + 2) * hd, w = ng * group;
+    const int64_t os = b * c.nq * hd, ob = c.nq * hd, og = c.per * hd;
+    const QStrides sq = q_strides(q, c.per);
+    if (127 * std::max({sq.s, k.stride(0), v.stride(0), os, b * w}) + 128 >= ((int64_t)1 << 31)) return none();
+    AttnGrads g;
+    int rc;
+    {
+      WithoutInterpreter free;
+      g.fused = at::empty({s, b, ng, c.per + 2, hd}, q.options());
+      g.mixed = g.fused.view({s, b, w});
+      g.dq = g.fused.as_strided({s, b, ng, c.per, hd}, {b * w, w, group, hd, 1}, 0);
+      g.dk = g.fused.as_strided({s, b, ng, hd}, {b * w, w, group, 1}, c.per * hd);
+      g.dv = g.fused.as_strided({s, b, ng, hd}, {b * w, w, group, 1}, (c.per + 1) * hd);
+      const size_t n = kr_attn_window_bwd_workspace_bytes(c.s, c.b, c.nq, c.nkv, c.hd, (int)window, (int)sinks);
+      const Tensor ws = bytes(n < 16 ? 16 : n, q);
+      rc = kr_attn_window_bwd(ptr(dout), ptr(q), ptr(k), ptr(v), ptr(o), (const float*)ptr(lse), ptr(g.dq), ptr(g.dk), ptr(g.dv),
+                              ptr(ws), c.s, c.b, c.nq, c.nkv, c.hd, (float)scale, sq.s, sq.b, sq.g, sq.h, k.stride(0), k.stride(1),
+                              k.stride(2), v.stride(0), v.stride(1), v.stride(2), os, ob, og, hd, os, ob, og, hd, b * w, w, group, hd,
+                              b * w, w, group, b * w, w, group, (int)window, (int)sinks, flags, stream());
+    }
+    if (rc != KR_OK) return failed(window_name("kr_attn_window_bwd", c, window, sinks), rc);
+    PyObject *pq = wrap(std::move(g.dq)), *pk = wrap(std::move(g.dk)), *pv = wrap(std::move(g.dv));
+    PyObject* pm = wrap(std::move(g.mixed));
+    PyObject* pf = wrap(std::move(g.fused));
+    return Py_BuildValue("(NNNNN)", pq, pk, pv, pm, pf);
+  });
+}
+
 // ---- gradient norm and clipping --------------------------------------------------------------------------------
 // The gradients of a list as the library takes them; false for any that the Python side has to word an error about.
 struct Gradients {
@@ -1636,6 +1727,8 @@ PyMethodDef kMethods[] = {
     {"attn_chain_bwd", (PyCFunction)(void*)py_attn_chain_bwd, METH_FASTCALL, nullptr},
     {"layernorm_fwd", (PyCFunction)(void*)py_layernorm_fwd, METH_FASTCALL, nullptr},
     {"layernorm_bwd", (PyCFunction)(void*)py_layernorm_bwd, METH_FASTCALL, nullptr},
+    {"attn_window_fwd", (PyCFunction)(void*)py_attn_window_fwd, METH_FASTCALL, nullptr},
+    {"attn_window_bwd", (PyCFunction)(void*)py_attn_window_bwd, METH_FASTCALL, nullptr},
     {"rope_axes_fused", (PyCFunction)(void*)py_rope_axes_fused, METH_FASTCALL, nullptr},
     {"grad_norm", (PyCFunction)(void*)py_grad_norm, METH_FASTCALL, nullptr},
     {"clip_grad_norm", (PyCFunction)(void*)py_clip_grad_norm, METH_FASTCALL, nullptr},
