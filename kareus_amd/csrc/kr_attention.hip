@@ -325,23 +325,6 @@ __device__ __forceinline__ int band_query_tiles(Band band, int key0, int sp) {
   const int64_t end = ((int64_t)key0 + 127 + band.window - 1) / TQ + 1;
   return end < sp / TQ ? (int)end : sp / TQ;
 }
-// What queries behind the window add to the gradients of the sinks' keys (attn_bwd_sinks_kernel): sums of `chunks` stretches of queries for
-// each 32-key block of a (batch, head) pair, in the layout of a wave's accumulators, [which][channel block, value][lane].
-template <int D>
-__device__ __forceinline__ void add_sink_sums(const float* sums, int chunks, int blocks, int pair, int block, int lane,
-                                              f32x16 (&dkacc)[D / 32], f32x16 (&dvacc)[D / 32]) {
-  constexpr int N = D / 32 * 16 * 64;
-  const float* at = sums + ((int64_t)pair * blocks + block) * chunks * 2 * N + lane;
-  for (int c = 0; c < chunks; ++c, at += 2 * N)
-#pragma unroll
-    for (int dt = 0; dt < D / 32; ++dt)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        dkacc[dt][e] += at[(dt * 16 + e) * 64];
-        dvacc[dt][e] += at[N + (dt * 16 + e) * 64];
-      }
-}
-
 struct QLayout {
   int64_t s_, b_, g_, h_;
   __device__ __forceinline__ int64_t at(int bi, int head, int per) const {
@@ -836,13 +819,13 @@ __global__ __launch_bounds__(512, 1) void attn_fwd_pp_kernel(
 // tiles (V(j+2)).  K(j) is read in periods 2j (half 0) and 2j+1 (half 1), V(j) in 2j+2 and 2j+3;
 // rings of three tiles each give every request three to four periods to land.  Half 0 needs two
 // tiles fewer than half 1 (its rows end 128 earlier) and idles through the last two steps.
-template <int D, bool RAGGED>
+template <int D, bool RAGGED, bool WIN>
 __global__ __launch_bounds__(512, 1) void attn_fwd_sh_kernel(
     const bf16* __restrict__ q, const bf16* __restrict__ k, const bf16* __restrict__ v,
     bf16* __restrict__ o, float* __restrict__ lse, int s, int nq, int nkv, float scale_log2,
     int64_t q_ss, int64_t q_sb, int64_t q_sg, int64_t q_sh, int64_t k_ss, int64_t k_sb,
     int64_t k_sh, int64_t v_ss, int64_t v_sb, int64_t v_sh, int64_t o_ss, int64_t o_sb,
-    int64_t o_sg, int64_t o_sh) {
+    int64_t o_sg, int64_t o_sh, Band band) {
   extern __shared__ __attribute__((aligned(16))) bf16 smem[];
   constexpr int NB = tile_rows<D> / 32;  // 32-key blocks of a tile
   constexpr int DT = D / 32, KK = D / 16;
@@ -854,12 +837,16 @@ __global__ __launch_bounds__(512, 1) void attn_fwd_sh_kernel(
   const int lane = tid & 63, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int nqt = (s + BQ2 - 1) / BQ2;
-  int rank, pair;
-  longest_first(blockIdx.x, gridDim.x, nqt, rank, pair);
-  const int qt = nqt - 1 - rank;
+  const int per = nq / nkv;
+  int qt, rank, pair;
+  if constexpr (WIN) {
+    band_order<true>(blockIdx.x, gridDim.x, nqt, nq, per, qt, pair);
+  } else {
+    longest_first(blockIdx.x, gridDim.x, nqt, rank, pair);
+    qt = nqt - 1 - rank;
+  }
   const int head = pair % nq;
   const int bi = pair / nq;
-  const int per = nq / nkv;
   const int kvh = head / per, hj = head % per;
 
   const int q0 = qt * BQ2;
@@ -881,8 +868,12 @@ __global__ __launch_bounds__(512, 1) void attn_fwd_sh_kernel(
     for (int e = 0; e < 16; ++e) oacc[dt][e] = 0.f;
   float m_run = -INFINITY, l_run = 0.f;
 
-  const int ntiles = (q0 + BQ2) / TK;                 // tiles the workgroup walks (>= 2)
-  const int nmine = (q0 + half * 128 + 128) / TK;     // tiles with keys this half's rows see
+  const BandTiles<TK> tiles(WIN ? band : Band{1, 0}, q0, BQ2);
+  const int ntiles = WIN ? tiles.total : (q0 + BQ2) / TK;                 // tiles the workgroup walks (>= 2)
+  const int nmine = WIN ? tiles.total - (1 - half) * 128 / TK : (q0 + half * 128 + 128) / TK;     // tiles with keys this half's rows see
+  auto key_of = [&](int j) { return (WIN ? tiles.of(j) : j) * TK; };
+  // (of a window's first tiles the first half's rows alone see keys)
+  auto is_mine = [&](int j) { return j < nmine && !(WIN && band_hides_all(band, key_of(j), TK, q0 + half * 128)); };
   constexpr uint32_t KBLK = 1024 + 16, VBLK = 1024 + 64, KTILE = 16 * KBLK, VTILE = 16 * VBLK;
   const uint32_t kring = (uint32_t)(uintptr_t)(KR_LDS const bf16*)smem;
   const uint32_t vring = kring + 3 * KTILE;
@@ -901,18 +892,18 @@ __global__ __launch_bounds__(512, 1) void attn_fwd_sh_kernel(
   const uint32_t r_lane_off = tile_lane_off<D>(lane, (int)r_ss);
   auto request_part = [&](uint32_t tile, int j, int i) {
     const uint32_t dst = tile + (wave + 4 * i) * r_blk;
-    if (RAGGED && (j + 1) * TK > s)
-      request_clamped<D>(half ? vb : kb, r_ss, j * TK, wave + 4 * i, s, lane, dst);
+    if (RAGGED && key_of(j) + TK > s)
+      request_clamped<D>(half ? vb : kb, r_ss, key_of(j), wave + 4 * i, s, lane, dst);
     else
-      dma_b128(req + i * r_rows4, r_lane_off, dst);
-    if (i == 3) req += r_next;
+      dma_b128((WIN ? req + (int64_t)key_of(j) * r_ss : req) + i * r_rows4, r_lane_off, dst);
+    if (!WIN && i == 3) req += r_next;
   };
   // rows of V tile j (ring slot `slot`) beyond the sequence: as in the kernel above
   auto zero_v_tail = [&](int j, int slot) {
-    if (RAGGED && half == 1 && (j + 1) * TK > s) {
+    if (RAGGED && half == 1 && key_of(j) + TK > s) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        zero_block_tail<D>(j * TK, wave + 4 * i, s, lane, vring + slot * VTILE + (wave + 4 * i) * VBLK);
+        zero_block_tail<D>(key_of(j), wave + 4 * i, s, lane, vring + slot * VTILE + (wave + 4 * i) * VBLK);
     }
   };
 #pragma unroll
@@ -966,9 +957,9 @@ __global__ __launch_bounds__(512, 1) void attn_fwd_sh_kernel(
   for (int j = 0; j < ntiles; ++j) {
     // ---- matrix period: O^T += V^T . P^T of tile j-1, then S^T = K . Q^T of tile j
     f32x16 sacc[NB];
-    const bool mine = j < nmine;
+    const bool mine = is_mine(j);
     __builtin_amdgcn_s_setprio(1);
-    if (j > 0 && j - 1 < nmine) pv_step(slot_prev);
+    if (j > 0 && is_mine(j - 1)) pv_step(slot_prev);
     if (mine) {
       uint32_t ka = kring + slot * KTILE + kfrag_lane;
       asm volatile("" : "+v"(ka));
@@ -1005,7 +996,7 @@ __global__ __launch_bounds__(512, 1) void attn_fwd_sh_kernel(
     const bool want = j + 2 < ntiles;
     const uint32_t r_dst = r_ring + slot_req * r_tile;
     if (mine) {
-      const int key0 = j * TK;
+      const int key0 = key_of(j);
       if (key0 + TK - 1 > qw0) {
         asm volatile("" ::: "memory");  // keeps this a branch: off the diagonal no mask code runs
         const int lim = qrow - key0 - 4 * h;  // element offsets beyond it are keys after the query
@@ -1014,6 +1005,18 @@ __global__ __launch_bounds__(512, 1) void attn_fwd_sh_kernel(
 #pragma unroll
           for (int e = 0; e < 16; ++e)
             if (t * 32 + 8 * (e >> 2) + (e & 3) > lim) sacc[t][e] = -INFINITY;
+      }
+      if (WIN && band_hides(band, key0, TK, qw0 + 31)) {
+        asm volatile("" ::: "memory");
+        const int at = key0 + 4 * h;
+        const int lim = qrow - band.window - at, from = band.sinks - at;  // offsets from `from` to lim are keys behind the window
+#pragma unroll
+        for (int t = 0; t < NB; ++t)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int c = t * 32 + 8 * (e >> 2) + (e & 3);
+            if (c <= lim && c >= from) sacc[t][e] = -INFINITY;
+          }
       }
       float mx = -INFINITY;
 #pragma unroll
@@ -1067,7 +1070,7 @@ __global__ __launch_bounds__(512, 1) void attn_fwd_sh_kernel(
     slot_req = slot_req == 2 ? 0 : slot_req + 1;
   }
   // last matrix period: the product of the final tile (half 1; half 0 finished two steps ago)
-  if (ntiles - 1 < nmine) {
+  if (is_mine(ntiles - 1)) {
     __builtin_amdgcn_s_setprio(1);
     pv_step(slot_prev);
     __builtin_amdgcn_s_setprio(0);
@@ -1159,8 +1162,7 @@ __global__ __launch_bounds__(512, 1) void attn_bwd_dkdv_kernel(
     const bf16* __restrict__ dout, const float* __restrict__ neg_lse2, const float* __restrict__ neg_delta,
     bf16* __restrict__ dk, bf16* __restrict__ dv, float* __restrict__ part_k,
     float* __restrict__ part_v, int s, int nq, int nkv, int qsplit, int hpw, float scale, float scale_log2,
-    QLayout ql, KLayout kl, KLayout vl, QLayout dol, KLayout dkl, KLayout dvl, Band band, const float* __restrict__ sink_sums,
-    int sink_chunks) {
+    QLayout ql, KLayout kl, KLayout vl, QLayout dol, KLayout dkl, KLayout dvl, Band band, int part_rows) {
   extern __shared__ __attribute__((aligned(16))) bf16 smem[];
   constexpr int D = HD, TQ = tile_rows<D>;  // queries of a tile: two blocks of 32
   constexpr int DT = D / 32, KK = D / 16;
@@ -1491,15 +1493,12 @@ __global__ __launch_bounds__(512, 1) void attn_bwd_dkdv_kernel(
     }
   }
 
-  if (WIN && part == 0 && kw0 < band.sinks)
-    for (int hh = 0; hh < hpw; ++hh)
-      add_sink_sums<D>(sink_sums, sink_chunks, (band.sinks + 31) / 32, bi * nq + head + hh, kw0 / 32, lane, dkacc, dvacc);
   // The hand-over slice this wave read last is its own: use the other one (block parity 0, read
   // one barrier earlier by this wave only) for the output transposition.
   RowStage rs;
   rs.init(reinterpret_cast<char*>(smem) + XCH + wave * 4096, lane);
-  if (PARTIAL) {
-    const int64_t prow = (((int64_t)bi * nhg + hgroup) * qsplit + part) * sp + kw0;
+  if (PARTIAL || (WIN && key0 < band.sinks)) {  // (what queries behind the window add to the sinks' keys is added to their sums)
+    const int64_t prow = (((int64_t)bi * nhg + hgroup) * qsplit + part) * (WIN ? part_rows : sp) + kw0;
     store_rows_f32<D>(rs, dkacc, scale, part_k + prow * D, D);
     store_rows_f32<D>(rs, dvacc, 1.0f, part_v + prow * D, D);
   } else {
@@ -1537,8 +1536,7 @@ __global__ __launch_bounds__(512, 1) void attn_bwd_dkdv64_kernel(
     const bf16* __restrict__ dout, const float* __restrict__ neg_lse2, const float* __restrict__ neg_delta,
     bf16* __restrict__ dk, bf16* __restrict__ dv, float* __restrict__ part_k,
     float* __restrict__ part_v, int s, int nq, int nkv, int qsplit, int hpw, float scale, float scale_log2,
-    QLayout ql, KLayout kl, KLayout vl, QLayout dol, KLayout dkl, KLayout dvl, Band band, const float* __restrict__ sink_sums,
-    int sink_chunks) {
+    QLayout ql, KLayout kl, KLayout vl, QLayout dol, KLayout dkl, KLayout dvl, Band band, int part_rows) {
   extern __shared__ __attribute__((aligned(16))) bf16 smem[];
   constexpr int D = 64, TQ = tile_rows<D>, DT = D / 32, KK = D / 16;
   constexpr uint32_t STAGE = 2 * BT_BYTES + 8 * TQ;  // Q tile | dO tile | -lse[TQ] fp32 | -delta[TQ] fp32
@@ -1830,9 +1828,6 @@ __global__ __launch_bounds__(512, 1) void attn_bwd_dkdv64_kernel(
     }
   }
   __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): the requests behind the last tile
-  if (WIN && part == 0 && half == 0 && kw0 < band.sinks)
-    for (int hh = 0; hh < hpw; ++hh)
-      add_sink_sums<D>(sink_sums, sink_chunks, (band.sinks + 31) / 32, bi * nq + head + hh, kw0 / 32, lane, dkacc, dvacc);
   // The stages are free.  Wave w of the first half gives its dV to wave w of the second and gets its dK ([value][wave]
   // [lane] layout, 32 KB each); the first half stores dK, the second dV, through 4 KB per wave behind them.
   kr_barrier();
@@ -1852,8 +1847,8 @@ __global__ __launch_bounds__(512, 1) void attn_bwd_dkdv64_kernel(
   RowStage rs;
   rs.init(reinterpret_cast<char*>(smem) + 65536 + wave8 * 4096, lane);
   const float mul = half == 0 ? scale : 1.0f;
-  if (PARTIAL) {
-    const int64_t prow = (((int64_t)bi * nhg + hgroup) * qsplit + part) * sp + kw0;
+  if (PARTIAL || (WIN && kt * 128 < band.sinks)) {
+    const int64_t prow = (((int64_t)bi * nhg + hgroup) * qsplit + part) * (WIN ? part_rows : sp) + kw0;
     store_rows_f32<D>(rs, acc, mul, (half == 0 ? part_k : part_v) + prow * D, D);
   } else if (half == 0) {
     store_rows_bf16<D, RAGGED>(rs, acc, mul, dk + dkl.at(bi, kvh) + (int64_t)kw0 * dkl.s_, dkl.s_, s - kw0);
@@ -1863,7 +1858,7 @@ __global__ __launch_bounds__(512, 1) void attn_bwd_dkdv64_kernel(
 }
 
 // dK and dV of the sinks' keys from the queries that have them behind their window, i - j >= window and j < sinks (the dK/dV kernels
-// above take i - j < window and add this kernel's sums to their accumulators).  These few keys are seen by every later query: a key
+// above take i - j < window; attn_window_reduce_kernel adds the two).  These few keys are seen by every later query: a key
 // tile's workgroup that took them too would run as many times longer than the others as a row is longer than its window.
 // A workgroup has 32 keys of one (batch, query head), their K and V fragments in every wave's registers, and a stretch of the
 // queries, 128 at a time, 32 to a wave; the waves' sums are added at the end.  `chunks` stretches to a key block, each leaving its sum.
@@ -1871,11 +1866,10 @@ template <int D, bool RAGGED>
 __global__ __launch_bounds__(256, 1) void attn_bwd_sinks_kernel(
     const bf16* __restrict__ q, const bf16* __restrict__ k, const bf16* __restrict__ v, const bf16* __restrict__ dout,
     const float* __restrict__ neg_lse2, const float* __restrict__ neg_delta, float* __restrict__ sums, int s, int nq, int nkv,
-    int chunks, float scale_log2, QLayout ql, KLayout kl, KLayout vl, QLayout dol, Band band) {
+    int chunks, float scale, float scale_log2, QLayout ql, KLayout kl, KLayout vl, QLayout dol, Band band) {
   extern __shared__ __attribute__((aligned(16))) bf16 smem[];
   constexpr int TQ = tile_rows<D>, NT = 128 / TQ, DT = D / 32, KK = D / 16, N = DT * 16 * 64;
   constexpr uint32_t STAGE = 2 * NT * BT_BYTES;  // Q tiles | dO tiles of 128 queries
-  static_assert(4 * 2 * N * 4 <= 2 * STAGE, "the waves' sums must fit");
 
   const int lane = threadIdx.x & 63, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -1986,17 +1980,98 @@ __global__ __launch_bounds__(256, 1) void attn_bwd_sinks_kernel(
     if (it + 1 < hi) zero_tail(it + 1, buf ^ 1);
     kr_barrier();
   }
-  float* const xch = reinterpret_cast<float*>(smem);  // [wave][which][value][lane]; the stages are free
+  // The stages are free: every wave leaves its sums there, [wave][which][row][channel], rows 4 floats longer than they are so that the
+  // lanes' 16 bytes are in banks of their own; all four waves' are added and stored as rows of D channels, dK's in front of dV's.
+  constexpr int LD = D + 4;
+  float* const xch = reinterpret_cast<float*>(smem);
+  float* const mine = xch + (wave * 64 + (lane & 31)) * LD + 4 * h;
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      xch[(wave * 2 * DT * 16 + dt * 16 + e) * 64 + lane] = dkacc[dt][e];
-      xch[(wave * 2 * DT * 16 + DT * 16 + dt * 16 + e) * 64 + lane] = dvacc[dt][e];
+    for (int g = 0; g < 4; ++g) {
+      f32x4 a, c;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        a[e] = dkacc[dt][4 * g + e] * scale;
+        c[e] = dvacc[dt][4 * g + e];
+      }
+      *reinterpret_cast<f32x4*>(mine + 32 * dt + 8 * g) = a;
+      *reinterpret_cast<f32x4*>(mine + 32 * LD + 32 * dt + 8 * g) = c;
     }
   kr_barrier();
   float* const to = sums + (int64_t)blockIdx.x * 2 * N;
-  for (int i = threadIdx.x; i < 2 * N; i += 256) to[i] = (xch[i] + xch[2 * N + i]) + (xch[4 * N + i] + xch[6 * N + i]);
+  for (int i = threadIdx.x * 4; i < 2 * N; i += 1024) {
+    const float* from = xch + i / D * LD + i % D;
+    f32x4 v[4];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) v[w] = *reinterpret_cast<const f32x4*>(from + w * 64 * LD);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[0][e] = (v[0][e] + v[1][e]) + (v[2][e] + v[3][e]);
+    *reinterpret_cast<f32x4*>(to + i) = v[0];
+  }
+}
+
+// dK and dV of the first `rows` keys: the fp32 sums of the dK/dV kernel over a group's `slots` workgroups, of part_rows rows each, one
+// thread per 8 channels.  The first `sink_blocks` workgroups have the sinks' keys, to which those of attn_bwd_sinks_kernel over the group's
+// heads and their stretches of queries are added, up to 16 of a head: 16 threads share them and add theirs in a fixed order.
+template <int D>
+__global__ __launch_bounds__(256) void attn_window_reduce_kernel(
+    const float* __restrict__ part_k, const float* __restrict__ part_v, const float* __restrict__ sums, bf16* __restrict__ dk,
+    bf16* __restrict__ dv, int rows, int part_rows, int slots, int nkv, int per, int chunks, int sink_blocks, int groups, KLayout dkl,
+    KLayout dvl, Band band) {
+  constexpr int VEC = D / 8, N = 2 * 32 * D;
+  __shared__ f32x4 red[4][16][16];  // [values][share][place]
+  const bool sinks = (int)blockIdx.x < sink_blocks;
+  const int share = sinks ? threadIdx.x / 16 : 0, place = threadIdx.x % 16;
+  // (bi, kvh, si, chunk of 8): of the sinks' keys, or of those behind them
+  const int64_t idx = sinks ? (int64_t)blockIdx.x * 16 + place : (int64_t)(blockIdx.x - sink_blocks) * 256 + threadIdx.x;
+  const int first = sinks ? 0 : band.sinks, count = sinks ? band.sinks : rows - band.sinks;
+  const int c = (int)(idx % VEC);
+  const int si = first + (int)((idx / VEC) % count);
+  const int64_t group = idx / VEC / count;  // bi * nkv + kvh
+  const bool there = group < groups;
+  if (!sinks && !there) return;
+  const int kvh = (int)(group % nkv), bi = (int)(group / nkv);
+  f32x4 a[4];  // dK, dV
+#pragma unroll
+  for (int i = 0; i < 4; ++i) a[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  auto add = [&](const float* pk, const float* pv) {
+    a[0] += *reinterpret_cast<const f32x4*>(pk);
+    a[1] += *reinterpret_cast<const f32x4*>(pk + 4);
+    a[2] += *reinterpret_cast<const f32x4*>(pv);
+    a[3] += *reinterpret_cast<const f32x4*>(pv + 4);
+  };
+  if (share == 0 && there) {
+    for (int j = 0; j < slots; ++j) {
+      const int64_t off = ((group * slots + j) * part_rows + si) * D + c * 8;
+      add(part_k + off, part_v + off);
+    }
+  }
+  if (sinks) {
+    const int blocks = (band.sinks + 31) / 32;
+    if (there) {
+      for (int j = 0; j < per; ++j)
+        for (int ch = share; ch < chunks; ch += 16) {
+          const float* at = sums + (((group * per + j) * blocks + si / 32) * chunks + ch) * N + (si % 32) * D + c * 8;
+          add(at, at + 32 * D);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) red[i][share][place] = a[i];
+    kr_barrier();
+    if (share || !there) return;
+    for (int j = 1; j < 16; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) a[i] += red[i][j][place];
+  }
+  bf16x8 ok, ov;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    ok[e] = (bf16)a[e >> 2][e & 3];
+    ov[e] = (bf16)a[2 + (e >> 2)][e & 3];
+  }
+  stg8(dk + dkl.at(bi, kvh) + (int64_t)si * dkl.s_ + c * 8, ok);
+  stg8(dv + dvl.at(bi, kvh) + (int64_t)si * dvl.s_ + c * 8, ov);
 }
 
 // dk/dv[b, kvh, i, :] = sum over the group's query heads of the fp32 partials; one thread per
@@ -2050,7 +2125,8 @@ __global__ __launch_bounds__(256 * HALVES, HALVES == 1 ? 2 : 1) void attn_bwd_dq
     const bf16* __restrict__ q, const bf16* __restrict__ k, const bf16* __restrict__ v,
     const bf16* __restrict__ dout, const float* __restrict__ lse, const float* __restrict__ neg_delta,
     bf16* __restrict__ dq, int s, int nq, int nkv, float scale, float scale_log2, QLayout ql,
-    KLayout kl, KLayout vl, QLayout dol, QLayout dql, Band band) {
+    KLayout kl, KLayout vl, QLayout dol, QLayout dql, Band band, const bf16* __restrict__ o, QLayout ol,
+    float* __restrict__ neg_delta_out, float* __restrict__ neg_lse2_out) {
   extern __shared__ __attribute__((aligned(16))) bf16 smem[];
   constexpr uint32_t STAGE = 2 * BT_BYTES;  // K tile | V tile (blocked tiles), bytes
   constexpr int TK = tile_rows<D>, NB = TK / 32, DT = D / 32, KK = D / 16;
@@ -2088,8 +2164,32 @@ __global__ __launch_bounds__(256 * HALVES, HALVES == 1 ? 2 : 1) void attn_bwd_dq
     dof[kk] = ldg8(dop + kk * 16 + h * 8);
   }
   const int64_t stat = (int64_t)bi * nq + head;
-  const float neg_lse = -lse[stat * s + qld] * kLog2e;
-  const float my_neg_delta = neg_delta[stat * sp + qld];
+  float neg_lse = -lse[stat * s + qld] * kLog2e;
+  float my_neg_delta;
+  if constexpr (WIN) {
+    // no pre-pass: delta of its rows from the dO fragments that a wave holds anyway, written with -lse in the log2 domain for the dK/dV
+    // kernels, which are launched behind this one
+    const bf16* op = o + ol.at(bi, head, per) + (int64_t)qld * ol.s_;
+    float dsum = 0.f;  // this lane's half of the row (channels 16 kk + 8 h ..)
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+      const bf16x8 of = ldg8(op + kk * 16 + h * 8);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) dsum += (float)dof[kk][e] * (float)of[e];
+    }
+    dsum += __shfl_xor(dsum, 32, KR_WAVE);
+    my_neg_delta = -dsum;
+    if (RAGGED && qrow >= s) {  // rows the dK/dV kernels must not see
+      my_neg_delta = 0.f;
+      neg_lse = -kPadLse * kLog2e;
+    }
+    if (h == 0 && half == 0) {
+      neg_delta_out[stat * sp + qrow] = my_neg_delta;
+      neg_lse2_out[stat * sp + qrow] = neg_lse;
+    }
+  } else {
+    my_neg_delta = neg_delta[stat * sp + qld];
+  }
 
   f32x16 dqacc[DT];
 #pragma unroll
@@ -2994,8 +3094,8 @@ namespace {
 int band_sink_chunks(int sp, int b, int nq, Band band) {
   if (!band.sinks) return 0;
   const int query_blocks = sp / 128 - band.window / 128, groups = b * nq * ((band.sinks + 31) / 32);
-  int chunks = (kr_compute_units() + groups - 1) / groups;
-  if (chunks > 8) chunks = 8;
+  int chunks = kr_compute_units() / groups;  // (one workgroup fills a unit's LDS)
+  chunks = chunks < 1 ? 1 : chunks > 16 ? 16 : chunks;
   return chunks < query_blocks ? chunks : query_blocks;
 }
 size_t band_sink_floats(int sp, int b, int nq, int hd, Band band) {
@@ -3035,7 +3135,9 @@ int attn_bwd_mfma(const BwdCall& c) {
   float* part_k = sink_sums + (WIN ? band_sink_floats(sp, b, nq, D, c.band) : 0);
   const AttnForms forms = WIN ? AttnForms{false, false, 1} : attn_forms(sp, b, nq, c.nkv, D, c.flags);
   const int qsplit = forms.qsplit;
-  float* part_v = part_k + rows * qsplit * D;
+  // (with a window and no partial results of a group's heads, the sinks' key tiles leave theirs alone)
+  const int sink_rows = (c.band.sinks + 127) / 128 * 128;
+  float* part_v = part_k + (WIN && nq == nkv ? (int64_t)b * nq * sink_rows : rows * qsplit) * D;
   // query heads of a KV group per dK/dV workgroup: as many as leave two workgroups per compute
   // unit (KR_DKDV_HPW_MAX: a build-time cap, for measurements)
   int hpw = 1;
@@ -3058,7 +3160,9 @@ int attn_bwd_mfma(const BwdCall& c) {
       return partial ? attn_bwd_dkdv_kernel<RAGGED, true, WIN> : attn_bwd_dkdv_kernel<RAGGED, false, WIN>;
   };
   constexpr size_t lds_dq = 2 * (2 * BT_BYTES);  // two stages of a K and a V tile
-  constexpr size_t lds_sinks = 2 * (2 * 128 / tile_rows<D> * BT_BYTES);  // two stages of 128 queries and their gradients
+  // two stages of 128 queries and their gradients; the waves' sums
+  constexpr size_t lds_sinks_stages = 2 * (2 * 128 / tile_rows<D> * BT_BYTES), lds_sinks_sums = 4 * 64 * (D + 4) * sizeof(float);
+  constexpr size_t lds_sinks = lds_sinks_stages > lds_sinks_sums ? lds_sinks_stages : lds_sinks_sums;
   constexpr size_t lds_dq_w64 = 3 * (2 * BT_BYTES) + 4 * 4096;  // three stages + a 4 KB output stage per wave
   static const hipError_t attr_status = [&] {
     hipError_t e = hipFuncSetAttribute((const void*)dkdv_kernel(false), hipFuncAttributeMaxDynamicSharedMemorySize,
@@ -3086,14 +3190,31 @@ int attn_bwd_mfma(const BwdCall& c) {
   const int per = nq / nkv;
   const float scale_log2 = scale * kLog2e;
   const int dq_blocks = (sp / BQ) * nq * b;
+  const auto launch_dq = [&] {
+    // few workgroups: the longest causal rows set the time; a window's are of one length, and two workgroups of four waves to a unit start
+    // and end beside each other (one of eight waves -> those, us of the whole backward: 384 workgroups, 3 x 2007 tokens, window 500 140 ->
+    // 133; 1024, 2 x 8192 of heads of 64, 128 168 -> 134, 16384 of 128, 4096 969 -> 946; 256, 4096, 512 63 -> 65)
+    if (dq_blocks <= (WIN ? kr_compute_units() : 4 * 256)) {
+      hipLaunchKernelGGL((attn_bwd_dq_kernel<D, RAGGED, 2, WIN>), dim3(dq_blocks), dim3(512), 2 * lds_dq, st,
+                         q, k, v, dout, lse,
+                         neg_delta, dq, s, nq, nkv, scale, scale_log2, ql, kl, vl, dol,
+                         dql, c.band, o, ol, neg_delta, neg_lse2);
+    } else {
+      hipLaunchKernelGGL((attn_bwd_dq_kernel<D, RAGGED, 1, WIN>), dim3(dq_blocks), dim3(256), lds_dq, st,
+                         q, k, v, dout, lse,
+                         neg_delta, dq, s, nq, nkv, scale, scale_log2, ql, kl, vl, dol,
+                         dql, c.band, o, ol, neg_delta, neg_lse2);
+    }
+  };
   int sink_chunks = 0;
-  if (forms.shared_dq) {
+  if constexpr (WIN) {
+    launch_dq();  // it comes first: the other kernels read the statistics that it leaves
+  } else if (forms.shared_dq) {
     // 256-query tiles (see attn_forms): one wave per SIMD, 64 rows each.
     // It comes first: it also computes delta and the log2-domain copy of lse that the dK/dV kernel reads.
-    if constexpr (!WIN)
-      hipLaunchKernelGGL((attn_bwd_dq_w64_kernel<D, RAGGED>), dim3(dq_blocks / 2), dim3(256), lds_dq_w64, st,
-                         q, k, v, dout, o, lse,
-                         neg_delta, neg_lse2, dq, s, nq, nkv, scale, scale_log2, ql, kl, vl, dol, ol, dql);
+    hipLaunchKernelGGL((attn_bwd_dq_w64_kernel<D, RAGGED>), dim3(dq_blocks / 2), dim3(256), lds_dq_w64, st,
+                       q, k, v, dout, o, lse,
+                       neg_delta, neg_lse2, dq, s, nq, nkv, scale, scale_log2, ql, kl, vl, dol, ol, dql);
   } else {
     hipLaunchKernelGGL((attn_delta_kernel<D>), dim3((unsigned)((rows * (D / 8) + 255) / 256)), dim3(256), 0, st,
                        dout, o, lse, neg_delta, neg_lse2, s, sp, nq, per, rows, dol, ol);
@@ -3103,7 +3224,7 @@ int attn_bwd_mfma(const BwdCall& c) {
     if (c.band.sinks) {
       sink_chunks = band_sink_chunks(sp, b, nq, c.band);
       hipLaunchKernelGGL((attn_bwd_sinks_kernel<D, RAGGED>), dim3((unsigned)(b * nq * ((c.band.sinks + 31) / 32) * sink_chunks)), dim3(256),
-                         lds_sinks, st, q, k, v, dout, neg_lse2, neg_delta, sink_sums, s, nq, nkv, sink_chunks, scale_log2, ql, kl, vl,
+                         lds_sinks, st, q, k, v, dout, neg_lse2, neg_delta, sink_sums, s, nq, nkv, sink_chunks, scale, scale_log2, ql, kl, vl,
                          dol, c.band);
       if (hipGetLastError() != hipSuccess) return KR_ELAUNCH;
     }
@@ -3111,8 +3232,18 @@ int attn_bwd_mfma(const BwdCall& c) {
   const dim3 grid_kv((sp / 128) * (nq / hpw) * b * qsplit);
   hipLaunchKernelGGL(dkdv_kernel(partial), grid_kv, dim3(512), lds_dkdv, st, q, k, v, dout, neg_lse2,
                      neg_delta, dk, dv, part_k, part_v, s, nq, nkv, partial ? qsplit : 1, hpw, scale, scale_log2, ql, kl,
-                     vl, dol, dkl, dvl, c.band, (const float*)sink_sums, sink_chunks);
-  if (partial) {
+                     vl, dol, dkl, dvl, c.band, partial ? sp : sink_rows);
+  if constexpr (WIN) {
+    const int reduced = partial ? s : sink_rows < s ? sink_rows : s;
+    if (reduced) {
+      if (hipGetLastError() != hipSuccess) return KR_ELAUNCH;
+      const int64_t sink_vectors = (int64_t)b * nkv * c.band.sinks * (D / 8), others = (int64_t)b * nkv * (reduced - c.band.sinks) * (D / 8);
+      const unsigned sink_blocks = (unsigned)((sink_vectors + 15) / 16);
+      hipLaunchKernelGGL((attn_window_reduce_kernel<D>), dim3(sink_blocks + (unsigned)((others + 255) / 256)), dim3(256), 0, st, part_k,
+                         part_v, sink_sums, dk, dv, reduced, partial ? sp : sink_rows, nq / hpw / nkv, nkv, per, sink_chunks,
+                         (int)sink_blocks, b * nkv, dkl, dvl, c.band);
+    }
+  } else if (partial) {
     if (hipGetLastError() != hipSuccess) return KR_ELAUNCH;
     const int64_t total = (int64_t)b * nkv * s * (D / 8);
     hipLaunchKernelGGL((attn_group_reduce_kernel<D>), dim3((unsigned)((total + 255) / 256)), dim3(256), 0,
@@ -3121,17 +3252,7 @@ int attn_bwd_mfma(const BwdCall& c) {
   }
   if (hipGetLastError() != hipSuccess) return KR_ELAUNCH;
   if (forms.shared_dq) return kr_launch_status();  // its dQ kernel ran in front of the dK/dV kernel
-  if (dq_blocks <= 4 * 256) {  // few workgroups: the longest causal rows set the time
-    hipLaunchKernelGGL((attn_bwd_dq_kernel<D, RAGGED, 2, WIN>), dim3(dq_blocks), dim3(512), 2 * lds_dq, st,
-                       q, k, v, dout, lse,
-                       neg_delta, dq, s, nq, nkv, scale, scale_log2, ql, kl, vl, dol,
-                       dql, c.band);
-  } else {
-    hipLaunchKernelGGL((attn_bwd_dq_kernel<D, RAGGED, 1, WIN>), dim3(dq_blocks), dim3(256), lds_dq, st,
-                       q, k, v, dout, lse,
-                       neg_delta, dq, s, nq, nkv, scale, scale_log2, ql, kl, vl, dol,
-                       dql, c.band);
-  }
+  if constexpr (!WIN) launch_dq();
   return kr_launch_status();
 }
 }  // namespace
@@ -3254,6 +3375,15 @@ extern "C" int kr_attn_bwd_flags(const void* dout, const void* q, const void* k,
 #endif  // KR_ATTN_WINDOW_TU
 
 namespace {
+// Whether a window's forward takes 256-query tiles.  Rows are of one length, so the launch takes as many rounds as it has
+// workgroups for a unit, and one of 256 queries takes 1.4 times one of 128: those where not all of them fit in one round.  (128 -> 256, us:
+// 128 workgroups of 256 queries, 4096 tokens of 8/2 heads of 128, window 512 18.9 -> 26.7; 192, 3 x 2048 of them, 500 38.6 -> 30.7; 16384 of
+// them, 4096 286 -> 255; 2 x 8192 of 16/4 heads of 64, 1024 136 -> 114, 128 86 -> 68.)
+bool band_shared_fwd(int s, int b, int nq, int flags) {
+  const int64_t tiles = (int64_t)((s + 255) / 256) * nq * b;
+  return s > 128 && ((flags & KR_ATTN_BESIDE_OTHER_STREAMS) != 0 || 2 * tiles > kr_compute_units());
+}
+
 struct FwdCall {
   const bf16 *q, *k, *v;
   bf16* o;
@@ -3270,15 +3400,15 @@ struct FwdCall {
 template <int D, bool RAGGED, bool WIN>
 int attn_fwd_mfma(const FwdCall& c) {
   const int s = c.s, b = c.b, nq = c.nq, sp = attn_padded_len(s);
-  if constexpr (!WIN) if (attn_forms(sp, b, nq, c.nkv, D, c.flags).shared_fwd) {
+  if (WIN ? band_shared_fwd(s, b, nq, c.flags) : attn_forms(sp, b, nq, c.nkv, D, c.flags).shared_fwd) {
     // 256-query tiles (see attn_forms): the halves share their K / V tiles
     constexpr size_t lds_sh = 3 * 16 * ((1024 + 16) + (1024 + 64));  // 100 KiB
     static const hipError_t attr_sh = hipFuncSetAttribute(
-        (const void*)attn_fwd_sh_kernel<D, RAGGED>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds_sh);
+        (const void*)attn_fwd_sh_kernel<D, RAGGED, WIN>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds_sh);
     if (attr_sh != hipSuccess) return KR_ELAUNCH;
-    hipLaunchKernelGGL((attn_fwd_sh_kernel<D, RAGGED>), dim3((sp / 256) * nq * b), dim3(512), lds_sh, c.st,
+    hipLaunchKernelGGL((attn_fwd_sh_kernel<D, RAGGED, WIN>), dim3((sp + 255) / 256 * nq * b), dim3(512), lds_sh, c.st,
                        c.q, c.k, c.v, c.o, c.lse, s, c.nq, c.nkv, c.scale * kLog2e, c.ql.s_, c.ql.b_, c.ql.g_, c.ql.h_, c.kl.s_,
-                       c.kl.b_, c.kl.h_, c.vl.s_, c.vl.b_, c.vl.h_, c.ol.s_, c.ol.b_, c.ol.g_, c.ol.h_);
+                       c.kl.b_, c.kl.h_, c.vl.s_, c.vl.b_, c.vl.h_, c.ol.s_, c.ol.b_, c.ol.g_, c.ol.h_, c.band);
     return kr_launch_status();
   }
   // two K and two V tiles of 17 KiB (padded blocks) per half; afterwards the same memory holds
@@ -3439,8 +3569,9 @@ extern "C" int kr_attn_window_fwd(const void* q, const void* k, const void* v, v
   const FwdCall c{(const bf16*)q, (const bf16*)k, (const bf16*)v, (bf16*)o, lse, s, b, nq, nkv, scale,
                   QLayout{q_ss, q_sb, q_sg, q_sh}, QLayout{o_ss, o_sb, o_sg, o_sh}, KLayout{k_ss, k_sb, k_sh},
                   KLayout{v_ss, v_sb, v_sh}, flags, (hipStream_t)stream, band};
-  if (hd == 64) return s % BQ ? attn_fwd_mfma<64, true, kWindow>(c) : attn_fwd_mfma<64, false, kWindow>(c);
-  return s % BQ ? attn_fwd_mfma<128, true, kWindow>(c) : attn_fwd_mfma<128, false, kWindow>(c);
+  const bool ragged = s % (band_shared_fwd(s, b, nq, flags) ? 256 : BQ) != 0;
+  if (hd == 64) return ragged ? attn_fwd_mfma<64, true, kWindow>(c) : attn_fwd_mfma<64, false, kWindow>(c);
+  return ragged ? attn_fwd_mfma<128, true, kWindow>(c) : attn_fwd_mfma<128, false, kWindow>(c);
 }
 
 extern "C" size_t kr_attn_window_bwd_workspace_bytes(int s, int b, int nq, int nkv, int hd, int window, int sinks) {
@@ -3449,7 +3580,8 @@ extern "C" size_t kr_attn_window_bwd_workspace_bytes(int s, int b, int nq, int n
   const int sp = attn_padded_len(s);
   if (!band.window) return attn_bwd_fast_bytes(sp, b, nq, nkv, hd);
   const size_t rows = (size_t)b * nq * sp;
-  return (2 * rows + band_sink_floats(sp, b, nq, hd, band) + (nq != nkv ? 2 * rows * hd : 0)) * sizeof(float);
+  const size_t parts = nq != nkv ? rows : (size_t)b * nq * ((band.sinks + 127) / 128 * 128);
+  return (2 * rows + band_sink_floats(sp, b, nq, hd, band) + 2 * parts * hd) * sizeof(float);
 }
 
 extern "C" int kr_attn_window_bwd(const void* dout, const void* q, const void* k, const void* v, const void* o, const float* lse,

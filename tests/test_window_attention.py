@@ -308,8 +308,8 @@ def test_refusals_of_the_library():
     stats, parts = 2 * 4 * 384 * 4, 2 * 4 * 384 * 64 * 4
     assert size(300, 1, 4, 2, 64, 50, 0) == stats + parts
     assert size(300, 1, 4, 4, 64, 50, 0) == stats
-    # four heads' 32 sinks, the queries from 50 on in three stretches of 128: 2 x 2048 sums each
-    assert size(300, 1, 4, 4, 64, 50, 20) == stats + 4 * 3 * 2 * 2048 * 4
+    # four heads' 32 sinks, the queries from 50 on in three stretches of 128: 2 x 2048 sums each, and the first key tile's own
+    assert size(300, 1, 4, 4, 64, 50, 20) == stats + 4 * 3 * 2 * 2048 * 4 + 2 * 4 * 128 * 64 * 4
     assert size(300, 1, 4, 2, 64, 300, 0) == size(300, 1, 4, 2, 64, 200, 100) == lib.kr_attn_bwd_workspace_bytes_strided(300, 1, 4, 2, 64, 64)
     assert size(300, 1, 4, 2, 80, 50, 0) == 0 and size(300, 1, 4, 2, 64, 0, 0) == 0
 
