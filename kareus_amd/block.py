@@ -24,18 +24,22 @@ from .operators import (
     BiasSwigluOp,
     BlockColumnParallelLinearOp,
     BlockRowParallelLinearOp,
+    MultiAxisRotaryEmbeddingOp,
     NoOpAllReduce,
+    PartitionableLayerNorm,
     PartitionableRMSNorm,
     QKVPostProcessOp,
     RMSNorm,
     ResidualForkOp,
     RotaryEmbeddingOp,
+    SlidingWindowAttentionOp,
     TEColumnParallelLinearOp,
     TEDotProductAttentionOp,
     TERowParallelLinearOp,
     rotary_frequencies,
 )
 from .partitions.op_context import operator_parameters
+from .rotary_axes import RotaryAxes, check_sections, inverse_frequencies, rotary_axes
 from .partitions.streams import stream_api
 from .partitions import (
     CommunicationType,
@@ -97,6 +101,16 @@ class LayerConfig:
     # an RMSNorm over the head dimension of every query head and of every key head, between the QKV split
     # and the rotary embedding (Qwen3-style models)
     qk_layernorm: bool = False
+    # "RMSNorm", or "LayerNorm" (mean and variance, weight and bias) in front of attention and MLP; layers with a layer norm, a window or
+    # several axes run their operators one by one
+    normalization: str = "RMSNorm"
+    # > 0: a token attends to the last attention_window tokens, itself among them, and to the first attention_sinks of its sequence
+    attention_window: int = 0
+    attention_sinks: int = 0
+    # positions on several axes (time, height, width: LayerStack.forward's position_ids): how many of the kv_channels / 2 frequencies
+    # each axis has, one axis behind the other or in turn
+    rotary_sections: Optional[Tuple[int, ...]] = None
+    rotary_interleaved: bool = False
     # Filled in by the driver / the training loop:
     kareus_scheduler: Optional[Any] = None
     nanobatch_streams: Optional[List[Any]] = field(default=None, repr=False)
@@ -142,7 +156,11 @@ class LayerConfig:
         t, h, hd, nq = seq * seqs, self.hidden_size, self.kv_channels, self.num_attention_heads
         weights = h * (self.qkv_width + nq * hd + 3 * self.ffn_hidden_size)
         blocks = self.linear_format != "bf16"
-        ms = (6.0 * t * weights / (1.5e12 if blocks else 0.75e12) + 7.0 * seqs * nq * hd * float(seq) ** 2 / 0.4e12
+        seen = float(seq) ** 2    # twice the (token, visible token) pairs
+        if self.attention_window:
+            hidden = max(seq - self.attention_window - self.attention_sinks, 0)
+            seen -= float(hidden) ** 2
+        ms = (6.0 * t * weights / (1.5e12 if blocks else 0.75e12) + 7.0 * seqs * nq * hd * seen / 0.4e12
               + 80.0 * t * h / 5e9 + 4.0 * weights / 4.5e9)
         return ms < self.in_line_below_ms * (2.3 if blocks else 1.0)
 
@@ -250,21 +268,30 @@ class DecoderLayer(torch.nn.Module):
         blocks = c.linear_format == "fp8_blocks"
         column = BlockColumnParallelLinearOp if blocks else TEColumnParallelLinearOp
         row = BlockRowParallelLinearOp if blocks else TERowParallelLinearOp
+        if c.normalization not in ("RMSNorm", "LayerNorm"):
+            raise ValueError(f"unknown normalization {c.normalization!r}; choose 'RMSNorm' or 'LayerNorm'")
+        if c.attention_window < 0 or c.attention_sinks < 0 or (c.attention_sinks and not c.attention_window):
+            raise ValueError(f"attention_window {c.attention_window} and attention_sinks {c.attention_sinks}: neither may be negative, and "
+                             "sinks stay visible beside a window")
+        if c.rotary_sections is not None:
+            check_sections(c.rotary_sections, c.kv_channels)
+        norm = PartitionableLayerNorm if c.normalization == "LayerNorm" else PartitionableRMSNorm
         lin = dict(config=c, init_method=init, bias=False, device=device, dtype=dt, backend=be)
         self.attn_residual_fork = ResidualForkOp(backend=be)
-        self.input_layernorm = PartitionableRMSNorm(c.hidden_size, c.layernorm_epsilon, device=device, dtype=dt, backend=be)
+        self.input_layernorm = norm(c.hidden_size, c.layernorm_epsilon, device=device, dtype=dt, backend=be)
         self.linear_qkv = column(c.hidden_size, c.qkv_width, skip_bias_add=False, **lin)
         head_norm = (lambda: RMSNorm(c.kv_channels, c.layernorm_epsilon, device=device, dtype=dt, backend=be)
                      ) if c.qk_layernorm else (lambda: None)
         self.qkv_postprocess = QKVPostProcessOp(c.num_query_groups, c.num_attention_heads, c.kv_channels,
                                                 q_layernorm=head_norm(), k_layernorm=head_norm(), backend=be)
-        self.rotary = RotaryEmbeddingOp(config=c, backend=be)
-        self.core_attention = TEDotProductAttentionOp(config=c, layer_number=layer_number, backend=be,
-                                                      attention_dropout=c.attention_dropout)
+        self.rotary = (RotaryEmbeddingOp if c.rotary_sections is None else MultiAxisRotaryEmbeddingOp)(config=c, backend=be)
+        attention = dict(config=c, layer_number=layer_number, backend=be, attention_dropout=c.attention_dropout)
+        self.core_attention = (SlidingWindowAttentionOp(c.attention_window, c.attention_sinks, **attention) if c.attention_window
+                               else TEDotProductAttentionOp(**attention))
         self.linear_proj = row(c.num_attention_heads * c.kv_channels, c.hidden_size, skip_bias_add=True, **lin)
         self.self_attn_bda = BiasDropoutAddOp(has_bias=c.add_bias_linear, dropout_prob=c.hidden_dropout, backend=be)
         self.mlp_residual_fork = ResidualForkOp(backend=be)
-        self.pre_mlp_layernorm = PartitionableRMSNorm(c.hidden_size, c.layernorm_epsilon, device=device, dtype=dt, backend=be)
+        self.pre_mlp_layernorm = norm(c.hidden_size, c.layernorm_epsilon, device=device, dtype=dt, backend=be)
         self.linear_fc1 = column(c.hidden_size, 2 * c.ffn_hidden_size, skip_bias_add=True, **lin)
         self.activation = BiasSwigluOp(has_bias=c.add_bias_linear, backend=be)
         self.linear_fc2 = row(c.ffn_hidden_size, c.hidden_size, skip_bias_add=True, **lin)
@@ -293,7 +320,8 @@ class DecoderLayer(torch.nn.Module):
 
 
 class LayerStack(torch.nn.Module):
-    """``forward(hidden_states [s, b, h], attention_mask=None, rotary_pos_emb [s,1,1,hd])``."""
+    """``forward(hidden_states [s, b, h], attention_mask=None, rotary_pos_emb [s,1,1,hd])``; with ``rotary_sections`` in the config
+    ``forward(hidden_states, position_ids=[axes, b, s])`` (int64; without them a token's place in its sequence on every axis)."""
 
     def __init__(self, config: LayerConfig, device=None, seed: Optional[int] = None) -> None:
         super().__init__()
@@ -403,9 +431,28 @@ class LayerStack(torch.nn.Module):
                                             device=device)
         return cache[key]
 
+    def _rotary_axes(self, s: int, b: int, position_ids, device) -> RotaryAxes:
+        c = self.config
+        cache = self.__dict__.setdefault("_inverse_frequencies", {})
+        inv = cache.get(str(device))
+        if inv is None:
+            inv = cache[str(device)] = inverse_frequencies(c.kv_channels, c.rotary_base, device)
+        if position_ids is None:
+            position_ids = torch.arange(s, dtype=torch.int64, device=device).expand(len(c.rotary_sections), b, s)
+        at = rotary_axes(position_ids, c.kv_channels, c.rotary_sections, interleaved=c.rotary_interleaved, inv_freq=inv)
+        try:
+            at.check(s, b, c.kv_channels)
+        except RuntimeError as e:
+            raise ValueError(f"position_ids: {e}") from None
+        return at
+
     # -- execution ----------------------------------------------------------------
-    def forward(self, hidden_states: torch.Tensor, attention_mask=None, rotary_pos_emb=None,
+    def forward(self, hidden_states: torch.Tensor, attention_mask=None, rotary_pos_emb=None, position_ids=None,
                 **unsupported) -> torch.Tensor:
+        if self.config.rotary_sections is None:
+            unsupported["position_ids"] = position_ids
+        elif rotary_pos_emb is not None:
+            raise NotImplementedError("layers with rotary_sections take position_ids, not a table of angles")
         for name, value in unsupported.items():
             if value is not None:
                 raise NotImplementedError(f"{name} is not supported by the partition engine")
@@ -419,7 +466,9 @@ class LayerStack(torch.nn.Module):
         s, b, _ = hidden_states.shape
         if b < n or b % n:
             raise ValueError(f"batch size {b} must be a positive multiple of {n} nanobatches")
-        if rotary_pos_emb is None:
+        if self.config.rotary_sections is not None:
+            rotary_pos_emb = self._rotary_axes(s, b, position_ids, hidden_states.device)
+        elif rotary_pos_emb is None:
             rotary_pos_emb = self.rotary_pos_emb(s, device=hidden_states.device)
 
         hs = _SplitNanobatches.apply(hidden_states, n, self.config.backend) if n > 1 else (hidden_states,)

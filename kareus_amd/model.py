@@ -25,6 +25,7 @@ from torch import Tensor
 
 from .backend import get_backend
 from .block import LayerConfig, LayerStack
+from .gradients import clip_grad_norm
 from .partitions.streams import stream_api
 
 
@@ -131,6 +132,27 @@ class _RMSNorm(torch.autograd.Function):
         return dx.view(dy.shape), dgamma, None, None
 
 
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gamma, beta, eps, backend):
+        x2d = x.reshape(-1, x.shape[-1])
+        y, mean, rstd = get_backend(backend).layernorm_fwd(x2d, gamma.detach(), beta.detach(), eps)
+        ctx.save_for_backward(x2d, mean, rstd, gamma)
+        ctx.backend = backend
+        return y.view(x.shape)
+
+    @staticmethod
+    def backward(ctx, dy):
+        x2d, mean, rstd, gamma = ctx.saved_tensors
+        dx, dgamma, dbeta = get_backend(ctx.backend).layernorm_bwd(dy.reshape(x2d.shape), x2d, mean, rstd, gamma.detach())
+        return dx.view(dy.shape), dgamma, dbeta, None, None
+
+
+def final_norm(x: Tensor, gamma: Tensor, beta: Optional[Tensor], eps: float, backend: str) -> Tensor:
+    """The norm behind the stack: a layer norm where there is a bias, else an RMSNorm."""
+    return _RMSNorm.apply(x, gamma, eps, backend) if beta is None else _LayerNorm.apply(x, gamma, beta, eps, backend)
+
+
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, backend):
@@ -203,8 +225,8 @@ class LanguageModelEmbedding(torch.nn.Module):
 
 
 class GPTModelShard(torch.nn.Module):
-    """``forward(input_ids [b, s], labels [b, s] or None)`` -> loss ``[b, s]`` (fp32) or logits
-    ``[s, b, vocab_rows]``.  ``embedding_scale``, ``embedding_sorted_gradient``, ``embedding_main_grad``: see
+    """``forward(input_ids [b, s], labels [b, s] or None, position_ids=None)`` -> loss ``[b, s]`` (fp32) or logits
+    ``[s, b, vocab_rows]``; ``position_ids`` as :class:`LayerStack`'s.  After ``backward()``, ``clip_grad_norm(max_norm)`` ends the step.  ``embedding_scale``, ``embedding_sorted_gradient``, ``embedding_main_grad``: see
     :class:`LanguageModelEmbedding`."""
 
     def __init__(self, config: LayerConfig, vocab_rows: int, vocab_start: int = 0, device=None,
@@ -218,14 +240,20 @@ class GPTModelShard(torch.nn.Module):
         self.decoder = LayerStack(config, device=device, seed=seed)
         self.final_layernorm = torch.nn.Parameter(
             torch.ones(config.hidden_size, device=device, dtype=config.params_dtype))
+        self.final_layernorm_bias = torch.nn.Parameter(
+            torch.zeros(config.hidden_size, device=device, dtype=config.params_dtype)) if config.normalization == "LayerNorm" else None
         w = torch.empty(vocab_rows, config.hidden_size, dtype=torch.float32)
         w.normal_(0.0, config.init_method_std, generator=gen)
         self.output_layer = torch.nn.Parameter(w.to(device=device, dtype=config.params_dtype))
 
-    def forward(self, input_ids: Tensor, labels: Optional[Tensor] = None) -> Tensor:
+    def clip_grad_norm(self, max_norm: float, eps: float = 1e-6, out=None) -> Tensor:
+        """:func:`kareus_amd.clip_grad_norm` of all parameters (the embedding's ``main_grad`` where it keeps one)."""
+        return clip_grad_norm(self.parameters(), max_norm, eps=eps, backend=self.config.backend, out=out)
+
+    def forward(self, input_ids: Tensor, labels: Optional[Tensor] = None, position_ids: Optional[Tensor] = None) -> Tensor:
         be = self.config.backend
-        hidden = self.decoder(self.embedding(input_ids))
-        hidden = _RMSNorm.apply(hidden, self.final_layernorm, self.config.layernorm_epsilon, be)
+        hidden = self.decoder(self.embedding(input_ids), position_ids=position_ids)
+        hidden = final_norm(hidden, self.final_layernorm, self.final_layernorm_bias, self.config.layernorm_epsilon, be)
         logits = _Linear.apply(hidden, self.output_layer, be)
         if labels is None:
             return logits

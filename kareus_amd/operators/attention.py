@@ -27,6 +27,7 @@ from ..partitions.tensor_graph import Channel, PartitionableOperator
 
 class TEDotProductAttentionOp(BasicOperation, PartitionableOperator):
     num_extra_inputs = 2
+    _band: dict = {}   # (a window and sinks, as the backends take them)
 
     def __init__(self, config=None, layer_number: int = 1, attn_mask_type: str = "causal",
                  attention_dropout: float = 0.0, softmax_scale=None, backend="hip") -> None:
@@ -62,7 +63,7 @@ class TEDotProductAttentionOp(BasicOperation, PartitionableOperator):
         scale = self.softmax_scale if self.softmax_scale is not None else 1.0 / math.sqrt(hd)
         ctx = basic_op_ctxs[0]
         out, lse = get_backend(self._backend_name).attn_fwd(q, key, value, scale, True,
-                                                            beside_other_streams=self.beside_other_streams)
+                                                            beside_other_streams=self.beside_other_streams, **self._band)
         if ctx.requires_grad:
             ctx.save_for_backward(q, key, value, out, lse)
             ctx.scale = scale
@@ -72,6 +73,17 @@ class TEDotProductAttentionOp(BasicOperation, PartitionableOperator):
         ctx = basic_op_ctxs[0]
         q, key, value, out, lse = ctx.saved_tensors
         dq, dk, dv = get_backend(self._backend_name).attn_bwd(
-            grad_output, q, key, value, out, lse, ctx.scale, True, beside_other_streams=self.beside_other_streams
+            grad_output, q, key, value, out, lse, ctx.scale, True, beside_other_streams=self.beside_other_streams, **self._band
         )
         return dq, [()], [(dk, dv)]
+
+
+class SlidingWindowAttentionOp(TEDotProductAttentionOp):
+    """A query sees the last ``window`` keys up to its own, and the first ``sinks`` of the sequence (Megatron's ``window_size =
+    (window - 1, 0)``, 3rdparty/Megatron-LM/megatron/core/transformer/transformer_config.py, with sink tokens beside it)."""
+
+    def __init__(self, window: int, sinks: int = 0, **kwargs) -> None:
+        super().__init__(**kwargs)
+        if window < 1 or sinks < 0:
+            raise ValueError(f"a window has at least one key and sinks are not negative, got {window} and {sinks}")
+        self._band = dict(window=int(window), sinks=int(sinks))

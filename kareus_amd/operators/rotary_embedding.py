@@ -22,6 +22,7 @@ import torch
 from ..backend import get_backend
 from ..partitions.op_context import BasicOperation
 from ..partitions.tensor_graph import Channel, PartitionableOperator
+from ..rotary_axes import RotaryAxes
 
 
 def rotary_frequencies(seq_len: int, dim: int, base: float = 10000.0, device=None) -> torch.Tensor:
@@ -84,4 +85,32 @@ class RotaryEmbeddingOp(BasicOperation, PartitionableOperator):
         else:
             dq = be.rope_bwd(grad_output, freqs)
             dk = be.rope_bwd(grad_key, freqs)
+        return dq, [()], [(dk, None)]
+
+
+class MultiAxisRotaryEmbeddingOp(RotaryEmbeddingOp):
+    """The same rotation by positions on several axes, of which every nanobatch gets its sequences' own (:class:`RotaryAxes`) where
+    :class:`RotaryEmbeddingOp` gets one table of angles for all."""
+
+    def _rotate(self, a, b, at, backward):
+        be = get_backend(self._backend_name)
+        fused = self._shared_fused(a, b)
+        if fused is not None:
+            be.rope_axes_fused(fused, fused.shape[3] - 2, at, backward=backward, out=fused)
+            return a, b
+        turn = be.rope_axes_bwd if backward else be.rope_axes_fwd
+        return turn(a, at), turn(b, at)
+
+    def fuser_forward(self, basic_op_ctxs, input_, *, basic_op_extra_inputs, basic_op_prev_ops,
+                      basic_op_next_ops, basic_op_kwargs):
+        key, at = basic_op_extra_inputs[0]
+        if not isinstance(at, RotaryAxes):
+            raise ValueError("rotary_pos_emb must be the positions of the nanobatch's sequences on several axes")
+        q_out, k_out = self._rotate(input_, key, at, False)
+        basic_op_ctxs[0].at = at    # (not a saved tensor: the layers and a recomputation share it)
+        return q_out, [(k_out,)]
+
+    def fuser_backward(self, basic_op_ctxs, grad_output, *, basic_op_grad_extra_outputs):
+        (grad_key,) = basic_op_grad_extra_outputs[0]
+        dq, dk = self._rotate(grad_output, grad_key, basic_op_ctxs[0].at, True)
         return dq, [()], [(dk, None)]

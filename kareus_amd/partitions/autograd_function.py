@@ -153,10 +153,14 @@ def _fused_producer_of_last(graph: TensorGraph) -> Optional[int]:
 
 
 def _seed_forward(ctxs, hs, rotary, mask, seed: SeedConfig) -> None:
+    sequences = getattr(rotary, "sequences", None)   # (positions of each sequence's own: a nanobatch gets those of its sequences)
+    lo = 0
     for ctx, h in zip(ctxs, hs):
         ctx.tensor_store.set(seed.h_tid, h)
         if rotary is not None and seed.rotary_tid is not None:
-            ctx.tensor_store.set(seed.rotary_tid, rotary, False)
+            own = rotary if sequences is None else sequences(lo, lo + h.shape[1])
+            ctx.tensor_store.set(seed.rotary_tid, own, False)
+        lo += h.shape[1]
         if mask is not None and seed.mask_tid is not None:
             ctx.tensor_store.set(seed.mask_tid, mask, False)
 

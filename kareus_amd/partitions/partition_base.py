@@ -36,8 +36,10 @@ _GROUP_BY_CLASS: Dict[str, str] = {
     "ResidualForkOp": "norm",
     "BiasDropoutAddOp": "norm",
     "PartitionableRMSNorm": "norm",
+    "PartitionableLayerNorm": "norm",
     "QKVPostProcessOp": "rope",
     "RotaryEmbeddingOp": "rope",
+    "MultiAxisRotaryEmbeddingOp": "rope",
     "BiasSwigluOp": "activation",
     "PartitionableLinear": "linear",
     "TEColumnParallelLinearOp": "linear",
@@ -45,6 +47,7 @@ _GROUP_BY_CLASS: Dict[str, str] = {
     "BlockColumnParallelLinearOp": "linear",
     "BlockRowParallelLinearOp": "linear",
     "TEDotProductAttentionOp": "attn",
+    "SlidingWindowAttentionOp": "attn",
 }
 _MEMORY_BOUND_GROUPS = frozenset({"norm", "rope", "activation"})
 

@@ -2,7 +2,7 @@
 
 Same five measurements and the same files as the reference's non-partition profiler
 (tests/bayesian/nonpartition/profile_nonpartition.py:92-486): ``preprocess`` (embedding forward),
-``preprocess_backward``, ``postprocess`` (concatenate the nanobatches, final RMSNorm, output layer),
+``preprocess_backward``, ``postprocess`` (concatenate the nanobatches, final norm, output layer),
 ``postprocess_backward`` and ``loss``, each written to
 ``<dir>/nonpartition/<freq>/<name>_energy.csv`` with the header
 ``time (s),total_energy (J),per_rank_energy (J)`` and one row.  ``read_nonpartition`` turns such a
@@ -20,7 +20,7 @@ import torch
 
 from ..block import LayerConfig
 from ..energy import PowerSampler
-from ..model import LanguageModelEmbedding, _CrossEntropy, _Linear, _RMSNorm
+from ..model import LanguageModelEmbedding, _CrossEntropy, _Linear, final_norm
 from .hardware import Trial, measure
 
 STEP_NAMES = ("preprocess", "preprocess_backward", "postprocess", "postprocess_backward", "loss")
@@ -41,6 +41,7 @@ class NonPartitionProfiler:
         n = config.num_nanobatches
         self.embedding = LanguageModelEmbedding(config, vocab_rows, 0, device=self.device, generator=gen)
         self.final_gamma = torch.ones(h, device=self.device, dtype=dt, requires_grad=True)
+        self.final_beta = torch.zeros(h, device=self.device, dtype=dt, requires_grad=True) if config.normalization == "LayerNorm" else None
         self.w_out = (torch.randn(vocab_rows, h, generator=gen) * config.init_method_std).to(self.device, dt).requires_grad_(True)
         rnd = lambda *shape: torch.randn(*shape, generator=gen).to(self.device, dt)
         self.input_ids = torch.randint(0, vocab_rows, (batch_size, seq_len), generator=gen).to(self.device)
@@ -54,7 +55,7 @@ class NonPartitionProfiler:
 
     def _postprocess(self, x):
         be = self.config.backend
-        return _Linear.apply(_RMSNorm.apply(x, self.final_gamma, self.config.layernorm_epsilon, be), self.w_out, be)
+        return _Linear.apply(final_norm(x, self.final_gamma, self.final_beta, self.config.layernorm_epsilon, be), self.w_out, be)
 
     def step(self, name: str) -> Callable[[], object]:
         be = self.config.backend
@@ -70,6 +71,8 @@ class NonPartitionProfiler:
         if name == "postprocess_backward":
             def run():
                 self.final_gamma.grad = self.w_out.grad = None
+                if self.final_beta is not None:
+                    self.final_beta.grad = None
                 x = torch.cat(self.hidden_parts, dim=1).requires_grad_(True)
                 self._postprocess(x).backward(self.grad_logits)
             return run

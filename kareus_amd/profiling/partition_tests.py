@@ -26,6 +26,7 @@ import torch
 from ..block import DecoderLayer, LayerConfig
 from ..operators import NoOpAllReduce
 from ..operators.rotary_embedding import rotary_frequencies
+from ..rotary_axes import rotary_axes
 from ..partitions.partition_base import _build_overlap_slots
 from ..partitions.streams import stream_api
 from ..partitions.tensor_graph import CommunicationType
@@ -98,6 +99,9 @@ class PartitionTest:
 
     def _tensor(self, channel: str) -> torch.Tensor:
         c = self.config
+        if channel == "rotary_pos_emb" and c.rotary_sections is not None:
+            place = torch.arange(self.seq_length, device=self.device).expand(len(c.rotary_sections), self.nano_batch_size, -1)
+            return rotary_axes(place, c.kv_channels, c.rotary_sections, c.rotary_base, c.rotary_interleaved)
         if channel == "rotary_pos_emb":
             return rotary_frequencies(self.seq_length, c.kv_channels, c.rotary_base, device=self.device)
         return self._randn(c.hidden_size)  # "main" (a partition's first op reads hidden-width rows) / "residual"
