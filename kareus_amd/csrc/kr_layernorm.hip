@@ -12,8 +12,10 @@
 
 namespace {
 
-constexpr int kMaxBwdBlocks = 512;   // two workgroups of four waves a unit: what their registers allow
 constexpr int kMaxCols = 16384;
+// Up to this many rows one launch does both (two launches -> one, us from Python: 257 x 512 13.9 -> 8.8, 1024 x 512 11.1 -> 8.6, 512 x 8192
+// 25.3 -> 12.1, 1024 x 4096 20.5 -> 14.9; 2048 x 4096 26.0 -> 26.8, 4096 x 512 11.1 -> 32.9).
+constexpr int kFewRows = 1024;
 
 template <int LPR>
 constexpr int kBlock = LPR > 256 ? LPR : 256;
@@ -116,15 +118,62 @@ __global__ __launch_bounds__(kBlock<LPR>) void layernorm_fwd_kernel(
   }
 }
 
+// The gradients of weight and bias in 32 columns, by one workgroup: 64 lanes along the rows with 8 columns each, their sums added in a
+// fixed order.
+constexpr int kFewCols = 32;
+__device__ __forceinline__ void column_sums(const bf16* dy, const bf16* x, const float* mean, const float* rstd, bf16* dgamma,
+                                            bf16* dbeta, int rows, int cols, int64_t dy_ld, int64_t x_ld, KrRuns x_runs, int block) {
+  __shared__ float red[2][64][kFewCols + 1];
+  const int vec = threadIdx.x & 3, rl = threadIdx.x >> 2, col = block * kFewCols + vec * 8;
+  float dg[8], db[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) dg[e] = db[e] = 0.f;
+  if (col < cols) {
+#pragma unroll 4
+    for (int row = rl; row < rows; row += 64) {
+      const bf16x8 xv = ldg8(x + kr_row_at(row, x_ld, x_runs) + col), dv = ldg8(dy + row * dy_ld + col);
+      const float mu = mean[row], rs = rstd[row];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        dg[e] = __builtin_fmaf((float)dv[e], ((float)xv[e] - mu) * rs, dg[e]);
+        db[e] += (float)dv[e];
+      }
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    red[0][rl][vec * 8 + e] = dg[e];
+    red[1][rl][vec * 8 + e] = db[e];
+  }
+  kr_barrier();
+  if (threadIdx.x < 2 * kFewCols) {
+    const int which = threadIdx.x / kFewCols, c = threadIdx.x % kFewCols;
+    if (block * kFewCols + c < cols) {
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int r = 0; r < 64; ++r) sum[r & 3] += red[which][r][c];
+      (which ? dbeta : dgamma)[block * kFewCols + c] = (bf16)((sum[0] + sum[1]) + (sum[2] + sum[3]));
+    }
+  }
+}
+
 // ADD: the gradient of the residual branch forked off in front of the norm is added before the one rounding.
-template <int LPR, int NCH, bool ADD>
+// FEW: the workgroups from `row_blocks` on have the columns, and no partial rows are left.
+template <int LPR, int NCH, bool ADD, bool FEW>
 __global__ __launch_bounds__(kBlock<LPR>) void layernorm_bwd_kernel(
     const bf16* __restrict__ dy, const bf16* __restrict__ x, const float* __restrict__ mean, const float* __restrict__ rstd,
     const bf16* __restrict__ gamma, const bf16* __restrict__ dres, bf16* __restrict__ dx, float* __restrict__ partial, int rows,
-    int cols, int64_t dy_ld, int64_t x_ld, int64_t dres_ld, int64_t dx_ld, KrRuns x_runs, KrRuns dres_runs, KrRuns dx_runs) {
+    int cols, int64_t dy_ld, int64_t x_ld, int64_t dres_ld, int64_t dx_ld, KrRuns x_runs, KrRuns dres_runs, KrRuns dx_runs,
+    int row_blocks, bf16* __restrict__ dgamma, bf16* __restrict__ dbeta) {
+  if constexpr (FEW) {
+    if ((int)blockIdx.x >= row_blocks) {
+      column_sums(dy, x, mean, rstd, dgamma, dbeta, rows, cols, dy_ld, x_ld, x_runs, blockIdx.x - row_blocks);
+      return;
+    }
+  }
   constexpr int kRows = kBlock<LPR> / LPR;
   __shared__ float slots[2][2][kBlock<LPR> / 64];
-  __shared__ float red[kRows > 1 ? kBlock<LPR> * 8 : 1];  // a chunk's column sums of every lane
+  __shared__ float red[kRows > 1 && !FEW ? kBlock<LPR> * 8 : 1];  // a chunk's column sums of every lane
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int at = threadIdx.x % LPR, slot = threadIdx.x / LPR;
   const int nvec = cols / 8;
@@ -139,7 +188,7 @@ __global__ __launch_bounds__(kBlock<LPR>) void layernorm_bwd_kernel(
     for (int e = 0; e < 8; ++e) dg[c][e] = db[c][e] = 0.f;
   }
   int use = 0;
-  for (int64_t base = (int64_t)blockIdx.x * kRows; base < rows; base += (int64_t)gridDim.x * kRows) {
+  for (int64_t base = (int64_t)blockIdx.x * kRows; base < rows; base += (int64_t)(FEW ? row_blocks : gridDim.x) * kRows) {
     const int64_t row = base + slot;
     const bool active = row < rows;
     const int64_t r = active ? row : 0;
@@ -164,8 +213,10 @@ __global__ __launch_bounds__(kBlock<LPR>) void layernorm_bwd_kernel(
         const float xh = ((float)xv[c][e] - mu) * rs, d = (float)dv[c][e], gv = d * (float)g[c][e];
         sum[0] += gv;
         sum[1] = __builtin_fmaf(gv, xh, sum[1]);
-        dg[c][e] = __builtin_fmaf(d, xh, dg[c][e]);
-        db[c][e] += d;
+        if (!FEW) {
+          dg[c][e] = __builtin_fmaf(d, xh, dg[c][e]);
+          db[c][e] += d;
+        }
       }
     row_sums<LPR>(sum, slots[use], wave, lane);
     use ^= 1;
@@ -188,6 +239,7 @@ __global__ __launch_bounds__(kBlock<LPR>) void layernorm_bwd_kernel(
       }
     }
   }
+  if constexpr (FEW) return;
   float* const mine = partial + (int64_t)blockIdx.x * 2 * cols;
 #pragma unroll
   for (int c = 0; c < NCH; ++c)
@@ -263,12 +315,17 @@ int lanes_per_row(int cols, int most) {
   while (l * most < nvec) l *= 2;
   return l;
 }
-constexpr int kFwdVectors = 8, kBwdVectors = 4;
+// (8 -> 4 in the forward, us: 6023 x 3584 17.9 -> 15.3, 8192 x 8192 50.7 -> 48.4, 4096 x 16384 50.9 -> 49.5; 2: 16.8, 48.2, and 32768 x
+// 4096, a wave a row or two, 95.5, 96.6, 108; backward 4 -> 2: 32768 x 4096 181 -> 183, without a residual 137 -> 144)
+constexpr int kFwdVectors = 4, kBwdVectors = 4;
 
+// Workgroups of the backward, each of which leaves 8 cols bytes that are read again: two a unit, what the registers of wide rows
+// allow, one where it has eight waves (4096 x 16384 in 512 and 256, us: 121, 109; 32768 x 4096 181, 220), four where rows share a
+// wave (100000 x 256 in 512 and 1024: 43.6, 40.4, without a residual 40.0, 32.6; 32768 x 1024 50.7, 53.5).
 int bwd_blocks(int rows, int cols) {
   const int lpr = lanes_per_row(cols, kBwdVectors), per = lpr > 256 ? 1 : 256 / lpr;
-  const int blocks = (rows + per - 1) / per;
-  return blocks < kMaxBwdBlocks ? blocks : kMaxBwdBlocks;
+  const int most = lpr > 256 ? 256 : lpr < 64 ? 1024 : 512, blocks = (rows + per - 1) / per;
+  return blocks < most ? blocks : most;
 }
 
 template <int LPR>
@@ -284,9 +341,7 @@ int launch_fwd(int nch, bool keep, int blocks, hipStream_t stream, const bf16* x
       case 1: KR_LN_FWD(1); break;
       case 2: KR_LN_FWD(2); break;
       case 3: KR_LN_FWD(3); break;
-      case 4: KR_LN_FWD(4); break;
-      case 5: case 6: KR_LN_FWD(6); break;
-      default: KR_LN_FWD(8);
+      default: KR_LN_FWD(4);
     }
   }
 #undef KR_LN_FWD
@@ -302,14 +357,19 @@ struct BwdArgs {
   int rows, cols;
   int64_t dy_ld, x_ld, dres_ld, dx_ld;
   KrRuns x_runs{0, 0}, dres_runs{0, 0}, dx_runs{0, 0};
+  bf16 *dgamma = nullptr, *dbeta = nullptr;  // few rows: theirs in the same launch
 };
 
 template <int LPR>
 int launch_bwd(int nch, int blocks, hipStream_t stream, const BwdArgs& a) {
 #define KR_LN_BWD(NCH)                                                                                                            \
-  hipLaunchKernelGGL((a.dres ? layernorm_bwd_kernel<LPR, NCH, true> : layernorm_bwd_kernel<LPR, NCH, false>), dim3(blocks),     \
-                     dim3(kBlock<LPR>), 0, stream, a.dy, a.x, a.mean, a.rstd, a.gamma, a.dres, a.dx, a.partial, a.rows, a.cols, \
-                     a.dy_ld, a.x_ld, a.dres_ld, a.dx_ld, a.x_runs, a.dres_runs, a.dx_runs)
+  hipLaunchKernelGGL((a.dgamma ? a.dres ? layernorm_bwd_kernel<LPR, NCH, true, kBlock<LPR> == 256>                               \
+                                        : layernorm_bwd_kernel<LPR, NCH, false, kBlock<LPR> == 256>                              \
+                      : a.dres ? layernorm_bwd_kernel<LPR, NCH, true, false>                                                     \
+                               : layernorm_bwd_kernel<LPR, NCH, false, false>),                                                  \
+                     dim3(blocks + (a.dgamma ? (a.cols + kFewCols - 1) / kFewCols : 0)), dim3(kBlock<LPR>), 0, stream, a.dy, a.x, \
+                     a.mean, a.rstd, a.gamma, a.dres, a.dx, a.partial, a.rows, a.cols, a.dy_ld, a.x_ld, a.dres_ld, a.dx_ld,      \
+                     a.x_runs, a.dres_runs, a.dx_runs, blocks, a.dgamma, a.dbeta)
   if constexpr (LPR < 64) {
     KR_LN_BWD(1);
   } else {
@@ -333,7 +393,7 @@ extern "C" int kr_layernorm_fwd(const void* x, const void* gamma, const void* be
   if (!kr_aligned16(x) || !kr_aligned16(y) || !kr_aligned16(gamma) || !kr_aligned16(beta)) return KR_EINVAL;
   KrRuns runs;
   if (const int rc = kr_make_runs(x_run_rows, x_run_ld, rows, &runs)) return rc;
-  const int lpr = lanes_per_row(cols, kFwdVectors), per = 256 / lpr, nch = (cols / 8 + lpr - 1) / lpr;
+  const int lpr = lanes_per_row(cols, kFwdVectors), per = lpr > 256 ? 1 : 256 / lpr, nch = (cols / 8 + lpr - 1) / lpr;
   int blocks = (rows + per - 1) / per;
   if (blocks > 256 * 8) blocks = 256 * 8;
   const bool keep = (int64_t)rows * cols <= (int64_t)8 << 20;  // (as the RMS norm's results)
@@ -346,7 +406,8 @@ extern "C" int kr_layernorm_fwd(const void* x, const void* gamma, const void* be
     case 32: KR_LN_CALL(32);
     case 64: KR_LN_CALL(64);
     case 128: KR_LN_CALL(128);
-    default: KR_LN_CALL(256);
+    case 256: KR_LN_CALL(256);
+    default: KR_LN_CALL(512);
   }
 #undef KR_LN_CALL
 }
@@ -388,6 +449,8 @@ extern "C" int kr_layernorm_bwd(const void* dy, const void* x, const float* mean
   if (const int rc = kr_make_runs(dx_run_rows, dx_run_ld, rows, &a.dx_runs)) return rc;
   const int lpr = lanes_per_row(cols, kBwdVectors), nch = (cols / 8 + lpr - 1) / lpr, blocks = bwd_blocks(rows, cols);
   const hipStream_t s = (hipStream_t)stream;
+  const bool few = dgamma && rows <= kFewRows && lpr <= 256;  // (workgroups of 256)
+  if (few) a.dgamma = (bf16*)dgamma, a.dbeta = (bf16*)dbeta;
   int rc;
   switch (lpr) {
     case 8: rc = launch_bwd<8>(nch, blocks, s, a); break;
@@ -398,6 +461,6 @@ extern "C" int kr_layernorm_bwd(const void* dy, const void* x, const float* mean
     case 256: rc = launch_bwd<256>(nch, blocks, s, a); break;
     default: rc = launch_bwd<512>(nch, blocks, s, a);
   }
-  if (rc != KR_OK || !dgamma) return rc;  // without a destination the caller sums the partial rows later
+  if (rc != KR_OK || !dgamma || few) return rc;  // without a destination the caller sums the partial rows later
   return kr_layernorm_dparams((const float*)workspace, blocks, cols, dgamma, dbeta, stream);
 }
