@@ -51,8 +51,8 @@ def check(grads, max_norm=1.0, eps=1e-6):
 
 
 @on_gpu
-@pytest.mark.parametrize("sizes", [[1], [-1], [7, -3], [8192], [8191, -8193], [-8192, 8200, 1], [0, 5, 0, -6, 0], [100000, -50001, 8],
-                                   [3] * 127, [3] * 128, [5] * 129, [17, -9] * 150, [1 << 24, 4096, -(1 << 22)]])
+@pytest.mark.parametrize("sizes", [[1], [-1], [7, -3], [4096], [8192], [8191, -8193], [-4097, 8200, 1], [0, 5, 0, -6, 0], [100000, -50001, 8],
+                                   [3] * 127, [3] * 128, [5] * 129, [17, -9] * 150, [1 << 24, 4096, -(1 << 22)], [1 << 25, -3, 5, 1]])
 @pytest.mark.parametrize("max_norm", [1.0, 1e9])
 def test_sizes(sizes, max_norm):
     check(make(sizes), max_norm)
@@ -202,7 +202,7 @@ def test_refusals_of_the_library():
     clip = lambda out, m=1.0, e=0.0: lib.kr_grad_clip(1, ptrs(16), counts(1), types(0), out, m, e, 16, 16, 1 << 20, None)  # noqa: E731
     assert clip(None, -1.0) == -1 and clip(None, float("nan")) == -1 and clip(None, 1.0, -1.0) == -1 and clip(ptrs(None)) == -1
     assert clip(ptrs(18)) == -1
-    assert lib.kr_grad_norm_workspace_bytes(128) == 16 + 8192 and lib.kr_grad_norm_workspace_bytes(129) == 16 + 2 * 8192
+    assert lib.kr_grad_norm_workspace_bytes(128) == 16 + 4096 * 8 and lib.kr_grad_norm_workspace_bytes(129) == 16 + 2 * 4096 * 8
     assert lib.kr_grad_norm_workspace_bytes(0) == 0
 
 
