@@ -2394,20 +2394,22 @@ __device__ __forceinline__ void dq_score_mfma(DqScores& x, int kk, int m, bf16x8
 }
 
 // One step (32 keys).  NEXT: issue the score MFMAs of the following 32 keys (fragments of sub-tile nt
-// at nk_rows / nv_rows) into `nxt`.  MASK: the step is on the causal diagonal; lim[qb] is the last
-// visible key of the lane's row, relative to the lane's first key of the step.
-template <int D, bool NEXT, bool MASK>
+// at nk_rows / nv_rows) into `nxt`.  MASK 1: the step is on the causal diagonal; lim[qb] is the last
+// visible key of the lane's row, relative to the lane's first key of the step.  MASK 2: some of its keys are behind a window;
+// lim[qb] is the last of them, `from` the first that is no sink.
+template <int D, bool NEXT, int MASK>
 __device__ __forceinline__ void dq_step(DqScores& nxt, const DqScores& cur, f32x16 (&dq)[2][D / 32],
                                         uint32_t nk_rows, uint32_t nv_rows, int nt, uint32_t k_cols, int t,
                                         const bf16x8 (&qf)[2][D / 16], const bf16x8 (&dof)[2][D / 16],
                                         float scale_log2, const float (&neg_lse)[2],
-                                        const f32x16 (&neg_delta)[2], const int (&lim)[2]) {
+                                        const f32x16 (&neg_delta)[2], const int (&lim)[2], int from = 0) {
   constexpr int KK = D / 16, DT = D / 32;
   bf16x8 dsb[2][2];
   auto one_score = [&](int g) {  // lane: query row of block g / 16, key 8 (e / 4) + e % 4 (+ 4 h) of the step
     const int qb = g >> 4, e = g & 15;
     float sv = cur.s[qb][e];
-    if (MASK) sv = 8 * (e >> 2) + (e & 3) > lim[qb] ? -INFINITY : sv;
+    if (MASK == 1) sv = 8 * (e >> 2) + (e & 3) > lim[qb] ? -INFINITY : sv;
+    if (MASK == 2) sv = 8 * (e >> 2) + (e & 3) <= lim[qb] && 8 * (e >> 2) + (e & 3) >= from ? -INFINITY : sv;
     const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sv, scale_log2, neg_lse[qb]));
     dsb[qb][e >> 3][e & 7] = (bf16)(p * cur.dp[qb][e]);  // dP - delta comes out of the MFMAs
   };
@@ -2458,13 +2460,13 @@ __device__ __forceinline__ void dq_step(DqScores& nxt, const DqScores& cur, f32x
 // The kernel also takes over the pre-pass of the backward: each wave forms delta = sum_d dO . O of its 64
 // rows from the dO fragments it holds anyway, uses it, and writes it (and -lse in the log2 domain) for
 // the dK/dV kernel, which the host launches behind this one.
-template <int D, bool RAGGED>
+template <int D, bool RAGGED, bool WIN>
 __global__ __launch_bounds__(256, 1) void attn_bwd_dq_w64_kernel(
     const bf16* __restrict__ q, const bf16* __restrict__ k, const bf16* __restrict__ v,
     const bf16* __restrict__ dout, const bf16* __restrict__ o, const float* __restrict__ lse,
     float* __restrict__ neg_delta_out, float* __restrict__ neg_lse2_out, bf16* __restrict__ dq, int s, int nq,
     int nkv, float scale, float scale_log2, QLayout ql, KLayout kl, KLayout vl, QLayout dol, QLayout ol,
-    QLayout dql) {
+    QLayout dql, Band band) {
   extern __shared__ __attribute__((aligned(16))) bf16 smem[];
   constexpr int TK = tile_rows<D>, NSUB = TK / 32, DT = D / 32, KK = D / 16;
   constexpr uint32_t STAGE = 2 * BT_BYTES;  // K tile | V tile
@@ -2475,12 +2477,16 @@ __global__ __launch_bounds__(256, 1) void attn_bwd_dq_w64_kernel(
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int sp = RAGGED ? (s + 127) / 128 * 128 : s;  // rows of the statistics (whole 256-query tiles here)
   const int nqt = sp / ROWS;
-  int rank, pair;
-  longest_first(blockIdx.x, gridDim.x, nqt, rank, pair);
-  const int qt = nqt - 1 - rank;
+  const int per = nq / nkv;
+  int qt, rank, pair;
+  if constexpr (WIN) {
+    band_order<true>(blockIdx.x, gridDim.x, nqt, nq, per, qt, pair);
+  } else {
+    longest_first(blockIdx.x, gridDim.x, nqt, rank, pair);
+    qt = nqt - 1 - rank;
+  }
   const int head = pair % nq;
   const int bi = pair / nq;
-  const int per = nq / nkv;
   const int kvh = head / per;
   const int q0 = qt * ROWS;
   const int qw0 = q0 + wave * 64;
@@ -2535,22 +2541,34 @@ __global__ __launch_bounds__(256, 1) void attn_bwd_dq_w64_kernel(
 #pragma unroll
       for (int e = 0; e < 16; ++e) dqacc[qb][dt][e] = 0.f;
 
-  const int ntiles = (q0 + ROWS) / TK;                              // key tiles of the workgroup
-  const int last = __builtin_amdgcn_readfirstlane(qw0 / TK);        // this wave's tile on the diagonal
+  const BandTiles<TK> tiles(WIN ? band : Band{1, 0}, q0, ROWS);
+  const int ntiles = WIN ? tiles.total : (q0 + ROWS) / TK;          // key tiles of the workgroup
+  // this wave's tile on the diagonal; in front of it, from `full` on, those that all its rows see whole (a window of 128 keys and more:
+  // none of the tile on the diagonal is behind it)
+  const int last = __builtin_amdgcn_readfirstlane(WIN ? tiles.total - (q0 + ROWS) / TK + qw0 / TK : qw0 / TK);
+  int full = 0;
+  if constexpr (WIN) {
+    const int hidden = qw0 + 63 - band.window;  // the last key that is behind the window of the wave's last row
+    const int ahead = hidden < 0 ? 0 : hidden / TK + 1 - tiles.first;
+    full = __builtin_amdgcn_readfirstlane(tiles.sink_tiles + (ahead > 0 ? ahead : 0));
+  }
+  auto key_of = [&](int j) { return (WIN ? tiles.of(j) : j) * TK; };
   const uint32_t area = (uint32_t)(uintptr_t)(KR_LDS const bf16*)smem;
   auto stage_request = [&](int j, int buf) {  // the four waves bring in the K and the V tile together
-    if (RAGGED && (j + 1) * TK > s) {
-      bt_request_clamped<D>(kb, kl.s_, j * TK, s, area + buf * STAGE, wave, lane);
-      bt_request_clamped<D>(vb, vl.s_, j * TK, s, area + buf * STAGE + BT_BYTES, wave, lane);
+    const int key0 = key_of(j);
+    if (RAGGED && key0 + TK > s) {
+      bt_request_clamped<D>(kb, kl.s_, key0, s, area + buf * STAGE, wave, lane);
+      bt_request_clamped<D>(vb, vl.s_, key0, s, area + buf * STAGE + BT_BYTES, wave, lane);
       return;
     }
-    bt_request<D>(kb + (int64_t)(j * TK) * kl.s_, kl.s_, area + buf * STAGE, wave, lane);
-    bt_request<D>(vb + (int64_t)(j * TK) * vl.s_, vl.s_, area + buf * STAGE + BT_BYTES, wave, lane);
+    bt_request<D>(kb + (int64_t)key0 * kl.s_, kl.s_, area + buf * STAGE, wave, lane);
+    bt_request<D>(vb + (int64_t)key0 * vl.s_, vl.s_, area + buf * STAGE + BT_BYTES, wave, lane);
   };
   auto zero_tail = [&](int j, int buf) {  // rows of tile j beyond the sequence, once it has landed
-    if (RAGGED && (j + 1) * TK > s) {
-      bt_zero_tail<D>(j * TK, s, area + buf * STAGE, wave, lane);
-      bt_zero_tail<D>(j * TK, s, area + buf * STAGE + BT_BYTES, wave, lane);
+    const int key0 = key_of(j);
+    if (RAGGED && key0 + TK > s) {
+      bt_zero_tail<D>(key0, s, area + buf * STAGE, wave, lane);
+      bt_zero_tail<D>(key0, s, area + buf * STAGE + BT_BYTES, wave, lane);
     }
   };
   stage_request(0, 0);
@@ -2587,9 +2605,40 @@ __global__ __launch_bounds__(256, 1) void attn_bwd_dq_w64_kernel(
     arrive(j);
     if (j + NSTAGE - 1 < ntiles) stage_request(j + NSTAGE - 1, buf == 0 ? NSTAGE - 1 : buf - 1);
   };
+  if constexpr (WIN) {  // the tiles in front of `full`: the sinks', those behind the window of some rows of the wave or of all
+    for (int j = 0; j < full; ++j) {
+      const int buf_next = buf == NSTAGE - 1 ? 0 : buf + 1;
+      uint32_t k_rows = area + buf * STAGE + rows_lane, v_rows = k_rows + BT_BYTES;
+      uint32_t k_cols = area + buf * STAGE + cols_lane;
+      uint32_t nk_rows = area + buf_next * STAGE + rows_lane, nv_rows = nk_rows + BT_BYTES;
+      asm volatile("" : "+v"(k_rows), "+v"(v_rows), "+v"(k_cols), "+v"(nk_rows), "+v"(nv_rows));
+      const int at = key_of(j) + 4 * h;
+      int from = band.sinks - at;
+#pragma unroll
+      for (int qb = 0; qb < 2; ++qb) lim[qb] = qw0 + 32 * qb + (lane & 31) - band.window - at;
+      auto next_keys = [&]() {
+        from -= 32;
+#pragma unroll
+        for (int qb = 0; qb < 2; ++qb) lim[qb] -= 32;
+      };
+#pragma unroll
+      for (int t = 0; t < NSUB; t += 2) {
+        dq_step<D, true, 2>(b, a, dqacc, k_rows, v_rows, t + 1, k_cols, t, qf, dof, scale_log2, neg_lse, neg_delta, lim, from);
+        next_keys();
+        if (t + 2 < NSUB) {
+          dq_step<D, true, 2>(a, b, dqacc, k_rows, v_rows, t + 2, k_cols, t + 1, qf, dof, scale_log2, neg_lse, neg_delta, lim, from);
+          next_keys();
+        } else {
+          turn(j);
+          dq_step<D, true, 2>(a, b, dqacc, nk_rows, nv_rows, 0, k_cols, t + 1, qf, dof, scale_log2, neg_lse, neg_delta, lim, from);
+        }
+      }
+      buf = buf_next;
+    }
+  }
 #pragma unroll
   for (int qb = 0; qb < 2; ++qb) lim[qb] = 0;
-  for (int j = 0; j < last; ++j) {
+  for (int j = full; j < last; ++j) {
     const int buf_next = buf == NSTAGE - 1 ? 0 : buf + 1;
     uint32_t k_rows = area + buf * STAGE + rows_lane, v_rows = k_rows + BT_BYTES;
     uint32_t k_cols = area + buf * STAGE + cols_lane;
@@ -2597,12 +2646,12 @@ __global__ __launch_bounds__(256, 1) void attn_bwd_dq_w64_kernel(
     asm volatile("" : "+v"(k_rows), "+v"(v_rows), "+v"(k_cols), "+v"(nk_rows), "+v"(nv_rows));
 #pragma unroll
     for (int t = 0; t < NSUB; t += 2) {
-      dq_step<D, true, false>(b, a, dqacc, k_rows, v_rows, t + 1, k_cols, t, qf, dof, scale_log2, neg_lse, neg_delta, lim);
+      dq_step<D, true, 0>(b, a, dqacc, k_rows, v_rows, t + 1, k_cols, t, qf, dof, scale_log2, neg_lse, neg_delta, lim);
       if (t + 2 < NSUB) {
-        dq_step<D, true, false>(a, b, dqacc, k_rows, v_rows, t + 2, k_cols, t + 1, qf, dof, scale_log2, neg_lse, neg_delta, lim);
+        dq_step<D, true, 0>(a, b, dqacc, k_rows, v_rows, t + 2, k_cols, t + 1, qf, dof, scale_log2, neg_lse, neg_delta, lim);
       } else {
         turn(j);
-        dq_step<D, true, false>(a, b, dqacc, nk_rows, nv_rows, 0, k_cols, t + 1, qf, dof, scale_log2, neg_lse, neg_delta, lim);
+        dq_step<D, true, 0>(a, b, dqacc, nk_rows, nv_rows, 0, k_cols, t + 1, qf, dof, scale_log2, neg_lse, neg_delta, lim);
       }
     }
     buf = buf_next;
@@ -2614,21 +2663,21 @@ __global__ __launch_bounds__(256, 1) void attn_bwd_dq_w64_kernel(
     uint32_t k_cols = area + buf * STAGE + cols_lane;
     asm volatile("" : "+v"(k_rows), "+v"(v_rows), "+v"(k_cols));
 #pragma unroll
-    for (int qb = 0; qb < 2; ++qb) lim[qb] = 32 * qb + (lane & 31) - 4 * h + (D == 64 ? qw0 - last * TK : 0);
+    for (int qb = 0; qb < 2; ++qb) lim[qb] = 32 * qb + (lane & 31) - 4 * h + (D == 64 ? qw0 - key_of(last) : 0);
     auto next_keys = [&]() {
 #pragma unroll
       for (int qb = 0; qb < 2; ++qb) lim[qb] -= 32;
     };
 #pragma unroll
     for (int t = 0; t < NSUB; t += 2) {
-      dq_step<D, true, true>(b, a, dqacc, k_rows, v_rows, t + 1, k_cols, t, qf, dof, scale_log2, neg_lse, neg_delta, lim);
+      dq_step<D, true, 1>(b, a, dqacc, k_rows, v_rows, t + 1, k_cols, t, qf, dof, scale_log2, neg_lse, neg_delta, lim);
       next_keys();
       if (t + 2 < NSUB) {
-        dq_step<D, true, true>(a, b, dqacc, k_rows, v_rows, t + 2, k_cols, t + 1, qf, dof, scale_log2, neg_lse, neg_delta, lim);
+        dq_step<D, true, 1>(a, b, dqacc, k_rows, v_rows, t + 2, k_cols, t + 1, qf, dof, scale_log2, neg_lse, neg_delta, lim);
         next_keys();
       } else {
         turn(last);
-        dq_step<D, false, true>(a, b, dqacc, 0, 0, 0, k_cols, t + 1, qf, dof, scale_log2, neg_lse, neg_delta, lim);
+        dq_step<D, false, 1>(a, b, dqacc, 0, 0, 0, k_cols, t + 1, qf, dof, scale_log2, neg_lse, neg_delta, lim);
       }
     }
     buf = buf == NSTAGE - 1 ? 0 : buf + 1;
@@ -3098,6 +3147,13 @@ int band_sink_chunks(int sp, int b, int nq, Band band) {
   chunks = chunks < 1 ? 1 : chunks > 16 ? 16 : chunks;
   return chunks < query_blocks ? chunks : query_blocks;
 }
+// Whether a window's dQ takes 256-query tiles, one wave per SIMD: long windows, which pay for its start, and a workgroup for every unit
+// (two waves per SIMD -> one, us of the whole backward: 16384 tokens of 8/2 heads of 128, 4 sinks, window 8192 1675 -> 1614, 4 x 8192,
+// 4096 1511 -> 1477, 2048 875 -> 878, 1024 523 -> 551; 16384 of 16/4 heads of 64, 4096 936 -> 864, 2048 524 -> 506, 2 x 8192, 1024 307 -> 320;
+// 4096 of 8/2 heads, 128 workgroups, 2048 127 -> 151).
+bool band_shared_dq(int sp, int b, int nq, int hd, Band band) {
+  return sp % 256 == 0 && band.window >= (hd == 64 ? 2048 : 4096) && (int64_t)(sp / 256) * nq * b >= kr_compute_units();
+}
 size_t band_sink_floats(int sp, int b, int nq, int hd, Band band) {
   return (size_t)b * nq * ((band.sinks + 31) / 32) * band_sink_chunks(sp, b, nq, band) * 2 * (hd / 32) * 16 * 64;
 }
@@ -3133,7 +3189,7 @@ int attn_bwd_mfma(const BwdCall& c) {
   float* neg_lse2 = neg_delta + rows;
   float* const sink_sums = neg_lse2 + rows;
   float* part_k = sink_sums + (WIN ? band_sink_floats(sp, b, nq, D, c.band) : 0);
-  const AttnForms forms = WIN ? AttnForms{false, false, 1} : attn_forms(sp, b, nq, c.nkv, D, c.flags);
+  const AttnForms forms = WIN ? AttnForms{false, band_shared_dq(sp, b, nq, D, c.band), 1} : attn_forms(sp, b, nq, c.nkv, D, c.flags);
   const int qsplit = forms.qsplit;
   // (with a window and no partial results of a group's heads, the sinks' key tiles leave theirs alone)
   const int sink_rows = (c.band.sinks + 127) / 128 * 128;
@@ -3175,12 +3231,12 @@ int attn_bwd_mfma(const BwdCall& c) {
     if (e == hipSuccess)
       e = hipFuncSetAttribute((const void*)attn_bwd_dq_kernel<D, RAGGED, 2, WIN>,
                               hipFuncAttributeMaxDynamicSharedMemorySize, (int)(2 * lds_dq));
-    if constexpr (WIN) {
+    if constexpr (WIN)
       if (e == hipSuccess)
         e = hipFuncSetAttribute((const void*)attn_bwd_sinks_kernel<D, RAGGED>, hipFuncAttributeMaxDynamicSharedMemorySize,
                                 (int)lds_sinks);
-    } else if (e == hipSuccess) {
-      e = hipFuncSetAttribute((const void*)attn_bwd_dq_w64_kernel<D, RAGGED>,
+    if (e == hipSuccess) {
+      e = hipFuncSetAttribute((const void*)attn_bwd_dq_w64_kernel<D, RAGGED, WIN>,
                               hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds_dq_w64);
     }
     return e;
@@ -3207,14 +3263,14 @@ int attn_bwd_mfma(const BwdCall& c) {
     }
   };
   int sink_chunks = 0;
-  if constexpr (WIN) {
+  if (WIN && !forms.shared_dq) {
     launch_dq();  // it comes first: the other kernels read the statistics that it leaves
   } else if (forms.shared_dq) {
     // 256-query tiles (see attn_forms): one wave per SIMD, 64 rows each.
     // It comes first: it also computes delta and the log2-domain copy of lse that the dK/dV kernel reads.
-    hipLaunchKernelGGL((attn_bwd_dq_w64_kernel<D, RAGGED>), dim3(dq_blocks / 2), dim3(256), lds_dq_w64, st,
+    hipLaunchKernelGGL((attn_bwd_dq_w64_kernel<D, RAGGED, WIN>), dim3(dq_blocks / 2), dim3(256), lds_dq_w64, st,
                        q, k, v, dout, o, lse,
-                       neg_delta, neg_lse2, dq, s, nq, nkv, scale, scale_log2, ql, kl, vl, dol, ol, dql);
+                       neg_delta, neg_lse2, dq, s, nq, nkv, scale, scale_log2, ql, kl, vl, dol, ol, dql, c.band);
   } else {
     hipLaunchKernelGGL((attn_delta_kernel<D>), dim3((unsigned)((rows * (D / 8) + 255) / 256)), dim3(256), 0, st,
                        dout, o, lse, neg_delta, neg_lse2, s, sp, nq, per, rows, dol, ol);

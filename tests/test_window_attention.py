@@ -123,6 +123,25 @@ def test_many_workgroups(hd, beside):
 
 
 @on_gpu
+@pytest.mark.parametrize("s,b,nq,hd,window,sinks", [(2304, 8, 4, 64, 2048, 5), (2816, 4, 6, 64, 2200, 0), (4352, 4, 4, 128, 4096, 70), (4864, 7, 2, 128, 4200, 0),
+                                                    (4864, 7, 2, 128, 4111, 130)])
+def test_long_windows(s, b, nq, hd, window, sinks):
+    """dQ over 256-query tiles, one wave per SIMD.  (The reference goes head by head: 64-bit scores of thousands of tokens.)"""
+    be = get_backend("hip")
+    q, k, v, do = make(s, b, nq, 1, hd)
+    q, k, v, do = (t.contiguous() for t in (q, k, v, do))
+    band = dict(window=window, sinks=sinks)
+    o, lse = be.attn_fwd(q, k, v, hd ** -0.5, **band)
+    dq, dk, dv = be.attn_bwd(do, q, k, v, o, lse, hd ** -0.5, **band)
+    for bi in (0, b - 1):
+        part = slice(bi, bi + 1)
+        want, tol = reference(q[:, part], k[:, part], v[:, part], do[:, part].contiguous(), hd ** -0.5, window, sinks)
+        for name, t in (("lse", lse[part]), ("o", o[:, part]), ("dv", dv[:, part]), ("dk", dk[:, part]), ("dq", dq[:, part])):
+            close(name, t, want[name], tol[name])
+    torch.cuda.empty_cache()
+
+
+@on_gpu
 @pytest.mark.parametrize("hd", [8, 40, 80, 96, 120])
 def test_other_head_dimensions(hd):
     check(*make(210, 2, 4, 2, hd), 50, 3)
@@ -403,9 +422,9 @@ def test_the_order_of_workgroups_is_a_permutation(tmp_path):
 
 
 def test_the_window_kernels_keep_their_reads_in_front_of_barriers(tmp_path):
-    """What tests/test_attention_asm.py reads in the plain dK/dV kernels, in those with a window."""
+    """What tests/test_attention_asm.py reads in the plain dK/dV and dQ kernels, in those with a window."""
     sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
-    from test_attention_asm import CSRC, HIPCC, _kernel_body
+    from test_attention_asm import CSRC, HIPCC, _kernel_body, early_readers
 
     if not os.path.exists(HIPCC):
         pytest.skip("hipcc is not installed")
@@ -422,5 +441,11 @@ def test_the_window_kernels_keep_their_reads_in_front_of_barriers(tmp_path):
             if mfmas == 16 and hand_over == 4:
                 blocks.append(fragments)
         assert len(blocks) >= 2 and set(blocks) == {32}, (name, blocks)
+    names = set(re.findall(r"^(_Z\w*attn_bwd_dq_w64_kernel\w*):", text, re.M))
+    assert len(names) == 4
+    for name in names:   # the hand-placed MFMAs: 128 of the plain kernel's, and the two steps of the loop over hidden keys
+        body = text[text.index("\n" + name + ":"):]
+        n_asm, bad = early_readers(body[:body.index(".Lfunc_end")].split("\n"))
+        assert n_asm == 192 and not bad, (name, n_asm, bad[:5])
     spills = [int(n) for n in re.findall(r"\.vgpr_spill_count:\s*(\d+)", text)]
     assert spills and not any(spills)
