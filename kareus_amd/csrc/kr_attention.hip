@@ -887,7 +887,8 @@ __global__ __launch_bounds__(512, 1) void attn_fwd_sh_kernel(
   const int64_t r_ss = half ? v_ss : k_ss;
   const uint32_t r_blk = half ? VBLK : KBLK, r_tile = half ? VTILE : KTILE;
   const uint32_t r_ring = half ? vring : kring;
-  const bf16* req = (half ? vb : kb) + (int64_t)wave * r_ss;
+  const bf16* req = (half ? vb : kb) + (int64_t)(key_of(0) + wave) * r_ss;
+  const int64_t r_gap = WIN ? (int64_t)(tiles.first - tiles.sink_tiles + 1) * TK * r_ss : 0;
   const int64_t r_next = (int64_t)TK * r_ss, r_rows4 = 4 * r_ss;
   const uint32_t r_lane_off = tile_lane_off<D>(lane, (int)r_ss);
   auto request_part = [&](uint32_t tile, int j, int i) {
@@ -895,8 +896,9 @@ __global__ __launch_bounds__(512, 1) void attn_fwd_sh_kernel(
     if (RAGGED && key_of(j) + TK > s)
       request_clamped<D>(half ? vb : kb, r_ss, key_of(j), wave + 4 * i, s, lane, dst);
     else
-      dma_b128((WIN ? req + (int64_t)key_of(j) * r_ss : req) + i * r_rows4, r_lane_off, dst);
-    if (!WIN && i == 3) req += r_next;
+      dma_b128(req + i * r_rows4, r_lane_off, dst);
+    // (of a window's tiles those between the sinks' and the first are left out)
+    if (i == 3) req += WIN && j + 1 == tiles.sink_tiles ? r_gap : r_next;
   };
   // rows of V tile j (ring slot `slot`) beyond the sequence: as in the kernel above
   auto zero_v_tail = [&](int j, int slot) {
@@ -952,6 +954,7 @@ __global__ __launch_bounds__(512, 1) void attn_fwd_sh_kernel(
     }
   };
 
+  bool mine_prev = false;
   int slot = 0, slot_prev = 2, slot_req = 2;  // j % 3, (j - 1) % 3, (j + 2) % 3
   settle_scalar_loads();
   for (int j = 0; j < ntiles; ++j) {
@@ -959,7 +962,8 @@ __global__ __launch_bounds__(512, 1) void attn_fwd_sh_kernel(
     f32x16 sacc[NB];
     const bool mine = is_mine(j);
     __builtin_amdgcn_s_setprio(1);
-    if (j > 0 && is_mine(j - 1)) pv_step(slot_prev);
+    if (WIN ? mine_prev : j > 0 && is_mine(j - 1)) pv_step(slot_prev);
+    mine_prev = mine;
     if (mine) {
       uint32_t ka = kring + slot * KTILE + kfrag_lane;
       asm volatile("" : "+v"(ka));
@@ -1070,7 +1074,7 @@ __global__ __launch_bounds__(512, 1) void attn_fwd_sh_kernel(
     slot_req = slot_req == 2 ? 0 : slot_req + 1;
   }
   // last matrix period: the product of the final tile (half 1; half 0 finished two steps ago)
-  if (is_mine(ntiles - 1)) {
+  if (WIN ? mine_prev : is_mine(ntiles - 1)) {
     __builtin_amdgcn_s_setprio(1);
     pv_step(slot_prev);
     __builtin_amdgcn_s_setprio(0);
