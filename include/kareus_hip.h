@@ -227,7 +227,8 @@ int kr_rmsnorm_bwd_add_noalloc(const void* dy, const void* x, const float* rstd,
  *   dx = bf16(rstd (g - mean(g) - xh mean(g xh)) + dres), g = dy gamma, xh = (x - mean) rstd; dres [rows, cols] may be NULL: the
  *   gradient of a residual branch forked off in front of the norm, added before the one rounding.
  *   dgamma = sum of dy xh, dbeta = sum of dy over the rows, in fp32 and in a fixed order, rounded once.
- * cols: a multiple of 8, at most 16384; strides multiples of 8.  dx overlaps no input; it may be a slice of a larger tensor.
+ * cols: a multiple of 8, at most 16384; strides multiples of 8.  dx may be a slice of a larger tensor, and dres itself; otherwise
+ * it overlaps no input (KR_EINVAL where it begins where x or dy does).
  * workspace: kr_layernorm_bwd_workspace_bytes() bytes, 16-byte aligned.  With dgamma and dbeta NULL the call leaves there its
  * kr_layernorm_bwd_partial_rows() fp32 rows of [2][cols] sums, and kr_layernorm_dparams adds those of several calls (the nanobatches
  * of a microbatch, workspaces back to back).  The queries return 0 for widths that are not supported.      */

@@ -135,6 +135,8 @@ class EagerBackend:
     def layernorm_bwd(self, dy: Tensor, x: Tensor, mean: Tensor, rstd: Tensor, gamma: Tensor, residual_grad: Tensor = None,
                       out: Tensor = None, partials_out: Tensor = None) -> Tuple[Tensor, Tensor, Tensor]:
         cols = x.shape[-1]
+        if out is not None and x.numel() and out.data_ptr() in (x.data_ptr(), dy.data_ptr()):
+            raise RuntimeError("layernorm_bwd: out must not be x or dy")
         xhat = (x.reshape(-1, cols).float() - mean[:, None]) * rstd[:, None]
         dyf = dy.reshape(-1, cols).float()
         g = dyf * gamma.float()

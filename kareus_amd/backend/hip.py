@@ -835,7 +835,8 @@ class HipBackend:
     def layernorm_bwd(self, dy: Tensor, x: Tensor, mean: Tensor, rstd: Tensor, gamma: Tensor, residual_grad: Tensor = None,
                       out: Tensor = None, partials_out: Tensor = None) -> Tuple[Tensor, Tensor, Tensor]:
         """The input gradient and the gradients of weight and bias.  ``residual_grad`` (rows as ``x``'s): the gradient of the residual branch
-        forked off in front of the norm, added before the one rounding.  ``out``: where the input gradient goes (rows, or rows in runs).
+        forked off in front of the norm, added before the one rounding.  ``out``: where the input gradient goes (rows, or rows in
+        runs; it may be ``residual_grad``, and overlaps no other input).
         ``partials_out`` ([layernorm_partial_rows, 2 cols] fp32, dense): the gradients of weight and bias are left there as partial rows
         for ``layernorm_dparams`` and None is returned in their place."""
         done = self._n.layernorm_bwd(dy, x, mean, rstd, gamma, residual_grad, out, partials_out)
@@ -869,6 +870,8 @@ class HipBackend:
             dx, dx_op = out, self._operand(out)
             if dx_op is None or dx_op[0] != rows or out.shape[-1] != cols or out.data_ptr() % 16:
                 raise RuntimeError(f"{name}: out must be [{rows}, {cols}] with a single row stride, or in row runs")
+            if rows and out.data_ptr() in (x.data_ptr(), dy.data_ptr()):
+                raise RuntimeError(f"{name}: out must not be x or dy")
             if rows == 1:
                 dx_op = (1, (cols + 7) // 8 * 8, 1, 0)
             tensors.append(out)

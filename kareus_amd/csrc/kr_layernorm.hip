@@ -441,6 +441,10 @@ extern "C" int kr_layernorm_bwd(const void* dy, const void* x, const float* mean
   if (!kr_aligned16(x) || !kr_aligned16(dy) || !kr_aligned16(dx) || !kr_aligned16(gamma) || !kr_aligned16(workspace) ||
       (dres && !kr_aligned16(dres)))
     return KR_EINVAL;
+  // (the gradients of the parameters are summed by other workgroups of the same launch, and a row's own may have left its place by then)
+  if (dx == dy || dx == x) return KR_EINVAL;
+  if (dx == dres && rows > 1 && (dx_ld != dres_ld || dx_run_rows != dres_run_rows || (dx_run_rows > 1 && dx_run_ld != dres_run_ld)))
+    return KR_EINVAL;
   BwdArgs a{(const bf16*)dy, (const bf16*)x, mean, rstd, (const bf16*)gamma, (const bf16*)dres, (bf16*)dx, (float*)workspace,
             rows, cols, dy_ld, x_ld, dres ? dres_ld : 0, dx_ld};
   if (const int rc = kr_make_runs(x_run_rows, x_run_ld, rows, &a.x_runs)) return rc;

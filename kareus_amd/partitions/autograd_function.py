@@ -253,6 +253,7 @@ class TransformerBlockAutogradFunction(torch.autograd.Function):
         func_ctx.seed_config = seed
         func_ctx.num_params = len(params) // n
         func_ctx.rotary_pos_emb = rotary
+        func_ctx.rotary_version = rotary.version() if hasattr(rotary, "version") else None
         func_ctx.attention_mask = mask
         func_ctx.checkpoint_activations = checkpoint_activations
         func_ctx.fuse_wgrad_accumulation = bool(getattr(config, "fuse_wgrad_accumulation", False))
@@ -289,6 +290,8 @@ class TransformerBlockAutogradFunction(torch.autograd.Function):
         seed: SeedConfig = func_ctx.seed_config
         streams = func_ctx.streams
         rotary, mask = func_ctx.rotary_pos_emb, func_ctx.attention_mask
+        if func_ctx.rotary_version is not None and rotary.version() != func_ctx.rotary_version:
+            raise RuntimeError("the positions of the forward pass were written to before its backward pass, which turns by them again")
         scheduler = func_ctx.scheduler
         schedule = scheduler.current_schedule if scheduler is not None else None
 

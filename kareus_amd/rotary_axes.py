@@ -29,6 +29,10 @@ class RotaryAxes(NamedTuple):
         """The positions of sequences ``lo`` to ``hi`` of the batch (a view)."""
         return self._replace(positions=self.positions[:, lo:hi])
 
+    def version(self) -> Optional[int]:
+        """Counts the writes to the positions (None: such a tensor does not)."""
+        return None if self.positions.is_inference() else self.positions._version
+
     def check(self, s: int, b: int, hd: int) -> None:
         """Raises unless these are the positions of ``[s, b]`` tokens with heads of ``hd`` channels."""
         p, f = self.positions, self.inv_freq

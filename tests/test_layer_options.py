@@ -145,6 +145,23 @@ def test_recomputation_and_streams_on_the_host():
     assert not rec.violations
 
 
+@pytest.mark.parametrize("again", [False, True])
+def test_positions_that_change_before_the_backward_pass(again):
+    """A buffer of positions that is filled for the next microbatch in between: refused, not turned by the wrong angles."""
+    c = config("eager", torch.float32, 2, checkpoint_activations=again, **OPTIONS["axes"])
+    model = stir(LayerStack(c, seed=1))
+    gen = torch.Generator().manual_seed(5)
+    x, dy = torch.randn(16, 2, 256, generator=gen), torch.randn(16, 2, 256, generator=gen)
+    at = positions(16, 2, 3, "cpu")
+    y = model(x.requires_grad_(True), position_ids=at)
+    at.copy_(at + 1)
+    with pytest.raises(RuntimeError, match="positions"):
+        y.backward(dy)
+    with torch.inference_mode():
+        frozen = at.clone()
+    near(run(model, x, dy, frozen), run(model, x, dy, at), 0.0)
+
+
 def test_slots_and_refusals():
     c = config("eager", torch.float32, layers=1, **OPTIONS["all"])
     model = LayerStack(c, seed=1)

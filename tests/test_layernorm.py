@@ -223,6 +223,31 @@ def test_refusals():
             bad()
 
 
+@on_gpu
+def test_the_residual_gradient_s_own_place_and_no_other():
+    """With few rows the parameters' gradients are summed beside the rows: dx must not be where x or dy is; dres is read before it is
+    written.  A gradient of a broadcast value is copied."""
+    be = get_backend("hip")
+    x, dy, res, w, b = make(37, 200)
+    want = check(x, dy, w, b, res=res)
+    _, mean, rstd = be.layernorm_fwd(x, w, b, 1e-5)
+    for out in (x, dy):
+        with pytest.raises(RuntimeError):
+            be.layernorm_bwd(dy, x, mean, rstd, w, out=out)
+    dx, _, _ = be.layernorm_bwd(dy, x, mean, rstd, w, residual_grad=res, out=res)
+    assert dx.data_ptr() == res.data_ptr() and torch.equal(dx, want[1])
+    check(x, dy[:1].expand(37, 200), w, b)
+
+
+def test_an_output_that_is_an_input_of_the_eager_backend():
+    be = get_backend("eager")
+    x, dy, _, w, b = make(7, 40, device="cpu", dtype=torch.float32)
+    _, mean, rstd = be.layernorm_fwd(x, w, b, 1e-5)
+    for out in (x, dy):
+        with pytest.raises(RuntimeError):
+            be.layernorm_bwd(dy, x, mean, rstd, w, out=out)
+
+
 def test_refusals_of_the_library():
     lib = hip.load_library()
     fwd = lambda *a: lib.kr_layernorm_fwd(*a, None)  # noqa: E731
@@ -237,6 +262,7 @@ def test_refusals_of_the_library():
         16, 16, 16, 16, 16, None, 16, dg, db, ws, rows, 64, ld, 64, 1, 0, 0, 1, 0, 64, 1, 0, None)
     assert bwd(16, None, 16) == -1 and bwd(16, 16, None) == -1 and bwd(16, 16, 24) == -1 and bwd(16, 16, 16, rows=0) == -1
     assert bwd(16, 16, 16, ld=68) == -2
+    assert bwd(16, 16, 16) == -1                                                # dx where x and dy are
     assert lib.kr_layernorm_dparams(16, 0, 64, 16, 16, None) == -1 and lib.kr_layernorm_dparams(16, 1, 64, 16, None, None) == -1
     assert lib.kr_layernorm_bwd_partial_rows(257, 512) == 65 and lib.kr_layernorm_bwd_workspace_bytes(257, 512) == 65 * 2 * 512 * 4
     assert lib.kr_layernorm_bwd_partial_rows(4, 60) == 0 and lib.kr_layernorm_bwd_workspace_bytes(4, 16392) == 0
