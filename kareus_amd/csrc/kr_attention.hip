@@ -319,9 +319,11 @@ namespace {
 
 
 // query-like tensors: head h of KV group g = h / per sits at g*g_ + (h % per)*h_
-// The query tile behind the last one that sees any of the keys key0 .. key0 + 127 in its window (sp: queries, in whole 128-row tiles).
+// The query tile behind the last one that sees any of the keys key0 .. key0 + 127 in its window, or, of sinks, at all (sp: queries, in whole
+// 128-row tiles).
 template <int TQ>
 __device__ __forceinline__ int band_query_tiles(Band band, int key0, int sp) {
+  if (key0 < band.sinks) return sp / TQ;
   const int64_t end = ((int64_t)key0 + 127 + band.window - 1) / TQ + 1;
   return end < sp / TQ ? (int)end : sp / TQ;
 }
@@ -1281,7 +1283,8 @@ __global__ __launch_bounds__(512, 1) void attn_bwd_dkdv_kernel(
         }
       }
       if (WIN && qs0 + 31 - kw0 >= band.window) {
-        const int lim = krow - qs0 - 4 * h + band.window;  // element offsets from it on are queries past the key's window
+        // element offsets from it on are queries past the key's window
+        const int lim = krow < band.sinks ? 1 << 30 : krow - qs0 - 4 * h + band.window;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           float x = 8 * (e >> 2) + (e & 3) >= lim ? -INFINITY : sacc[e];
@@ -1501,7 +1504,7 @@ __global__ __launch_bounds__(512, 1) void attn_bwd_dkdv_kernel(
   // one barrier earlier by this wave only) for the output transposition.
   RowStage rs;
   rs.init(reinterpret_cast<char*>(smem) + XCH + wave * 4096, lane);
-  if (PARTIAL || (WIN && key0 < band.sinks)) {  // (what queries behind the window add to the sinks' keys is added to their sums)
+  if (PARTIAL || (WIN && key0 < part_rows)) {  // (what queries behind the window add to the sinks' keys is added to their sums)
     const int64_t prow = (((int64_t)bi * nhg + hgroup) * qsplit + part) * (WIN ? part_rows : sp) + kw0;
     store_rows_f32<D>(rs, dkacc, scale, part_k + prow * D, D);
     store_rows_f32<D>(rs, dvacc, 1.0f, part_v + prow * D, D);
@@ -1687,7 +1690,8 @@ __global__ __launch_bounds__(512, 1) void attn_bwd_dkdv64_kernel(
       }
     }
     if (WIN && qs0 + 31 - kw0 >= band.window) {
-      const int lim = krow - qs0 - 4 * h + band.window;  // element offsets from it on are queries past the key's window
+      // element offsets from it on are queries past the key's window
+      const int lim = krow < band.sinks ? 1 << 30 : krow - qs0 - 4 * h + band.window;
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         float v = 8 * (e >> 2) + (e & 3) >= lim ? -INFINITY : x.s[e];
@@ -1851,7 +1855,7 @@ __global__ __launch_bounds__(512, 1) void attn_bwd_dkdv64_kernel(
   RowStage rs;
   rs.init(reinterpret_cast<char*>(smem) + 65536 + wave8 * 4096, lane);
   const float mul = half == 0 ? scale : 1.0f;
-  if (PARTIAL || (WIN && kt * 128 < band.sinks)) {
+  if (PARTIAL || (WIN && kt * 128 < part_rows)) {
     const int64_t prow = (((int64_t)bi * nhg + hgroup) * qsplit + part) * (WIN ? part_rows : sp) + kw0;
     store_rows_f32<D>(rs, acc, mul, (half == 0 ? part_k : part_v) + prow * D, D);
   } else if (half == 0) {
@@ -1861,8 +1865,8 @@ __global__ __launch_bounds__(512, 1) void attn_bwd_dkdv64_kernel(
   }
 }
 
-// dK and dV of the sinks' keys from the queries that have them behind their window, i - j >= window and j < sinks (the dK/dV kernels
-// above take i - j < window; attn_window_reduce_kernel adds the two).  These few keys are seen by every later query: a key
+// dK and dV of the sinks' keys from the queries that have them behind their window, i - j >= window and j < sinks (of sinks set apart the
+// dK/dV kernels above take i - j < window; attn_window_reduce_kernel adds the two).  These few keys are seen by every later query: a key
 // tile's workgroup that took them too would run as many times longer than the others as a row is longer than its window.
 // A workgroup has 32 keys of one (batch, query head), their K and V fragments in every wave's registers, and a stretch of the
 // queries, 128 at a time, 32 to a wave; the waves' sums are added at the end.  `chunks` stretches to a key block, each leaving its sum.
@@ -3158,6 +3162,15 @@ int band_sink_chunks(int sp, int b, int nq, Band band) {
 bool band_shared_dq(int sp, int b, int nq, int hd, Band band) {
   return sp % 256 == 0 && band.window >= (hd == 64 ? 2048 : 4096) && (int64_t)(sp / 256) * nq * b >= kr_compute_units();
 }
+// The sinks whose keys the dK/dV kernel leaves, behind their window, to a kernel of their own: all, or, where a walk over the few queries
+// behind the window costs less than that launch and the one that adds its sums, none (apart -> by the dK/dV kernel, us of the whole
+// backward, 4 sinks: 257 tokens of 8 heads of 64, window 64 30.4 -> 22.0, 512, 128 32.1 -> 25.2, 768, 128 32.3 -> 28.6, 4 x 1024 of 8/2, 256
+// 46.7 -> 46.4; heads of 128: 2 x 512 of 8/2, 128 47.0 -> 42.5, 768 of 8, 200 47.0 -> 43.3, 2 x 768 of 8/2, 128 50.0 -> 51.2, 8 x 1024 of
+// 8/2, 512 117 -> 123).
+Band band_apart(int sp, int hd, Band band) {
+  if ((sp - band.window) / 128 <= (hd == 64 ? 6 : 3)) band.sinks = 0;
+  return band;
+}
 size_t band_sink_floats(int sp, int b, int nq, int hd, Band band) {
   return (size_t)b * nq * ((band.sinks + 31) / 32) * band_sink_chunks(sp, b, nq, band) * 2 * (hd / 32) * 16 * 64;
 }
@@ -3185,6 +3198,7 @@ int attn_bwd_mfma(const BwdCall& c) {
   bf16 *dq = c.dq, *dk = c.dk, *dv = c.dv;
   const int s = c.s, b = c.b, nq = c.nq, nkv = c.nkv, sp = attn_padded_len(s);
   const float scale = c.scale;
+  const Band apart = band_apart(sp, D, c.band);
   const QLayout ql = c.ql, ol = c.ol, dol = c.dol, dql = c.dql;
   const KLayout kl = c.kl, vl = c.vl, dkl = c.dkl, dvl = c.dvl;
   hipStream_t st = c.st;
@@ -3192,11 +3206,11 @@ int attn_bwd_mfma(const BwdCall& c) {
   const int64_t rows = (int64_t)b * nq * sp;
   float* neg_lse2 = neg_delta + rows;
   float* const sink_sums = neg_lse2 + rows;
-  float* part_k = sink_sums + (WIN ? band_sink_floats(sp, b, nq, D, c.band) : 0);
+  float* part_k = sink_sums + (WIN ? band_sink_floats(sp, b, nq, D, apart) : 0);
   const AttnForms forms = WIN ? AttnForms{false, band_shared_dq(sp, b, nq, D, c.band), 1} : attn_forms(sp, b, nq, c.nkv, D, c.flags);
   const int qsplit = forms.qsplit;
   // (with a window and no partial results of a group's heads, the sinks' key tiles leave theirs alone)
-  const int sink_rows = (c.band.sinks + 127) / 128 * 128;
+  const int sink_rows = (apart.sinks + 127) / 128 * 128;
   float* part_v = part_k + (WIN && nq == nkv ? (int64_t)b * nq * sink_rows : rows * qsplit) * D;
   // query heads of a KV group per dK/dV workgroup: as many as leave two workgroups per compute
   // unit (KR_DKDV_HPW_MAX: a build-time cap, for measurements)
@@ -3281,27 +3295,27 @@ int attn_bwd_mfma(const BwdCall& c) {
   }
   if (hipGetLastError() != hipSuccess) return KR_ELAUNCH;
   if constexpr (WIN) {
-    if (c.band.sinks) {
-      sink_chunks = band_sink_chunks(sp, b, nq, c.band);
-      hipLaunchKernelGGL((attn_bwd_sinks_kernel<D, RAGGED>), dim3((unsigned)(b * nq * ((c.band.sinks + 31) / 32) * sink_chunks)), dim3(256),
+    if (apart.sinks) {
+      sink_chunks = band_sink_chunks(sp, b, nq, apart);
+      hipLaunchKernelGGL((attn_bwd_sinks_kernel<D, RAGGED>), dim3((unsigned)(b * nq * ((apart.sinks + 31) / 32) * sink_chunks)), dim3(256),
                          lds_sinks, st, q, k, v, dout, neg_lse2, neg_delta, sink_sums, s, nq, nkv, sink_chunks, scale, scale_log2, ql, kl, vl,
-                         dol, c.band);
+                         dol, apart);
       if (hipGetLastError() != hipSuccess) return KR_ELAUNCH;
     }
   }
   const dim3 grid_kv((sp / 128) * (nq / hpw) * b * qsplit);
   hipLaunchKernelGGL(dkdv_kernel(partial), grid_kv, dim3(512), lds_dkdv, st, q, k, v, dout, neg_lse2,
                      neg_delta, dk, dv, part_k, part_v, s, nq, nkv, partial ? qsplit : 1, hpw, scale, scale_log2, ql, kl,
-                     vl, dol, dkl, dvl, c.band, partial ? sp : sink_rows);
+                     vl, dol, dkl, dvl, apart.sinks ? Band{c.band.window, 0} : c.band, partial ? sp : sink_rows);
   if constexpr (WIN) {
     const int reduced = partial ? s : sink_rows < s ? sink_rows : s;
     if (reduced) {
       if (hipGetLastError() != hipSuccess) return KR_ELAUNCH;
-      const int64_t sink_vectors = (int64_t)b * nkv * c.band.sinks * (D / 8), others = (int64_t)b * nkv * (reduced - c.band.sinks) * (D / 8);
+      const int64_t sink_vectors = (int64_t)b * nkv * apart.sinks * (D / 8), others = (int64_t)b * nkv * (reduced - apart.sinks) * (D / 8);
       const unsigned sink_blocks = (unsigned)((sink_vectors + 15) / 16);
       hipLaunchKernelGGL((attn_window_reduce_kernel<D>), dim3(sink_blocks + (unsigned)((others + 255) / 256)), dim3(256), 0, st, part_k,
                          part_v, sink_sums, dk, dv, reduced, partial ? sp : sink_rows, nq / hpw / nkv, nkv, per, sink_chunks,
-                         (int)sink_blocks, b * nkv, dkl, dvl, c.band);
+                         (int)sink_blocks, b * nkv, dkl, dvl, apart);
     }
   } else if (partial) {
     if (hipGetLastError() != hipSuccess) return KR_ELAUNCH;
@@ -3640,8 +3654,9 @@ extern "C" size_t kr_attn_window_bwd_workspace_bytes(int s, int b, int nq, int n
   const int sp = attn_padded_len(s);
   if (!band.window) return attn_bwd_fast_bytes(sp, b, nq, nkv, hd);
   const size_t rows = (size_t)b * nq * sp;
-  const size_t parts = nq != nkv ? rows : (size_t)b * nq * ((band.sinks + 127) / 128 * 128);
-  return (2 * rows + band_sink_floats(sp, b, nq, hd, band) + 2 * parts * hd) * sizeof(float);
+  const Band apart = band_apart(sp, hd, band);
+  const size_t parts = nq != nkv ? rows : (size_t)b * nq * ((apart.sinks + 127) / 128 * 128);
+  return (2 * rows + band_sink_floats(sp, b, nq, hd, apart) + 2 * parts * hd) * sizeof(float);
 }
 
 extern "C" int kr_attn_window_bwd(const void* dout, const void* q, const void* k, const void* v, const void* o, const float* lse,

@@ -114,6 +114,15 @@ def test_heads(b, nq, nkv, hd, s, window, sinks):
     check(*make(s, b, nq, nkv, hd), window, sinks)
 
 
+# rows that leave the sinks' keys to a kernel of their own, and those around the shortest that do
+@on_gpu
+@pytest.mark.parametrize("hd,nq,nkv", [(64, 2, 2), (64, 6, 2), (128, 3, 3), (128, 4, 1)])
+@pytest.mark.parametrize("s,window,sinks", [(896, 127, 3), (896, 128, 3), (897, 128, 130), (512, 127, 4), (512, 128, 4), (513, 129, 33), (1153, 1, 33),
+                                            (1280, 100, 200), (1300, 30, 1), (1408, 65, 65), (1536, 128, 32), (1111, 63, 129)])
+def test_sinks_of_long_rows(s, window, sinks, hd, nq, nkv):
+    check(*make(s, 2, nq, nkv, hd, seed=s), window, sinks)
+
+
 @on_gpu
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("beside", [False, True])
@@ -326,9 +335,9 @@ def test_refusals_of_the_library():
     size = lambda *a: lib.kr_attn_window_bwd_workspace_bytes(*a)  # noqa: E731
     stats, parts = 2 * 4 * 384 * 4, 2 * 4 * 384 * 64 * 4
     assert size(300, 1, 4, 2, 64, 50, 0) == stats + parts
-    assert size(300, 1, 4, 4, 64, 50, 0) == stats
-    # four heads' 32 sinks, the queries from 50 on in three stretches of 128: 2 x 2048 sums each, and the first key tile's own
-    assert size(300, 1, 4, 4, 64, 50, 20) == stats + 4 * 3 * 2 * 2048 * 4 + 2 * 4 * 128 * 64 * 4
+    assert size(300, 1, 4, 4, 64, 50, 0) == size(300, 1, 4, 4, 64, 50, 20) == stats
+    # four heads' 32 sinks, the queries from 50 on in eleven stretches of 128: 2 x 2048 sums each, and the first key tile's own
+    assert size(1300, 1, 4, 4, 64, 50, 20) == 2 * 4 * 1408 * 4 + 4 * 11 * 2 * 2048 * 4 + 2 * 4 * 128 * 64 * 4
     assert size(300, 1, 4, 2, 64, 300, 0) == size(300, 1, 4, 2, 64, 200, 100) == lib.kr_attn_bwd_workspace_bytes_strided(300, 1, 4, 2, 64, 64)
     assert size(300, 1, 4, 2, 80, 50, 0) == 0 and size(300, 1, 4, 2, 64, 0, 0) == 0
 
@@ -361,8 +370,8 @@ extern "C" int keys(int tk, int window, int sinks, int q0, int rows, int* list) 
   if (tk == 64) {{ BandTiles<64> t(Band{{window, sinks}}, q0, rows); for (int n = 0; n < t.total + 1; ++n) list[n] = t.of(n); return t.total; }}
   BandTiles<128> t(Band{{window, sinks}}, q0, rows); for (int n = 0; n < t.total + 1; ++n) list[n] = t.of(n); return t.total;
 }}
-extern "C" int queries(int tq, int window, int key0, int sp) {{
-  return tq == 64 ? band_query_tiles<64>(Band{{window, 0}}, key0, sp) : band_query_tiles<128>(Band{{window, 0}}, key0, sp);
+extern "C" int queries(int tq, int window, int sinks, int key0, int sp) {{
+  return tq == 64 ? band_query_tiles<64>(Band{{window, sinks}}, key0, sp) : band_query_tiles<128>(Band{{window, sinks}}, key0, sp);
 }}
 extern "C" void order(int grouped, int nblocks, int ntiles, int nheads, int per, int* tile, int* pair) {{
   for (int i = 0; i < nblocks; ++i)
@@ -403,10 +412,11 @@ def test_tiles_that_the_kernels_walk(tmp_path):
                                 assert lib.hides(window, sinks, t * tk, tk, q0 + r + 31)
                             if lib.hides_all(window, sinks, t * tk, tk, q0 + r):
                                 assert not bool(part.any())
-                near = visible(sp, window, 0, "cpu")
-                for key0 in range(0, sp, 128):
-                    end = lib.queries(tk, window, key0, sp)
-                    assert key0 // tk < end <= sp // tk and not bool(near[end * tk:, key0:key0 + 128].any())
+                for some in (0, sinks):
+                    near = visible(sp, window, some, "cpu")
+                    for key0 in range(0, sp, 128):
+                        end = lib.queries(tk, window, some, key0, sp)
+                        assert key0 // tk < end <= sp // tk and not bool(near[end * tk:, key0:key0 + 128].any())
 
 
 def test_the_order_of_workgroups_is_a_permutation(tmp_path):
