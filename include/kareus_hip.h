@@ -442,8 +442,9 @@ int kr_attn_bwd_flags(const void* dout, const void* q, const void* k, const void
  * among them) or j < sinks (the first keys stay visible to all).  Tensors, strides, lse and flags as kr_attn_fwd_flags' and
  * kr_attn_bwd_flags' (KR_ATTN_BESIDE_OTHER_STREAMS at most); hd 64 or 128, sequence strides below 2^31 / 127 elements unless hd = 128
  * and s is a multiple of 128 (KR_EUNSUPPORTED otherwise); scale positive.  Only key tiles with a visible key are read: work and
- * time go with s * (window + sinks).  Where window + sinks reach s nothing is hidden and the calls are those above.  Keys and values
- * have to be finite, hidden ones too: a tile's hidden probabilities are zeros that its values are multiplied by.
+ * time go with s * (window + sinks).  Where window + sinks reach s nothing is hidden, and from s = 513 on the calls are those above.
+ * Rows with few keys form their dO . O from the scores (a row whose probabilities are nearly all one key's has gradients of which
+ * nothing is left behind O's rounding).  Keys and values have to be finite, hidden ones too: a tile's hidden probabilities are zeros that its values are multiplied by.
  * workspace: kr_attn_window_bwd_workspace_bytes() bytes, 16-byte aligned.                         */
 int kr_attn_window_fwd(const void* q, const void* k, const void* v, void* o, float* lse,
                        int s, int b, int nq, int nkv, int hd, float scale,

@@ -108,8 +108,8 @@ __device__ __forceinline__ void longest_first(int pid, int nblocks, int ntiles, 
 // diagonal cuts.  All rows are of one length, so tiles go in sequence (band_order) instead of longest first.  The backward goes dQ, which
 // forms delta = sum dO . O on the way, then dK/dV by key tiles over the queries that have them in their window, and what queries further
 // on add to the sinks' keys apart (attn_bwd_sinks_kernel) unless they are few (band_apart); fp32 sums of a group's heads are added last.
-// 16384 tokens of 8/2 heads of 128, window 4096, 64 sinks, us: forward 262 (0.92 PFLOP/s of visible pairs), dQ 360, sinks 25, dK/dV 537
-// (0.83 together), sums 15; 2 x 8192 tokens of 16/4 heads of 64, window 1024: forward 110 (0.59, the exponentials).
+// 16384 tokens of 8/2 heads of 128, window 4096, 64 sinks, us: forward 262 (0.93 PFLOP/s of visible pairs), dQ 360, sinks 25, dK/dV 537
+// (0.66 together, counted as the five products that need be), sums 15; 2 x 8192 tokens of 16/4 heads of 64, window 1024: forward 110 (0.59, the exponentials).
 struct Band {
   int window, sinks;
 };
@@ -2136,6 +2136,10 @@ __global__ __launch_bounds__(256) void attn_group_reduce_kernel(
 // LDS at the end.  Chosen by the host when there are few workgroups.
 // When there are more 256-query tiles than compute units (or other streams run beside the launch; see attn_forms)
 // the host takes attn_bwd_dq_w64_kernel below instead.
+// Windows up to this many keys, and every row's first 128 queries, form delta from the scores (2-norm errors of dQ, of which 0.0017 are its
+// own rounding, delta from O -> from the scores: 2 tokens, window 1, a sink 0.038 -> 0.0027, 24, 19 0.0042 -> 0.0026, 351, 1 0.0037 -> 0.0024,
+// 257, 64 0.0025 -> 0.0024; backward of 257 tokens of 8 heads of 64, window 64, 22.0 -> 24.2 us, 3 x 2007 of 8/2 of 128, 500 no difference).
+constexpr int kDeltaFromScores = 64;
 template <int D, bool RAGGED, int HALVES, bool WIN>
 __global__ __launch_bounds__(256 * HALVES, HALVES == 1 ? 2 : 1) void attn_bwd_dq_kernel(
     const bf16* __restrict__ q, const bf16* __restrict__ k, const bf16* __restrict__ v,
@@ -2182,19 +2186,10 @@ __global__ __launch_bounds__(256 * HALVES, HALVES == 1 ? 2 : 1) void attn_bwd_dq
   const int64_t stat = (int64_t)bi * nq + head;
   float neg_lse = -lse[stat * s + qld] * kLog2e;
   float my_neg_delta;
-  if constexpr (WIN) {
-    // no pre-pass: delta of its rows from the dO fragments that a wave holds anyway, written with -lse in the log2 domain for the dK/dV
-    // kernels, which are launched behind this one
-    const bf16* op = o + ol.at(bi, head, per) + (int64_t)qld * ol.s_;
-    float dsum = 0.f;  // this lane's half of the row (channels 16 kk + 8 h ..)
-#pragma unroll
-    for (int kk = 0; kk < KK; ++kk) {
-      const bf16x8 of = ldg8(op + kk * 16 + h * 8);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) dsum += (float)dof[kk][e] * (float)of[e];
-    }
-    dsum += __shfl_xor(dsum, 32, KR_WAVE);
-    my_neg_delta = -dsum;
+  // Rows with few keys form delta from the scores, sum P dP, in a walk of its own in front: O is rounded, and where a row's few dP - delta
+  // are much smaller than delta that rounding is all that is left of them.
+  const bool from_scores = WIN && (q0 == 0 || band.window <= kDeltaFromScores);
+  auto leave_statistics = [&]() {
     if (RAGGED && qrow >= s) {  // rows the dK/dV kernels must not see
       my_neg_delta = 0.f;
       neg_lse = -kPadLse * kLog2e;
@@ -2202,6 +2197,23 @@ __global__ __launch_bounds__(256 * HALVES, HALVES == 1 ? 2 : 1) void attn_bwd_dq
     if (h == 0 && half == 0) {
       neg_delta_out[stat * sp + qrow] = my_neg_delta;
       neg_lse2_out[stat * sp + qrow] = neg_lse;
+    }
+  };
+  if constexpr (WIN) {
+    // no pre-pass: delta of its rows from the dO fragments that a wave holds anyway, written with -lse in the log2 domain for the dK/dV
+    // kernels, which are launched behind this one
+    if (!from_scores) {
+      const bf16* op = o + ol.at(bi, head, per) + (int64_t)qld * ol.s_;
+      float dsum = 0.f;  // this lane's half of the row (channels 16 kk + 8 h ..)
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) {
+        const bf16x8 of = ldg8(op + kk * 16 + h * 8);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) dsum += (float)dof[kk][e] * (float)of[e];
+      }
+      dsum += __shfl_xor(dsum, 32, KR_WAVE);
+      my_neg_delta = -dsum;
+      leave_statistics();
     }
   } else {
     my_neg_delta = neg_delta[stat * sp + qld];
@@ -2243,57 +2255,112 @@ __global__ __launch_bounds__(256 * HALVES, HALVES == 1 ? 2 : 1) void attn_bwd_dq
   zero_tail(0, 0);
   kr_barrier();
 
+  // S^T and dP^T of 32 keys, hidden scores -inf; lane: query row qrow, keys key0 + 32t + 8g + 4h + e
+  auto scores = [&](int key0, int t, uint32_t k_rows, uint32_t v_rows, f32x16& sacc, f32x16& dpacc) __attribute__((always_inline)) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      sacc[e] = 0.f;
+      dpacc[e] = 0.f;
+    }
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+      sacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bt_rows<D>(k_rows, t, kk), qf[kk], sacc, 0, 0, 0);
+      dpacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bt_rows<D>(v_rows, t, kk), dof[kk], dpacc, 0, 0, 0);
+    }
+    if (key0 + TK - 1 > qw0) {  // wave-uniform: the tile on the diagonal
+      // Off the diagonal no mask code must run.  Left alone the compiler turns the branch
+      // into 16 unconditional selects; values that pass through an (empty) volatile asm can
+      // only be produced where the asm executes, i.e. inside the branch.
+      const int lim = qrow - key0 - t * 32 - 4 * h;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        float v = 8 * (e >> 2) + (e & 3) > lim ? -INFINITY : sacc[e];
+        asm volatile("" : "+v"(v));
+        sacc[e] = v;
+      }
+    }
+    if (WIN && band_hides(band, key0 + 32 * t, 32, qw0 + 31)) {
+      const int at = key0 + t * 32 + 4 * h, lim = qrow - band.window - at, from = band.sinks - at;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int c = 8 * (e >> 2) + (e & 3);
+        float v = c <= lim && c >= from ? -INFINITY : sacc[e];
+        asm volatile("" : "+v"(v));
+        sacc[e] = v;
+      }
+    }
+  };
+  auto sees_tile = [&](int key0) { return key0 <= qw0 + 31 && !(WIN && band_hides_all(band, key0, TK, qw0)); };
+  auto sees_block = [&](int key0, int t) {
+    if ((D == 64 || WIN) && key0 + 32 * t > qw0 + 31) return false;  // wave-uniform: beyond the diagonal
+    return !(WIN && band_hides_all(band, key0 + 32 * t, 32, qw0));
+  };
   settle_scalar_loads();
+  bool held = false;  // the walk that formed delta has left all tiles in the stages
+  int start = 0;      // stage of the first tile
+  if constexpr (WIN) {
+    if (from_scores) {
+      held = ntiles <= 2;
+      start = held ? 0 : ntiles & 1;
+      float psum = 0.f, pdp = 0.f;  // of this lane's scores: P, P dP
+      for (int j = 0; j < ntiles; ++j) {
+        const int cur = j & 1, next = j + 1 < ntiles ? j + 1 : 0;
+        if (next || !held) stage_request(__builtin_amdgcn_readfirstlane(next), cur ^ 1);
+        const int key0 = key_of(j);
+        if (sees_tile(key0)) {
+          uint32_t k_rows = area + cur * STAGE + bt_rows_lane(lane);
+          uint32_t v_rows = k_rows + BT_BYTES;
+          asm volatile("" : "+v"(k_rows), "+v"(v_rows));
+#pragma unroll
+          for (int t = 0; t < NB; ++t) {
+            if (!sees_block(key0, t)) continue;
+            f32x16 sacc, dpacc;
+            scores(key0, t, k_rows, v_rows, sacc, dpacc);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[e], scale_log2, neg_lse));
+              psum += p;
+              pdp = __builtin_fmaf(p, dpacc[e], pdp);
+            }
+          }
+        }
+        __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+        if (RAGGED && (next || !held)) zero_tail(next, cur ^ 1);
+        if (j + 1 < ntiles) kr_barrier();
+      }
+      psum += __shfl_xor(psum, 32, KR_WAVE);
+      pdp += __shfl_xor(pdp, 32, KR_WAVE);
+      // (both halves' sums: behind the stages, pairs by [half][wave][row])
+      float* const sums = reinterpret_cast<float*>(reinterpret_cast<char*>(smem) + 4 * STAGE) + (wave * 32 + (lane & 31)) * 2;
+      if (HALVES == 2 && h == 0) {
+        sums[half * 256] = psum;
+        sums[half * 256 + 1] = pdp;
+      }
+      kr_barrier();
+      if (HALVES == 2) {
+        psum += sums[(half ^ 1) * 256];
+        pdp += sums[(half ^ 1) * 256 + 1];
+      }
+      my_neg_delta = -pdp / psum;
+      leave_statistics();
+    }
+  }
   for (int j = 0; j < ntiles; ++j) {
-    const int cur = j & 1;
-    if (j + 1 < ntiles) stage_request(j + 1, cur ^ 1);
+    const int cur = __builtin_amdgcn_readfirstlane((j + start) & 1);
+    if (j + 1 < ntiles && !held) stage_request(j + 1, cur ^ 1);
     const int key0 = key_of(j);
-    if (key0 <= qw0 + 31 && !(WIN && band_hides_all(band, key0, TK, qw0))) {
+    if (sees_tile(key0)) {
       // one base register per tile and read direction; everything else is an immediate
       uint32_t k_rows = area + cur * STAGE + bt_rows_lane(lane);
       uint32_t v_rows = k_rows + BT_BYTES;
       uint32_t k_cols = area + cur * STAGE + bt_cols_lane(lane);
       asm volatile("" : "+v"(k_rows), "+v"(v_rows), "+v"(k_cols));
-      const bool need_mask = key0 + TK - 1 > qw0;  // wave-uniform: the tile on the diagonal
 #pragma unroll
       for (int t = 0; t < NB; ++t) {
-        if ((D == 64 || WIN) && key0 + 32 * t > qw0 + 31) continue;  // wave-uniform: beyond the diagonal
-        if (WIN && band_hides_all(band, key0 + 32 * t, 32, qw0)) continue;
+        if (!sees_block(key0, t)) continue;
         f32x16 sacc, dpacc;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          sacc[e] = 0.f;
-          dpacc[e] = 0.f;
-        }
-#pragma unroll
-        for (int kk = 0; kk < KK; ++kk) {
-          sacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bt_rows<D>(k_rows, t, kk), qf[kk], sacc, 0, 0, 0);
-          dpacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bt_rows<D>(v_rows, t, kk), dof[kk], dpacc, 0, 0, 0);
-        }
-        // lane: query row qrow, keys key0 + 32t + 8g + 4h + e
+        scores(key0, t, k_rows, v_rows, sacc, dpacc);
         bf16x8 dsb[2];
-        if (need_mask) {
-          // Off the diagonal no mask code must run.  Left alone the compiler turns the branch
-          // into 16 unconditional selects; values that pass through an (empty) volatile asm can
-          // only be produced where the asm executes, i.e. inside the branch.
-          const int lim = qrow - key0 - t * 32 - 4 * h;
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            float v = 8 * (e >> 2) + (e & 3) > lim ? -INFINITY : sacc[e];
-            asm volatile("" : "+v"(v));
-            sacc[e] = v;
-          }
-        }
-        if (WIN && band_hides(band, key0 + 32 * t, 32, qw0 + 31)) {
-          const int at = key0 + t * 32 + 4 * h, lim = qrow - band.window - at, from = band.sinks - at;
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int c = 8 * (e >> 2) + (e & 3);
-            float v = c <= lim && c >= from ? -INFINITY : sacc[e];
-            asm volatile("" : "+v"(v));
-            sacc[e] = v;
-          }
-        }
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[e], scale_log2, neg_lse));
@@ -2309,7 +2376,7 @@ __global__ __launch_bounds__(256 * HALVES, HALVES == 1 ? 2 : 1) void attn_bwd_dq
       }
     }
     __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's share of the next tiles has landed
-    if (RAGGED && j + 1 < ntiles) zero_tail(j + 1, cur ^ 1);
+    if (RAGGED && j + 1 < ntiles && !held) zero_tail(j + 1, cur ^ 1);
     kr_barrier();
   }
 
@@ -3242,6 +3309,7 @@ int attn_bwd_mfma(const BwdCall& c) {
       return partial ? attn_bwd_dkdv_kernel<RAGGED, true, WIN> : attn_bwd_dkdv_kernel<RAGGED, false, WIN>;
   };
   constexpr size_t lds_dq = 2 * (2 * BT_BYTES);  // two stages of a K and a V tile
+  constexpr size_t lds_dq2 = 2 * lds_dq + (WIN ? 2 * 128 * 2 * sizeof(float) : 0);  // of either half, and a window's sums of both
   // two stages of 128 queries and their gradients; the waves' sums
   constexpr size_t lds_sinks_stages = 2 * (2 * 128 / tile_rows<D> * BT_BYTES), lds_sinks_sums = 4 * 64 * (D + 4) * sizeof(float);
   constexpr size_t lds_sinks = lds_sinks_stages > lds_sinks_sums ? lds_sinks_stages : lds_sinks_sums;
@@ -3256,7 +3324,7 @@ int attn_bwd_mfma(const BwdCall& c) {
                               hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds_dq);
     if (e == hipSuccess)
       e = hipFuncSetAttribute((const void*)attn_bwd_dq_kernel<D, RAGGED, 2, WIN>,
-                              hipFuncAttributeMaxDynamicSharedMemorySize, (int)(2 * lds_dq));
+                              hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds_dq2);
     if constexpr (WIN)
       if (e == hipSuccess)
         e = hipFuncSetAttribute((const void*)attn_bwd_sinks_kernel<D, RAGGED>, hipFuncAttributeMaxDynamicSharedMemorySize,
@@ -3277,7 +3345,7 @@ int attn_bwd_mfma(const BwdCall& c) {
     // and end beside each other (one of eight waves -> those, us of the whole backward: 384 workgroups, 3 x 2007 tokens, window 500 140 ->
     // 133; 1024, 2 x 8192 of heads of 64, 128 168 -> 134, 16384 of 128, 4096 969 -> 946; 256, 4096, 512 63 -> 65)
     if (dq_blocks <= (WIN ? kr_compute_units() : 4 * 256)) {
-      hipLaunchKernelGGL((attn_bwd_dq_kernel<D, RAGGED, 2, WIN>), dim3(dq_blocks), dim3(512), 2 * lds_dq, st,
+      hipLaunchKernelGGL((attn_bwd_dq_kernel<D, RAGGED, 2, WIN>), dim3(dq_blocks), dim3(512), lds_dq2, st,
                          q, k, v, dout, lse,
                          neg_delta, dq, s, nq, nkv, scale, scale_log2, ql, kl, vl, dol,
                          dql, c.band, o, ol, neg_delta, neg_lse2);
@@ -3609,13 +3677,17 @@ extern "C" int kr_attn_fwd_ws(const void* q, const void* k, const void* v, void*
 }
 #else  // KR_ATTN_WINDOW_TU
 namespace {
-// What a call asks for, as the kernels take it: no window where every key up to its own is visible to every query.
+// What a call asks for, as the kernels take it: no window where every key up to its own is visible to every query, unless rows are so short
+// that those with few keys count (attn_bwd_dq_kernel forms their delta from the scores: 2-norm errors of dQ, 2 tokens 0.013 -> 0.0037, 31
+// 0.0040 -> 0.0022; from 512 on the plain kernels have 0.0025 as well).
+constexpr int kShortRows = 512;
 int make_band(int s, int hd, float scale, int window, int sinks, int flags, Band* band) {
   if (window <= 0 || sinks < 0 || !(scale > 0.f)) return KR_EINVAL;
   if (flags & ~KR_ATTN_BESIDE_OTHER_STREAMS) return KR_EINVAL;
   if (hd != 64 && hd != 128) return KR_EUNSUPPORTED;
   if (sinks > s) sinks = s;
-  *band = (int64_t)window + sinks >= s ? Band{0, 0} : Band{window, sinks};
+  const bool all = (int64_t)window + sinks >= s;
+  *band = all ? Band{s <= kShortRows ? s : 0, 0} : Band{window, sinks};
   return KR_OK;
 }
 int check_tensors(int s, int hd, std::initializer_list<const void*> ptrs, std::initializer_list<int64_t> seq,

@@ -6,6 +6,8 @@ Bounds, element by element, from what is rounded.  u = 2^-24, half a bf16 step 2
   o            probabilities rounded to bf16, then o: 2^-8 |o| + (2^-8 + e) sum p |v|
   dV           the same with P and dO: 2^-8 |dV| + sum (2^-8 + e) P |dO|
   delta        dO . o with the rounded o: D = sum |dO| (bound of o) + hd u sum |dO o|
+               of a row's first 128 queries and windows up to 64, sum P dP over sum P: their errors weigh what dP is off delta by,
+               D = sum P (e |dP - delta| + hd u sum |dO V|) + (s + 8) u sum P |dP|
   dS           rounded to bf16 behind P (dP - delta): ds = 2^-8 |dS| + P (e |dP - delta| + hd u sum |dO V| + D)
   dQ, dK       2^-8 of the result + scale sum ds |k|, scale sum ds |q|"""
 
@@ -44,7 +46,7 @@ def visible(s, window, sinks, device):
     return (back >= 0) & ((back < window) | (i < sinks))
 
 
-def reference(q, k, v, do, scale, window, sinks):
+def reference(q, k, v, do, scale, window, sinks, from_scores=False):
     s, b, nkv, per, hd = q.shape
     rows = lambda t: t.double().permute(1, 2, 3, 0, 4)                    # noqa: E731  [b, nkv, per, s, hd]
     q, g = rows(q), rows(do.view(s, b, nkv, per, hd))
@@ -64,6 +66,8 @@ def reference(q, k, v, do, scale, window, sinks):
     delta = (g * o).sum(-1, keepdim=True)
     d_off = (g.abs() * tol["o"]).sum(-1, keepdim=True) + hd * U * (g * o).abs().sum(-1, keepdim=True)
     ds = p * (dp - delta)
+    if from_scores:
+        d_off = (p * (e * (dp - delta).abs() + hd * U * (g.abs() @ t(v).abs()) + (s + 8) * U * dp.abs())).sum(-1, keepdim=True)
     ds_off = HALF * ds.abs() + p * (e * (dp - delta).abs() + hd * U * (g.abs() @ t(v).abs()) + d_off)
     group = lambda m: m.sum(2, keepdim=True)                               # noqa: E731
     out["dv"], out["dq"], out["dk"] = group(t(p) @ g), scale * (ds @ k), scale * group(t(ds) @ q)
@@ -82,13 +86,13 @@ def close(name, got, want, tol):
     assert bool((off <= tol + 1e-30).all()), (name, float((off / (tol + 1e-30)).max()))
 
 
-def check(q, k, v, do, window, sinks, scale=None, beside=False):
+def check(q, k, v, do, window, sinks, scale=None, beside=False, from_scores=False):
     be = get_backend("hip")
     scale = q.shape[-1] ** -0.5 if scale is None else scale
     band = dict(window=window, sinks=sinks, beside_other_streams=beside)
     o, lse = be.attn_fwd(q, k, v, scale, **band)
     dq, dk, dv = be.attn_bwd(do, q, k, v, o, lse, scale, **band)
-    want, tol = reference(q, k, v, do, scale, window, sinks)
+    want, tol = reference(q, k, v, do, scale, window, sinks, from_scores)
     for name, t in (("lse", lse), ("o", o), ("dv", dv), ("dk", dk), ("dq", dq)):
         close(name, t, want[name], tol[name])
     return o, lse, dq, dk, dv
@@ -112,6 +116,17 @@ def test_lengths_windows_and_sinks(s, window, sinks, hd):
 @pytest.mark.parametrize("s,window,sinks", [(333, 100, 5), (256, 96, 0)])
 def test_heads(b, nq, nkv, hd, s, window, sinks):
     check(*make(s, b, nq, nkv, hd), window, sinks)
+
+
+# rows with few keys: of a window, of a short sequence, all but one of them with next to no probability
+@on_gpu
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("scale", [None, 1.0])
+@pytest.mark.parametrize("s,b,nq,nkv,window,sinks", [(2, 1, 2, 1, 1, 1), (2, 2, 1, 1, 2, 0), (3, 1, 4, 2, 1, 40), (24, 1, 2, 1, 19, 1), (31, 1, 2, 2, 12, 40),
+                                                     (100, 2, 3, 1, 100, 0), (128, 1, 4, 4, 70, 9), (300, 1, 2, 2, 64, 4), (515, 1, 4, 2, 33, 130),
+                                                     (700, 2, 2, 1, 1, 1), (1300, 8, 16, 4, 20, 0), (1300, 8, 16, 4, 64, 66)])
+def test_rows_with_few_keys(s, b, nq, nkv, window, sinks, scale, hd):
+    check(*make(s, b, nq, nkv, hd, seed=s), window, sinks, scale=scale, from_scores=True)
 
 
 # rows that leave the sinks' keys to a kernel of their own, and those around the shortest that do
@@ -171,10 +186,12 @@ def test_scores_over_a_wide_range():
 @pytest.mark.parametrize("hd", [64, 128])
 def test_a_window_that_hides_nothing_is_plain_attention(hd):
     be = get_backend("hip")
-    q, k, v, do = make(300, 2, 4, 2, hd)
+    for window, sinks in ((300, 0), (1 << 40, 0), (299, 1), (100, 200), (1, 1 << 40)):    # (short rows keep to the window's kernels)
+        check(*make(300, 2, 4, 2, hd), window, sinks)
+    q, k, v, do = make(520, 2, 4, 2, hd)
     plain = be.attn_fwd(q, k, v, 0.1)
     grads = be.attn_bwd(do, q, k, v, *plain, 0.1)
-    for window, sinks in ((300, 0), (1 << 40, 0), (299, 1), (100, 200), (1, 1 << 40)):
+    for window, sinks in ((520, 0), (1 << 40, 0), (519, 1), (320, 200), (1, 1 << 40)):
         got = be.attn_fwd(q, k, v, 0.1, window=window, sinks=sinks)
         assert all(torch.equal(a, b) for a, b in zip(plain, got))
         assert all(torch.equal(a, b) for a, b in zip(grads, be.attn_bwd(do, q, k, v, *got, 0.1, window=window, sinks=sinks)))
@@ -338,7 +355,8 @@ def test_refusals_of_the_library():
     assert size(300, 1, 4, 4, 64, 50, 0) == size(300, 1, 4, 4, 64, 50, 20) == stats
     # four heads' 32 sinks, the queries from 50 on in eleven stretches of 128: 2 x 2048 sums each, and the first key tile's own
     assert size(1300, 1, 4, 4, 64, 50, 20) == 2 * 4 * 1408 * 4 + 4 * 11 * 2 * 2048 * 4 + 2 * 4 * 128 * 64 * 4
-    assert size(300, 1, 4, 2, 64, 300, 0) == size(300, 1, 4, 2, 64, 200, 100) == lib.kr_attn_bwd_workspace_bytes_strided(300, 1, 4, 2, 64, 64)
+    assert size(600, 1, 4, 2, 64, 600, 0) == size(600, 1, 4, 2, 64, 400, 200) == lib.kr_attn_bwd_workspace_bytes_strided(600, 1, 4, 2, 64, 64)
+    assert size(300, 1, 4, 2, 64, 300, 0) == size(300, 1, 4, 2, 64, 200, 100) == stats + parts
     assert size(300, 1, 4, 2, 80, 50, 0) == 0 and size(300, 1, 4, 2, 64, 0, 0) == 0
 
 
