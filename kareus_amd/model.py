@@ -1,5 +1,5 @@
 """The two ends around the layer stack, so that a stack computes a loss from token ids:
-embedding -> LayerStack -> final RMSNorm -> output layer -> cross entropy.
+embedding -> LayerStack -> final norm -> output layer -> cross entropy; and the clipping of its gradients.
 
 What the reference runs outside its partitions ("non-partition" work,
 tests/bayesian/nonpartition/profile_nonpartition.py:148-486): ``LanguageModelEmbedding``
@@ -226,8 +226,8 @@ class LanguageModelEmbedding(torch.nn.Module):
 
 class GPTModelShard(torch.nn.Module):
     """``forward(input_ids [b, s], labels [b, s] or None, position_ids=None)`` -> loss ``[b, s]`` (fp32) or logits
-    ``[s, b, vocab_rows]``; ``position_ids`` as :class:`LayerStack`'s.  After ``backward()``, ``clip_grad_norm(max_norm)`` ends the step.  ``embedding_scale``, ``embedding_sorted_gradient``, ``embedding_main_grad``: see
-    :class:`LanguageModelEmbedding`."""
+    ``[s, b, vocab_rows]``; ``position_ids`` as :class:`LayerStack`'s.  After ``backward()``, ``clip_grad_norm(max_norm)`` ends the step.
+    ``embedding_scale``, ``embedding_sorted_gradient``, ``embedding_main_grad``: see :class:`LanguageModelEmbedding`."""
 
     def __init__(self, config: LayerConfig, vocab_rows: int, vocab_start: int = 0, device=None,
                  seed: Optional[int] = None, embedding_scale: float = 1.0, embedding_sorted_gradient: bool = False,
