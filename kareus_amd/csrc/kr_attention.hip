@@ -134,6 +134,18 @@ __device__ __forceinline__ bool band_hides(Band band, int key0, int n, int q_las
 __device__ __forceinline__ bool band_hides_all(Band band, int key0, int n, int q_first) {
   return q_first - (key0 + n - 1) >= band.window && key0 >= band.sinks;
 }
+// Whether the key c behind key0 is out of a query's sight, behind its window and no sink: one unsigned comparison (for two and their
+// conjunction; forward, us: 257 tokens of 8 heads of 64, window 64 13.5 -> 12.8, 2 x 8192 of 16/4, 128 72.5 -> 70.0, heads of 128 no difference).
+struct BandHidden {
+  int from;
+  uint32_t count;
+  __device__ __forceinline__ BandHidden(Band band, int query, int key0) {
+    from = band.sinks - key0;
+    const int past = query - band.window - key0 + 1;  // the first key in the window
+    count = past > from ? (uint32_t)(past - from) : 0u;
+  }
+  __device__ __forceinline__ bool at(int c) const { return (uint32_t)(c - from) < count; }
+};
 // Workgroup -> (tile, (batch, head) pair): rows of a window are of one length, so tiles go in sequence, a contiguous range of them to an
 // XCD; the heads of a KV group side by side (GROUPED), which share their keys, or a head's tiles, which share its queries.
 template <bool GROUPED>
@@ -708,13 +720,12 @@ __global__ __launch_bounds__(512, 1) void attn_fwd_pp_kernel(
       if (WIN && band_hides(band, key0, TK, qw0 + 31)) {
         asm volatile("" ::: "memory");
         const int at = key0 + 4 * h;
-        const int lim = qrow - band.window - at, from = band.sinks - at;  // offsets from `from` to lim are keys behind the window
+        const BandHidden hidden(band, qrow, at);
 #pragma unroll
         for (int t = 0; t < NB; ++t)
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            const int c = t * 32 + 8 * (e >> 2) + (e & 3);
-            if (c <= lim && c >= from) sacc[t][e] = -INFINITY;
+            if (hidden.at(t * 32 + 8 * (e >> 2) + (e & 3))) sacc[t][e] = -INFINITY;
           }
       }
       float mx = -INFINITY;
@@ -1022,13 +1033,12 @@ __global__ __launch_bounds__(512, 1) void attn_fwd_sh_kernel(
       if (WIN && band_hides(band, key0, TK, qw0 + 31)) {
         asm volatile("" ::: "memory");
         const int at = key0 + 4 * h;
-        const int lim = qrow - band.window - at, from = band.sinks - at;  // offsets from `from` to lim are keys behind the window
+        const BandHidden hidden(band, qrow, at);
 #pragma unroll
         for (int t = 0; t < NB; ++t)
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            const int c = t * 32 + 8 * (e >> 2) + (e & 3);
-            if (c <= lim && c >= from) sacc[t][e] = -INFINITY;
+            if (hidden.at(t * 32 + 8 * (e >> 2) + (e & 3))) sacc[t][e] = -INFINITY;
           }
       }
       float mx = -INFINITY;
@@ -2280,11 +2290,10 @@ __global__ __launch_bounds__(256 * HALVES, HALVES == 1 ? 2 : 1) void attn_bwd_dq
       }
     }
     if (WIN && band_hides(band, key0 + 32 * t, 32, qw0 + 31)) {
-      const int at = key0 + t * 32 + 4 * h, lim = qrow - band.window - at, from = band.sinks - at;
+      const BandHidden hidden(band, qrow, key0 + t * 32 + 4 * h);
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        const int c = 8 * (e >> 2) + (e & 3);
-        float v = c <= lim && c >= from ? -INFINITY : sacc[e];
+        float v = hidden.at(8 * (e >> 2) + (e & 3)) ? -INFINITY : sacc[e];
         asm volatile("" : "+v"(v));
         sacc[e] = v;
       }
