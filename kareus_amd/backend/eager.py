@@ -268,6 +268,7 @@ class EagerBackend:
         return out
 
     # The 2-norm over all tensors in 64 bits, and all tensors times min(1, max_norm / (norm + eps))
+    @torch.no_grad()
     def grad_norm(self, tensors) -> Tensor:
         tensors = list(tensors)
         check_gradients(tensors)
@@ -275,6 +276,7 @@ class EagerBackend:
             return torch.zeros(())
         return torch.stack([t.double().square().sum() for t in tensors]).sum().sqrt().float()
 
+    @torch.no_grad()
     def clip_grad_norm(self, tensors, max_norm: float, eps: float = 1e-6, out=None) -> Tensor:
         tensors = list(tensors)
         check_gradients(tensors, max_norm, eps, out)

@@ -3,17 +3,17 @@
 
 from __future__ import annotations
 
-from typing import Iterable, List, Optional, Sequence
+from typing import Iterable, List, Optional, Sequence, Union
 
 import torch
 from torch import Tensor
 
 
-def gradients_of(parameters: Iterable[torch.nn.Parameter]) -> List[Tensor]:
+def gradients_of(parameters: Union[Tensor, Iterable[torch.nn.Parameter]]) -> List[Tensor]:
     """The gradients that there are, one for each parameter object: its ``main_grad``, or where it keeps none its ``grad``.  One that has
     both raises: which of them a step goes by is not for this function to say."""
     found, seen = [], set()
-    for p in parameters:
+    for p in [parameters] if isinstance(parameters, Tensor) else parameters:    # (of a tensor alone the rows would be gone through)
         if id(p) in seen:
             continue
         seen.add(id(p))
@@ -26,14 +26,14 @@ def gradients_of(parameters: Iterable[torch.nn.Parameter]) -> List[Tensor]:
     return found
 
 
-def grad_norm(parameters: Iterable[torch.nn.Parameter], backend: str = "hip") -> Tensor:
+def grad_norm(parameters: Union[Tensor, Iterable[torch.nn.Parameter]], backend: str = "hip") -> Tensor:
     """The 2-norm of all gradients as one vector, fp32 on the gradients' device; nothing waits for it."""
     from .backend import get_backend
 
     return get_backend(backend).grad_norm(gradients_of(parameters))
 
 
-def clip_grad_norm(parameters: Iterable[torch.nn.Parameter], max_norm: float, eps: float = 1e-6, backend: str = "hip",
+def clip_grad_norm(parameters: Union[Tensor, Iterable[torch.nn.Parameter]], max_norm: float, eps: float = 1e-6, backend: str = "hip",
                    out: Optional[Sequence[Tensor]] = None) -> Tensor:
     """Scales all gradients by ``min(1, max_norm / (norm + eps))`` and returns their norm before that, fp32 on their device; nothing
     waits for it.  ``out``: fp32 tensors, one for each gradient in order, that receive the scaled gradients (an optimizer's own), and

@@ -221,3 +221,14 @@ def test_parameters():
     with pytest.raises(RuntimeError, match="main_grad and a grad"):
         grad_norm([b], backend="eager")
     assert float(grad_norm([c], backend="eager")) == 0.0
+
+
+def test_one_parameter_and_gradients_with_a_history():
+    """A parameter by itself is one, not its rows; gradients of a graph that is kept are scaled in place all the same."""
+    p = torch.nn.Parameter(torch.full((2, 3), 2.0))
+    (p.grad,) = torch.autograd.grad((p ** 3).sum(), p, create_graph=True)
+    want = float(p.grad.detach().double().norm())
+    assert float(grad_norm(p, backend="eager")) == pytest.approx(want, rel=1e-6)
+    assert float(clip_grad_norm(p, 0.5 * want, eps=0.0, backend="eager")) == pytest.approx(want, rel=1e-6)
+    assert p.grad.detach().flatten().tolist() == [6.0] * 6
+    p.grad = None
