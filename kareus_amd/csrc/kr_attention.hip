@@ -2038,26 +2038,25 @@ __global__ __launch_bounds__(256, 1) void attn_bwd_sinks_kernel(
 }
 
 // dK and dV of the first `rows` keys: the fp32 sums of the dK/dV kernel over a group's `slots` workgroups, of part_rows rows each, one
-// thread per 8 channels.  The first `sink_blocks` workgroups have the sinks' keys, to which those of attn_bwd_sinks_kernel over the group's
+// thread per 8 channels.  Of the `blocks` workgroups of a (batch, KV head) pair the first `sink_blocks` have the sinks' keys, to which those of attn_bwd_sinks_kernel over the group's
 // heads and their stretches of queries are added, up to 16 of a head: 16 threads share them and add theirs in a fixed order.
 template <int D>
 __global__ __launch_bounds__(256) void attn_window_reduce_kernel(
     const float* __restrict__ part_k, const float* __restrict__ part_v, const float* __restrict__ sums, bf16* __restrict__ dk,
-    bf16* __restrict__ dv, int rows, int part_rows, int slots, int nkv, int per, int chunks, int sink_blocks, int groups, KLayout dkl,
+    bf16* __restrict__ dv, int rows, int part_rows, int slots, int nkv, int per, int chunks, int sink_blocks, int blocks, KLayout dkl,
     KLayout dvl, Band band) {
   constexpr int VEC = D / 8, N = 2 * 32 * D;
   __shared__ f32x4 red[4][16][16];  // [values][share][place]
-  const bool sinks = (int)blockIdx.x < sink_blocks;
+  const int pair = blockIdx.x / blocks, block = blockIdx.x - pair * blocks;
+  const bool sinks = block < sink_blocks;
   const int share = sinks ? threadIdx.x / 16 : 0, place = threadIdx.x % 16;
-  // (bi, kvh, si, chunk of 8): of the sinks' keys, or of those behind them
-  const int64_t idx = sinks ? (int64_t)blockIdx.x * 16 + place : (int64_t)(blockIdx.x - sink_blocks) * 256 + threadIdx.x;
-  const int first = sinks ? 0 : band.sinks, count = sinks ? band.sinks : rows - band.sinks;
-  const int c = (int)(idx % VEC);
-  const int si = first + (int)((idx / VEC) % count);
-  const int64_t group = idx / VEC / count;  // bi * nkv + kvh
-  const bool there = group < groups;
+  // (si, chunk of 8): of the sinks' keys, or of those behind them
+  const int idx = sinks ? block * 16 + place : (block - sink_blocks) * 256 + threadIdx.x;
+  const int c = idx % VEC, si = (sinks ? 0 : band.sinks) + idx / VEC;
+  const bool there = si < (sinks ? band.sinks : rows);
   if (!sinks && !there) return;
-  const int kvh = (int)(group % nkv), bi = (int)(group / nkv);
+  const int64_t group = pair;  // bi * nkv + kvh
+  const int kvh = pair % nkv, bi = pair / nkv;
   f32x4 a[4];  // dK, dV
 #pragma unroll
   for (int i = 0; i < 4; ++i) a[i] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -2068,17 +2067,18 @@ __global__ __launch_bounds__(256) void attn_window_reduce_kernel(
     a[3] += *reinterpret_cast<const f32x4*>(pv + 4);
   };
   if (share == 0 && there) {
+#pragma unroll 4
     for (int j = 0; j < slots; ++j) {
       const int64_t off = ((group * slots + j) * part_rows + si) * D + c * 8;
       add(part_k + off, part_v + off);
     }
   }
   if (sinks) {
-    const int blocks = (band.sinks + 31) / 32;
+    const int key_blocks = (band.sinks + 31) / 32;
     if (there) {
       for (int j = 0; j < per; ++j)
         for (int ch = share; ch < chunks; ch += 16) {
-          const float* at = sums + (((group * per + j) * blocks + si / 32) * chunks + ch) * N + (si % 32) * D + c * 8;
+          const float* at = sums + (((group * per + j) * key_blocks + si / 32) * chunks + ch) * N + (si % 32) * D + c * 8;
           add(at, at + 32 * D);
         }
     }
@@ -3396,11 +3396,10 @@ int attn_bwd_mfma(const BwdCall& c) {
     const int reduced = partial ? s : sink_rows < s ? sink_rows : s;
     if (reduced) {
       if (hipGetLastError() != hipSuccess) return KR_ELAUNCH;
-      const int64_t sink_vectors = (int64_t)b * nkv * apart.sinks * (D / 8), others = (int64_t)b * nkv * (reduced - apart.sinks) * (D / 8);
-      const unsigned sink_blocks = (unsigned)((sink_vectors + 15) / 16);
-      hipLaunchKernelGGL((attn_window_reduce_kernel<D>), dim3(sink_blocks + (unsigned)((others + 255) / 256)), dim3(256), 0, st, part_k,
+      const int sink_blocks = (apart.sinks * (D / 8) + 15) / 16, blocks = sink_blocks + ((reduced - apart.sinks) * (D / 8) + 255) / 256;
+      hipLaunchKernelGGL((attn_window_reduce_kernel<D>), dim3((unsigned)(b * nkv * blocks)), dim3(256), 0, st, part_k,
                          part_v, sink_sums, dk, dv, reduced, partial ? sp : sink_rows, nq / hpw / nkv, nkv, per, sink_chunks,
-                         (int)sink_blocks, b * nkv, dkl, dvl, apart);
+                         sink_blocks, blocks, dkl, dvl, apart);
     }
   } else if (partial) {
     if (hipGetLastError() != hipSuccess) return KR_ELAUNCH;
