@@ -157,6 +157,14 @@ __device__ __forceinline__ void column_sums(const bf16* dy, const bf16* x, const
   }
 }
 
+// Where a row's loads are asked for while the row before is worked on: eight waves to a row, which have no other workgroup beside them, and
+// a wave to a row (without -> with a residual, us, at once -> ahead: 12000 x 8200 140 -> 111, 166 -> 146, 8192 x 12288 124 -> 108, 154 -> 141,
+// 65536 x 512 49.5 -> 42, 55 -> 49, 50000 x 768 50 -> 44, 56 -> 58, 32768 x 1024 39.6 -> 39.8, 49.4 -> 48.7; two waves: 32768 x 4096 136 -> 142,
+// 180 -> 175, 2560 89 -> 89, 115 -> 122, four: 11577 x 6552 97 -> 99, 117 -> 130; four vectors to a lane leave no registers, 7395 x 15696
+// 145 -> 174, 182 -> 285).
+template <int LPR, int NCH>
+constexpr bool kAhead = (LPR == 64 && NCH <= 2) || (LPR == 512 && NCH <= 3);
+
 // ADD: the gradient of the residual branch forked off in front of the norm is added before the one rounding.
 // FEW: the workgroups from `row_blocks` on have the columns, and no partial rows are left.
 template <int LPR, int NCH, bool ADD, bool FEW>
@@ -187,24 +195,43 @@ __global__ __launch_bounds__(kBlock<LPR>) void layernorm_bwd_kernel(
 #pragma unroll
     for (int e = 0; e < 8; ++e) dg[c][e] = db[c][e] = 0.f;
   }
-  int use = 0;
-  for (int64_t base = (int64_t)blockIdx.x * kRows; base < rows; base += (int64_t)(FEW ? row_blocks : gridDim.x) * kRows) {
-    const int64_t row = base + slot;
+  constexpr bool AHEAD = kAhead<LPR, NCH>;
+  bf16x8 xn[NCH], dn[NCH], rn[ADD ? NCH : 1];
+  float mu_n = 0.f, rs_n = 0.f;
+  auto load = [&](int64_t row) {
     const bool active = row < rows;
     const int64_t r = active ? row : 0;
     const bf16* xr = x + kr_row_at(r, x_ld, x_runs);
     const bf16* dr = dy + r * dy_ld;
     const bf16* rr = ADD ? dres + kr_row_at(r, dres_ld, dres_runs) : nullptr;
-    bf16x8 xv[NCH], dv[NCH], rv[ADD ? NCH : 1];
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
       const int v = at + c * LPR;
       const bool in = active && v < nvec;
-      xv[c] = in ? ldg8_stream(xr + v * 8) : zero8();
-      dv[c] = in ? ldg8_stream(dr + v * 8) : zero8();
-      if (ADD) rv[c] = in ? ldg8_stream(rr + v * 8) : zero8();
+      xn[c] = in ? ldg8_stream(xr + v * 8) : zero8();
+      dn[c] = in ? ldg8_stream(dr + v * 8) : zero8();
+      if (ADD) rn[c] = in ? ldg8_stream(rr + v * 8) : zero8();
     }
-    const float mu = active ? mean[r] : 0.f, rs = active ? rstd[r] : 0.f;
+    mu_n = active ? mean[r] : 0.f;
+    rs_n = active ? rstd[r] : 0.f;
+  };
+  int use = 0;
+  const int64_t step = (int64_t)(FEW ? row_blocks : gridDim.x) * kRows;
+  if (AHEAD) load((int64_t)blockIdx.x * kRows + slot);
+  for (int64_t base = (int64_t)blockIdx.x * kRows; base < rows; base += step) {
+    const int64_t row = base + slot;
+    const bool active = row < rows;
+    const int64_t r = active ? row : 0;
+    if (!AHEAD) load(row);
+    bf16x8 xv[NCH], dv[NCH], rv[ADD ? NCH : 1];
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) {
+      xv[c] = xn[c];
+      dv[c] = dn[c];
+      if (ADD) rv[c] = rn[c];
+    }
+    const float mu = mu_n, rs = rs_n;
+    if (AHEAD && base + step < rows) load(row + step);
     float sum[2] = {0.f, 0.f};  // of g and of g xh
 #pragma unroll
     for (int c = 0; c < NCH; ++c)
@@ -318,12 +345,16 @@ int lanes_per_row(int cols, int most) {
 // (8 -> 4 in the forward, us: 6023 x 3584 17.9 -> 15.3, 8192 x 8192 50.7 -> 48.4, 4096 x 16384 50.9 -> 49.5; 2: 16.8, 48.2, and 32768 x
 // 4096, a wave a row or two, 95.5, 96.6, 108; backward 4 -> 2: 32768 x 4096 181 -> 183, without a residual 137 -> 144)
 constexpr int kFwdVectors = 4, kBwdVectors = 4;
+// In the backward rows of more than 5632 columns take eight waves, with loads ahead (four waves of 4 vectors -> those, without and with a
+// residual, us: 11577 x 6552 94 -> 93, 117 -> 110, 12000 x 8192 109 -> 105, 140 -> 131, 16384 x 6144 109 -> 103, 144 -> 137, 5120 92 -> 92, 119
+// -> 121), unless they are few and their columns are read in the same launch.
+int bwd_lanes(int rows, int cols) { return cols > 5632 && rows > kFewRows ? 512 : lanes_per_row(cols, kBwdVectors); }
 
 // Workgroups of the backward, each of which leaves 8 cols bytes that are read again: two a unit, what the registers of wide rows
 // allow, one where it has eight waves (4096 x 16384 in 512 and 256, us: 121, 109; 32768 x 4096 181, 220), four where rows share a
 // wave (100000 x 256 in 512 and 1024: 43.6, 40.4, without a residual 40.0, 32.6; 32768 x 1024 50.7, 53.5).
 int bwd_blocks(int rows, int cols) {
-  const int lpr = lanes_per_row(cols, kBwdVectors), per = lpr > 256 ? 1 : 256 / lpr;
+  const int lpr = bwd_lanes(rows, cols), per = lpr > 256 ? 1 : 256 / lpr;
   const int most = lpr > 256 ? 256 : lpr < 64 ? 1024 : 512, blocks = (rows + per - 1) / per;
   return blocks < most ? blocks : most;
 }
@@ -451,7 +482,7 @@ extern "C" int kr_layernorm_bwd(const void* dy, const void* x, const float* mean
   if (dres)
     if (const int rc = kr_make_runs(dres_run_rows, dres_run_ld, rows, &a.dres_runs)) return rc;
   if (const int rc = kr_make_runs(dx_run_rows, dx_run_ld, rows, &a.dx_runs)) return rc;
-  const int lpr = lanes_per_row(cols, kBwdVectors), nch = (cols / 8 + lpr - 1) / lpr, blocks = bwd_blocks(rows, cols);
+  const int lpr = bwd_lanes(rows, cols), nch = (cols / 8 + lpr - 1) / lpr, blocks = bwd_blocks(rows, cols);
   const hipStream_t s = (hipStream_t)stream;
   const bool few = dgamma && rows <= kFewRows && lpr <= 256;  // (workgroups of 256)
   if (few) a.dgamma = (bf16*)dgamma, a.dbeta = (bf16*)dbeta;

@@ -81,7 +81,8 @@ def test_widths(rows, cols):
 
 
 @on_gpu
-@pytest.mark.parametrize("rows,cols", [(6023, 3584), (4099, 200), (33000, 64), (2100, 4096), (1030, 16384)])
+@pytest.mark.parametrize("rows,cols", [(6023, 3584), (4099, 200), (33000, 64), (2100, 4096), (1030, 16384), (1030, 8192), (1100, 5640),
+                                       (1281, 6152), (1537, 12288), (5000, 520), (2051, 1024)])
 def test_more_rows_than_workgroups(rows, cols):
     x, dy, res, w, b = make(rows, cols)
     first = check(x, dy, w, b, res=res)
