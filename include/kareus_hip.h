@@ -229,9 +229,12 @@ int kr_rmsnorm_bwd_add_noalloc(const void* dy, const void* x, const float* rstd,
  *   dgamma = sum of dy xh, dbeta = sum of dy over the rows, in fp32 and in a fixed order, rounded once.
  * cols: a multiple of 8, at most 16384; strides multiples of 8.  dx may be a slice of a larger tensor, and dres itself; otherwise
  * it overlaps no input (KR_EINVAL where it begins where x or dy does).
- * workspace: kr_layernorm_bwd_workspace_bytes() bytes, 16-byte aligned.  With dgamma and dbeta NULL the call leaves there its
+ * workspace: kr_layernorm_bwd_workspace_bytes() bytes, 16-byte aligned; NULL where dgamma and dbeta are asked for of up to
+ * KR_LAYERNORM_FEW_ROWS rows of up to KR_LAYERNORM_FEW_COLS columns.  With dgamma and dbeta NULL the call leaves there its
  * kr_layernorm_bwd_partial_rows() fp32 rows of [2][cols] sums, and kr_layernorm_dparams adds those of several calls (the nanobatches
  * of a microbatch, workspaces back to back).  The queries return 0 for widths that are not supported.      */
+#define KR_LAYERNORM_FEW_ROWS 1024
+#define KR_LAYERNORM_FEW_COLS 8192
 int kr_layernorm_fwd(const void* x, const void* gamma, const void* beta, void* y, float* mean, float* rstd, int rows, int cols,
                      int64_t x_ld, int x_run_rows, int64_t x_run_ld, float eps, void* stream);
 size_t kr_layernorm_bwd_workspace_bytes(int rows, int cols);

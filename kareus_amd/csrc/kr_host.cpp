@@ -1435,10 +1435,10 @@ PyObject* py_layernorm_bwd(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
       if (!ws.defined()) {
         dgamma = at::empty({ox.cols}, x.options());
         dbeta = at::empty({ox.cols}, x.options());
-        ws = bytes(kr_layernorm_bwd_workspace_bytes(rows, cols), x);
+        if (rows > KR_LAYERNORM_FEW_ROWS || cols > KR_LAYERNORM_FEW_COLS) ws = bytes(kr_layernorm_bwd_workspace_bytes(rows, cols), x);
       }
       rc = kr_layernorm_bwd(ptr(dy), ptr(x), (const float*)ptr(mean), (const float*)ptr(rstd), ptr(gamma), ptr_or_null(a[5]), ptr(dx),
-                            dgamma.defined() ? ptr(dgamma) : nullptr, dbeta.defined() ? ptr(dbeta) : nullptr, ptr(ws), rows, cols,
+                            dgamma.defined() ? ptr(dgamma) : nullptr, dbeta.defined() ? ptr(dbeta) : nullptr, ws.defined() ? ptr(ws) : nullptr, rows, cols,
                             od.ld, ox.ld, ox.run_rows, ox.run_ld, orr.ld, orr.run_rows, orr.run_ld, oc.ld, oc.run_rows, oc.run_ld,
                             stream());
     }

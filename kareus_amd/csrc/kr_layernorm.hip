@@ -15,7 +15,7 @@ namespace {
 constexpr int kMaxCols = 16384;
 // Up to this many rows one launch does both (two launches -> one, us from Python: 257 x 512 13.9 -> 8.8, 1024 x 512 11.1 -> 8.6, 512 x 8192
 // 25.3 -> 12.1, 1024 x 4096 20.5 -> 14.9; 2048 x 4096 26.0 -> 26.8, 4096 x 512 11.1 -> 32.9).
-constexpr int kFewRows = 1024;
+constexpr int kFewRows = KR_LAYERNORM_FEW_ROWS;
 
 template <int LPR>
 constexpr int kBlock = LPR > 256 ? LPR : 256;
@@ -465,7 +465,8 @@ extern "C" int kr_layernorm_bwd(const void* dy, const void* x, const float* mean
                                 int64_t dy_ld, int64_t x_ld, int x_run_rows, int64_t x_run_ld, int64_t dres_ld,
                                 int dres_run_rows, int64_t dres_run_ld, int64_t dx_ld, int dx_run_rows, int64_t dx_run_ld,
                                 void* stream) {
-  if (!dy || !x || !mean || !rstd || !gamma || !dx || !workspace || rows <= 0 || cols <= 0 || dy_ld < cols || x_ld < cols ||
+  const bool few = dgamma && rows <= kFewRows && cols <= KR_LAYERNORM_FEW_COLS;  // (workgroups of 256)
+  if (!dy || !x || !mean || !rstd || !gamma || !dx || (!workspace && !few) || rows <= 0 || cols <= 0 || dy_ld < cols || x_ld < cols ||
       dx_ld < cols || (dres && dres_ld < cols) || !dgamma != !dbeta)
     return KR_EINVAL;
   if (cols % 8 || dy_ld % 8 || x_ld % 8 || dx_ld % 8 || (dres && dres_ld % 8) || cols > kMaxCols) return KR_EUNSUPPORTED;
@@ -484,7 +485,6 @@ extern "C" int kr_layernorm_bwd(const void* dy, const void* x, const float* mean
   if (const int rc = kr_make_runs(dx_run_rows, dx_run_ld, rows, &a.dx_runs)) return rc;
   const int lpr = bwd_lanes(rows, cols), nch = (cols / 8 + lpr - 1) / lpr, blocks = bwd_blocks(rows, cols);
   const hipStream_t s = (hipStream_t)stream;
-  const bool few = dgamma && rows <= kFewRows && lpr <= 256;  // (workgroups of 256)
   if (few) a.dgamma = (bf16*)dgamma, a.dbeta = (bf16*)dbeta;
   int rc;
   switch (lpr) {

@@ -261,7 +261,7 @@ def test_refusals_of_the_library():
     assert fwd(16, 16, 16, 16, 16, 16, 4, 64, 64, 8, 512, 1e-5) == -2           # ... that divide the rows
     bwd = lambda dg, db, ws, rows=4, ld=64: lib.kr_layernorm_bwd(  # noqa: E731
         16, 16, 16, 16, 16, None, 16, dg, db, ws, rows, 64, ld, 64, 1, 0, 0, 1, 0, 64, 1, 0, None)
-    assert bwd(16, None, 16) == -1 and bwd(16, 16, None) == -1 and bwd(16, 16, 24) == -1 and bwd(16, 16, 16, rows=0) == -1
+    assert bwd(16, None, 16) == -1 and bwd(16, 16, None, rows=1025) == -1 and bwd(None, None, None) == -1 and bwd(16, 16, 24) == -1 and bwd(16, 16, 16, rows=0) == -1
     assert bwd(16, 16, 16, ld=68) == -2
     assert bwd(16, 16, 16) == -1                                                # dx where x and dy are
     assert lib.kr_layernorm_dparams(16, 0, 64, 16, 16, None) == -1 and lib.kr_layernorm_dparams(16, 1, 64, 16, None, None) == -1
