@@ -134,6 +134,19 @@ def test_back_and_forth_is_the_input():
 
 
 @on_gpu
+def test_more_than_2_to_31_elements():
+    be = get_backend("hip")
+    s, b, heads, hd = 420000, 1, 40, 128
+    t = torch.randn(1000, b, heads, hd, device="cuda").bfloat16().repeat(s // 1000, 1, 1, 1)
+    at = rotary_axes(torch.arange(s, device="cuda").expand(3, b, s), hd, (24, 20, 20))
+    turned = be.rope_axes_fwd(t, at)
+    part = be.rope_axes_fwd(t[-1000:].contiguous(), at._replace(positions=at.positions[:, :, -1000:]))
+    assert t.numel() > 1 << 31 and torch.equal(turned[-1000:], part)
+    del t, turned
+    torch.cuda.empty_cache()
+
+
+@on_gpu
 def test_captured():
     be = get_backend("hip")
     t, at = make(389, 1, 10, 128, 3)
