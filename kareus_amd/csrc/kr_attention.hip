@@ -2141,15 +2141,17 @@ __global__ __launch_bounds__(256) void attn_group_reduce_kernel(
   stg8(dv + dvl.at(bi, kvh) + (int64_t)si * dvl.s_ + c * 8, ov);
 }
 
+// Windows up to this many keys, and every row's first 128 queries, form delta from the scores (2-norm errors of dQ, of which 0.0017 are its
+// own rounding, delta from O -> from the scores: 2 tokens, window 1, a sink 0.038 -> 0.0027, 24, 19 0.0042 -> 0.0026, 351, 1 0.0037 -> 0.0024,
+// 257, 64 0.0025 -> 0.0024, 924, 125 no difference; backward of 257 tokens of 8 heads of 64, window 64, 22.0 -> 24.2 us, 3 x 2007 of 8/2 of
+// 128, 500 no difference; with a limit of 256, 2 x 8192 of 16/4 heads of 64, window 128 would take 145 us for 124).
+constexpr int kDeltaFromScores = 64;
+
 // HALVES = 2: as in the forward kernel, two halves of an 8-wave workgroup own the same 128
 // queries and walk the even / odd key tiles; half 1's dQ partial is added to half 0's through
 // LDS at the end.  Chosen by the host when there are few workgroups.
 // When there are more 256-query tiles than compute units (or other streams run beside the launch; see attn_forms)
 // the host takes attn_bwd_dq_w64_kernel below instead.
-// Windows up to this many keys, and every row's first 128 queries, form delta from the scores (2-norm errors of dQ, of which 0.0017 are its
-// own rounding, delta from O -> from the scores: 2 tokens, window 1, a sink 0.038 -> 0.0027, 24, 19 0.0042 -> 0.0026, 351, 1 0.0037 -> 0.0024,
-// 257, 64 0.0025 -> 0.0024; backward of 257 tokens of 8 heads of 64, window 64, 22.0 -> 24.2 us, 3 x 2007 of 8/2 of 128, 500 no difference).
-constexpr int kDeltaFromScores = 64;
 template <int D, bool RAGGED, int HALVES, bool WIN>
 __global__ __launch_bounds__(256 * HALVES, HALVES == 1 ? 2 : 1) void attn_bwd_dq_kernel(
     const bf16* __restrict__ q, const bf16* __restrict__ k, const bf16* __restrict__ v,
