@@ -477,3 +477,24 @@ def test_the_window_kernels_keep_their_reads_in_front_of_barriers(tmp_path):
         assert n_asm == 192 and not bad, (name, n_asm, bad[:5])
     spills = [int(n) for n in re.findall(r"\.vgpr_spill_count:\s*(\d+)", text)]
     assert spills and not any(spills)
+
+
+def long_window(s, b, nq, hd, window, sinks):
+    be = get_backend("hip")
+    q, k, v, do = (t.contiguous() for t in make(s, b, nq, 1, hd))
+    o, lse = be.attn_fwd(q, k, v, hd ** -0.5, window=window, sinks=sinks)
+    return (q, k, v, do), o, lse, *be.attn_bwd(do, q, k, v, o, lse, hd ** -0.5, window=window, sinks=sinks)
+
+
+@on_gpu
+@pytest.mark.parametrize("s,b,nq,hd,window,sinks", [(2300, 8, 4, 64, 2048, 5), (2177, 8, 4, 64, 2050, 0), (4340, 4, 4, 128, 4096, 70),
+                                                    (4737, 7, 2, 128, 4111, 130)])
+def test_long_windows_of_ragged_rows(s, b, nq, hd, window, sinks):
+    """dQ over 256-query tiles, the last of which rows leave: its second half with one token and with nearly all of them."""
+    (q, k, v, do), o, lse, dq, dk, dv = long_window(s, b, nq, hd, window, sinks)
+    for bi in (0, b - 1):
+        part = slice(bi, bi + 1)
+        want, tol = reference(q[:, part], k[:, part], v[:, part], do[:, part].contiguous(), hd ** -0.5, window, sinks)
+        for name, t in (("lse", lse[part]), ("o", o[:, part]), ("dv", dv[:, part]), ("dk", dk[:, part]), ("dq", dq[:, part])):
+            close(name, t, want[name], tol[name])
+    torch.cuda.empty_cache()
