@@ -446,8 +446,8 @@ int kr_attn_bwd_flags(const void* dout, const void* q, const void* k, const void
  * kr_attn_bwd_flags' (KR_ATTN_BESIDE_OTHER_STREAMS at most); hd 64 or 128, sequence strides below 2^31 / 127 elements unless hd = 128
  * and s is a multiple of 128 (KR_EUNSUPPORTED otherwise); scale positive.  Only key tiles with a visible key are read: work and
  * time go with s * (window + sinks).  Where window + sinks reach s nothing is hidden, and from s = 513 on the calls are those above.
- * Rows with few keys form their dO . O from the scores (a row whose probabilities are nearly all one key's has gradients of which
- * nothing is left behind O's rounding).  Keys and values have to be finite, hidden ones too: a tile's hidden probabilities are zeros that its values are multiplied by.
+ * The first 128 queries of a sequence, and all where window <= 64, form their dO . O from the scores (a row whose probabilities are
+ * nearly all one key's has gradients of which nothing is left behind O's rounding); the others, and all of the calls above, from O.  Keys and values have to be finite, hidden ones too: a tile's hidden probabilities are zeros that its values are multiplied by.
  * workspace: kr_attn_window_bwd_workspace_bytes() bytes, 16-byte aligned.                         */
 int kr_attn_window_fwd(const void* q, const void* k, const void* v, void* o, float* lse,
                        int s, int b, int nq, int nkv, int hd, float scale,

@@ -2143,8 +2143,11 @@ __global__ __launch_bounds__(256) void attn_group_reduce_kernel(
 
 // Windows up to this many keys, and every row's first 128 queries, form delta from the scores (2-norm errors of dQ, of which 0.0017 are its
 // own rounding, delta from O -> from the scores: 2 tokens, window 1, a sink 0.038 -> 0.0027, 24, 19 0.0042 -> 0.0026, 351, 1 0.0037 -> 0.0024,
-// 257, 64 0.0025 -> 0.0024, 924, 125 no difference; backward of 257 tokens of 8 heads of 64, window 64, 22.0 -> 24.2 us, 3 x 2007 of 8/2 of
-// 128, 500 no difference; with a limit of 256, 2 x 8192 of 16/4 heads of 64, window 128 would take 145 us for 124).
+// 257, 64 0.0025 -> 0.0024, 924, 125 no difference; tokens 1, 1 to 15 and 16 to 127 of 2304, window 2048 0.0037 -> 0.0023, 0.0029 -> 0.0024,
+// 0.0024; backward of 257 tokens of 8 heads of 64, window 64, 22.0 -> 24.2 us, 3 x 2007 of 8/2 of 128, 500 no difference; with a limit of 256,
+// 2 x 8192 of 16/4 heads of 64, window 128 would take 145 us for 124; of one wave per SIMD, 8 x 2304 of 4/1 heads of 64, 2048 148 -> 151,
+// 16384 of 8/2 heads of 128, 4096 no difference).
+// A window that hides nothing of more than kShortRows tokens is plain attention, whose kernels form it from O for every row.
 constexpr int kDeltaFromScores = 64;
 
 // HALVES = 2: as in the forward kernel, two halves of an 8-wave workgroup own the same 128
@@ -2551,9 +2554,48 @@ __device__ __forceinline__ void dq_step(DqScores& nxt, const DqScores& cur, f32x
   }
 }
 
+// delta = sum P dP / sum P of 32 queries from row q0 on, whose keys up to their own are all visible, from the scores: operands come from
+// memory, a fragment of 32 keys at a time.  qp, dop: the lane's row.  (For the first 128 rows alone: four blocks of keys at most.)
+template <int D>
+__device__ __forceinline__ float delta_from_scores(const bf16* qp, const bf16* dop, const bf16* kb, int64_t k_ss, const bf16* vb,
+                                                   int64_t v_ss, int q0, float scale_log2, float neg_lse, int lane) {
+  constexpr int KK = D / 16;
+  const int h = lane >> 5;
+  bf16x8 qf[KK], dof[KK];
+#pragma unroll
+  for (int kk = 0; kk < KK; ++kk) {
+    qf[kk] = ldg8(qp + kk * 16 + h * 8);
+    dof[kk] = ldg8(dop + kk * 16 + h * 8);
+  }
+  float psum = 0.f, pdp = 0.f;
+  for (int key0 = 0; key0 <= q0; key0 += 32) {
+    const bf16* kp = kb + (int64_t)(key0 + (lane & 31)) * k_ss + h * 8;
+    const bf16* vp = vb + (int64_t)(key0 + (lane & 31)) * v_ss + h * 8;
+    f32x16 sacc, dpacc;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) sacc[e] = dpacc[e] = 0.f;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+      sacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ldg8(kp + kk * 16), qf[kk], sacc, 0, 0, 0);
+      dpacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ldg8(vp + kk * 16), dof[kk], dpacc, 0, 0, 0);
+    }
+    const int lim = q0 + (lane & 31) - key0 - 4 * h;  // element offsets beyond it are keys after the query
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float p = 8 * (e >> 2) + (e & 3) > lim ? 0.f : __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[e], scale_log2, neg_lse));
+      psum += p;
+      pdp = __builtin_fmaf(p, dpacc[e], pdp);
+    }
+  }
+  psum += __shfl_xor(psum, 32, KR_WAVE);
+  pdp += __shfl_xor(pdp, 32, KR_WAVE);
+  return pdp / psum;
+}
+
 // The kernel also takes over the pre-pass of the backward: each wave forms delta = sum_d dO . O of its 64
 // rows from the dO fragments it holds anyway, uses it, and writes it (and -lse in the log2 domain) for
-// the dK/dV kernel, which the host launches behind this one.
+// the dK/dV kernel, which the host launches behind this one.  (With a window the first 128 rows, which have few keys, form it from the
+// scores instead, as in attn_bwd_dq_kernel.)
 template <int D, bool RAGGED, bool WIN>
 __global__ __launch_bounds__(256, 1) void attn_bwd_dq_w64_kernel(
     const bf16* __restrict__ q, const bf16* __restrict__ k, const bf16* __restrict__ v,
@@ -2601,8 +2643,9 @@ __global__ __launch_bounds__(256, 1) void attn_bwd_dq_w64_kernel(
     // delta from a second read of the dO row: the fragments kept for the MFMAs must stay values that
     // only the MFMAs read, or the compiler keeps them in VGPRs and copies them into accumulation
     // registers in front of every MFMA
-    const bf16* dop2 = dop;
+    const bf16 *dop2 = dop, *qp2 = qp;
     asm volatile("" : "+v"(dop2));
+    if (WIN) asm volatile("" : "+v"(qp2));
     float dsum = 0.f;  // this lane's half of the row (channels 16 kk + 8 h ..)
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) {
@@ -2615,6 +2658,8 @@ __global__ __launch_bounds__(256, 1) void attn_bwd_dq_w64_kernel(
     dsum += __shfl_xor(dsum, 32, KR_WAVE);
     const int64_t stat = ((int64_t)bi * nq + head) * sp + qrow;
     neg_lse[qb] = -lse[((int64_t)bi * nq + head) * s + qld] * kLog2e;
+    if (WIN && qw0 < 128)  // (such windows and rows are longer than that)
+      dsum = delta_from_scores<D>(qp2, dop2, kb, kl.s_, vb, vl.s_, qw0 + 32 * qb, scale_log2, neg_lse[qb], lane);
     if (RAGGED && qrow >= s) {  // rows the dK/dV kernel must not see
       dsum = 0.f;
       neg_lse[qb] = -kPadLse * kLog2e;

@@ -498,3 +498,15 @@ def test_long_windows_of_ragged_rows(s, b, nq, hd, window, sinks):
         for name, t in (("lse", lse[part]), ("o", o[:, part]), ("dv", dv[:, part]), ("dk", dk[:, part]), ("dq", dq[:, part])):
             close(name, t, want[name], tol[name])
     torch.cuda.empty_cache()
+
+
+@on_gpu
+@pytest.mark.parametrize("s,b,nq,hd,window,sinks", [(2304, 8, 4, 64, 2048, 5), (2300, 8, 4, 64, 2048, 0), (4352, 4, 4, 128, 4096, 70), (4340, 4, 4, 128, 4096, 0)])
+def test_first_tokens_under_a_long_window(s, b, nq, hd, window, sinks):
+    """The first 128 queries form delta from the scores in every form of dQ.  (They see one another alone; the reference's 256 tokens
+    leave room in sum P |dP| for delta's own way through the matrix unit's sums, hd u |delta|, beside the 66 additions of a lane.)"""
+    (q, k, v, do), _, _, dq, _, _ = long_window(s, b, nq, hd, window, sinks)
+    for bi in (0, b - 1):
+        part = [t[:256, bi:bi + 1].contiguous() for t in (q, k, v, do)]
+        want, tol = reference(*part, hd ** -0.5, 256, 0, from_scores=True)
+        close("dq", dq[:128, bi:bi + 1], want["dq"][:128], tol["dq"][:128])
