@@ -378,8 +378,9 @@ int kr_attn_fwd(const void* q, const void* k, const void* v, void* o, float* lse
  * streams run beside this launch and use the compute units it leaves idle (the engine's nanobatch
  * streams), so the launch is shaped for the least compute-unit time rather than for its own latency:
  * whole rows / whole key tiles per workgroup whatever their number, no second pass and no merge.
- * The two shapes sum in different orders: results agree to rounding, and for a given flags word they
- * do not depend on the batch size.  No counterpart in the reference's call
+ * The two shapes sum in different orders: results agree to rounding.  With the flag a sequence's o, lse and
+ * dQ have the same bits in a batch of any size (without a window: where s is a multiple of 256).  No counterpart
+ * in the reference's call
  * (kareus/flash_attn/flash_attn_interface.py:66-80 runs one kernel at a time).                   */
 #define KR_ATTN_BESIDE_OTHER_STREAMS 0x100
 #define KR_ATTN_GENERAL_KERNELS 0x200
@@ -447,7 +448,8 @@ int kr_attn_bwd_flags(const void* dout, const void* q, const void* k, const void
  * and s is a multiple of 128 (KR_EUNSUPPORTED otherwise); scale positive.  Only key tiles with a visible key are read: work and
  * time go with s * (window + sinks).  Where window + sinks reach s nothing is hidden, and from s = 513 on the calls are those above.
  * The first 128 queries of a sequence, and all where window <= 64, form their dO . O from the scores (a row whose probabilities are
- * nearly all one key's has gradients of which nothing is left behind O's rounding); the others, and all of the calls above, from O.  Keys and values have to be finite, hidden ones too: a tile's hidden probabilities are zeros that its values are multiplied by.
+ * nearly all one key's has gradients of which nothing is left behind O's rounding); the others, and all of the calls above, from O.
+ * Keys and values have to be finite, hidden ones too: a tile's hidden probabilities are zeros that its values are multiplied by.
  * workspace: kr_attn_window_bwd_workspace_bytes() bytes, 16-byte aligned.                         */
 int kr_attn_window_fwd(const void* q, const void* k, const void* v, void* o, float* lse,
                        int s, int b, int nq, int nkv, int hd, float scale,

@@ -3289,9 +3289,9 @@ int band_sink_chunks(int sp, int b, int nq, Band band) {
 // Whether a window's dQ takes 256-query tiles, one wave per SIMD: long windows, which pay for its start, and a workgroup for every unit
 // (two waves per SIMD -> one, us of the whole backward: 16384 tokens of 8/2 heads of 128, 4 sinks, window 8192 1675 -> 1614, 4 x 8192,
 // 4096 1511 -> 1477, 2048 875 -> 878, 1024 523 -> 551; 16384 of 16/4 heads of 64, 4096 936 -> 864, 2048 524 -> 506, 2 x 8192, 1024 307 -> 320;
-// 4096 of 8/2 heads, 128 workgroups, 2048 127 -> 151).
-bool band_shared_dq(int sp, int b, int nq, int hd, Band band) {
-  return sp % 256 == 0 && band.window >= (hd == 64 ? 2048 : 4096) && (int64_t)(sp / 256) * nq * b >= kr_compute_units();
+// 4096 of 8/2 heads, 128 workgroups, 2048 127 -> 151).  Beside other streams their kernels have the units that it leaves.
+bool band_shared_dq(int sp, int b, int nq, int hd, Band band, bool beside) {
+  return sp % 256 == 0 && band.window >= (hd == 64 ? 2048 : 4096) && (beside || (int64_t)(sp / 256) * nq * b >= kr_compute_units());
 }
 // The sinks whose keys the dK/dV kernel leaves, behind their window, to a kernel of their own: all, or, where a walk over the few queries
 // behind the window costs less than that launch and the one that adds its sums, none (apart -> by the dK/dV kernel, us of the whole
@@ -3338,7 +3338,8 @@ int attn_bwd_mfma(const BwdCall& c) {
   float* neg_lse2 = neg_delta + rows;
   float* const sink_sums = neg_lse2 + rows;
   float* part_k = sink_sums + (WIN ? band_sink_floats(sp, b, nq, D, apart) : 0);
-  const AttnForms forms = WIN ? AttnForms{false, band_shared_dq(sp, b, nq, D, c.band), 1} : attn_forms(sp, b, nq, c.nkv, D, c.flags);
+  const bool beside = (c.flags & KR_ATTN_BESIDE_OTHER_STREAMS) != 0;
+  const AttnForms forms = WIN ? AttnForms{false, band_shared_dq(sp, b, nq, D, c.band, beside), 1} : attn_forms(sp, b, nq, c.nkv, D, c.flags);
   const int qsplit = forms.qsplit;
   // (with a window and no partial results of a group's heads, the sinks' key tiles leave theirs alone)
   const int sink_rows = (apart.sinks + 127) / 128 * 128;
@@ -3399,8 +3400,11 @@ int attn_bwd_mfma(const BwdCall& c) {
   const auto launch_dq = [&] {
     // few workgroups: the longest causal rows set the time; a window's are of one length, and two workgroups of four waves to a unit start
     // and end beside each other (one of eight waves -> those, us of the whole backward: 384 workgroups, 3 x 2007 tokens, window 500 140 ->
-    // 133; 1024, 2 x 8192 of heads of 64, 128 168 -> 134, 16384 of 128, 4096 969 -> 946; 256, 4096, 512 63 -> 65)
-    if (dq_blocks <= (WIN ? kr_compute_units() : 4 * 256)) {
+    // 133; 1024, 2 x 8192 of heads of 64, 128 168 -> 134, 16384 of 128, 4096 969 -> 946; 256, 4096, 512 63 -> 65).  Beside other streams it
+    // is two of four, and one wave per SIMD under long windows, whatever their number: least time of a unit's, and the same bits in any batch
+    // (backward of one sequence of 8/2 heads on each of four streams, us: 2007 tokens, 128 channels, window 500, 5 sinks 118 -> 113, 4096, 64,
+    // 2048 217 -> 203; 512, 128, 100 78.1 -> 77.7; alone on the device 67.7 -> 70.4, 73.8 -> 91.8, 32.9 -> 32.2).
+    if (WIN ? !beside && dq_blocks <= kr_compute_units() : dq_blocks <= 4 * 256) {
       hipLaunchKernelGGL((attn_bwd_dq_kernel<D, RAGGED, 2, WIN>), dim3(dq_blocks), dim3(512), lds_dq2, st,
                          q, k, v, dout, lse,
                          neg_delta, dq, s, nq, nkv, scale, scale_log2, ql, kl, vl, dol,

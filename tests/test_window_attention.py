@@ -510,3 +510,20 @@ def test_first_tokens_under_a_long_window(s, b, nq, hd, window, sinks):
         part = [t[:256, bi:bi + 1].contiguous() for t in (q, k, v, do)]
         want, tol = reference(*part, hd ** -0.5, 256, 0, from_scores=True)
         close("dq", dq[:128, bi:bi + 1], want["dq"][:128], tol["dq"][:128])
+
+
+@on_gpu
+@pytest.mark.parametrize("s,nq,nkv,hd,window,sinks", [(384, 8, 2, 64, 100, 3), (512, 8, 2, 128, 100, 3), (700, 4, 4, 128, 65, 0), (512, 4, 2, 64, 600, 0),
+                                                      (2304, 4, 1, 64, 2048, 5), (4340, 2, 1, 128, 4096, 0)])
+def test_beside_other_streams(s, nq, nkv, hd, window, sinks):
+    """Whole rows to a workgroup whatever their number: the same bits for a sequence in a batch of any size."""
+    be = get_backend("hip")
+    big = 40 if s < 1024 else 10
+    q, k, v, do = make(s, 1, nq, nkv, hd)
+    band = dict(window=window, sinks=sinks, beside_other_streams=True)
+    o, lse = be.attn_fwd(q, k, v, hd ** -0.5, **band)
+    dq, dk, dv = be.attn_bwd(do, q, k, v, o, lse, hd ** -0.5, **band)
+    q, k, v, do = (t.repeat_interleave(big, dim=1) for t in (q, k, v, do))
+    o2, lse2 = be.attn_fwd(q, k, v, hd ** -0.5, **band)
+    assert torch.equal(o2[:, 7:8], o) and torch.equal(lse2[7:8], lse)
+    assert torch.equal(be.attn_bwd(do, q, k, v, o2, lse2, hd ** -0.5, **band)[0][:, 7:8], dq)
