@@ -292,8 +292,8 @@ int kr_rope(const void* t, void* out, const float* freqs,
  * positions[axis(f)][bi][si] * inv_freq[f], formed in 64 bits.  positions: [axes, b, s] int64 through strides; inv_freq: [hd / 2]
  * fp64; axes: 1 to KR_ROPE_MAX_AXES.  sections [axes] (host memory, read before the call returns): how many frequencies an axis
  * has, hd / 2 in all: one axis behind the other, or, interleaved != 0, in turn (f % axes) while that axis has any left, the first
- * axis behind that.  t, out, their strides and groups as kr_rope's; heads that are not rotated are copied unless out is t.
- * out is t or overlaps it nowhere.  hd: a multiple of 16, at most 256.                          */
+ * axis behind that (of 64 frequencies, sections 16, 24, 24 in turn come out as 22, 21, 21).  t, out, their strides and groups as
+ * kr_rope's; heads that are not rotated are copied unless out is t.  out is t or overlaps it nowhere.  hd: a multiple of 16, at most 256.                          */
 #define KR_ROPE_MAX_AXES 4
 int kr_rope_axes(const void* t, void* out, const int64_t* positions, int64_t p_stride_axis, int64_t p_stride_b,
                  int64_t p_stride_s, int axes, const double* inv_freq, const int* sections, int interleaved,

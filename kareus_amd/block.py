@@ -39,7 +39,7 @@ from .operators import (
     rotary_frequencies,
 )
 from .partitions.op_context import operator_parameters
-from .rotary_axes import RotaryAxes, check_sections, inverse_frequencies, rotary_axes
+from .rotary_axes import RotaryAxes, check_sections, check_sections_in_turn, inverse_frequencies, rotary_axes
 from .partitions.streams import stream_api
 from .partitions import (
     CommunicationType,
@@ -108,7 +108,8 @@ class LayerConfig:
     attention_window: int = 0
     attention_sinks: int = 0
     # positions on several axes (time, height, width: LayerStack.forward's position_ids): how many of the kv_channels / 2 frequencies
-    # each axis has, one axis behind the other or in turn
+    # each axis has, one axis behind the other or in turn (the first axis then has what is behind the others' last turn; sections that
+    # turns do not give are refused)
     rotary_sections: Optional[Tuple[int, ...]] = None
     rotary_interleaved: bool = False
     # Filled in by the driver / the training loop:
@@ -275,6 +276,8 @@ class DecoderLayer(torch.nn.Module):
                              "sinks stay visible beside a window")
         if c.rotary_sections is not None:
             check_sections(c.rotary_sections, c.kv_channels)
+            if c.rotary_interleaved:
+                check_sections_in_turn(c.rotary_sections)
         norm = PartitionableLayerNorm if c.normalization == "LayerNorm" else PartitionableRMSNorm
         lin = dict(config=c, init_method=init, bias=False, device=device, dtype=dt, backend=be)
         self.attn_residual_fork = ResidualForkOp(backend=be)

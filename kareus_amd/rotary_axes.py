@@ -18,7 +18,8 @@ MAX_AXES = 4
 class RotaryAxes(NamedTuple):
     """``positions`` ``[axes, b, s]`` int64; ``inv_freq`` ``[hd / 2]`` float64, in radians per position; ``sections``: how many of the
     frequencies each axis has, ``hd / 2`` in all.  They lie one axis behind the other, or ``interleaved``: in turn while an axis has any
-    left, and the first axis has what is behind that.  Angles are formed in 64 bits."""
+    left, and the first axis has what is behind that, also where an axis gets fewer than its section for want of turns (layers refuse
+    such sections).  Angles are formed in 64 bits."""
 
     positions: Tensor
     inv_freq: Tensor
@@ -50,6 +51,13 @@ class RotaryAxes(NamedTuple):
 def check_sections(sections: Sequence[int], hd: int) -> None:
     if not 1 <= len(sections) <= MAX_AXES or min(sections) < 0 or sum(sections) != hd // 2:
         raise RuntimeError(f"sections {tuple(sections)} are not the {hd // 2} frequencies of {hd} channels on 1 to {MAX_AXES} axes")
+
+
+def check_sections_in_turn(sections: Sequence[int]) -> None:
+    """Raises unless frequencies dealt in turn give every axis as many as its section says: of 64, (4, 28, 32) would become 22, 21 and 21."""
+    dealt = torch.bincount(axis_of_frequency(sections, True), minlength=len(sections)).tolist()
+    if dealt != list(sections):
+        raise RuntimeError(f"sections {tuple(sections)} cannot be had in turn: the axes would get {tuple(dealt)} frequencies")
 
 
 def axis_of_frequency(sections: Sequence[int], interleaved: bool, device=None) -> Tensor:

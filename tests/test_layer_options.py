@@ -303,3 +303,18 @@ def test_a_step_captured_and_replayed():
         want = step()
         torch.cuda.synchronize()
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and all(torch.equal(a, b) for a, b in zip(got[2], want[2]))
+
+
+@pytest.mark.parametrize("sections,had", [((12, 10, 10), True), ((11, 11, 10), True), ((16, 16), True), ((32,), True), ((17, 15), True), ((8, 12, 12), False),
+                                          ((2, 14, 16), False), ((15, 17), False), ((0, 16, 16), False)])
+def test_sections_in_turn_are_what_the_axes_get(sections, had):
+    """Dealt in turn an axis has at most every n-th frequency: a layer refuses sections that say more."""
+    counts = torch.bincount(axis_of_frequency(sections, True), minlength=len(sections)).tolist()
+    assert (counts == list(sections)) == had
+    LayerStack(config("eager", torch.float32, layers=1, rotary_sections=sections))
+    c = config("eager", torch.float32, layers=1, rotary_sections=sections, rotary_interleaved=True)
+    if had:
+        LayerStack(c)
+    else:
+        with pytest.raises(RuntimeError, match="in turn"):
+            LayerStack(c)
