@@ -198,7 +198,7 @@ int check(int n, const void* const* grads, const int64_t* counts, const int* fp3
     const uintptr_t at = reinterpret_cast<uintptr_t>(grads[i]);
     if (!at || at % (fp32[i] ? 4 : 2)) return KR_EINVAL;
     if (out && (!out[i] || reinterpret_cast<uintptr_t>(out[i]) % 4)) return KR_EINVAL;
-    if (counts[i] >= (int64_t)1 << 37) return KR_EUNSUPPORTED;  // (128 of them: below 2^32 chunks)
+    if (counts[i] > ((int64_t)1 << 37) - kChunk) return KR_EUNSUPPORTED;  // (kTensors of them: below 2^32 chunks)
   }
   return KR_OK;
 }

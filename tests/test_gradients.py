@@ -232,3 +232,15 @@ def test_one_parameter_and_gradients_with_a_history():
     assert float(clip_grad_norm(p, 0.5 * want, eps=0.0, backend="eager")) == pytest.approx(want, rel=1e-6)
     assert p.grad.detach().flatten().tolist() == [6.0] * 6
     p.grad = None
+
+
+def test_the_chunks_of_a_launch_are_counted_in_32_bits():
+    """128 tensors to a launch, chunks of 4096 elements: the largest that is taken, 128 times, stays below 2^32 of them."""
+    import ctypes
+
+    lib = hip.load_library()
+    # (without a place for the norm a count that is taken is refused for that, before anything is launched)
+    norm = lambda n: lib.kr_grad_norm(1, (ctypes.c_void_p * 1)(16), (ctypes.c_int64 * 1)(n), (ctypes.c_int * 1)(0), None, 16, 1 << 20, None)  # noqa: E731
+    most = (1 << 37) - 4096
+    assert 128 * -(-most // 4096) < 1 << 32 <= 128 * -(-(most + 1) // 4096)
+    assert norm(most) == -1 and norm(most + 1) == norm((1 << 37) - 1) == -2
