@@ -166,12 +166,13 @@ __device__ __forceinline__ void column_sums(const bf16* dy, const bf16* x, const
 template <int LPR, int NCH>
 constexpr bool kAhead = (LPR == 64 && NCH <= 2) || (LPR == 512 && NCH <= 3);
 
-// ADD: the gradient of the residual branch forked off in front of the norm is added before the one rounding.
+// ADD: the gradient of the residual branch forked off in front of the norm is added before the one rounding.  dx may be dres (neither is
+// __restrict__): a lane reads its piece before it writes there, and the row asked for ahead is another one.
 // FEW: the workgroups from `row_blocks` on have the columns, and no partial rows are left.
 template <int LPR, int NCH, bool ADD, bool FEW>
 __global__ __launch_bounds__(kBlock<LPR>) void layernorm_bwd_kernel(
     const bf16* __restrict__ dy, const bf16* __restrict__ x, const float* __restrict__ mean, const float* __restrict__ rstd,
-    const bf16* __restrict__ gamma, const bf16* __restrict__ dres, bf16* __restrict__ dx, float* __restrict__ partial, int rows,
+    const bf16* __restrict__ gamma, const bf16* dres, bf16* dx, float* __restrict__ partial, int rows,
     int cols, int64_t dy_ld, int64_t x_ld, int64_t dres_ld, int64_t dx_ld, KrRuns x_runs, KrRuns dres_runs, KrRuns dx_runs,
     int row_blocks, bf16* __restrict__ dgamma, bf16* __restrict__ dbeta) {
   if constexpr (FEW) {

@@ -294,3 +294,21 @@ def test_the_eager_backend(res):
     want, _ = reference(x, dy, w, b, 1e-5, r if res else None)
     for name, t in (("y", y), ("dx", dx), ("dw", dw), ("db", db)):
         assert torch.allclose(t.double(), want[name], rtol=1e-5, atol=1e-5)
+
+
+@on_gpu
+@pytest.mark.parametrize("rows,cols", [(3000, 64), (3000, 200), (2100, 512), (2500, 768), (1500, 1024), (1300, 2048), (1100, 4096), (1100, 5120),
+                                       (1100, 8192), (1100, 12288), (1100, 16384), (1024, 8192), (700, 512), (5, 16384)])
+def test_the_residual_gradient_s_own_place_in_every_form(rows, cols):
+    """Rows of few lanes to eight waves, with the next row's loads ahead and without, few rows and many, a row stride: the same bits in
+    the residual gradient's place as elsewhere."""
+    be = get_backend("hip")
+    x, dy, res, w, b = make(rows, cols)
+    _, mean, rstd = be.layernorm_fwd(x, w, b, 1e-5)
+    want = be.layernorm_bwd(dy, x, mean, rstd, w, residual_grad=res)
+    wide = torch.full((rows, cols + 24), 7.0, device="cuda").bfloat16()
+    wide[:, 8:8 + cols] = res
+    for place in (res, wide[:, 8:8 + cols]):
+        got = be.layernorm_bwd(dy, x, mean, rstd, w, residual_grad=place, out=place)
+        assert got[0].data_ptr() == place.data_ptr() and all(torch.equal(p, q) for p, q in zip(got, want))
+    assert bool((wide[:, :8] == 7.0).all()) and bool((wide[:, 8 + cols:] == 7.0).all())
