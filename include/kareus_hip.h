@@ -563,10 +563,11 @@ int kr_block_gemm_segments(int M, int N, int nseg, const int* K, const void* con
 
 /* ---- Gradient norm and clipping -----------------------------------------------------------------
  * n tensors, the i-th of counts[i] elements one behind the other at grads[i] (any alignment of its type; 0 elements: the pointer is
- * not looked at), bf16 or, fp32[i] != 0, fp32.  The arrays are in host memory and read before the call returns.
+ * not looked at; at most 2^37 - 4096), bf16 or, fp32[i] != 0, fp32.  The arrays are in host memory and read before the call returns.
  * kr_grad_norm: norm = sqrt(sum of all squares), 64-bit sums in a fixed order, one fp32 on the device.
  * kr_grad_clip: the norm, and every gradient times min(1, max_norm / (norm + eps)): in place (out NULL; rounded once; with a factor of
  * 1 nothing is written), or in fp32 at out[i].  A norm that is infinite or not a number gives the factor that the formula gives.
+ * Both are of these tensors alone: a norm over several devices is the caller's to add up, and to scale by.
  * A tensor that appears twice, or overlaps another or an output, is the caller's to leave out.
  * workspace: kr_grad_norm_workspace_bytes() bytes, 16-byte aligned.                                  */
 size_t kr_grad_norm_workspace_bytes(int n);

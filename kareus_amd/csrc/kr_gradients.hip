@@ -1,4 +1,4 @@
-// The global norm of a step's gradients and clipping by it: norm = sqrt(sum g^2) over all tensors, factor = min(1, max_norm /
+// The norm of all gradients that a process holds and clipping by it: norm = sqrt(sum g^2) over all tensors, factor = min(1, max_norm /
 // (norm + eps)), g factor in place or in fp32 elsewhere.  HBM-bound: the norm reads every gradient once, clipping once more, and
 // writes it.
 // Tensors come as a table in the launch's own arguments, kTensors to a launch: nothing has to be copied to the device first, and a

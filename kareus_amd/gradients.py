@@ -1,5 +1,9 @@
-"""The end of a training step: the global 2-norm of the gradients and clipping by it
-(3rdparty/Megatron-LM/megatron/core/optimizer/clip_grads.py: ``get_grad_norm_fp32``, ``clip_grad_by_total_norm_fp32``)."""
+"""The end of a training step: the 2-norm of the gradients that one process holds and clipping by it, the local part of
+3rdparty/Megatron-LM/megatron/core/optimizer/clip_grads.py (``get_grad_norm_fp32``, ``clip_grad_by_total_norm_fp32``).
+
+Nothing here is reduced over ranks.  Where a model's gradients are split over processes, ``clip_grad_norm`` on each would scale each by a
+factor of its own: take ``grad_norm`` of each part (those that every rank holds counted once), add the squares over the ranks, and scale
+by the factor of that sum."""
 
 from __future__ import annotations
 
@@ -27,7 +31,8 @@ def gradients_of(parameters: Union[Tensor, Iterable[torch.nn.Parameter]]) -> Lis
 
 
 def grad_norm(parameters: Union[Tensor, Iterable[torch.nn.Parameter]], backend: str = "hip") -> Tensor:
-    """The 2-norm of all gradients as one vector, fp32 on the gradients' device; nothing waits for it."""
+    """The 2-norm of all these gradients as one vector, fp32 on their device; nothing waits for it.  Of this process alone: the squares of
+    several shards' norms are the caller's to add."""
     from .backend import get_backend
 
     return get_backend(backend).grad_norm(gradients_of(parameters))
@@ -35,8 +40,8 @@ def grad_norm(parameters: Union[Tensor, Iterable[torch.nn.Parameter]], backend: 
 
 def clip_grad_norm(parameters: Union[Tensor, Iterable[torch.nn.Parameter]], max_norm: float, eps: float = 1e-6, backend: str = "hip",
                    out: Optional[Sequence[Tensor]] = None) -> Tensor:
-    """Scales all gradients by ``min(1, max_norm / (norm + eps))`` and returns their norm before that, fp32 on their device; nothing
-    waits for it.  ``out``: fp32 tensors, one for each gradient in order, that receive the scaled gradients (an optimizer's own), and
+    """Scales all these gradients by ``min(1, max_norm / (norm + eps))`` and returns their norm before that, fp32 on their device; nothing
+    waits for it.  The norm is that of these gradients: nothing is reduced over ranks.  ``out``: fp32 tensors, one for each gradient in order, that receive the scaled gradients (an optimizer's own), and
     the gradients stay as they are."""
     from .backend import get_backend
 

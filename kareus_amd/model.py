@@ -226,7 +226,8 @@ class LanguageModelEmbedding(torch.nn.Module):
 
 class GPTModelShard(torch.nn.Module):
     """``forward(input_ids [b, s], labels [b, s] or None, position_ids=None)`` -> loss ``[b, s]`` (fp32) or logits
-    ``[s, b, vocab_rows]``; ``position_ids`` as :class:`LayerStack`'s.  After ``backward()``, ``clip_grad_norm(max_norm)`` ends the step.
+    ``[s, b, vocab_rows]``; ``position_ids`` as :class:`LayerStack`'s.  After ``backward()``, ``clip_grad_norm(max_norm)`` ends the step of
+    a model that is one shard.
     ``embedding_scale``, ``embedding_sorted_gradient``, ``embedding_main_grad``: see :class:`LanguageModelEmbedding`."""
 
     def __init__(self, config: LayerConfig, vocab_rows: int, vocab_start: int = 0, device=None,
@@ -247,7 +248,8 @@ class GPTModelShard(torch.nn.Module):
         self.output_layer = torch.nn.Parameter(w.to(device=device, dtype=config.params_dtype))
 
     def clip_grad_norm(self, max_norm: float, eps: float = 1e-6, out=None) -> Tensor:
-        """:func:`kareus_amd.clip_grad_norm` of all parameters (the embedding's ``main_grad`` where it keeps one)."""
+        """:func:`kareus_amd.clip_grad_norm` of all parameters (the embedding's ``main_grad`` where it keeps one).  The norm is this shard's:
+        of a model in several shards each would be scaled by a factor of its own."""
         return clip_grad_norm(self.parameters(), max_norm, eps=eps, backend=self.config.backend, out=out)
 
     def forward(self, input_ids: Tensor, labels: Optional[Tensor] = None, position_ids: Optional[Tensor] = None) -> Tensor:
