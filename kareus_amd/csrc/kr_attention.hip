@@ -336,8 +336,6 @@ inline bool attn_strides_ok(const int64_t (&seq)[N], std::initializer_list<int64
 // =============================================================================================
 namespace {
 
-
-// query-like tensors: head h of KV group g = h / per sits at g*g_ + (h % per)*h_
 // The query tile behind the last one that sees any of the keys key0 .. key0 + 127 in its window, or, of sinks, at all (sp: queries, in whole
 // 128-row tiles).
 template <int TQ>
@@ -346,6 +344,8 @@ __device__ __forceinline__ int band_query_tiles(Band band, int key0, int sp) {
   const int64_t end = ((int64_t)key0 + 127 + band.window - 1) / TQ + 1;
   return end < sp / TQ ? (int)end : sp / TQ;
 }
+
+// query-like tensors: head h of KV group g = h / per sits at g*g_ + (h % per)*h_
 struct QLayout {
   int64_t s_, b_, g_, h_;
   __device__ __forceinline__ int64_t at(int bi, int head, int per) const {
