@@ -15,6 +15,10 @@
 //   contraction index of an MFMA can be permuted freely as long as both operands agree), and
 //   V^T fragments come out of LDS through the transposing read ds_read_b64_tr_b16.  Neither
 //   P nor V is ever transposed through memory.
+// Rounded to bf16 on the way is what the matrix instructions take: P in front of P.V and of dV, dS in front of dQ and dK.  Scores, row
+// statistics, delta and all sums stay in fp32.  2-norm errors against 64 bits are 0.0021 to 0.0025 with it, where P and dS in fp32 leave
+// the results' own rounding, 0.0016 to 0.0017.  (P and dS as a high and a low half each would keep those bits for more
+// matrix work: three products for two in the forward, eight for five in the backward.)
 // Tensors are addressed through (seq, batch, head) strides, so sequence-major [s, b, h, d]
 // views of the fused QKV projection are consumed in place.
 // This file is built twice: with KR_ATTN_WINDOW_TU for attention with a window and sinks (WIN instances of the kernels and the
@@ -109,7 +113,9 @@ __device__ __forceinline__ void longest_first(int pid, int nblocks, int ntiles, 
 // forms delta = sum dO . O on the way, then dK/dV by key tiles over the queries that have them in their window, and what queries further
 // on add to the sinks' keys apart (attn_bwd_sinks_kernel) unless they are few (band_apart); fp32 sums of a group's heads are added last.
 // 16384 tokens of 8/2 heads of 128, window 4096, 64 sinks, us: forward 262 (0.93 PFLOP/s of visible pairs), dQ 360, sinks 25, dK/dV 537
-// (0.66 together, counted as the five products that need be), sums 15; 2 x 8192 tokens of 16/4 heads of 64, window 1024: forward 110 (0.59, the exponentials).
+// (0.66 together, counted as the five products that need be), sums 15; 2 x 8192 tokens of 16/4 heads of 64, window 1024: forward 104 (0.62;
+// vector instructions take 0.44 of the cycles, the exponentials among them 0.13, matrix instructions 0.25, and waves wait 0.40 of their time),
+// backward 263 (0.61); 16384 of them, window 4096: 308 (0.78), 835 (0.72).
 struct Band {
   int window, sinks;
 };
@@ -2038,8 +2044,9 @@ __global__ __launch_bounds__(256, 1) void attn_bwd_sinks_kernel(
 }
 
 // dK and dV of the first `rows` keys: the fp32 sums of the dK/dV kernel over a group's `slots` workgroups, of part_rows rows each, one
-// thread per 8 channels.  Of the `blocks` workgroups of a (batch, KV head) pair the first `sink_blocks` have the sinks' keys, to which those of attn_bwd_sinks_kernel over the group's
-// heads and their stretches of queries are added, up to 16 of a head: 16 threads share them and add theirs in a fixed order.
+// thread per 8 channels.  Of the `blocks` workgroups of a (batch, KV head) pair the first `sink_blocks` have the sinks' keys, to which
+// those of attn_bwd_sinks_kernel over the group's heads and their stretches of queries are added, up to 16 of a head: 16 threads share
+// them and add theirs in a fixed order.
 template <int D>
 __global__ __launch_bounds__(256) void attn_window_reduce_kernel(
     const float* __restrict__ part_k, const float* __restrict__ part_v, const float* __restrict__ sums, bf16* __restrict__ dk,

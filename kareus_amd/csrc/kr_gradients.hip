@@ -11,7 +11,8 @@
 // elsewhere goes past them, in whole 1 KB pieces to a wave.  Norm and scaled copy of 218 M bf16 and 131 M fp32 elements (0.96 GB read twice, 1.4
 // GB written), us: 8 elements to a lane, 1024 workgroups of 8192 elements 237 + 479, 2048 209 + 482, from the last chunk on 209 + 472; 4
 // elements to a lane 209 + 443; its stores past the caches, which leave the next step's first pass clean ones, 164 + 464; 4096 workgroups of
-// 4096 elements 156 + 460: 5.4 TB/s.
+// 4096 elements 156 + 460: 5.4 TB/s.  In place, norm and scaling of 0.96 GB in bf16 and fp32 544 (5.3 TB/s of two reads and a write), of 0.35
+// GB 209; with a factor of 1 170 and 87, the norm's own time.
 #include "kr_common.h"
 
 namespace {

@@ -8,7 +8,8 @@
 // The weight's and the bias' gradients are column sums over all rows: a lane has the same columns of every row it comes by and sums
 // them in registers, a workgroup adds its rows' through LDS in a fixed order and leaves one fp32 row of both, [2][cols], and a
 // second launch adds the workgroups' rows.
-// 32768 x 4096: forward 95 us (5.6 TB/s), backward 137 (5.9), with a residual 180 (6.0).
+// 32768 x 4096: forward 95 us (5.6 TB/s), backward 137 (5.9), with a residual 180 (6.0); right behind the forward, of whose rows the caches
+// still hold some, 154 with its sums' launch.  (The times below are of operands that come from memory.)
 #include "kr_common.h"
 
 namespace {

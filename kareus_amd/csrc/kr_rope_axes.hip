@@ -5,7 +5,8 @@
 // A wave takes a token.  A lane has 8 frequencies and every 64 / (hd / 16)-th head, whose 16 bytes of either half it turns; the angles
 // themselves, some hundred instructions each, are formed one to a lane and handed over through LDS.  (Formed by every lane that turns by
 // them, 4 x 4096 tokens of 8/2 heads took 26.5 us for 18.5.  Vectors of whole rows to a wave, the halves exchanged between its lanes: 154.4
-// at best for 154.4, and 19.7 for 18.5.)
+// at best for 154.4, and 19.7 for 18.5.)  In place, as a layer turns its fused buffer, value heads are left alone: 4 x 8191 tokens of 32/8
+// heads of 128 take 121 us (5.5 TB/s), into a new buffer 154.
 // Angles are taken in 64 bits, as turns, and only what is left of the whole turns is rounded to 32: in 32 bits a position of a
 // million at frequency 1 would be off by a sixteenth of a radian.
 #include "kr_common.h"

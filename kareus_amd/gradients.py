@@ -41,8 +41,8 @@ def grad_norm(parameters: Union[Tensor, Iterable[torch.nn.Parameter]], backend: 
 def clip_grad_norm(parameters: Union[Tensor, Iterable[torch.nn.Parameter]], max_norm: float, eps: float = 1e-6, backend: str = "hip",
                    out: Optional[Sequence[Tensor]] = None) -> Tensor:
     """Scales all these gradients by ``min(1, max_norm / (norm + eps))`` and returns their norm before that, fp32 on their device; nothing
-    waits for it.  The norm is that of these gradients: nothing is reduced over ranks.  ``out``: fp32 tensors, one for each gradient in order, that receive the scaled gradients (an optimizer's own), and
-    the gradients stay as they are."""
+    waits for it.  The norm is that of these gradients: nothing is reduced over ranks.  ``out``: fp32 tensors, one for each gradient in
+    order, that receive the scaled gradients (an optimizer's own), and the gradients stay as they are."""
     from .backend import get_backend
 
     return get_backend(backend).clip_grad_norm(gradients_of(parameters), max_norm, eps=eps, out=out)

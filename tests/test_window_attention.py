@@ -501,7 +501,8 @@ def test_long_windows_of_ragged_rows(s, b, nq, hd, window, sinks):
 
 
 @on_gpu
-@pytest.mark.parametrize("s,b,nq,hd,window,sinks", [(2304, 8, 4, 64, 2048, 5), (2300, 8, 4, 64, 2048, 0), (4352, 4, 4, 128, 4096, 70), (4340, 4, 4, 128, 4096, 0)])
+@pytest.mark.parametrize("s,b,nq,hd,window,sinks", [(2304, 8, 4, 64, 2048, 5), (2300, 8, 4, 64, 2048, 0), (4352, 4, 4, 128, 4096, 70),
+                                                    (4340, 4, 4, 128, 4096, 0)])
 def test_first_tokens_under_a_long_window(s, b, nq, hd, window, sinks):
     """The first 128 queries form delta from the scores in every form of dQ.  (They see one another alone; the reference's 256 tokens
     leave room in sum P |dP| for delta's own way through the matrix unit's sums, hd u |delta|, beside the 66 additions of a lane.)"""
