@@ -6,7 +6,7 @@ What Megatron's multimodal rotary embedding makes a table of angles for, ``[s, b
 
 from __future__ import annotations
 
-from typing import NamedTuple, Optional, Sequence, Tuple
+from typing import List, NamedTuple, Optional, Sequence, Tuple
 
 import torch
 from torch import Tensor
@@ -55,19 +55,22 @@ def check_sections(sections: Sequence[int], hd: int) -> None:
 
 def check_sections_in_turn(sections: Sequence[int]) -> None:
     """Raises unless frequencies dealt in turn give every axis as many as its section says: of 64, (4, 28, 32) would become 22, 21 and 21."""
-    dealt = torch.bincount(axis_of_frequency(sections, True), minlength=len(sections)).tolist()
-    if dealt != list(sections):
-        raise RuntimeError(f"sections {tuple(sections)} cannot be had in turn: the axes would get {tuple(dealt)} frequencies")
+    axes = _axes(sections, True)
+    dealt = tuple(axes.count(a) for a in range(len(sections)))
+    if dealt != tuple(sections):
+        raise RuntimeError(f"sections {tuple(sections)} cannot be had in turn: the axes would get {dealt} frequencies")
+
+
+def _axes(sections: Sequence[int], interleaved: bool) -> List[int]:
+    n = len(sections)
+    if interleaved:
+        return [i % n if i // n < sections[i % n] else 0 for i in range(sum(sections))]
+    return [a for a, size in enumerate(sections) for _ in range(size)]
 
 
 def axis_of_frequency(sections: Sequence[int], interleaved: bool, device=None) -> Tensor:
     """The axis of each frequency, ``[hd / 2]`` int64."""
-    n = len(sections)
-    if interleaved:
-        axis = [i % n if i // n < sections[i % n] else 0 for i in range(sum(sections))]
-    else:
-        axis = [a for a, size in enumerate(sections) for _ in range(size)]
-    return torch.tensor(axis, dtype=torch.int64, device=device)
+    return torch.tensor(_axes(sections, interleaved), dtype=torch.int64, device=device)
 
 
 def rotary_axes(positions: Tensor, dim: int, sections: Sequence[int], base: float = 10000.0, interleaved: bool = False,

@@ -318,3 +318,11 @@ def test_sections_in_turn_are_what_the_axes_get(sections, had):
     else:
         with pytest.raises(RuntimeError, match="in turn"):
             LayerStack(c)
+
+
+def test_sections_are_looked_at_without_a_device():
+    """Layers are made under any default device, whose tensors may hold no values."""
+    with torch.device("meta"):
+        LayerStack(config("eager", torch.float32, layers=1, rotary_sections=(12, 10, 10), rotary_interleaved=True))
+        with pytest.raises(RuntimeError, match="in turn"):
+            LayerStack(config("eager", torch.float32, layers=1, rotary_sections=(8, 12, 12), rotary_interleaved=True))
